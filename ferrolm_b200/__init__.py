@@ -3,9 +3,10 @@
 The package is a thin host-side mirror of the reference's Rust interface over the C ABI of
 `include/ferrovec.h`; all search code is hand-written CUDA in `csrc/`.
 """
+from .kv import KvCache
 from .vector import (NEIGHBOR, Context, FerrovecError, FlatIndex, Hnsw, HnswParams, IvfPq, IvfPqParams, Metric,
                      datagen, datagen_dev, kmeans_assign, kmeans_train, merge_topk_static, neighbors_from_tensor, normalize, padded,
                      recall)
 
-__all__ = ["NEIGHBOR", "Context", "FerrovecError", "FlatIndex", "Hnsw", "HnswParams", "IvfPq", "IvfPqParams", "Metric",
+__all__ = ["NEIGHBOR", "Context", "FerrovecError", "FlatIndex", "Hnsw", "HnswParams", "IvfPq", "IvfPqParams", "KvCache", "Metric",
            "datagen", "datagen_dev", "kmeans_assign", "kmeans_train", "merge_topk_static", "neighbors_from_tensor", "normalize", "padded", "recall"]

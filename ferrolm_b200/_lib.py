@@ -54,6 +54,17 @@ class fv_hnsw_params(C.Structure):
     _fields_ = [("m", C.c_size_t), ("ef_construction", C.c_size_t), ("seed", C.c_uint64)]
 
 
+class fv_kv(C.Structure):
+    _fields_ = [("device", C.c_int), ("dtype", C.c_int), ("kind", C.c_int), ("page_size", C.c_uint32), ("heads", C.c_uint32),
+                ("dim", C.c_uint32), ("pages", C.c_uint64), ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("bounds", C.c_void_p), ("bound_codes", C.c_void_p), ("bound_scale", C.c_void_p)]
+
+
+class fv_kv_batch(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("table_stride", C.c_size_t), ("table_width", C.c_size_t), ("lens", C.c_void_p),
+                ("cu", C.c_void_p), ("nseq", C.c_size_t), ("rows", C.c_size_t)]
+
+
 _vp, _sz, _i, _u32, _u64 = C.c_void_p, C.c_size_t, C.c_int, C.c_uint32, C.c_uint64
 _pp = C.POINTER(C.c_void_p)
 
@@ -139,6 +150,8 @@ SIGNATURES = {
     "fv_read_fvecs": (_i, [C.c_char_p, _sz, _pp, C.POINTER(_sz), C.POINTER(_sz)]),
     "fv_read_ivecs": (_i, [C.c_char_p, _sz, _pp, C.POINTER(_sz), C.POINTER(_sz)]),
     "fv_free": (None, [_vp]),
+    "fv_kv_add_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _sz]),
+    "fv_kv_vectors_dev": (_i, [_vp, _vp, _vp, _vp, _vp]),
     "fv_datagen_dev": (_i, [_vp, _u64, _sz, _sz, _sz, _sz, _vp]),
 }
 

@@ -1,0 +1,166 @@
+// Shared by the operators on a key/value cache (kv_rows.cu, kv_search.cu, kv_attend.cu): where the rows of a call stand, 16-bit
+// and 8-bit values, warp-wide matrix products, launches.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <atomic>
+
+#include "internal.h"
+
+namespace fv {
+
+// ---------------------------------------------------------------------------------------------
+// host side
+int kv_check(const fv_kv* kv, const fv_kv_batch* batch, const char* who);  // kv_rows.cu
+inline bool kv_aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+// Returns fn<type, kind, dim>(...) for what the cache holds.  kv_check has looked at the three.
+#define FV_KV_DISPATCH(kv, fn, ...)                                                                                     \
+  do {                                                                                                                  \
+    const int _d = int((kv)->dim), _k = (kv)->kind;                                                                     \
+    if ((kv)->dtype == FV_KV_BF16) FV_KV_KIND_(__nv_bfloat16, fn, __VA_ARGS__) else FV_KV_KIND_(__half, fn, __VA_ARGS__) \
+  } while (0)
+#define FV_KV_KIND_(T, fn, ...)                                                     \
+  {                                                                                 \
+    if (_k == FV_KV_SAME) FV_KV_DIM_(T, FV_KV_SAME, fn, __VA_ARGS__)                \
+    else if (_k == FV_KV_INT8) FV_KV_DIM_(T, FV_KV_INT8, fn, __VA_ARGS__)           \
+    else FV_KV_DIM_(T, FV_KV_E4M3, fn, __VA_ARGS__)                                 \
+  }
+#define FV_KV_DIM_(T, K, fn, ...)                      \
+  {                                                    \
+    if (_d == 64) return fn<T, K, 64>(__VA_ARGS__);    \
+    if (_d == 96) return fn<T, K, 96>(__VA_ARGS__);    \
+    return fn<T, K, 128>(__VA_ARGS__);                 \
+  }
+
+// Allows a kernel its dynamic shared memory on the current device, once for each device.
+template <auto* kern>
+int kv_allow_smem(int device, size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = 1ull << (device & 63);
+  if (bytes <= 48 * 1024 || (device < 64 && (done.load(std::memory_order_acquire) & bit))) return FV_OK;
+  FV_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+  done.fetch_or(bit, std::memory_order_release);
+  return FV_OK;
+}
+
+#ifdef __CUDACC__
+// ---------------------------------------------------------------------------------------------
+// the batch, as kernels take it
+struct KvBatch {
+  const int32_t* table;
+  size_t table_stride;
+  int table_width;
+  const int32_t* lens;
+  const int32_t* cu;
+  int nseq;
+  int rows;
+  unsigned pages;
+  int page_shift;
+
+  __device__ __forceinline__ int cu_at(int b) const {  // rows before sequence b, never outside of the call's tensors
+    return cu ? min(max(__ldg(cu + b), 0), rows) : min(b, rows);
+  }
+  // page of block j of sequence b, or -1
+  __device__ __forceinline__ int page(int b, int j) const {
+    if (j < 0 || j >= table_width) return -1;
+    const int p = __ldg(table + size_t(b) * table_stride + j);
+    return unsigned(p) < pages ? p : -1;
+  }
+};
+inline KvBatch kv_batch(const fv_kv* kv, const fv_kv_batch* b) {
+  return KvBatch{b->table, b->table_stride, int(b->table_width), b->lens, b->cu, int(b->nseq), int(b->rows),
+                 unsigned(kv->pages), __builtin_ctz(kv->page_size)};
+}
+
+// The sequence whose work holds item `i` when that of sequence b begins at item cu[b] / per + extra * b: the largest such b.
+// Items are handed out without a prefix sum over the sequences that way: floor(x) + floor(y) <= floor(x + y), so a
+// sequence of n rows has n / per + extra items at least to itself.  Whole warps call it; 32 sequences are looked at at once.
+__device__ __forceinline__ int kv_find(const KvBatch& m, int i, int shift, int extra) {
+  int lo = 0, n = m.nseq;  // the answer is in lo .. lo + n - 1
+  const int lane = lane_id();
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int b = lo + lane * step;
+    const bool before = lane * step < n && (m.cu_at(b) >> shift) + extra * b <= i;
+    const int w = 31 - __clz(int(__ballot_sync(FV_FULL, before)) | 1);  // lane 0's begins at item 0
+    lo += w * step;
+    n = min(step, n - w * step);
+  }
+  return lo;
+}
+
+// ---------------------------------------------------------------------------------------------
+// 16-bit values in pairs
+template <class T>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 to_float(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ uint32_t from_float(float lo, float hi) {  // to nearest even
+    uint32_t w;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+  }
+};
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ float2 to_float(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+  static __device__ __forceinline__ uint32_t from_float(float lo, float hi) {
+    uint32_t w;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+  }
+};
+
+// ---------------------------------------------------------------------------------------------
+// 8-bit values.  A code is top * x / most rounded to nearest even, and most, x of 8 or 11 significant bits make the quotient
+// either the border of two codes exactly or further from it than half a step of 32 bits: with a correctly rounded division
+// the code is that of the true quotient.  Values beyond 2^64 are divided by 2^32 first, for top * x to stay finite.
+__device__ __forceinline__ float kv_down(float most) { return most > 0x1p64f ? 0x1p-32f : 1.0f; }
+__device__ __forceinline__ bool kv_finite(float x) { return fabsf(x) < INFINITY; }
+
+template <int KIND>
+struct Eight;
+template <>
+struct Eight<FV_KV_INT8> {
+  static constexpr float top = 127.0f;
+  // four quotients to four codes
+  static __device__ __forceinline__ uint32_t pack(const float* y) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (uint32_t(__float2int_rn(y[i])) & 0xFFu) << (8 * i);
+    return w;
+  }
+  static __device__ __forceinline__ void unpack(uint32_t w, float* y) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = float(int32_t(w << (24 - 8 * i)) >> 24);
+  }
+};
+template <>
+struct Eight<FV_KV_E4M3> {
+  static constexpr float top = 448.0f;
+  static __device__ __forceinline__ uint32_t pack(const float* y) {
+    uint16_t a, b;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a) : "f"(y[1]), "f"(y[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(y[3]), "f"(y[2]));
+    return uint32_t(a) | uint32_t(b) << 16;
+  }
+  static __device__ __forceinline__ void unpack(uint32_t w, float* y) {
+    uint32_t a, b;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"(uint16_t(w)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"(uint16_t(w >> 16)));
+    const float2 x = Pair<__half>::to_float(a), z = Pair<__half>::to_float(b);
+    y[0] = x.x, y[1] = x.y, y[2] = z.x, y[3] = z.y;
+  }
+};
+
+#endif  // __CUDACC__
+
+}  // namespace fv

@@ -290,6 +290,63 @@ int fv_merge_topk_static_dev(int device, void* stream, const fv_neighbor* d_part
                              size_t nparts, size_t nq, size_t k_in, size_t k_out, fv_neighbor* d_out,
                              uint32_t* d_counts);
 
+/* ---- the key/value cache of a language model as an index over its blocks (no counterpart in src/vector: the reference's
+ * own cache is src/kv.rs, on the host).  The rows are a model's keys and values, in pages of `page_size` rows for each
+ * key head; the metric is the inner product; what a search finds are blocks (one page of one sequence), and what is
+ * wanted of them is attention.
+ *
+ * All memory is the caller's, on `device`, and is laid out [pages][heads][page_size][dim] (k, v), [pages][heads][page_size]
+ * (scales), [pages][heads][2][dim] (bounds: the componentwise minima and maxima of a block's keys; bound_codes: the same in
+ * 8 bits), [pages][heads] (bound_scale), contiguous.  k and v hold `dtype` (FV_KV_SAME) or 8 bits: a row is
+ * code * scale with scale = max|x| / 127 (int8) or / 448 (e4m3), and a row with a value that is not finite reads back
+ * as NaN; k_scale and v_scale are NULL for FV_KV_SAME.  k, v and bounds begin on 16 bytes, bound_codes on 16, scales on 4.
+ * dim is 64, 96 or 128, page_size 16, 32, 64 or 128.
+ *
+ * The calls take a cudaStream_t of that device (NULL: its default stream), launch one kernel on it and return: they allocate
+ * nothing, wait for nothing and may be captured into a graph.  Calls on one cache are ordered by their streams; nothing in
+ * the library is shared between them.
+ *
+ * A batch: sequence b has its pages in table[b][0..table_width) and lens[b] rows, those of this call among them.  The call
+ * is about its last n_b rows: row i of them stands at position lens[b] - n_b + i, and they are rows cu[b] .. cu[b+1] of the
+ * call's tensors (cu: nseq + 1 ascending numbers from 0; NULL: one row each, rows = nseq).  Rows from cu[nseq] on are not
+ * touched.  Positions below 0 or in a block from table_width on, and blocks whose table entry is not a page of the cache
+ * (-1, say), are skipped: nothing is read or written there, and nothing attends to them.  A page that add writes to belongs
+ * to one sequence of the call. */
+enum { FV_KV_BF16 = 0, FV_KV_FP16 = 1 };                 /* dtype */
+enum { FV_KV_SAME = 0, FV_KV_INT8 = 1, FV_KV_E4M3 = 2 }; /* kind */
+typedef struct fv_kv {
+  int device;
+  int dtype;
+  int kind;
+  uint32_t page_size;
+  uint32_t heads; /* key heads */
+  uint32_t dim;
+  uint64_t pages;
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  void* bounds;
+  int8_t* bound_codes;
+  float* bound_scale;
+} fv_kv;
+typedef struct fv_kv_batch {
+  const int32_t* table;
+  size_t table_stride; /* from one sequence's pages to the next one's */
+  size_t table_width;
+  const int32_t* lens;
+  const int32_t* cu;
+  size_t nseq;
+  size_t rows; /* of the call's tensors */
+} fv_kv_batch;
+/* Writes the rows k and v ([rows][heads][dim] of dtype; *_row and *_head: strides in elements, multiples of 8) and keeps the
+ * blocks' bounds.  A block that gets its first row forgets the bounds from before; components that are not finite count as
+ * zero in them. */
+int fv_kv_add_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* k, size_t k_row, size_t k_head,
+                  const void* v, size_t v_row, size_t v_head);
+/* Reads rows back, as dtype, to k_out and v_out ([rows][heads][dim], contiguous). */
+int fv_kv_vectors_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, void* k_out, void* v_out);
+
 /* ---- seeded synthetic data for benchmarks and tests: a mixture of `clusters` Gaussians.
  * kind 0: centres uniform in [0,255]^dim, sigma 30, clipped to [0,255] and rounded (SIFT-like integers);
  * kind 1: centres normal*3, sigma 1, rows then scaled to unit length (embedding-like).
