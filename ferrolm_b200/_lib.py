@@ -152,6 +152,7 @@ SIGNATURES = {
     "fv_free": (None, [_vp]),
     "fv_kv_add_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _sz]),
     "fv_kv_vectors_dev": (_i, [_vp, _vp, _vp, _vp, _vp]),
+    "fv_kv_search_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _vp]),
     "fv_datagen_dev": (_i, [_vp, _u64, _sz, _sz, _sz, _sz, _vp]),
 }
 

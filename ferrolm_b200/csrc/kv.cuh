@@ -41,7 +41,9 @@ int kv_allow_smem(int device, size_t bytes) {
   static std::atomic<uint64_t> done{0};
   const uint64_t bit = 1ull << (device & 63);
   if (bytes <= 48 * 1024 || (device < 64 && (done.load(std::memory_order_acquire) & bit))) return FV_OK;
-  FV_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+  cudaFuncAttributes at;
+  FV_CUDA(cudaFuncGetAttributes(&at, kern));
+  FV_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - int(at.sharedSizeBytes)));
   done.fetch_or(bit, std::memory_order_release);
   return FV_OK;
 }

@@ -142,6 +142,36 @@ class KvCache:
         check(lib().fv_kv_vectors_dev(self._ref, self._stream(), self._batch(table, lens, cu, rows), k.data_ptr(), v.data_ptr()))
         return k, v
 
+    # ---- search
+    def search_blocks(self, q, table, lens, k: int, cu=None, first: int = 1, recent: int = 2, out=None):
+        """For every row of the call and key head the `k` blocks that promise the queries the largest inner products:
+        (rows, heads, k) int32, ascending, -1 behind the last.
+
+        `q` is (rows, heads * group, dim), the query heads of a key head one behind the other.  A block's score is the sum
+        over those heads of the largest inner product that the block's bounds allow, worked out in whole numbers, so that
+        it does not depend on how the work is cut; of equal scores the lower block is taken.  The first `first` blocks
+        and the last `recent` ones up to the query's own are always among the `k`, blocks behind the query's position and
+        blocks without a page never."""
+        import torch
+
+        q, qp, qr, qh = self._rows(q, "q")
+        rows, group = q.shape[0], self._group(q)
+        if first < 0 or recent < 0 or k < 1:
+            _refuse(f"k is 1 or more, first and recent are 0 or more: got {k}, {first}, {recent}")
+        shape = (rows, self.heads, k)
+        if out is None:
+            out = torch.empty(shape, dtype=self._i32, device=self.device)
+        elif tuple(out.shape) != shape or out.dtype != self._i32 or out.device != self.device or not out.is_contiguous():
+            _refuse(f"out is a contiguous int32 tensor of {shape} on {self.device}")
+        check(lib().fv_kv_search_dev(self._ref, self._stream(), self._batch(table, lens, cu, rows), qp, qr, qh, group, k, first, recent, out.data_ptr()))
+        return out
+
+    def _group(self, q) -> int:
+        group, more = divmod(q.shape[1], self.heads)
+        if more or not group:
+            _refuse(f"q has a multiple of the cache's {self.heads} heads: got {q.shape[1]}")
+        return group
+
 
 def _contiguous():
     import torch

@@ -346,6 +346,15 @@ int fv_kv_add_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const
                   const void* v, size_t v_row, size_t v_head);
 /* Reads rows back, as dtype, to k_out and v_out ([rows][heads][dim], contiguous). */
 int fv_kv_vectors_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, void* k_out, void* v_out);
+/* For every row and key head the k blocks that promise its queries the largest inner products: out is [rows][heads][k], block
+ * numbers (not pages) ascending, -1 behind the last.  q: [rows][heads * group][dim], query heads group*h .. group*h + group-1
+ * belonging to key head h.  The score of a block is the sum over those heads of the largest inner product that its bounds
+ * allow, in 8 bits: whole numbers, the same on every path; of equals the lower block is taken.  The first `first` blocks and
+ * the last `recent` ones up to the query's own are always among the k.  Blocks behind the query's own position and blocks
+ * without a page are never.  k and group are at most 4096 and 128, table_width at most 50000. */
+enum { FV_KV_MAX_BLOCKS = 4096 };
+int fv_kv_search_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* q, size_t q_row, size_t q_head,
+                     size_t group, size_t k, size_t first, size_t recent, int32_t* out);
 
 /* ---- seeded synthetic data for benchmarks and tests: a mixture of `clusters` Gaussians.
  * kind 0: centres uniform in [0,255]^dim, sigma 30, clipped to [0,255] and rounded (SIFT-like integers);

@@ -76,3 +76,25 @@ class PlainCache:
                     for h in range(self.heads):
                         out[r, h] = self.value(name, page, h, pos % self.page_size).float().to(self.dtype).double()
         return out_k, out_v
+
+    def search(self, q, table, lens, k, cu, first, recent, out):
+        """Into the given int64 tensor.  Sums of whole numbers in 64 bits; the score has the definition's two roundings to 32."""
+        group = q.shape[1] // self.heads
+        for r, b, pos in self.places(table, lens, cu):
+            for h in range(self.heads):
+                x = q[r, h * group : (h + 1) * group]
+                x = torch.where(torch.isfinite(x), x, 0).double()
+                codes = coded(x.flatten(), "int8")[0].view(group, -1)
+                parts = torch.cat((codes.clamp(max=0).sum(0), codes.clamp(min=0).sum(0)))
+                parts = (parts * 127.0 / parts.abs().max().clamp(min=1)).round()
+                last, scored = pos // self.page_size if pos >= 0 else -1, []
+                for j in range(last + 1):
+                    page = self.page(table, b, j)
+                    if page < 0:
+                        continue
+                    s = (parts * self.bound_codes[page, h].flatten()).sum().float() * self.bound_scale[page, h].float()
+                    forced = j < first or j > last - recent
+                    scored.append((-math.inf if forced else -float(s), j))
+                chosen = sorted(j for _, j in sorted(scored)[:k])
+                out[r, h] = torch.tensor(chosen + [-1] * (k - len(chosen)))
+        return out

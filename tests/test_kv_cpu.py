@@ -40,6 +40,7 @@ def calls(fv):
     return {
         "fv_kv_add_dev": lambda c, b: L.fv_kv_add_dev(C.byref(c), None, C.byref(b), AT, 1024, 128, AT, 1024, 128),
         "fv_kv_vectors_dev": lambda c, b: L.fv_kv_vectors_dev(C.byref(c), None, C.byref(b), AT, AT),
+        "fv_kv_search_dev": lambda c, b: L.fv_kv_search_dev(C.byref(c), None, C.byref(b), AT, 4096, 128, 4, 8, 1, 2, AT),
     }
 
 
@@ -78,9 +79,26 @@ def test_null_arguments(fv):
     assert L.fv_kv_vectors_dev(C.byref(c), None, C.byref(b), AT + 2, AT) == ARG
 
 
+def test_searches_that_are_refused(fv):
+    L, c, b = fv.kv.lib(), cache(), batch()
+
+    def search(q=AT, row=4096, head=128, group=4, k=8, first=1, recent=2, out=AT, batch=b):
+        return L.fv_kv_search_dev(C.byref(c), None, C.byref(batch), q, row, head, group, k, first, recent, out)
+
+    assert search(group=0) == search(group=129) == search(k=0) == search(k=4097) == UNSUPPORTED
+    assert search(batch=batch(table_width=50001)) == UNSUPPORTED
+    assert search(q=None) == search(out=None) == search(q=AT + 8) == search(row=4100) == search(head=4) == search(out=AT + 2) == ARG
+
+
 def test_nothing_to_do_is_no_error(fv):
     for call in calls(fv).values():
         assert call(cache(), batch(nseq=0, rows=0, table=None, lens=None)) == 0
+        assert call(cache(pages=0), batch(nseq=0, rows=0)) == 0
+
+
+def test_rows_of_a_cache_without_pages(fv):
+    for name in ("fv_kv_add_dev", "fv_kv_vectors_dev"):
+        call = calls(fv)[name]
         assert call(cache(pages=0, k=None, v=None, k_scale=None, v_scale=None, bounds=None, bound_codes=None, bound_scale=None), batch()) == 0
 
 
