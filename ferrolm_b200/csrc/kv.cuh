@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "internal.h"
 
@@ -80,13 +81,13 @@ inline KvBatch kv_batch(const fv_kv* kv, const fv_kv_batch* b) {
 // The sequence whose work holds item `i` when that of sequence b begins at item cu[b] / per + extra * b: the largest such b.
 // Items are handed out without a prefix sum over the sequences that way: floor(x) + floor(y) <= floor(x + y), so a
 // sequence of n rows has n / per + extra items at least to itself.  Whole warps call it; 32 sequences are looked at at once.
-__device__ __forceinline__ int kv_find(const KvBatch& m, int i, int shift, int extra) {
+__device__ __forceinline__ int kv_find(const KvBatch& m, int i, int per, int extra) {
   int lo = 0, n = m.nseq;  // the answer is in lo .. lo + n - 1
   const int lane = lane_id();
   while (n > 1) {
     const int step = (n + 31) / 32;
     const int b = lo + lane * step;
-    const bool before = lane * step < n && (m.cu_at(b) >> shift) + extra * b <= i;
+    const bool before = lane * step < n && unsigned(m.cu_at(b)) / unsigned(per) + extra * b <= unsigned(i);
     const int w = 31 - __clz(int(__ballot_sync(FV_FULL, before)) | 1);  // lane 0's begins at item 0
     lo += w * step;
     n = min(step, n - w * step);
@@ -162,6 +163,64 @@ struct Eight<FV_KV_E4M3> {
     y[0] = x.x, y[1] = x.y, y[2] = z.x, y[3] = z.y;
   }
 };
+
+// ---------------------------------------------------------------------------------------------
+// attention (kv_attend.cu, kv_prompt.cu)
+struct KvAttend {
+  const unsigned char* q;
+  size_t q_row, q_head;  // bytes
+  int heads, group;
+  const int32_t* blocks;  // [rows][heads][k], or NULL: all of them
+  int k;
+  float scale;  // of the products, times log2(e)
+  const unsigned char *kp, *vp;
+  const float *k_scale, *v_scale;
+  unsigned char* out;
+  float* lse;
+};
+
+// c += a b: 16 x 16 by 16 x 8, sums in 32 bits
+template <class T>
+__device__ __forceinline__ void mma_16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four 8-bit codes as two pairs of fp16, exactly: (0, 1) and (2, 3).
+template <int KIND>
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& a, uint32_t& b) {
+  if constexpr (KIND == FV_KV_E4M3) {
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"(uint16_t(w)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"(uint16_t(w >> 16)));
+  } else {  // code + 128 in the low byte of 1024 .. 1279, whose step in fp16 is 1
+    w ^= 0x80808080u;
+    const uint32_t x = __byte_perm(w, 0x64646464u, 0x4140), y = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
+    __half2 u = __hsub2(*reinterpret_cast<const __half2*>(&x), off), v = __hsub2(*reinterpret_cast<const __half2*>(&y), off);
+    a = *reinterpret_cast<uint32_t*>(&u), b = *reinterpret_cast<uint32_t*>(&v);
+  }
+}
+__device__ __forceinline__ float exp2_of(float x) {  // to 2 units in the last place; 0 for -inf, NaN for NaN
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {  // of 8 x 8 values of 16 bits, a row on four lanes
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// The power of two that brings numbers of at most `most` below 2^14, so that they fit fp16 with all their bits.
+__device__ __forceinline__ float half_factor(float most) {
+  const int e = int(__float_as_uint(most) >> 23);  // biased; 255: not finite
+  if (e == 255 || most == 0.f) return 1.f;
+  return __uint_as_float(uint32_t(min(max(127 + 13 - (e - 127), 1), 254)) << 23);
+}
 
 #endif  // __CUDACC__
 

@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(128) kv_add_kernel(KvPool pool, KvBatch m, KvI
   const int head = WARPS > 1 ? int(blockIdx.y) : int(blockIdx.y) * 4 + warp, part = WARPS > 1 ? warp : 0;
   if (head >= pool.heads) return;  // whole warps, and with WARPS > 1 whole blocks
   const int shift = pool.page_shift, size = 1 << shift, item = blockIdx.x;
-  const int b = m.cu ? kv_find(m, item, shift, 2) : item;
+  const int b = m.cu ? kv_find(m, item, size, 2) : item;
   const int r0 = m.cu_at(b), r1 = max(m.cu_at(b + 1), r0), len = __ldg(m.lens + b);
   const int pos0 = len - (r1 - r0);  // of row r0
   const int j = (max(pos0, 0) >> shift) + (m.cu ? item - ((r0 >> shift) + 2 * b) : 0);

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(KV_SEARCH_THREADS) kv_search_kernel(KvSearch a
   int b, row, rows;  // the CTA's rows are row .. row + rows - 1
   {
     const int item = blockIdx.x;
-    b = m.cu ? kv_find(m, item, SHIFT, R > 1) : item;
+    b = m.cu ? kv_find(m, item, R, R > 1) : item;
     const int r0 = m.cu_at(b), r1 = max(m.cu_at(b + 1), r0);
     row = R > 1 ? r0 + ((item - ((r0 >> SHIFT) + b)) << SHIFT) : item;
     rows = min(R, r1 - row);

@@ -166,6 +166,41 @@ class KvCache:
         check(lib().fv_kv_search_dev(self._ref, self._stream(), self._batch(table, lens, cu, rows), qp, qr, qh, group, k, first, recent, out.data_ptr()))
         return out
 
+    # ---- attention
+    def attend(self, q, table, lens, cu=None, blocks=None, scale: float | None = None, return_lse: bool = False, out=None):
+        """softmax(scale q k^T) v over the rows at and before each query's own position: (rows, heads * group, dim), and with
+        `return_lse` also the natural logarithms of the sums, (rows, heads * group) float32.
+
+        `blocks`: the blocks that each row and key head attends to, (rows, heads, k) int32 as `search_blocks` gives them;
+        without it, all of them.  Entries that are no block the query can see, and entries not above all of those before
+        them, are skipped.  A row with nothing to attend to gets zeros and -inf.  `scale` is dim ** -0.5 unless given.
+        `out`: the tensor to write to (with `return_lse` a pair)."""
+        import torch
+
+        q, qp, qr, qh = self._rows(q, "q")
+        rows, heads = q.shape[0], q.shape[1]
+        group, at, k = self._group(q), None, 0
+        if blocks is not None:
+            if blocks.dtype != self._i32 or blocks.device != self.device or blocks.dim() != 3 or tuple(blocks.shape[:2]) != (rows, self.heads) or not blocks.is_contiguous():
+                _refuse(f"blocks is a contiguous int32 tensor of ({rows}, {self.heads}, k) on {self.device}")
+            at, k = blocks.data_ptr(), blocks.shape[2]
+            if k == 0:
+                _refuse("blocks has no entry for a row; leave it out to attend to all blocks")
+        lse = None
+        if out is None:
+            out = torch.empty((rows, heads, self.dim), dtype=self.dtype, device=self.device)
+            if return_lse:
+                lse = torch.empty((rows, heads), dtype=torch.float32, device=self.device)
+        else:
+            out, lse = out if return_lse else (out, None)
+            if tuple(out.shape) != (rows, heads, self.dim) or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() & 15:
+                _refuse(f"out is a contiguous {self.dtype} tensor of {(rows, heads, self.dim)} on {self.device}")
+            if return_lse and (tuple(lse.shape) != (rows, heads) or lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous()):
+                _refuse(f"lse is a contiguous float32 tensor of {(rows, heads)} on {self.device}")
+        check(lib().fv_kv_attend_dev(self._ref, self._stream(), self._batch(table, lens, cu, rows), qp, qr, qh, group, at, k,
+                                     self.dim**-0.5 if scale is None else scale, out.data_ptr(), None if lse is None else lse.data_ptr()))
+        return (out, lse) if return_lse else out
+
     def _group(self, q) -> int:
         group, more = divmod(q.shape[1], self.heads)
         if more or not group:

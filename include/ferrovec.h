@@ -355,6 +355,14 @@ int fv_kv_vectors_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, v
 enum { FV_KV_MAX_BLOCKS = 4096 };
 int fv_kv_search_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* q, size_t q_row, size_t q_head,
                      size_t group, size_t k, size_t first, size_t recent, int32_t* out);
+/* Attention of the call's rows: out [rows][heads * group][dim] of dtype = softmax(scale q k^T) v over the rows at and before a
+ * query's own position, lse [rows][heads * group] (NULL: not wanted) the natural logarithm of the sum.  blocks [rows][heads][k]: the
+ * blocks that each row and key head attends to, as fv_kv_search_dev gives them (ascending; an entry that is no block the
+ * query can see, or is not above all before it that are, is skipped), or NULL for all of them.  A row with nothing to
+ * attend to gets zeros and -inf.  Scores, maxima and sums are 32-bit floats; weights are rounded to 16 bits before they meet the
+ * values. */
+int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* q, size_t q_row, size_t q_head,
+                     size_t group, const int32_t* blocks, size_t k, float scale, void* out, float* lse);
 
 /* ---- seeded synthetic data for benchmarks and tests: a mixture of `clusters` Gaussians.
  * kind 0: centres uniform in [0,255]^dim, sigma 30, clipped to [0,255] and rounded (SIFT-like integers);

@@ -98,3 +98,48 @@ class PlainCache:
                 chosen = sorted(j for _, j in sorted(scored)[:k])
                 out[r, h] = torch.tensor(chosen + [-1] * (k - len(chosen)))
         return out
+
+    def attend(self, q, table, lens, cu, blocks, scale, out, lse):
+        """Into the given float64 tensors, and how far a result may be off: (out, lse, out's tolerance, lse's tolerance).
+
+        A score of dim products summed in 32 bits, then multiplied three times, is off by at most (dim + 4) 2^-24 times the sum
+        of the products' absolute values; a weight by that of its own and of the largest score (all are relative to it), by
+        2^-11 for its rounding to 16 bits (2^-8 where `out`'s type is bf16 and the rows are a prompt's), by 2^-20 for 2^x and
+        the factors that join parts; a sum of n terms in 32 bits by n 2^-24 of the sum of absolute values, and so is the sum
+        of weights.  All of it scales sum |p v|; on top comes the result's own rounding.  A weight in fp16, where 2^14 stands
+        for 1 and the step of the smallest numbers is 2^-24, is off by up to 2^-25 / 2^14 = 2^-39 however small it is; it is
+        held relative to a power of two of at most twice the largest scale, and the sum of weights is at least 1: n rows add
+        n 2^-38 times the largest scale times the largest code."""
+        group, half = q.shape[1] // self.heads, torch.finfo(self.dtype).eps / 2
+        tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
+        for r, b, pos in self.places(table, lens, cu):
+            for h in range(self.heads):
+                if blocks is None:
+                    chosen = range(pos // self.page_size + 1 if pos >= 0 else 0)
+                else:
+                    chosen, most = [], -1
+                    for e in blocks[r, h].tolist():
+                        if most < e < table.shape[1] and e * self.page_size <= pos:
+                            chosen.append(e)
+                            most = e
+                at = [(self.page(table, b, j), j) for j in chosen]
+                rows = [(p, j * self.page_size + s, s) for p, j in at if p >= 0 for s in range(self.page_size) if j * self.page_size + s <= pos]
+                sl = slice(h * group, (h + 1) * group)
+                if not rows:
+                    out[r, sl], lse[r, sl] = 0, -math.inf
+                    continue
+                pages, slots = torch.tensor([x[0] for x in rows]), torch.tensor([x[2] for x in rows])
+                k, v = self.k[pages, h, slots], self.v[pages, h, slots]
+                if self.kind != "same":
+                    k, v = k * self.k_scale[pages, h, slots][:, None], v * self.v_scale[pages, h, slots][:, None]
+                x = q[r, sl].double()
+                s = x @ k.T * scale
+                off = (self.dim + 4) * 2.0**-24 * float((x.abs() @ k.abs().T).nan_to_num(posinf=0).max()) * abs(scale)
+                p = torch.softmax(s, -1)
+                out[r, sl], lse[r, sl] = p @ v, torch.logsumexp(s, -1)
+                n = len(rows)
+                floor = self.v[pages, h, slots].nan_to_num(posinf=0, neginf=0).abs().max() * (1 if self.kind == "same" else self.v_scale[pages, h, slots].nan_to_num().max())
+                weight = (2.0**-8 if self.dtype == torch.bfloat16 and self.kind == "same" else 2.0**-11) + 2 * off + 2 * n * 2.0**-24 + 2.0**-20
+                tol[r, sl] = (p @ v.abs()) * weight + out[r, sl].abs() * half * 1.001 + n * 2.0**-38 * floor + torch.finfo(self.dtype).smallest_normal * half
+                ltol[r, sl] = off + n * 2.0**-24 + lse[r, sl].abs() * 2.0**-22 + 2.0**-20
+        return out, lse, tol, ltol

@@ -41,6 +41,7 @@ def calls(fv):
         "fv_kv_add_dev": lambda c, b: L.fv_kv_add_dev(C.byref(c), None, C.byref(b), AT, 1024, 128, AT, 1024, 128),
         "fv_kv_vectors_dev": lambda c, b: L.fv_kv_vectors_dev(C.byref(c), None, C.byref(b), AT, AT),
         "fv_kv_search_dev": lambda c, b: L.fv_kv_search_dev(C.byref(c), None, C.byref(b), AT, 4096, 128, 4, 8, 1, 2, AT),
+        "fv_kv_attend_dev": lambda c, b: L.fv_kv_attend_dev(C.byref(c), None, C.byref(b), AT, 4096, 128, 4, AT, 8, 0.1, AT, AT),
     }
 
 
@@ -88,6 +89,18 @@ def test_searches_that_are_refused(fv):
     assert search(group=0) == search(group=129) == search(k=0) == search(k=4097) == UNSUPPORTED
     assert search(batch=batch(table_width=50001)) == UNSUPPORTED
     assert search(q=None) == search(out=None) == search(q=AT + 8) == search(row=4100) == search(head=4) == search(out=AT + 2) == ARG
+
+
+def test_attentions_that_are_refused(fv):
+    L, c, b = fv.kv.lib(), cache(), batch()
+
+    def attend(q=AT, row=4096, head=128, group=4, blocks=AT, k=8, scale=0.1, out=AT, lse=AT):
+        return L.fv_kv_attend_dev(C.byref(c), None, C.byref(b), q, row, head, group, blocks, k, scale, out, lse)
+
+    assert attend(group=0) == attend(group=129) == attend(k=0) == attend(k=4097) == UNSUPPORTED
+    assert attend(scale=float("nan")) == attend(scale=float("inf")) == ARG
+    assert attend(q=None) == attend(out=None) == attend(q=AT + 8) == attend(row=4100) == attend(head=4) == ARG
+    assert attend(out=AT + 8) == attend(lse=AT + 2) == attend(blocks=AT + 1) == ARG
 
 
 def test_nothing_to_do_is_no_error(fv):
