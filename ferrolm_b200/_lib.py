@@ -153,7 +153,8 @@ SIGNATURES = {
     "fv_kv_add_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _sz]),
     "fv_kv_vectors_dev": (_i, [_vp, _vp, _vp, _vp, _vp]),
     "fv_kv_search_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _vp]),
-    "fv_kv_attend_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, C.c_float, _vp, _vp]),
+    "fv_kv_attend_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, C.c_float, _vp, _vp, _vp, _sz]),
+    "fv_kv_attend_work": (_sz, [_vp, _vp, _sz]),
     "fv_datagen_dev": (_i, [_vp, _u64, _sz, _sz, _sz, _sz, _vp]),
 }
 

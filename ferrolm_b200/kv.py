@@ -197,8 +197,12 @@ class KvCache:
                 _refuse(f"out is a contiguous {self.dtype} tensor of {(rows, heads, self.dim)} on {self.device}")
             if return_lse and (tuple(lse.shape) != (rows, heads) or lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous()):
                 _refuse(f"lse is a contiguous float32 tensor of {(rows, heads)} on {self.device}")
-        check(lib().fv_kv_attend_dev(self._ref, self._stream(), self._batch(table, lens, cu, rows), qp, qr, qh, group, at, k,
-                                     self.dim**-0.5 if scale is None else scale, out.data_ptr(), None if lse is None else lse.data_ptr()))
+        batch = self._batch(table, lens, cu, rows)
+        size, work = lib().fv_kv_attend_work(self._ref, batch, group), None
+        if size:
+            work = torch.empty(size, dtype=torch.uint8, device=self.device)
+        check(lib().fv_kv_attend_dev(self._ref, self._stream(), batch, qp, qr, qh, group, at, k, self.dim**-0.5 if scale is None else scale,
+                                     out.data_ptr(), None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), size))
         return (out, lse) if return_lse else out
 
     def _group(self, q) -> int:

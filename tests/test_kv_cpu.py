@@ -41,7 +41,7 @@ def calls(fv):
         "fv_kv_add_dev": lambda c, b: L.fv_kv_add_dev(C.byref(c), None, C.byref(b), AT, 1024, 128, AT, 1024, 128),
         "fv_kv_vectors_dev": lambda c, b: L.fv_kv_vectors_dev(C.byref(c), None, C.byref(b), AT, AT),
         "fv_kv_search_dev": lambda c, b: L.fv_kv_search_dev(C.byref(c), None, C.byref(b), AT, 4096, 128, 4, 8, 1, 2, AT),
-        "fv_kv_attend_dev": lambda c, b: L.fv_kv_attend_dev(C.byref(c), None, C.byref(b), AT, 4096, 128, 4, AT, 8, 0.1, AT, AT),
+        "fv_kv_attend_dev": lambda c, b: L.fv_kv_attend_dev(C.byref(c), None, C.byref(b), AT, 4096, 128, 4, AT, 8, 0.1, AT, AT, None, 0),
     }
 
 
@@ -94,13 +94,13 @@ def test_searches_that_are_refused(fv):
 def test_attentions_that_are_refused(fv):
     L, c, b = fv.kv.lib(), cache(), batch()
 
-    def attend(q=AT, row=4096, head=128, group=4, blocks=AT, k=8, scale=0.1, out=AT, lse=AT):
-        return L.fv_kv_attend_dev(C.byref(c), None, C.byref(b), q, row, head, group, blocks, k, scale, out, lse)
+    def attend(q=AT, row=4096, head=128, group=4, blocks=AT, k=8, scale=0.1, out=AT, lse=AT, work=None, size=0):
+        return L.fv_kv_attend_dev(C.byref(c), None, C.byref(b), q, row, head, group, blocks, k, scale, out, lse, work, size)
 
     assert attend(group=0) == attend(group=129) == attend(k=0) == attend(k=4097) == UNSUPPORTED
     assert attend(scale=float("nan")) == attend(scale=float("inf")) == ARG
     assert attend(q=None) == attend(out=None) == attend(q=AT + 8) == attend(row=4100) == attend(head=4) == ARG
-    assert attend(out=AT + 8) == attend(lse=AT + 2) == attend(blocks=AT + 1) == ARG
+    assert attend(out=AT + 8) == attend(lse=AT + 2) == attend(blocks=AT + 1) == attend(work=AT + 8) == ARG
 
 
 def test_nothing_to_do_is_no_error(fv):
