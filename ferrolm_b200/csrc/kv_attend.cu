@@ -21,6 +21,8 @@
 
 namespace fv {
 
+int kv_prompt_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a);  // kv_prompt.cu
+
 // up to so many rows and tasks the work is cut into equal parts, for as many warps
 enum { KV_PARTS_ROWS = 2048, KV_PARTS_TASKS = 2048, KV_PARTS_WARPS = 160 * 16 };
 
@@ -794,5 +796,7 @@ extern "C" int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch
                        scale * 1.44269504088896341f, static_cast<const unsigned char*>(kv->k), static_cast<const unsigned char*>(kv->v),
                        kv->k_scale, kv->v_scale, static_cast<unsigned char*>(out), lse};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // the bits of a prompt's union of lists are kept in shared memory: 8 KB of them at most
+  if (batch->rows > 4 * batch->nseq && batch->table_width <= 65536) return fv::kv_prompt_attend(kv, s, batch, a);
   return fv::kv_token_attend(kv, s, batch, a, work, work_bytes);
 }

@@ -135,11 +135,14 @@ class PlainCache:
                 x = q[r, sl].double()
                 s = x @ k.T * scale
                 off = (self.dim + 4) * 2.0**-24 * float((x.abs() @ k.abs().T).nan_to_num(posinf=0).max()) * abs(scale)
-                p = torch.softmax(s, -1)
-                out[r, sl], lse[r, sl] = p @ v, torch.logsumexp(s, -1)
+                w = torch.exp(s - s.amax(-1, keepdim=True))
+                w = torch.where(w < 2.0**-126, 0.0, w)  # the smallest power of two in 32 bits: what is below has no weight
+                p = w / w.sum(-1, keepdim=True)
+                out[r, sl] = torch.where(p[..., None] > 0, p[..., None] * v, torch.where(p.isnan(), torch.nan, 0.0)[..., None]).sum(1)
+                lse[r, sl] = torch.logsumexp(s, -1)
                 n = len(rows)
                 floor = self.v[pages, h, slots].nan_to_num(posinf=0, neginf=0).abs().max() * (1 if self.kind == "same" else self.v_scale[pages, h, slots].nan_to_num().max())
                 weight = (2.0**-8 if self.dtype == torch.bfloat16 and self.kind == "same" else 2.0**-11) + 2 * off + 2 * n * 2.0**-24 + 2.0**-20
-                tol[r, sl] = (p @ v.abs()) * weight + out[r, sl].abs() * half * 1.001 + n * 2.0**-38 * floor + torch.finfo(self.dtype).smallest_normal * half
+                tol[r, sl] = (p @ v.abs().nan_to_num(posinf=0)) * weight + out[r, sl].abs().nan_to_num(posinf=0) * half * 1.001 + n * 2.0**-38 * floor + torch.finfo(self.dtype).smallest_normal * half
                 ltol[r, sl] = off + n * 2.0**-24 + lse[r, sl].abs() * 2.0**-22 + 2.0**-20
         return out, lse, tol, ltol
