@@ -7,10 +7,10 @@
 // mma.sync, at a quarter of the rate, pay for those of eight rows.  Bound by these products and, where lists have little in
 // common, by the copies.
 //
-// S^T = K Q^T, O^T = V^T P^T as in kv_attend.cu: the queries are the columns, their weights come from S^T by a transposition in
-// registers, and a column's maximum and sum are held by the four lanes of its place.  32 rows of keys share a read of the
-// queries.  Values that are not finite would reach rows that do not see them as 0 * inf: stages that hold some are worked on
-// without them, and they are added where they are seen.
+// S = Q K^T with 16 queries to a tile, whose weights are the operand of O = P V as they stand in registers.  32 rows of keys share
+// a read of the queries.  A maximum that grows by less than a factor of 2 (fp16) or 256 (bf16) is left as it was: the weights
+// stay within their type, and the sums need not be scaled as often.  Values that are not finite would reach rows that do not
+// see them as 0 * inf: stages that hold some are worked on without them, and they are added where they are seen.
 #include <climits>
 
 #include "kv.cuh"
@@ -19,7 +19,7 @@ namespace fv {
 
 namespace {
 
-enum { KV_PROMPT_THREADS = 128, KV_PROMPT_WARPS = 4, KV_PROMPT_NT = 4, KV_PROMPT_COLS = 32 };
+enum { KV_PROMPT_THREADS = 128, KV_PROMPT_WARPS = 4, KV_PROMPT_COLS = 32 };
 
 template <int KIND, int D>
 struct Tile {
@@ -42,18 +42,26 @@ __device__ __forceinline__ void ldmatrix_t(uint32_t* r, uint32_t at) {
 
 // 0x7F80 or 0x7C00 in both halves: the exponent of what is not finite
 template <class T>
-__device__ __forceinline__ constexpr uint32_t exponent_bits() { return std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u; }
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {  // zeros in the halves that are not finite
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+  return w & ~__vcmpeq2(w & e, e);
+}
+// x + 0 * w in both halves: NaN from the first that is not finite on
 template <class T>
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {  // ones in the halves that are not finite
-  return __vcmpeq2(w & exponent_bits<T>(), exponent_bits<T>());
+__device__ __forceinline__ uint32_t watch(uint32_t x, uint32_t w) {
+  uint32_t y;
+  if constexpr (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(w), "r"(0u), "r"(x));
+  else asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(w), "r"(0u), "r"(x));
+  return y;
 }
 
 template <class T, int KIND, int D>
 __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAttend a, KvBatch m, int tiles) {
   using S = Tile<KIND, D>;
   using M = typename std::conditional<KIND == FV_KV_SAME, T, __half>::type;
-  constexpr int NT = KV_PROMPT_NT, COLS = KV_PROMPT_COLS, W = KV_PROMPT_WARPS;
+  constexpr int COLS = KV_PROMPT_COLS, W = KV_PROMPT_WARPS;  // columns: a row and a query head
   constexpr float ONE = std::is_same<M, __half>::value ? 14.f : 0.f;  // log2 of what stands for a weight of 1
+  constexpr float GROWN = std::is_same<M, __half>::value ? 1.f : 8.f;   // log2 of what a maximum may lag behind by
   unsigned char* const ring = dyn_smem() + S::Q;
   uint32_t* const bits = reinterpret_cast<uint32_t*>(dyn_smem() + S::SMEM);
   const int warp = threadIdx.x >> 5, lane = lane_id(), g = lane >> 2, t = lane & 3;
@@ -84,7 +92,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
   }
   // the queries, a column each: in 8 bits as fp16 times a power of two, and in the order in which the codes come
   unsigned char* const sq = dyn_smem() + warp * (COLS * S::Q_PITCH);
-  float by[NT][2];
+  float by[2][2];  // of a lane's columns: 16 x + 8 i + g
   {
     float f[COLS / 4];  // of column 4 i + lane / 8, by the eight lanes that have it
 #pragma unroll
@@ -135,20 +143,21 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
       }
     }
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = 2 * t + i;  // column 8 x + c is 4 (2 x + c / 4) + c % 4
-        const float lo = __shfl_sync(FV_FULL, f[2 * x], (c & 3) * 8), hi = __shfl_sync(FV_FULL, f[2 * x + 1], (c & 3) * 8);
-        by[x][i] = a.scale / (c < 4 ? lo : hi);
+      for (int i = 0; i < 2; ++i) {  // column 4 j + lane / 8 of f[j]
+        const float lo = __shfl_sync(FV_FULL, f[4 * x + 2 * i], (g & 3) * 8), hi = __shfl_sync(FV_FULL, f[4 * x + 2 * i + 1], (g & 3) * 8);
+        by[x][i] = a.scale / (g < 4 ? lo : hi);
       }
   }
-  uint32_t row_of[2] = {0u, 0u};  // of a lane's eight columns, a byte each; 255: none
+  int row_of[2][2];  // of a lane's columns; 31, which no warp has with a column to spare, for none
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int c = 8 * (j >> 1) + 2 * t + (j & 1);
-    row_of[j >> 2] |= uint32_t(c < cols && c / per < mine ? c / per : 255) << (8 * (j & 3));
-  }
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = 16 * x + 8 * i + g;
+      row_of[x][i] = c < cols && c / per < mine ? c / per : 31;
+    }
   __syncthreads();
 
   // the walk over the pieces of the union: block `at`, whose page is `page`, piece `sub`; the block after it is known already
@@ -177,8 +186,10 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
       if (start < 0) continue;
       const size_t from = ((size_t(page) * a.heads + head) << m.page_shift) + sub * 16;
       ++sub;
-      for (int u = threadIdx.x; u < S::ROW; u += KV_PROMPT_THREADS) {
-        const int r = u / (S::ROW / 16), x = (u - r * (S::ROW / 16)) * 16, bytes = start + r <= last ? 16 : 0;
+#pragma unroll
+      for (int i = 0; i < (S::ROW + KV_PROMPT_THREADS - 1) / KV_PROMPT_THREADS; ++i) {
+        const int u = threadIdx.x + i * KV_PROMPT_THREADS, r = u / (S::ROW / 16), x = (u - r * (S::ROW / 16)) * 16, bytes = start + r <= last ? 16 : 0;
+        if (S::ROW % KV_PROMPT_THREADS && u >= S::ROW) break;
         const uint32_t dst = to + (16 * p + r) * S::PITCH + x;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(a.kp + from * S::ROW + u * 16), "r"(bytes));
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + S::ROWS * S::PITCH), "l"(a.vp + from * S::ROW + u * 16), "r"(bytes));
@@ -202,17 +213,210 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
   const int32_t* const list = a.blocks ? a.blocks + (size_t(row + (lane < mine ? lane : 0)) * a.heads + head) * a.k : nullptr;
   int entry = -1, ahead = a.blocks && lane < mine ? __ldg(list) : 0, index = 0;
 
-  float o[D / 16][NT][4], top[NT][2], l[NT][2];
+  float o[2][D / 8][4], top[2][2], l[2][2];  // tiles of 16 columns; of 8 components
   int unit = 0;  // 8 bits: values stand for multiples of 2^(unit - 126)
 #pragma unroll
-  for (int x = 0; x < NT; ++x) {
+  for (int x = 0; x < 2; ++x) {
     top[x][0] = top[x][1] = -INFINITY, l[x][0] = l[x][1] = 0.f;
 #pragma unroll
-    for (int u = 0; u < D / 16; ++u)
+    for (int u = 0; u < D / 8; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[u][x][i] = 0.f;
+      for (int i = 0; i < 4; ++i) o[x][u][i] = 0.f;
   }
-  const uint32_t q_at = uint32_t(__cvta_generic_to_shared(sq)) + ((lane & 7) + (lane >> 4) * 8) * S::Q_PITCH + (lane >> 3 & 1) * 16;
+  const int r8 = lane & 7, second = lane >> 3 & 1, third = lane >> 4;  // which row of which of four 8 x 8 tiles a lane points at
+  const uint32_t q_at = uint32_t(__cvta_generic_to_shared(sq)) + (r8 + second * 8) * S::Q_PITCH + third * 16;
+
+  // 32 rows of the cache, in two pieces that begin at start[0] and start[1] and are seen by who[0] and who[1]; ALL: by every row of
+  // the warp, whole.  ODD: some of their values are not finite.
+  auto take = [&](const unsigned char* s, int pair, const int* start, const unsigned* who, auto all_of, auto odd_of) {
+    constexpr bool ALL = decltype(all_of)::value, ODD = decltype(odd_of)::value;
+    const uint32_t keys = uint32_t(__cvta_generic_to_shared(s)) + 32 * pair * S::PITCH, values = keys + S::ROWS * S::PITCH;
+    [[maybe_unused]] const float* const scales = reinterpret_cast<const float*>(s + 2 * S::ROWS * S::PITCH) + 32 * pair;
+    float sc[2][4][4] = {};  // tiles of columns; of 8 rows of the cache
+    if constexpr (KIND == FV_KV_SAME) {
+      const uint32_t k_at = keys + (r8 + third * 8) * S::PITCH + second * 16;
+#pragma unroll
+      for (int st = 0; st < D / 16; ++st) {
+        uint32_t q[2][4], k[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) ldmatrix(q[x], q_at + x * 16 * S::Q_PITCH + st * 32), ldmatrix(k[x], k_at + x * 16 * S::PITCH + st * 32);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) mma_16<M>(sc[x][j], q[x][0], q[x][1], q[x][2], q[x][3], k[j >> 1][(j & 1) * 2], k[j >> 1][(j & 1) * 2 + 1]);
+      }
+    } else {
+      const uint32_t k_at = keys + (r8 + second * 8) * S::PITCH + third * 16;
+#pragma unroll
+      for (int st = 0; st < D / 32; ++st) {
+        uint32_t c[2][4];  // 16 rows each: rows 0-7 and 8-15 of 16 components, then of the next 16
+#pragma unroll
+        for (int h = 0; h < 2; ++h) ldmatrix(c[h], k_at + h * 16 * S::PITCH + st * 32);
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          uint32_t q[2][4], k[4][2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) ldmatrix(q[x], q_at + x * 16 * S::Q_PITCH + (2 * st + z) * 32);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) codes_to_half<KIND>(c[j >> 1][2 * z + (j & 1)], k[j][0], k[j][1]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) mma_16<M>(sc[x][j], q[x][0], q[x][1], q[x][2], q[x][3], k[j][0], k[j][1]);
+        }
+      }
+    }
+    [[maybe_unused]] float vs[4][2];  // of a lane's rows of the cache: 8 j + 2 t + i
+    float grown = 1.f;
+    if constexpr (KIND != FV_KV_SAME) {
+      float most = 0.f;  // leaves NaN out: it reaches the sums through its weight
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 ks = *reinterpret_cast<const float2*>(scales + 8 * j + 2 * t);
+        float2 v = *reinterpret_cast<const float2*>(scales + S::ROWS + 8 * j + 2 * t);
+        if (!ALL && start[j >> 1] < 0) v = make_float2(0.f, 0.f);
+        most = fmaxf(most, fmaxf(v.x, v.y));
+        vs[j][0] = v.x, vs[j][1] = v.y;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) sc[x][j][0] *= ks.x, sc[x][j][1] *= ks.y, sc[x][j][2] *= ks.x, sc[x][j][3] *= ks.y;
+      }
+      const int e = max(unit, int(__reduce_max_sync(FV_FULL, __float_as_uint(most)) >> 23));
+      grown = __uint_as_float(uint32_t(max(127 + unit - e, 0)) << 23);
+      unit = e;
+      const float down = __uint_as_float(uint32_t(max(253 - e, 1)) << 23);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vs[j][0] *= down, vs[j][1] *= down;
+    }
+    bool moved = grown != 1.f;
+    float to[2][2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float y = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool seen = ALL || (who[j >> 1] >> row_of[x][i] & 1u);
+          const int ahead = pos + row_of[x][i] - start[j >> 1] - 8 * (j & 1) - 2 * t;  // rows of the cache up to the column's own
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            float& v = sc[x][j][2 * i + z];
+            v *= by[x][i];
+            if (!ALL && !(seen && z <= ahead)) v = -INFINITY;
+            y = fmaxf(y, v);
+          }
+        }
+        to[x][i] = y;
+        moved = moved || y > top[x][i] + GROWN;  // -inf + GROWN is -inf
+      }
+    if (__any_sync(FV_FULL, moved)) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float y = fmaxf(top[x][i], to[x][i]);
+          y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 1));
+          y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 2));
+          const float by_l = y > top[x][i] ? exp2_of(top[x][i] - y) : 1.f, by_o = by_l * grown;
+          top[x][i] = y;
+          l[x][i] *= by_l;
+#pragma unroll
+          for (int u = 0; u < D / 8; ++u) o[x][u][2 * i] *= by_o, o[x][u][2 * i + 1] *= by_o;
+        }
+    }
+    // weights, rounded to 16 bits: tiles of 16 columns by 16 rows of the cache
+    uint32_t p[2][2][4];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float off = top[x][i] == -INFINITY ? 0.f : ONE - top[x][i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float y[2];
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            y[z] = exp2_of(sc[x][j][2 * i + z] + off);
+            l[x][i] += y[z];
+            if constexpr (KIND != FV_KV_SAME) y[z] = y[z] != 0.f ? y[z] * vs[j][z] : 0.f;
+            if constexpr (ODD) sc[x][j][2 * i + z] = y[z];
+          }
+          p[x][j >> 1][i + 2 * (j & 1)] = Pair<M>::from_float(y[0], y[1]);
+        }
+      }
+    if constexpr (KIND == FV_KV_SAME) {
+      const uint32_t v_at = values + (r8 + second * 8) * S::PITCH + third * 16;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (!ALL && start[h] < 0) continue;  // its place holds anything
+#pragma unroll
+        for (int u = 0; u < D / 8; u += 2) {
+          uint32_t v[4];
+          ldmatrix_t(v, v_at + h * 16 * S::PITCH + u * 16);
+          if constexpr (ODD) {
+#pragma unroll
+            for (int z = 0; z < 4; ++z) v[z] = finite_only<T>(v[z]);
+          }
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) mma_16<M>(o[x][u + z], p[x][h][0], p[x][h][1], p[x][h][2], p[x][h][3], v[2 * z], v[2 * z + 1]);
+        }
+        if constexpr (ODD) {  // what was left out, to the columns that have a weight for it
+#pragma unroll 1
+          for (int j = 0; j < 16; ++j) {
+            const T* vr = reinterpret_cast<const T*>(s + (S::ROWS + 32 * pair + 16 * h + j) * S::PITCH);
+            float w[2][2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float y = 0.f;  // tile j / 8 of the piece, lane j / 2 % 4, number j % 2
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                  const float here = __shfl_sync(FV_FULL, sc[x][2 * h + (z >> 1)][2 * i + (z & 1)], (lane & ~3) + (j >> 1 & 3));
+                  if ((j >> 3) == (z >> 1) && (j & 1) == (z & 1)) y = here;
+                }
+                w[x][i] = y;
+              }
+#pragma unroll
+            for (int u = 0; u < D / 8; ++u)
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const float v = float(vr[8 * u + 2 * t + z]);
+                if (kv_finite(v)) continue;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                  for (int i = 0; i < 2; ++i)
+                    if (w[x][i] != 0.f) o[x][u][2 * i + z] += w[x][i] * v;
+              }
+          }
+        }
+      }
+    } else {
+      const uint32_t v_at = values + (r8 + second * 8) * S::PITCH + third * 16;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (!ALL && start[h] < 0) continue;
+#pragma unroll
+        for (int u = 0; u < D / 8; u += 4) {
+          uint32_t c[4];  // rows 0-7 and 8-15 of 16 components, then of the next 16
+          ldmatrix_t(c, v_at + h * 16 * S::PITCH + u * 8);
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            uint32_t v[2][2];  // the even and the odd components of 16, of two neighbouring rows each
+#pragma unroll
+            for (int i = 0; i < 2; ++i) codes_to_half<KIND>(__byte_perm(c[2 * z + i], 0, 0x3120), v[0][i], v[1][i]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) mma_16<M>(o[x][u + 2 * z + i], p[x][h][0], p[x][h][1], p[x][h][2], p[x][h][3], v[i][0], v[i][1]);
+          }
+        }
+      }
+    }
+  };
 
 #pragma unroll 1
   for (int stage = 0;; stage = stage + 1 == S::STAGES ? 0 : stage + 1) {
@@ -221,21 +425,22 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
     int odd = 0;
     if constexpr (KIND == FV_KV_SAME) {  // each thread looks at what it has copied
       uint32_t found = 0u;
+#pragma unroll
       for (int p = 0; p < 4; ++p)
-        for (int u = threadIdx.x; u < S::ROW; u += KV_PROMPT_THREADS) {
-          const int r = u / (S::ROW / 16), x = (u - r * (S::ROW / 16)) * 16;
+#pragma unroll
+        for (int i = 0; i < (S::ROW + KV_PROMPT_THREADS - 1) / KV_PROMPT_THREADS; ++i) {
+          const int u = threadIdx.x + i * KV_PROMPT_THREADS, r = u / (S::ROW / 16), x = (u - r * (S::ROW / 16)) * 16;
+          if (S::ROW % KV_PROMPT_THREADS && u >= S::ROW) break;
           const uint4 v = *reinterpret_cast<const uint4*>(s + (S::ROWS + 16 * p + r) * S::PITCH + x);
-          found |= not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w);
+          found = watch<T>(watch<T>(watch<T>(watch<T>(found, v.x), v.y), v.z), v.w);
         }
-      odd = __syncthreads_or(found != 0u);
+      odd = __syncthreads_or(found != 0u);  // 0 * w is 0 or -0, and 0 + -0 is 0
     } else {
       __syncthreads();
     }
     const int* const where = reinterpret_cast<const int*>(s + S::STAGE - 16);
     if (where[0] < 0) break;  // the union is done
     fill(stage == 0 ? S::STAGES - 1 : stage - 1);  // the stage that everybody has left
-    const uint32_t keys = uint32_t(__cvta_generic_to_shared(s)), values = keys + S::ROWS * S::PITCH;
-    const float* const scales = reinterpret_cast<const float*>(s + 2 * S::ROWS * S::PITCH);
 #pragma unroll 1
     for (int pair = 0; pair < 2; ++pair) {
       int start[2];
@@ -260,187 +465,11 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
         all = all && who[h] == everyone && start[h] + 15 <= pos;
       }
       if ((who[0] | who[1]) == 0u) continue;
-      // scores
-      float sc[2][NT][4] = {};
-      const uint32_t k_at = keys + (32 * pair + (lane & 7) + (lane >> 3 & 1) * 8) * S::PITCH + (lane >> 4) * 16;
-      if constexpr (KIND == FV_KV_SAME) {
-#pragma unroll
-        for (int st = 0; st < D / 16; ++st) {
-          uint32_t q[2][4], k[4];
-          ldmatrix(q[0], q_at + st * 32);
-          ldmatrix(q[1], q_at + 16 * S::Q_PITCH + st * 32);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            ldmatrix(k, k_at + h * 16 * S::PITCH + st * 32);
-#pragma unroll
-            for (int x = 0; x < NT; ++x) mma_16<M>(sc[h][x], k[0], k[1], k[2], k[3], q[x >> 1][(x & 1) * 2], q[x >> 1][(x & 1) * 2 + 1]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int st = 0; st < D / 32; ++st) {
-          uint32_t k[2][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) ldmatrix(k[h], k_at + h * 16 * S::PITCH + st * 32);
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            uint32_t q[2][4];
-            ldmatrix(q[0], q_at + (2 * st + z) * 32);
-            ldmatrix(q[1], q_at + 16 * S::Q_PITCH + (2 * st + z) * 32);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t c[4];
-              codes_to_half<KIND>(k[h][2 * z], c[0], c[2]);
-              codes_to_half<KIND>(k[h][2 * z + 1], c[1], c[3]);
-#pragma unroll
-              for (int x = 0; x < NT; ++x) mma_16<M>(sc[h][x], c[0], c[1], c[2], c[3], q[x >> 1][(x & 1) * 2], q[x >> 1][(x & 1) * 2 + 1]);
-            }
-          }
-        }
-      }
-      float vs[2][2], grown = 1.f;
-      if constexpr (KIND != FV_KV_SAME) {
-        float most = 0.f;  // leaves NaN out: it reaches the sums through its weight
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int r = 32 * pair + 16 * h + 8 * i + g;
-            const float ks = scales[r];
-            vs[h][i] = start[h] >= 0 ? scales[S::ROWS + r] : 0.f;
-            most = fmaxf(most, vs[h][i]);
-#pragma unroll
-            for (int x = 0; x < NT; ++x) sc[h][x][2 * i] *= ks, sc[h][x][2 * i + 1] *= ks;
-          }
-        const int e = max(unit, int(__reduce_max_sync(FV_FULL, __float_as_uint(most)) >> 23));
-        grown = __uint_as_float(uint32_t(max(127 + unit - e, 0)) << 23);
-        unit = e;
-        const float down = __uint_as_float(uint32_t(max(253 - e, 1)) << 23);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) vs[h][0] *= down, vs[h][1] *= down;
-      }
-      bool moved = grown != 1.f;
-      float to[NT][2];
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float y = -INFINITY;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              float& v = sc[h][x][2 * z + i];
-              v *= by[x][i];
-              if (!all) {
-                const int r = row_of[x >> 1] >> (8 * (2 * (x & 1) + i)) & 255u;
-                if (!(who[h] >> (r & 31) & 1u) || start[h] + g + 8 * z > pos + r) v = -INFINITY;
-              }
-              y = fmaxf(y, v);
-            }
-          to[x][i] = y;
-          moved = moved || y > top[x][i];
-        }
-      if (__any_sync(FV_FULL, moved)) {
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float y = fmaxf(top[x][i], to[x][i]);
-            y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 4));
-            y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 8));
-            y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 16));
-            const float by_l = y > top[x][i] ? exp2_of(top[x][i] - y) : 1.f, by_o = by_l * grown;
-            top[x][i] = y;
-            l[x][i] *= by_l;
-#pragma unroll
-            for (int u = 0; u < D / 16; ++u) o[u][x][i] *= by_o, o[u][x][i + 2] *= by_o;
-          }
-      }
-      // weights: to 16 bits, and from rows to columns
-      uint32_t p[2][NT][2];
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            float y[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              y[i] = exp2_of(sc[h][x][2 * z + i] - (top[x][i] == -INFINITY ? 0.f : top[x][i]) + ONE);
-              l[x][i] += y[i];
-              if constexpr (KIND != FV_KV_SAME) y[i] = y[i] != 0.f ? y[i] * vs[h][z] : 0.f;
-              else if (odd) sc[h][x][2 * z + i] = y[i];
-            }
-            p[h][x][z] = transposed(Pair<M>::from_float(y[0], y[1]));
-          }
-      // values
-      if constexpr (KIND == FV_KV_SAME) {
-        const uint32_t v_at = values + (32 * pair + (lane & 7) + (lane >> 4) * 8) * S::PITCH + (lane >> 3 & 1) * 16;
-#pragma unroll
-        for (int u = 0; u < D / 16; ++u)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (start[h] < 0) continue;  // its place holds anything
-            uint32_t v[4];
-            ldmatrix_t(v, v_at + h * 16 * S::PITCH + u * 32);
-            if (odd) {
-#pragma unroll
-              for (int z = 0; z < 4; ++z) v[z] &= ~not_finite<T>(v[z]);
-            }
-#pragma unroll
-            for (int x = 0; x < NT; ++x) mma_16<M>(o[u][x], v[0], v[1], v[2], v[3], p[h][x][0], p[h][x][1]);
-          }
-        if (odd) {  // what was left out, to the columns that have a weight for it
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (start[h] < 0) continue;
-#pragma unroll 1
-            for (int j = 0; j < 16; ++j) {
-              const unsigned char* vr = s + (S::ROWS + 32 * pair + 16 * h + j) * S::PITCH;
-              float w[NT][2];
-#pragma unroll
-              for (int x = 0; x < NT; ++x)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  const float lo = __shfl_sync(FV_FULL, sc[h][x][i], (j & 7) * 4 + t), hi = __shfl_sync(FV_FULL, sc[h][x][2 + i], (j & 7) * 4 + t);
-                  w[x][i] = j < 8 ? lo : hi;
-                }
-#pragma unroll
-              for (int u = 0; u < D / 16; ++u)
-#pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                  const float v = float(reinterpret_cast<const T*>(vr)[16 * u + 8 * z + g]);
-                  if (kv_finite(v)) continue;
-#pragma unroll
-                  for (int x = 0; x < NT; ++x)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                      if (w[x][i] != 0.f) o[u][x][2 * z + i] += w[x][i] * v;
-                }
-            }
-          }
-        }
-      } else {
-        const uint32_t v_at = values + (32 * pair + (lane & 7) + (lane >> 3 & 1) * 8) * S::PITCH + (lane >> 4) * 16;
-#pragma unroll
-        for (int u = 0; u < D / 16; u += 2)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t c[4];
-            ldmatrix_t(c, v_at + h * 16 * S::PITCH + u * 16);
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              uint32_t v[4];  // components 2 g and 2 g + 1 of 16, of two neighbouring rows each
-              codes_to_half<KIND>(__byte_perm(c[2 * z], 0, 0x3120), v[0], v[1]);
-              codes_to_half<KIND>(__byte_perm(c[2 * z + 1], 0, 0x3120), v[2], v[3]);
-              if (start[h] < 0) v[0] = v[1] = v[2] = v[3] = 0u;  // codes of e4m3 that nobody wrote may be NaN
-#pragma unroll
-              for (int x = 0; x < NT; ++x) mma_16<M>(o[u + z][x], v[0], v[1], v[2], v[3], p[h][x][0], p[h][x][1]);
-            }
-          }
-      }
+      using Yes = std::true_type;
+      using No = std::false_type;
+      if (KIND == FV_KV_SAME && odd) take(s, pair, start, who, No(), std::integral_constant<bool, KIND == FV_KV_SAME>());
+      else if (all) take(s, pair, start, who, Yes(), No());
+      else take(s, pair, start, who, No(), No());
     }
   }
   asm volatile("cp.async.wait_all;");
@@ -449,27 +478,27 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
   const float f = KIND != FV_KV_SAME ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
   __syncwarp();
 #pragma unroll
-  for (int x = 0; x < NT; ++x)
+  for (int x = 0; x < 2; ++x)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float y = l[x][i];
-      y += __shfl_xor_sync(FV_FULL, y, 4);
-      y += __shfl_xor_sync(FV_FULL, y, 8);
-      y += __shfl_xor_sync(FV_FULL, y, 16);
-      const int c = 8 * x + 2 * t + i, tok = c / per;
+      y += __shfl_xor_sync(FV_FULL, y, 1);
+      y += __shfl_xor_sync(FV_FULL, y, 2);
+      const int c = 16 * x + 8 * i + g, tok = c / per;
       const float down = y == 0.f ? 0.f : f / y;
-      T* to = reinterpret_cast<T*>(sq + c * S::Q_PITCH);
+      uint32_t* to = reinterpret_cast<uint32_t*>(sq + c * S::Q_PITCH);
 #pragma unroll
-      for (int u = 0; u < D / 16; ++u) {
-        const uint32_t w = y == 0.f ? 0u : Pair<T>::from_float(o[u][x][i] * down, o[u][x][i + 2] * down);
-        const uint16_t lo = uint16_t(w), hi = uint16_t(w >> 16);
+      for (int u = 0; u < D / 8; u += 2) {
+        float v[4] = {o[x][u][2 * i], o[x][u][2 * i + 1], o[x][u + 1][2 * i], o[x][u + 1][2 * i + 1]};
+#pragma unroll
+        for (int z = 0; z < 4; ++z) v[z] = y == 0.f ? 0.f : v[z] * down;
         if constexpr (KIND == FV_KV_SAME) {
-          reinterpret_cast<uint16_t*>(to)[16 * u + g] = lo, reinterpret_cast<uint16_t*>(to)[16 * u + 8 + g] = hi;
-        } else {
-          reinterpret_cast<uint32_t*>(to)[8 * u + g] = w;
+          to[4 * u + t] = Pair<T>::from_float(v[0], v[1]), to[4 * u + 4 + t] = Pair<T>::from_float(v[2], v[3]);
+        } else {  // components 4 t, 4 t + 2, 4 t + 1, 4 t + 3 of 16
+          *reinterpret_cast<uint2*>(to + 4 * u + 2 * t) = make_uint2(Pair<T>::from_float(v[0], v[2]), Pair<T>::from_float(v[1], v[3]));
         }
       }
-      if (a.lse && g == 0 && c < cols && tok < mine)
+      if (a.lse && t == 0 && c < cols && tok < mine)
         a.lse[size_t(row + tok) * a.heads * a.group + size_t(head) * a.group + first + c - tok * per] =
             y == 0.f ? -INFINITY : (top[x][i] - ONE + log2f(y)) * 0.693147180559945309f;
     }
