@@ -66,7 +66,7 @@ class fv_kv_batch(C.Structure):
 
 
 _vp, _sz, _i, _u32, _u64 = C.c_void_p, C.c_size_t, C.c_int, C.c_uint32, C.c_uint64
-_pp = C.POINTER(C.c_void_p)
+_pp, _kvb = C.POINTER(C.c_void_p), C.POINTER(fv_kv_batch)
 
 # every symbol include/ferrovec.h declares: name -> (restype, argtypes)
 SIGNATURES = {
@@ -150,11 +150,11 @@ SIGNATURES = {
     "fv_read_fvecs": (_i, [C.c_char_p, _sz, _pp, C.POINTER(_sz), C.POINTER(_sz)]),
     "fv_read_ivecs": (_i, [C.c_char_p, _sz, _pp, C.POINTER(_sz), C.POINTER(_sz)]),
     "fv_free": (None, [_vp]),
-    "fv_kv_add_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _sz, _sz]),
-    "fv_kv_vectors_dev": (_i, [_vp, _vp, _vp, _vp, _vp]),
-    "fv_kv_search_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _vp]),
-    "fv_kv_attend_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, C.c_float, _vp, _vp, _vp, _sz]),
-    "fv_kv_attend_work": (_sz, [_vp, _vp, _sz]),
+    "fv_kv_add_dev": (_i, [_vp, _vp, _kvb, _vp, _sz, _sz, _vp, _sz, _sz]),
+    "fv_kv_vectors_dev": (_i, [_vp, _vp, _kvb, _vp, _vp]),
+    "fv_kv_search_dev": (_i, [_vp, _vp, _kvb, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _vp]),
+    "fv_kv_attend_dev": (_i, [_vp, _vp, _kvb, _vp, _sz, _sz, _sz, _vp, _sz, C.c_float, _vp, _vp, _vp, _sz]),
+    "fv_kv_attend_work": (_sz, [_vp, _kvb, _sz]),
     "fv_datagen_dev": (_i, [_vp, _u64, _sz, _sz, _sz, _sz, _vp]),
 }
 

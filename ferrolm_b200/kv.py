@@ -19,7 +19,6 @@ from __future__ import annotations
 
 import ctypes as C
 
-from . import _lib
 from ._lib import FV_ERR_ARG, FerrovecError, check, fv_kv, fv_kv_batch, lib
 
 KINDS = ("same", "int8", "e4m3")
@@ -75,40 +74,51 @@ class KvCache:
         at = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
         self._c = fv_kv(self.device.index, int(dtype == torch.float16), KINDS.index(kind), page_size, heads, dim, pages, at(self.k),
                         at(self.v), at(self.k_scale), at(self.v_scale), at(self.bounds), at(self.bound_codes), at(self.bound_scale))
-        self._ref = C.byref(self._c)
-        self._i32, self._get_stream = torch.int32, torch._C._cuda_getCurrentRawStream
+        self._ready()
+
+    def _ready(self):
+        """What every call uses, looked up once."""
+        import torch
+
+        L = lib()
+        self._ref, self._i32, self._f32, self._index = C.byref(self._c), torch.int32, torch.float32, self.device.index
+        self._empty_like, self._contiguous = torch.empty_like, torch.contiguous_format
+        self._get_stream, self._work_sizes = torch._C._cuda_getCurrentRawStream, {}
+        self._add, self._vectors, self._search, self._attend = L.fv_kv_add_dev, L.fv_kv_vectors_dev, L.fv_kv_search_dev, L.fv_kv_attend_dev
 
     # ---- the batch and the rows of a call
     def _batch(self, table, lens, cu, rows: int):
         i32, dev = self._i32, self.device
-        if table.dtype != i32 or lens.dtype != i32 or table.device != dev or lens.device != dev or table.dim() != 2:
+        if table.dtype is not i32 or lens.dtype is not i32 or table.device != dev or lens.device != dev or table.dim() != 2:
             _refuse("table (sequences, blocks) and lens are int32 tensors on the cache's device")
         n, width = table.shape
-        if lens.shape != (n,) or lens.stride(0) != 1 and n > 1 or table.stride(1) != 1 and width > 1 or table.stride(0) < 0:
-            _refuse("lens has an entry for each row of table, and rows of table are contiguous")
+        stride, next_one = table.stride()
+        if lens.dim() != 1 or len(lens) != n or not lens.is_contiguous() or next_one != 1 and width > 1:
+            _refuse("lens is contiguous and has an entry for each row of table, and rows of table are contiguous")
         at = None
         if cu is not None:
-            if cu.dtype != i32 or cu.device != dev or cu.shape != (n + 1,) or not cu.is_contiguous():
+            if cu.dtype is not i32 or cu.device != dev or cu.dim() != 1 or len(cu) != n + 1 or not cu.is_contiguous():
                 _refuse("cu is a contiguous int32 tensor on the cache's device, with one entry more than there are sequences")
             at = cu.data_ptr()
         elif rows != n:
             _refuse(f"without cu every sequence brings one row: got {rows} rows for {n} sequences")
-        return C.byref(fv_kv_batch(table.data_ptr(), table.stride(0), width, lens.data_ptr(), at, n, rows))
+        return fv_kv_batch(table.data_ptr(), stride, width, lens.data_ptr(), at, n, rows)
 
-    def _rows(self, x, what: str, heads: int | None = None):
-        """(rows, heads, dim) with any strides of whole 16 bytes; copied where it is not like that."""
-        if x.dim() != 3 or x.shape[2] != self.dim or heads is not None and x.shape[1] != heads:
-            _refuse(f"{what} is (rows, heads, dim) with dim {self.dim}" + (f" and {heads} heads" if heads is not None else "") + f": got {tuple(x.shape)}")
-        if x.dtype != self.dtype or x.device != self.device:
+    def _rows(self, x, what: str, heads: int):
+        """(rows, heads, dim) with any strides of whole 16 bytes, copied where it is not like that: it, its address, strides and
+        rows.  `heads`: 0 for any."""
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.dim or heads and shape[1] != heads:
+            _refuse(f"{what} is (rows, heads, dim) with dim {self.dim}" + (f" and {heads} heads" if heads else "") + f": got {tuple(shape)}")
+        if x.dtype is not self.dtype or x.device != self.device:
             _refuse(f"{what} is {self.dtype} on {self.device}: got {x.dtype} on {x.device}")
         r, h, d = x.stride()
-        if d != 1 or (r | h) & 7 or r < 0 or h < 0 or x.data_ptr() & 15:
-            x = x.clone(memory_format=_contiguous())
+        at = x.data_ptr()
+        if d != 1 or (r | h) & 7 or at & 15:
+            x = x.clone(memory_format=self._contiguous)
             r, h, d = x.stride()
-        return x, x.data_ptr(), r, h
-
-    def _stream(self) -> int:
-        return self._get_stream(self.device.index)
+            at = x.data_ptr()
+        return x, at, r, h, shape[0]
 
     # ---- rows
     def add(self, k, v, table, lens, cu=None):
@@ -117,30 +127,36 @@ class KvCache:
         A page that is written to belongs to one sequence of the call.  A block that gets its first row forgets what its
         bounds were; one that is written again from its middle on keeps the bounds of the rows that were there.  Key
         components that are not finite count as zero in the bounds."""
-        k, kp, kr, kh = self._rows(k, "k", self.heads)
-        v, vp, vr, vh = self._rows(v, "v", self.heads)
-        if k.shape != v.shape:
-            _refuse(f"k and v have as many rows: got {k.shape[0]} and {v.shape[0]}")
-        check(lib().fv_kv_add_dev(self._ref, self._stream(), self._batch(table, lens, cu, k.shape[0]), kp, kr, kh, vp, vr, vh))
+        k, kp, kr, kh, rows = self._rows(k, "k", self.heads)
+        v, vp, vr, vh, more = self._rows(v, "v", self.heads)
+        if rows != more:
+            _refuse(f"k and v have as many rows: got {rows} and {more}")
+        status = self._add(self._ref, self._get_stream(self._index), self._batch(table, lens, cu, rows), kp, kr, kh, vp, vr, vh)
+        if status:
+            check(status)
 
     def vectors(self, table, lens, cu=None, rows: int | None = None, out=None):
         """The last rows of every sequence as the cache holds them: (k, v), each (rows, heads, dim) of `dtype`.
 
         `rows`: how many rows the call has; without it cu[-1] is read, for which the host waits.  `out`: the two tensors to
         write to; what stands for no row of the cache stays as it was in them."""
-        import torch
-
         if rows is None:
             rows = table.shape[0] if cu is None else int(cu[-1]) if out is None else out[0].shape[0]
+        shape = (rows, self.heads, self.dim)
         if out is None:
-            k, v = torch.empty((2, rows, self.heads, self.dim), dtype=self.dtype, device=self.device).unbind(0)
+            k, v = self.bounds.new_empty(shape), self.bounds.new_empty(shape)
         else:
             k, v = out
-            for x in out:
-                if tuple(x.shape) != (rows, self.heads, self.dim) or x.dtype != self.dtype or x.device != self.device or not x.is_contiguous() or x.data_ptr() & 15:
-                    _refuse(f"out is two contiguous {self.dtype} tensors of {(rows, self.heads, self.dim)} on {self.device}")
-        check(lib().fv_kv_vectors_dev(self._ref, self._stream(), self._batch(table, lens, cu, rows), k.data_ptr(), v.data_ptr()))
+            self._check_out(k, shape)
+            self._check_out(v, shape)
+        status = self._vectors(self._ref, self._get_stream(self._index), self._batch(table, lens, cu, rows), k.data_ptr(), v.data_ptr())
+        if status:
+            check(status)
         return k, v
+
+    def _check_out(self, x, shape):
+        if tuple(x.shape) != shape or x.dtype is not self.dtype or x.device != self.device or not x.is_contiguous() or x.data_ptr() & 15:
+            _refuse(f"what is written to is a contiguous {self.dtype} tensor of {shape} on {self.device}")
 
     # ---- search
     def search_blocks(self, q, table, lens, k: int, cu=None, first: int = 1, recent: int = 2, out=None):
@@ -152,18 +168,18 @@ class KvCache:
         it does not depend on how the work is cut; of equal scores the lower block is taken.  The first `first` blocks
         and the last `recent` ones up to the query's own are always among the `k`, blocks behind the query's position and
         blocks without a page never."""
-        import torch
-
-        q, qp, qr, qh = self._rows(q, "q")
-        rows, group = q.shape[0], self._group(q)
+        q, qp, qr, qh, rows = self._rows(q, "q", 0)
+        group = self._group(q)
         if first < 0 or recent < 0 or k < 1:
             _refuse(f"k is 1 or more, first and recent are 0 or more: got {k}, {first}, {recent}")
-        shape = (rows, self.heads, k)
+        shape, batch = (rows, self.heads, k), self._batch(table, lens, cu, rows)
         if out is None:
-            out = torch.empty(shape, dtype=self._i32, device=self.device)
-        elif tuple(out.shape) != shape or out.dtype != self._i32 or out.device != self.device or not out.is_contiguous():
+            out = table.new_empty(shape)
+        elif tuple(out.shape) != shape or out.dtype is not self._i32 or out.device != self.device or not out.is_contiguous():
             _refuse(f"out is a contiguous int32 tensor of {shape} on {self.device}")
-        check(lib().fv_kv_search_dev(self._ref, self._stream(), self._batch(table, lens, cu, rows), qp, qr, qh, group, k, first, recent, out.data_ptr()))
+        status = self._search(self._ref, self._get_stream(self._index), batch, qp, qr, qh, group, k, first, recent, out.data_ptr())
+        if status:
+            check(status)
         return out
 
     # ---- attention
@@ -175,34 +191,38 @@ class KvCache:
         without it, all of them.  Entries that are no block the query can see, and entries not above all of those before
         them, are skipped.  A row with nothing to attend to gets zeros and -inf.  `scale` is dim ** -0.5 unless given.
         `out`: the tensor to write to (with `return_lse` a pair)."""
-        import torch
-
-        q, qp, qr, qh = self._rows(q, "q")
-        rows, heads = q.shape[0], q.shape[1]
-        group, at, k = self._group(q), None, 0
+        q, qp, qr, qh, rows = self._rows(q, "q", 0)
+        heads, group, at, k = q.shape[1], self._group(q), None, 0
         if blocks is not None:
-            if blocks.dtype != self._i32 or blocks.device != self.device or blocks.dim() != 3 or tuple(blocks.shape[:2]) != (rows, self.heads) or not blocks.is_contiguous():
+            shape = blocks.shape
+            if blocks.dtype is not self._i32 or blocks.device != self.device or len(shape) != 3 or shape[0] != rows or shape[1] != self.heads or not blocks.is_contiguous():
                 _refuse(f"blocks is a contiguous int32 tensor of ({rows}, {self.heads}, k) on {self.device}")
-            at, k = blocks.data_ptr(), blocks.shape[2]
+            at, k = blocks.data_ptr(), shape[2]
             if k == 0:
                 _refuse("blocks has no entry for a row; leave it out to attend to all blocks")
-        lse = None
+        lse = lse_at = None
         if out is None:
-            out = torch.empty((rows, heads, self.dim), dtype=self.dtype, device=self.device)
+            out = self._empty_like(q, memory_format=self._contiguous)
             if return_lse:
-                lse = torch.empty((rows, heads), dtype=torch.float32, device=self.device)
+                lse = self.bound_scale.new_empty((rows, heads))
         else:
             out, lse = out if return_lse else (out, None)
-            if tuple(out.shape) != (rows, heads, self.dim) or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous() or out.data_ptr() & 15:
-                _refuse(f"out is a contiguous {self.dtype} tensor of {(rows, heads, self.dim)} on {self.device}")
-            if return_lse and (tuple(lse.shape) != (rows, heads) or lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous()):
+            self._check_out(out, (rows, heads, self.dim))
+            if return_lse and (tuple(lse.shape) != (rows, heads) or lse.dtype is not self._f32 or lse.device != self.device or not lse.is_contiguous()):
                 _refuse(f"lse is a contiguous float32 tensor of {(rows, heads)} on {self.device}")
-        batch = self._batch(table, lens, cu, rows)
-        size, work = lib().fv_kv_attend_work(self._ref, batch, group), None
+        if return_lse:
+            lse_at = lse.data_ptr()
+        batch, work_at = self._batch(table, lens, cu, rows), None
+        size = self._work_sizes.get((rows, batch.nseq, heads, batch.table_width > 65536))  # depends on these alone
+        if size is None:
+            size = self._work_sizes[rows, batch.nseq, heads, batch.table_width > 65536] = lib().fv_kv_attend_work(self._ref, batch, group)
         if size:
-            work = torch.empty(size, dtype=torch.uint8, device=self.device)
-        check(lib().fv_kv_attend_dev(self._ref, self._stream(), batch, qp, qr, qh, group, at, k, self.dim**-0.5 if scale is None else scale,
-                                     out.data_ptr(), None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), size))
+            work = self.bound_scale.new_empty(size >> 2)
+            work_at = work.data_ptr()
+        status = self._attend(self._ref, self._get_stream(self._index), batch, qp, qr, qh, group, at, k, self.dim**-0.5 if scale is None else scale,
+                              out.data_ptr(), lse_at, work_at, size)
+        if status:
+            check(status)
         return (out, lse) if return_lse else out
 
     def _group(self, q) -> int:
@@ -210,12 +230,6 @@ class KvCache:
         if more or not group:
             _refuse(f"q has a multiple of the cache's {self.heads} heads: got {q.shape[1]}")
         return group
-
-
-def _contiguous():
-    import torch
-
-    return torch.contiguous_format
 
 
 __all__ = ["KvCache"]
