@@ -36,12 +36,13 @@ inline bool kv_aligned(const void* p, size_t to) { return (reinterpret_cast<uint
     return fn<T, K, 128>(__VA_ARGS__);                 \
   }
 
-// Allows a kernel its dynamic shared memory on the current device, once for each device.
+// Allows a kernel its dynamic shared memory on the current device, once for each device.  Without that it gets 48 KB, its static
+// shared memory (up to 18 KB here) among them.
 template <auto* kern>
 int kv_allow_smem(int device, size_t bytes) {
   static std::atomic<uint64_t> done{0};
   const uint64_t bit = 1ull << (device & 63);
-  if (bytes <= 48 * 1024 || (device < 64 && (done.load(std::memory_order_acquire) & bit))) return FV_OK;
+  if (bytes <= 24 * 1024 || (device < 64 && (done.load(std::memory_order_acquire) & bit))) return FV_OK;
   cudaFuncAttributes at;
   FV_CUDA(cudaFuncGetAttributes(&at, kern));
   FV_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - int(at.sharedSizeBytes)));
@@ -125,9 +126,20 @@ struct Pair<__half> {
 // ---------------------------------------------------------------------------------------------
 // 8-bit values.  A code is top * x / most rounded to nearest even, and most, x of 8 or 11 significant bits make the quotient
 // either the border of two codes exactly or further from it than half a step of 32 bits: with a correctly rounded division
-// the code is that of the true quotient.  Values beyond 2^64 are divided by 2^32 first, for top * x to stay finite.
-__device__ __forceinline__ float kv_down(float most) { return most > 0x1p64f ? 0x1p-32f : 1.0f; }
+// the code is that of the true quotient.  Values beyond 2^64 or below 2^-64 are brought nearer to 1 first, by a power of two,
+// for top * x and 1 / most to stay finite.
+__device__ __forceinline__ float kv_down(float most) { return most > 0x1p64f ? 0x1p-32f : most < 0x1p-64f ? 0x1p64f : 1.0f; }
 __device__ __forceinline__ bool kv_finite(float x) { return fabsf(x) < INFINITY; }
+
+// num / den to the nearest whole number, halves to the even one, from inv = 1 / den to within a unit in the last place: num and
+// den have at most 21 and 14 significant bits and |num / den| <= 127, so num * inv leads to one of the two nearest, and what that
+// leaves of num is exact and says whether the quotient is a half.  A third of the steps of a division.
+__device__ __forceinline__ int kv_whole(float num, float den, float inv) {
+  const int r = __float2int_rn(num * inv);
+  const float left = __fmaf_rn(-float(r), den, num);
+  const bool half = fabsf(left) + fabsf(left) == den;
+  return half && (r & 1) ? (left > 0.f ? r + 1 : r - 1) : r;
+}
 
 template <int KIND>
 struct Eight;

@@ -14,6 +14,8 @@
 //                   block of equals) up to k in all, in ascending order, -1 behind the last
 #include <climits>
 
+#include <cooperative_groups.h>
+
 #include "kv.cuh"
 
 namespace fv {
@@ -28,9 +30,7 @@ struct KvSearch {
   int32_t* out;
 };
 
-enum { KV_SEARCH_THREADS = 256, KV_SEARCH_WARPS = 8 };
-
-__device__ __forceinline__ int whole(float num, float den) { return __float2int_rn(__fdiv_rn(num, den)); }
+enum { KV_SEARCH_THREADS = 256, KV_SEARCH_WARPS = 8, KV_SEARCH_LIST = 128 };
 
 // The 2 D codes of one row's group of queries to dst, by a warp: lanes 0 .. D/4-1 have 4 components each.
 template <class T, int D>
@@ -53,13 +53,13 @@ __device__ __forceinline__ void query_codes(const KvSearch& a, int row, int head
     for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(x[i]));
   }
   most = __uint_as_float(__reduce_max_sync(FV_FULL, __float_as_uint(most)));  // none is negative: ordered like whole numbers
-  const float down = kv_down(most), den = most > 0.f ? most * down : 1.f, up = 127.f * down;
+  const float down = kv_down(most), den = most > 0.f ? most * down : 1.f, up = 127.f * down, inv = __fdiv_rn(1.f, den);
   int p[4] = {}, n[4] = {};
   for (int g = 0; g < a.group; ++g) {
     load(g, x);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int c = whole(x[i] * up, den);
+      const int c = kv_whole(x[i] * up, den, inv);
       p[i] += max(c, 0), n[i] += max(-c, 0);
     }
   }
@@ -67,12 +67,12 @@ __device__ __forceinline__ void query_codes(const KvSearch& a, int row, int head
 #pragma unroll
   for (int i = 0; i < 4; ++i) top = max(top, max(p[i], n[i]));
   top = __reduce_max_sync(FV_FULL, top);
-  const float by = float(max(top, 1));  // at most 127 * 2^16: exact, and far enough from the borders for the quotients too
+  const float by = float(max(top, 1)), inv2 = __fdiv_rn(1.f, by);  // at most 127 * 128, 14 bits
   uint32_t wp = 0, wn = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    wp |= (uint32_t(whole(127.f * float(p[i]), by)) & 0xFFu) << (8 * i);
-    wn |= (uint32_t(whole(-127.f * float(n[i]), by)) & 0xFFu) << (8 * i);
+    wp |= (uint32_t(kv_whole(127.f * float(p[i]), by, inv2)) & 0xFFu) << (8 * i);
+    wn |= (uint32_t(kv_whole(-127.f * float(n[i]), by, inv2)) & 0xFFu) << (8 * i);
   }
   if (on) {
     reinterpret_cast<uint32_t*>(dst)[lane] = wn;          // with the lower bounds
@@ -88,10 +88,11 @@ __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_
 }
 
 // The largest `k` of n keys in shared memory, 0 standing for none, to out in ascending order.  TEAM warps work on one row: a
-// warp, or the whole block (then every thread calls it).  The threshold is found bit by bit from the highest in which two
-// keys differ; HELD keys a thread stay in registers meanwhile (0: they are read again for each bit).
+// warp, or the whole block (then every thread calls it).  HELD keys a thread stay in registers (0: they are read again each time).
+// The threshold is found bit by bit between the largest key and the smallest of the threads' own largest ones, from which on there
+// are at least as many keys as threads, and, for a warp, among those keys alone.
 template <int TEAM, int HELD>
-__device__ __forceinline__ void choose(const uint32_t* keys, int n, int k, int32_t* out, int* s_team) {
+__device__ __forceinline__ void choose(const uint32_t* keys, int n, int k, int32_t* out, int* s_team, uint2* s_list) {
   const int lane = lane_id(), me = TEAM > 1 ? int(threadIdx.x) : lane, warp = TEAM > 1 ? int(threadIdx.x >> 5) : 0;
   constexpr int STEP = 32 * TEAM;
   uint32_t held[HELD > 0 ? HELD : 1];
@@ -131,32 +132,101 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int n, int k, int32
     }
     return x;
   };
-  int there = 0, forced = 0;
-  uint32_t hi = 0, low = 0;  // largest key that is not forced, and largest complement of one
+  int counts = 0;  // candidates, and forced ones times 2^16
+  uint32_t hi = 0, second = 0;  // a thread's two largest keys that are not forced
   each([&](uint32_t x) {
-    there += x != 0u, forced += x == 0xFFFFFFFFu;
-    if (x != 0u && x != 0xFFFFFFFFu) hi = max(hi, x), low = max(low, ~x);
+    counts += (x != 0u) + (x == 0xFFFFFFFFu ? 1 << 16 : 0);
+    const uint32_t y = x == 0xFFFFFFFFu ? 0u : x;
+    second = max(second, min(hi, y)), hi = max(hi, y);
   });
-  there = total(there);
-  uint32_t t = 1u;  // keys from t on are taken, of those equal to t the first ones
+  counts = total(counts);
+  const int there = counts & 0xFFFF, forced = counts >> 16;
+  const unsigned before = (1u << lane) - 1u;
+  auto bisect = [&](uint32_t lo, uint32_t up, auto&& over, uint32_t& t) {  // the least t with at most k keys from it on, or the k-th key
+    const uint32_t differ = up ^ lo;
+    int bit = differ ? 31 - __clz(int(differ)) : -1;
+    t = bit < 0 ? up : up & ~((2u << bit) - 1u);
+    for (; bit >= 0; --bit) {
+      const uint32_t c = t | 1u << bit;
+      int cnt = 0;
+      over([&](uint32_t x) { cnt += x >= c; });
+      cnt = total(cnt);
+      if (cnt >= k) t = c;
+      if (cnt == k) return true;
+    }
+    return false;
+  };
+  uint32_t t = 1u;  // keys from t on are taken
+  bool exact = true;  // and there are no more of them than k; else, of those equal to t the first ones
   if (there > k) {
-    forced = total(forced);
+    exact = false;
     if (forced >= k) {
       t = 0xFFFFFFFFu;
     } else {
-      hi = largest(hi), low = ~largest(low);
-      const uint32_t differ = hi ^ low;
-      int bit = differ ? 31 - __clz(int(differ)) : -1;
-      t = bit < 0 ? hi : hi & ~((2u << bit) - 1u);
-      for (; bit >= 0; --bit) {
-        const uint32_t c = t | 1u << bit;
-        int cnt = 0;
-        each([&](uint32_t x) { cnt += x >= c; });
-        cnt = total(cnt);
-        if (cnt >= k) t = c;
-        if (cnt == k) break;
+      // as many keys as threads, or twice as many, are at least as large as this; 0: some thread has none
+      const uint32_t least = k <= STEP ? ~largest(~hi) : k <= 2 * STEP ? ~largest(~second) : 0u;
+      if constexpr (TEAM == 1) {
+        if (least != 0u) {  // those in order to a list of their own: mostly not many more than k
+          int count = 0;
+          auto file = [&](uint32_t x, int i) {
+            const unsigned in = __ballot_sync(FV_FULL, x >= least);
+            const int to = count + __popc(in & before);
+            if (x >= least && to < KV_SEARCH_LIST) s_list[to] = make_uint2(x, uint32_t(i));
+            count += __popc(in);
+          };
+          if constexpr (HELD > 0) {
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) file(held[i], 32 * i + lane);
+          } else {
+            for (int i0 = 0; i0 < n; i0 += 32) file(i0 + lane < n ? keys[i0 + lane] : 0u, i0 + lane);
+          }
+          if (count <= KV_SEARCH_LIST) {
+            __syncwarp();
+            uint2 few[KV_SEARCH_LIST / 32];
+#pragma unroll
+            for (int i = 0; i < KV_SEARCH_LIST / 32; ++i) few[i] = 32 * i + lane < count ? s_list[32 * i + lane] : make_uint2(0u, 0u);
+            exact = bisect(least, largest(hi), [&](auto&& f) {
+#pragma unroll
+              for (int i = 0; i < KV_SEARCH_LIST / 32; ++i) f(few[i].x);
+            }, t);
+            if (exact) {
+              int at = 0;
+#pragma unroll
+              for (int i = 0; i < KV_SEARCH_LIST / 32; ++i) {
+                const unsigned takes = __ballot_sync(FV_FULL, few[i].x >= t);
+                if (few[i].x >= t) out[at + __popc(takes & before)] = int(few[i].y);
+                at += __popc(takes);
+              }
+              __syncwarp();
+              return;
+            }
+            __syncwarp();
+          } else {
+            exact = bisect(least, largest(hi), each, t);
+          }
+        } else {
+          exact = bisect(1u, largest(hi), each, t);
+        }
+      } else {
+        exact = bisect(max(least, 1u), largest(hi), each, t);
       }
     }
+  }
+  if (TEAM == 1 && exact) {
+    int at = 0;
+    auto put = [&](uint32_t x, int i) {
+      const unsigned takes = __ballot_sync(FV_FULL, x >= t);
+      if (x >= t) out[at + __popc(takes & before)] = i;
+      at += __popc(takes);
+    };
+    if constexpr (HELD > 0) {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) put(held[i], 32 * i + lane);
+    } else {
+      for (int i0 = 0; i0 < n; i0 += 32) put(i0 + lane < n ? keys[i0 + lane] : 0u, i0 + lane);
+    }
+    for (int i = at + lane; i < k; i += 32) out[i] = -1;
+    return;
   }
   // every warp of the team has a stretch of the keys
   const int per = TEAM > 1 ? ((n + TEAM - 1) / TEAM + 31) / 32 * 32 : n;
@@ -181,7 +251,7 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int n, int k, int32
     const int i = i0 + lane;
     const uint32_t x = i < end ? keys[i] : 0u;
     const bool eq = i < end && x == t;
-    const unsigned eqs = __ballot_sync(FV_FULL, eq), before = (1u << lane) - 1u;
+    const unsigned eqs = __ballot_sync(FV_FULL, eq);
     const bool take = i < end && (x > t || (eq && seen + __popc(eqs & before) < room));
     const unsigned takes = __ballot_sync(FV_FULL, take);
     if (take) out[at + __popc(takes & before)] = i;
@@ -191,29 +261,35 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int n, int k, int32
     for (int i = at + lane; i < k; i += 32) out[i] = -1;
 }
 
-// TEAM = 8: one row of the call to a CTA (a token).  TEAM = 1: 8 * NT consecutive rows of one sequence (a prompt), which share
+// TEAM = 8: one row of the call to a CTA (a token), or to a cluster of up to 8 where there are few.  TEAM = 1: 8 * NT consecutive rows of one sequence (a prompt), which share
 // what is read of the bounds.  A warp takes 16 blocks at a time straight from memory into the operands of a matrix product:
 // the components are a sum, so lane t of four may hold 16 neighbouring ones where the product would have it hold 4 of each 16,
 // on both sides.
 template <class T, int D, int NT, int TEAM>
-__global__ void __launch_bounds__(KV_SEARCH_THREADS) kv_search_kernel(KvSearch a, KvBatch m, int pitch) {
+__global__ void __launch_bounds__(KV_SEARCH_THREADS, TEAM > 1 ? 3 : 2) kv_search_kernel(KvSearch a, KvBatch m, int pitch, int splits) {
   constexpr int R = TEAM > 1 ? 1 : 8 * NT, CHUNKS = 2 * D / 64;
   constexpr int SHIFT = R == 1 ? 0 : R == 8 ? 3 : R == 16 ? 4 : 5;
   __shared__ __align__(16) int8_t s_codes[8 * NT][2 * D + 16];
   __shared__ int s_team[2 * KV_SEARCH_WARPS];
-  uint32_t* keys = reinterpret_cast<uint32_t*>(dyn_smem());  // [R][pitch]
+  __shared__ uint2 s_list[KV_SEARCH_WARPS][TEAM > 1 ? 1 : KV_SEARCH_LIST];
+  uint32_t* const keys = reinterpret_cast<uint32_t*>(dyn_smem());  // [R][pitch]
   const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = lane_id(), g = lane >> 2, t = lane & 3;
+  const int rank = TEAM > 1 ? int(blockIdx.x) % splits : 0;
   int b, row, rows;  // the CTA's rows are row .. row + rows - 1
   {
-    const int item = blockIdx.x;
+    const int item = TEAM > 1 ? int(blockIdx.x) / splits : int(blockIdx.x);
     b = m.cu ? kv_find(m, item, R, R > 1) : item;
     const int r0 = m.cu_at(b), r1 = max(m.cu_at(b + 1), r0);
     row = R > 1 ? r0 + ((item - ((r0 >> SHIFT) + b)) << SHIFT) : item;
     rows = min(R, r1 - row);
-    if (row < r0 || rows <= 0) return;
+    if (row < r0 || rows <= 0) return;  // the same for a whole cluster
   }
   const int pos0 = __ldg(m.lens + b) - max(m.cu_at(b + 1), row + 1) + row;  // of the first row
   const int n = min(m.table_width, pos0 + rows - 1 < 0 ? 0 : ((pos0 + rows - 1) >> m.page_shift) + 1);
+  const int begin = (rank * KV_SEARCH_WARPS + warp) * 16, step = splits * KV_SEARCH_WARPS * 16;
+  int ahead[2];  // the pages that are next
+#pragma unroll
+  for (int i = 0; i < 2; ++i) ahead[i] = begin + g + 8 * i < n ? m.page(b, begin + g + 8 * i) : -1;
   for (int r = warp; r < 8 * NT; r += KV_SEARCH_WARPS) {
     if (r < rows) {
       query_codes<T, D>(a, row + r, head, s_codes[r]);
@@ -221,30 +297,31 @@ __global__ void __launch_bounds__(KV_SEARCH_THREADS) kv_search_kernel(KvSearch a
       for (int i = lane; i < 2 * D / 4; i += 32) reinterpret_cast<uint32_t*>(s_codes[r])[i] = 0u;
     }
   }
-  __syncthreads();
+  if (TEAM > 1 && splits > 1) cooperative_groups::this_cluster().sync();  // also: the first CTA is there to be written to
+  else __syncthreads();
   uint4 q[NT][CHUNKS];
 #pragma unroll
   for (int x = 0; x < NT; ++x)
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) q[x][c] = *reinterpret_cast<const uint4*>(&s_codes[8 * x + g][64 * c + 16 * t]);
-  for (int j0 = warp * 16; j0 < n; j0 += KV_SEARCH_WARPS * 16) {
+  // the keys of a row's cluster come together in its first CTA
+  uint32_t* const to = TEAM > 1 && splits > 1 ? cooperative_groups::this_cluster().map_shared_rank(keys, 0) : keys;
+  for (int j0 = begin; j0 < n; j0 += step) {
     int acc[NT][4] = {};
     int page[2];
     float scale[2];
     uint4 w[2][CHUNKS];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int j = j0 + g + 8 * i;
-      page[i] = j < n ? m.page(b, j) : -1;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
+      page[i] = ahead[i];
       const size_t at = size_t(max(page[i], 0)) * a.heads + head;
       scale[i] = page[i] >= 0 ? __ldg(a.scale + at) : 0.f;
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c)
         w[i][c] = page[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.codes + at * (2 * D) + 64 * c + 16 * t)) : make_uint4(0, 0, 0, 0);
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ahead[i] = j0 + step + g + 8 * i < n ? m.page(b, j0 + step + g + 8 * i) : -1;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
@@ -255,25 +332,33 @@ __global__ void __launch_bounds__(KV_SEARCH_THREADS) kv_search_kernel(KvSearch a
 #pragma unroll
     for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 8 * x + 2 * t + (i & 1), j = j0 + g + (i & 2) * 4;
-        if (r < R && j < n) {
-          const int last = pos0 + r < 0 ? -1 : (pos0 + r) >> m.page_shift;
+      for (int z = 0; z < 2; ++z) {
+        const int r = 8 * x + 2 * t + z, last = (pos0 + r) >> m.page_shift;  // negative where the row has no position
+        if (r >= R) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = j0 + g + 8 * i;
           // + 0: of the two zeros the one that is not negative
-          uint32_t key = order_bits(__fadd_rn(__fmul_rn(float(acc[x][i]), scale[i >> 1]), 0.f));
+          uint32_t key = order_bits(__fadd_rn(__fmul_rn(float(acc[x][2 * i + z]), scale[i]), 0.f));
           if (j < a.first || j > last - a.recent) key = 0xFFFFFFFFu;
-          if (j > last || page[i >> 1] < 0) key = 0u;
-          keys[size_t(r) * pitch + j] = key;
+          if (j > last || page[i] < 0) key = 0u;
+          if (j < n) to[size_t(r) * pitch + j] = key;
         }
       }
+  }
+  if constexpr (TEAM > 1) {
+    if (splits > 1) {
+      cooperative_groups::this_cluster().sync();
+      if (rank) return;
+    }
   }
   __syncthreads();
   auto pick = [&](int r) {
     const uint32_t* mine = keys + size_t(r) * pitch;
     int32_t* out = a.out + (size_t(row + r) * a.heads + head) * a.k;
-    if (n <= 4 * 32 * TEAM) choose<TEAM, 4>(mine, n, a.k, out, s_team);
-    else if (n <= 16 * 32 * TEAM) choose<TEAM, 16>(mine, n, a.k, out, s_team);
-    else choose<TEAM, 0>(mine, n, a.k, out, s_team);
+    if (n <= 8 * 32 * TEAM) choose<TEAM, 8>(mine, n, a.k, out, s_team, s_list[warp]);
+    else if (n <= 20 * 32 * TEAM) choose<TEAM, 20>(mine, n, a.k, out, s_team, s_list[warp]);
+    else choose<TEAM, 0>(mine, n, a.k, out, s_team, s_list[warp]);
   };
   if constexpr (TEAM > 1) {
     pick(0);
@@ -290,7 +375,23 @@ int search_launch(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const K
   const int pitch = search_pitch(b->table_width);
   const size_t smem = size_t(R) * pitch * 4, items = R == 1 ? b->rows : b->rows / R + b->nseq;
   FV_TRY((kv_allow_smem<kv_search_kernel<T, D, NT, TEAM>>(kv->device, smem)));
-  kv_search_kernel<T, D, NT, TEAM><<<dim3(unsigned(items), kv->heads), KV_SEARCH_THREADS, smem, s>>>(a, kv_batch(kv, b), pitch);
+  int splits = 1;  // CTAs to a row: while the GPU has room for more, and each warp has some of the blocks
+  while (R == 1 && splits < 8 && items * kv->heads * splits <= 148 && b->table_width > size_t(splits) * KV_SEARCH_WARPS * 16) splits *= 2;
+  if (splits > 1) {
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {unsigned(splits), 1, 1};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(items * splits), kv->heads);
+    cfg.blockDim = dim3(KV_SEARCH_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    FV_CUDA(cudaLaunchKernelEx(&cfg, kv_search_kernel<T, D, NT, TEAM>, a, kv_batch(kv, b), pitch, splits));
+    return FV_OK;
+  }
+  kv_search_kernel<T, D, NT, TEAM><<<dim3(unsigned(items), kv->heads), KV_SEARCH_THREADS, smem, s>>>(a, kv_batch(kv, b), pitch, 1);
   FV_CUDA(cudaGetLastError());
   return FV_OK;
 }
