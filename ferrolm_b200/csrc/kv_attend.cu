@@ -22,6 +22,7 @@
 namespace fv {
 
 int kv_prompt_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a);  // kv_prompt.cu
+bool kv_prompt_fits(const fv_kv_batch* b, size_t group, bool lists, size_t k);
 
 // up to so many rows and tasks the work is cut into equal parts, for as many warps
 enum { KV_PARTS_ROWS = 2048, KV_PARTS_TASKS = 2048, KV_PARTS_WARPS = 160 * 16 };
@@ -767,8 +768,10 @@ int token_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAtte
 
 }  // namespace
 
-// The bits of a prompt's union of lists are kept in shared memory: 8 KB of them at most.
-static bool is_prompt(const fv_kv_batch* b) { return b->rows > 4 * b->nseq && b->table_width <= 65536; }
+// Several rows of a sequence on average, and room for the union of their lists.
+static bool is_prompt(const fv_kv_batch* b, size_t group, bool lists, size_t k) {
+  return b->rows > 4 * b->nseq && kv_prompt_fits(b, group, lists, k);
+}
 
 int kv_token_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a, void* work, size_t work_bytes) {
   FV_KV_DISPATCH(kv, token_of, kv, s, b, a, work, work_bytes);
@@ -778,7 +781,7 @@ int kv_token_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const
 
 // Shares that are worth their room: beyond that many tasks a CTA for each of them leaves no SM without work for long.
 extern "C" size_t fv_kv_attend_work(const fv_kv* kv, const fv_kv_batch* batch, size_t group) {
-  if (!kv || !batch || group == 0 || group > 128 || batch->rows > fv::KV_PARTS_ROWS || fv::is_prompt(batch)) return 0;
+  if (!kv || !batch || group == 0 || group > 128 || batch->rows > fv::KV_PARTS_ROWS) return 0;
   const size_t cols = group <= 8 ? 8 : 16, tasks = batch->rows * kv->heads * ((group + cols - 1) / cols);
   return tasks && tasks <= fv::KV_PARTS_TASKS ? (tasks + fv::KV_PARTS_WARPS) * cols * (kv->dim + 2) * 4 : 0;
 }
@@ -799,6 +802,6 @@ extern "C" int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch
                        scale * 1.44269504088896341f, static_cast<const unsigned char*>(kv->k), static_cast<const unsigned char*>(kv->v),
                        kv->k_scale, kv->v_scale, static_cast<unsigned char*>(out), lse};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (fv::is_prompt(batch)) return fv::kv_prompt_attend(kv, s, batch, a);
+  if (kv->pages && fv::is_prompt(batch, group, blocks != nullptr, k)) return fv::kv_prompt_attend(kv, s, batch, a);
   return fv::kv_token_attend(kv, s, batch, a, work, work_bytes);
 }

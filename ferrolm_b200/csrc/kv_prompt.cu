@@ -1,50 +1,85 @@
-// Attention of many rows of a sequence (a prompt, or a piece of one) over blocks of a key/value cache.
+// Attention of many rows of a sequence (a prompt, or a piece of one) over blocks of a key/value cache, on the tensor cores.
 //
-// Every row has a list of blocks of its own, and neighbours have many of them in common.  A CTA has 32 queries for each of its
-// four warps (8 rows of a group of 4 heads, say), goes once over the union of their lists in ascending order, 64 rows of the
-// cache at a time, and a warp passes over pieces of 16 rows that none of its own rows has.  With one 128-row tile for the CTA,
-// as a tcgen05 product wants it, every row of the tile would pay for the blocks of all others; the warps' own tiles of
-// mma.sync, at a quarter of the rate, pay for those of eight rows.  Bound by these products and, where lists have little in
-// common, by the copies.
+// Every row has a list of blocks of its own, and neighbours have many of them in common.  A CTA has 128 queries (32 rows of a
+// group of 4 heads, say) and goes once over the union of their lists in ascending order, 64 rows of the cache at a time:
 //
-// S = Q K^T with 16 queries to a tile, whose weights are the operand of O = P V as they stand in registers.  32 rows of keys share
-// a read of the queries.  A maximum that grows by less than a factor of 2 (fp16) or 256 (bf16) is left as it was: the weights
-// stay within their type, and the sums need not be scaled as often.  Values that are not finite would reach rows that do not
-// see them as 0 * inf: stages that hold some are worked on without them, and they are added where they are seen.
+//   S = Q K^T (128 x 64) and O += P V (128 x dim): tcgen05.mma from shared memory into tensor memory, P read from there
+//   P = 2^(scale S - max): a thread to a query, which has a whole row of S in its registers: no exchange between lanes
+//
+// Warps 0-3 turn S into P, warp 4 issues the products, warp 5 brings keys and warp 6 values, each two tiles ahead at most; S has
+// two places, so that the next one is worked out while this one becomes P.  P takes the place of its S.  Two CTAs share an SM, and
+// the other one's products and copies fill the time in which the first one's threads compute powers of two: 16 an SM and clock,
+// so 512 clocks for a tile whose products take about 250.  That, and the share of a tile that its rows do not have in
+// common, bounds it; tiles of their own for every 8 rows, on mma.sync with its quarter of the rate, were tried and took
+// three times as long.
+//
+// A maximum that grows by less than a factor of 2 (fp16) or 256 (bf16) is left as it was: the weights stay within their type, and
+// O, in tensor memory, need not be scaled as often.  Values that are not finite would reach rows that do not see them as
+// 0 * inf: they are taken out on their way in, and added by the threads whose rows see them.  In 8 bits the codes become fp16,
+// exactly, on their way in; a key's scale multiplies its column of S, a value's its weight (kv_attend.cu).
 #include <climits>
 
 #include "kv.cuh"
+#include "tc.cuh"
 
 namespace fv {
 
 namespace {
 
-enum { KV_PROMPT_THREADS = 128, KV_PROMPT_WARPS = 4, KV_PROMPT_COLS = 32 };
+enum { KV_PROMPT_COLS = 128, KV_PROMPT_WARPS = 7, KV_PROMPT_THREADS = 32 * KV_PROMPT_WARPS };
+
+struct PromptBars {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done, all_done;
+  uint32_t tmem;
+  int abort, odd[2], exponent[2], entries;
+};
 
 template <int KIND, int D>
 struct Tile {
-  static constexpr int BYTES = KIND == FV_KV_SAME ? 2 : 1, ROW = D * BYTES;
-  static constexpr int PITCH = ROW + 16;  // an odd number of 16 bytes: eight rows lie in different banks
-  static constexpr int ROWS = 64;         // of the cache, in a stage
-  static constexpr int STAGE = 2 * ROWS * PITCH + (KIND == FV_KV_SAME ? 0 : 2 * ROWS * 4) + 16;  // keys, values, scales, positions
-  static constexpr int STAGES = KIND == FV_KV_SAME ? 2 : 3;
-  static constexpr int Q_PITCH = 2 * D + 16;
-  static constexpr int Q = KV_PROMPT_WARPS * KV_PROMPT_COLS * Q_PITCH;
-  static constexpr int SMEM = Q + STAGES * STAGE;  // and the bits of the union behind it
+  static constexpr int ROWS = 64;                        // of the cache
+  static constexpr int HALVES = (D + 63) / 64;           // of 64 components: rows of 128 bytes
+  static constexpr int HALF = ROWS * 128;                // bytes
+  static constexpr int STAGE = HALVES * HALF;            // keys or values of one tile
+  static constexpr int Q_HALF = KV_PROMPT_COLS * 128;
+  static constexpr int Q = HALVES * Q_HALF;
+  static constexpr int SCALES = KIND == FV_KV_SAME ? 0 : 2 * 2 * ROWS * 4;  // [stage][keys, values][ROWS]
+  static constexpr int K_AT = Q, V_AT = Q + 2 * STAGE, SCALE_AT = Q + 4 * STAGE, BARS_AT = SCALE_AT + SCALES;
+  static constexpr int LIST_AT = BARS_AT + (int(sizeof(PromptBars)) + 15) / 16 * 16;
+  static constexpr int O_COL = 128;  // columns of tensor memory: S or P 0-63, 64-127, O from 128 on
 };
 
-__device__ __forceinline__ void ldmatrix(uint32_t* r, uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
-}
-__device__ __forceinline__ void ldmatrix_t(uint32_t* r, uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
-}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 0x7F80 or 0x7C00 in both halves: the exponent of what is not finite
+// D (tensor memory) += A (tensor memory: two 16-bit values to a column) B (shared memory)
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t to, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(to)
+      : "memory");
+}
+__device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// zeros in the halves that are not finite, and whether there are any
 template <class T>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w) {  // zeros in the halves that are not finite
+__device__ __forceinline__ uint32_t finite_only(uint32_t w, uint32_t& found) {
   constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
-  return w & ~__vcmpeq2(w & e, e);
+  const uint32_t bad = __vcmpeq2(w & e, e);
+  found |= bad;
+  return w & ~bad;
 }
 // x + 0 * w in both halves: NaN from the first that is not finite on
 template <class T>
@@ -55,33 +90,110 @@ __device__ __forceinline__ uint32_t watch(uint32_t x, uint32_t w) {
   return y;
 }
 
+// What all warps of a CTA know about its work.
+struct PromptWork {
+  int head, last, pieces, tiles;  // position of the last row; pieces of 16 rows of the cache, tiles of four of them
+  const int2* list;               // (block, page) of the union, ascending
+  // piece p: where it begins, and its first row in the pages; false: it is none, or has no page
+  __device__ __forceinline__ bool piece(const KvAttend& a, const KvBatch& m, int p, int& start, size_t& from) const {
+    if (p >= pieces) return false;
+    const int per = m.page_shift - 4, sub = (p & ((1 << per) - 1)) << 4;
+    const int2 at = list[p >> per];
+    start = (at.x << m.page_shift) + sub;
+    from = ((size_t(max(at.y, 0)) * a.heads + head) << m.page_shift) + sub;
+    return at.y >= 0;
+  }
+};
+
+// One warp brings tile i of the keys (or values) to `to`: rows of 128 bytes, 16-byte pieces exchanged by the row's number as the
+// tensor cores read them, zeros for rows that are none.  Piece u of a row of 16 bytes in 16 bits, of 8 codes in 8.
 template <class T, int KIND, int D>
-__global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAttend a, KvBatch m, int tiles) {
+struct Bring {
+  using S = Tile<KIND, D>;
+  static constexpr int UNITS = D / 8;  // 16-byte pieces of a row as it is brought
+  static __device__ __forceinline__ uint32_t place(int r, int u) { return (u >> 3) * S::HALF + r * 128 + (((u & 7) ^ (r & 7)) << 4); }
+
+  static __device__ __forceinline__ void start(const KvAttend& a, const KvBatch& m, const PromptWork& w, int i, const unsigned char* src, uint32_t to, int lane) {
+    static_assert(KIND == FV_KV_SAME, "");
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      int begin = 0;
+      size_t from = 0;
+      const bool on = w.piece(a, m, 4 * i + p, begin, from);
+#pragma unroll
+      for (int x = 0; x < 16 * UNITS / 32; ++x) {
+        const int n = lane + 32 * x, r = n / UNITS, u = n - r * UNITS;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + place(16 * p + r, u)), "l"(src + (on ? from * (2 * D) + n * 16 : 0)),
+                     "r"(on && begin + r <= w.last ? 16 : 0));
+      }
+    }
+    asm volatile("cp.async.commit_group;");
+  }
+  // 8 bits: through registers, where the codes become fp16
+  static __device__ __forceinline__ void convert(const KvAttend& a, const KvBatch& m, const PromptWork& w, int i, const unsigned char* src, unsigned char* to, int lane) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      int begin = 0;
+      size_t from = 0;
+      const bool on = w.piece(a, m, 4 * i + p, begin, from);
+      uint2 c[16 * UNITS / 32];
+#pragma unroll
+      for (int x = 0; x < 16 * UNITS / 32; ++x) {
+        const int n = lane + 32 * x, r = n / UNITS;
+        c[x] = make_uint2(0, 0);
+        if (on && begin + r <= w.last) c[x] = __ldg(reinterpret_cast<const uint2*>(src + from * D + n * 8));
+      }
+#pragma unroll
+      for (int x = 0; x < 16 * UNITS / 32; ++x) {
+        const int n = lane + 32 * x, r = n / UNITS, u = n - r * UNITS;
+        uint4 y;
+        codes_to_half<KIND>(c[x].x, y.x, y.y);
+        codes_to_half<KIND>(c[x].y, y.z, y.w);
+        *reinterpret_cast<uint4*>(to + place(16 * p + r, u)) = y;
+      }
+    }
+  }
+};
+
+template <class T, int KIND, int D>
+__global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAttend a, KvBatch m) {
   using S = Tile<KIND, D>;
   using M = typename std::conditional<KIND == FV_KV_SAME, T, __half>::type;
-  constexpr int COLS = KV_PROMPT_COLS, W = KV_PROMPT_WARPS;  // columns: a row and a query head
-  constexpr float ONE = std::is_same<M, __half>::value ? 14.f : 0.f;  // log2 of what stands for a weight of 1
-  constexpr float GROWN = std::is_same<M, __half>::value ? 1.f : 8.f;   // log2 of what a maximum may lag behind by
-  unsigned char* const ring = dyn_smem() + S::Q;
-  uint32_t* const bits = reinterpret_cast<uint32_t*>(dyn_smem() + S::SMEM);
-  const int warp = threadIdx.x >> 5, lane = lane_id(), g = lane >> 2, t = lane & 3;
+  using B = Bring<T, KIND, D>;
+  constexpr bool HALF = std::is_same<M, __half>::value;
+  constexpr float ONE = HALF ? 14.f : 0.f;   // log2 of what stands for a weight of 1
+  constexpr float GROWN = HALF ? 1.f : 8.f;  // log2 of what a maximum may lag behind by
+  unsigned char* const smem = dyn_smem();
+  PromptBars* const bars = reinterpret_cast<PromptBars*>(smem + S::BARS_AT);
+  int2* const list = reinterpret_cast<int2*>(smem + S::LIST_AT);
+  const int warp = threadIdx.x >> 5, lane = lane_id(), head = blockIdx.y;
 
   // which rows of which sequence
-  const int tw = a.group <= COLS ? COLS / a.group : 1, tc = tw * W;  // rows of a warp and of the CTA
-  const int head = blockIdx.y / tiles, first = (blockIdx.y % tiles) * COLS;
-  const int cols = tiles > 1 ? min(COLS, a.group - first) : tw * a.group;  // of a warp
-  const int per = tiles > 1 ? COLS : a.group;                             // columns of a row
-  const int item = int(gridDim.x - 1 - blockIdx.x);                        // the rows that see most come first
-  const int b = m.cu ? kv_find(m, item, tc, 1) : min(item, m.nseq - 1);
+  const int tc = KV_PROMPT_COLS / a.group;                // rows of a CTA
+  const int item = int(gridDim.x - 1 - blockIdx.x);       // the rows that see most come first
+  const int b = m.cu ? kv_find(m, item, tc, 1) : item;
   const int r0 = m.cu_at(b), r1 = max(m.cu_at(b + 1), r0);
   const int row0 = m.cu ? r0 + (item - (r0 / tc + b)) * tc : r0, rows = min(tc, r1 - row0);
-  if (row0 < r0 || rows <= 0 || (!m.cu && item >= m.nseq)) return;
-  const int pos_cta = __ldg(m.lens + b) - r1 + row0, last = pos_cta + rows - 1;  // positions of the first and the last row
+  if (row0 < r0 || rows <= 0) return;
+  const int pos0 = __ldg(m.lens + b) - r1 + row0, last = pos0 + rows - 1;  // positions of the first and the last row
   const int blocks = min(m.table_width, last < 0 ? 0 : (last >> m.page_shift) + 1);
-  const int row = row0 + warp * tw, mine = min(tw, max(0, rows - warp * tw)), pos = pos_cta + warp * tw;
-  const unsigned everyone = mine == 32 ? ~0u : (1u << mine) - 1u;
 
-  // the union of the lists
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&bars->tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->k_full[i], 32), mbar_init(&bars->k_empty[i], 1), mbar_init(&bars->v_full[i], 32), mbar_init(&bars->v_empty[i], 1);
+      mbar_init(&bars->s_full[i], 1), mbar_init(&bars->p_full[i], KV_PROMPT_COLS);
+      bars->odd[i] = 0;
+    }
+    mbar_init(&bars->pv_done, 1), mbar_init(&bars->all_done, 1);
+    bars->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // the union of the lists: its bits, where keys will be, then its blocks and their pages in order
+  uint32_t* const bits = reinterpret_cast<uint32_t*>(smem + S::K_AT);  // room for 2^18 blocks and more
   if (a.blocks) {
     for (int i = threadIdx.x; i < (blocks + 31) / 32; i += KV_PROMPT_THREADS) bits[i] = 0u;
     __syncthreads();
@@ -89,441 +201,418 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
       const int r = i / a.k, e = __ldg(a.blocks + (size_t(row0 + r) * a.heads + head) * a.k + (i - r * a.k));
       if (e >= 0 && e < blocks) atomicOr(bits + (e >> 5), 1u << (e & 31));
     }
+    __syncthreads();
+    if (warp == 5) {
+      int n = 0;
+      for (int w0 = 0; w0 < (blocks + 31) / 32; w0 += 32) {
+        uint32_t x = w0 + lane < (blocks + 31) / 32 ? bits[w0 + lane] : 0u;
+        int up = __popc(x);  // up to this lane
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(FV_FULL, up, o);
+          if (lane >= o) up += y;
+        }
+        int at = n + up - __popc(x);
+        for (; x; x &= x - 1) list[at++].x = (w0 + lane) * 32 + __ffs(int(x)) - 1;
+        n += __shfl_sync(FV_FULL, up, 31);
+      }
+      if (lane == 0) bars->entries = n;
+    }
+  } else if (threadIdx.x == 0) {
+    bars->entries = blocks;
   }
-  // the queries, a column each: in 8 bits as fp16 times a power of two, and in the order in which the codes come
-  unsigned char* const sq = dyn_smem() + warp * (COLS * S::Q_PITCH);
-  float by[2][2];  // of a lane's columns: 16 x + 8 i + g
-  {
-    float f[COLS / 4];  // of column 4 i + lane / 8, by the eight lanes that have it
+  // the queries: a thread to a query.  In 8 bits as fp16 times a power of two.  A negative scale turns their sign, 0 makes them 0.
+  const int tok = int(threadIdx.x) / a.group, h = int(threadIdx.x) - tok * a.group;  // of a query's thread
+  const bool mine = threadIdx.x < KV_PROMPT_COLS && tok < rows;
+  float by = a.scale == 0.f ? 1.f : fabsf(a.scale);
+  if (warp < 4) {
+    const uint4* src = reinterpret_cast<const uint4*>(a.q + size_t(row0 + (mine ? tok : 0)) * a.q_row + size_t(head * a.group + (mine ? h : 0)) * a.q_head);
+    float most = 0.f;
+    if constexpr (!std::is_same<M, T>::value) {
+      for (int u = 0; u < D / 8; ++u) {
+        const uint4 x = __ldg(src + u);
 #pragma unroll
-    for (int i = 0; i < COLS / 4; ++i) {
-      const int c = 4 * i + (lane >> 3), tok = c / per, h = first + c - tok * per;
-      const bool on = tok < mine && c < cols && h < a.group;
-      const unsigned char* src = a.q + size_t(row + (on ? tok : 0)) * a.q_row + size_t(head * a.group + (on ? h : 0)) * a.q_head;
-      uint4 w[(D / 8 + 7) / 8];
-      float most = 0.f;
+        for (int z = 0; z < 4; ++z) {
+          const float2 y = Pair<T>::to_float(reinterpret_cast<const uint32_t*>(&x)[z]);
+          most = fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y)));
+        }
+      }
+    }
+    const float f = std::is_same<M, T>::value ? 1.f : half_factor(most);
+    by = fmaxf(by / f, __uint_as_float(1u));  // never 0: what is not seen is -inf times it
+    const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u, keep = mine && a.scale != 0.f ? ~0u : 0u;
+    for (int u = 0; u < D / 8; ++u) {
+      uint4 x = __ldg(src + u);
+      uint32_t* w = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
-      for (int x = 0; x < (D / 8 + 7) / 8; ++x) {
-        const int p = (lane & 7) + 8 * x;
-        w[x] = make_uint4(0, 0, 0, 0);
-        if (on && p < D / 8) w[x] = __ldg(reinterpret_cast<const uint4*>(src) + p);
+      for (int z = 0; z < 4; ++z) {
         if constexpr (!std::is_same<M, T>::value) {
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const float2 y = Pair<T>::to_float(reinterpret_cast<const uint32_t*>(&w[x])[z]);
-            most = fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y)));
-          }
+          const float2 y = Pair<T>::to_float(w[z]);
+          w[z] = Pair<M>::from_float(y.x * f, y.y * f);
         }
+        w[z] = (w[z] ^ sign) & keep;
       }
-      f[i] = 1.f;
-      if constexpr (!std::is_same<M, T>::value) {
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(FV_FULL, most, o));
-        f[i] = half_factor(most);
-      }
-#pragma unroll
-      for (int x = 0; x < (D / 8 + 7) / 8; ++x) {
-        const int p = (lane & 7) + 8 * x;
-        if (p >= D / 8) continue;
-        if constexpr (KIND == FV_KV_SAME) {
-          *reinterpret_cast<uint4*>(sq + c * S::Q_PITCH + p * 16) = w[x];
-        } else {
-          // components 4 t .. 4 t + 3 of 16 stand at 2 t, 2 t + 1, 8 + 2 t, 8 + 2 t + 1; these 8 are the first or second half
-          uint32_t* to = reinterpret_cast<uint32_t*>(sq + c * S::Q_PITCH + (p >> 1) * 32);
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            uint32_t y = reinterpret_cast<const uint32_t*>(&w[x])[z];
-            if constexpr (!std::is_same<M, T>::value) {
-              const float2 v = Pair<T>::to_float(y);
-              y = Pair<M>::from_float(v.x * f[i], v.y * f[i]);
-            }
-            to[(p & 1) * 2 + (z >> 1) + (z & 1) * 4] = y;
-          }
-        }
-      }
+      const int r = threadIdx.x;
+      *reinterpret_cast<uint4*>(smem + (u >> 3) * S::Q_HALF + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = x;
     }
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {  // column 4 j + lane / 8 of f[j]
-        const float lo = __shfl_sync(FV_FULL, f[4 * x + 2 * i], (g & 3) * 8), hi = __shfl_sync(FV_FULL, f[4 * x + 2 * i + 1], (g & 3) * 8);
-        by[x][i] = a.scale / (g < 4 ? lo : hi);
-      }
+    fence_async();
   }
-  int row_of[2][2];  // of a lane's columns; 31, which no warp has with a column to spare, for none
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c = 16 * x + 8 * i + g;
-      row_of[x][i] = c < cols && c / per < mine ? c / per : 31;
-    }
   __syncthreads();
+  PromptWork work;
+  work.head = head, work.last = last, work.list = list;
+  const int entries = bars->entries;
+  for (int i = threadIdx.x; i < entries; i += KV_PROMPT_THREADS) {
+    const int block = a.blocks ? list[i].x : i;
+    list[i] = make_int2(block, m.page(b, block));
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const int per = m.page_shift - 4;
+  // of the last block only the pieces up to the last row
+  work.pieces = entries ? ((entries - 1) << per) + min(1 << per, ((last - (list[entries - 1].x << m.page_shift)) >> 4) + 1) : 0;
+  work.tiles = (work.pieces + 3) / 4;
+  const int tiles = work.tiles;
+  const uint32_t tmem = bars->tmem;
+  const AbortCtl abort{&bars->abort, WAIT_LIMIT_CYCLES};
 
-  // the walk over the pieces of the union: block `at`, whose page is `page`, piece `sub`; the block after it is known already
-  int at = -1, page = -1, sub = 0, after = -1, after_page = -1;
-  auto look = [&]() {  // the next block with a page
-    at = after, page = after_page, sub = 0;
-    if (after >= blocks) return;
-    ++after;
-    if (a.blocks) {
-      int w = after >> 5;
-      uint32_t x = after < blocks ? bits[w] & (~0u << (after & 31)) : 0u;
-      while (x == 0u && ++w < (blocks + 31) / 32) x = bits[w];
-      after = x ? w * 32 + __ffs(int(x)) - 1 : blocks;
-    }
-    after_page = m.page(b, after < blocks ? after : -1);
-  };
-  const int pieces = 1 << (m.page_shift - 4);
-  auto fill = [&](int stage) {
-    unsigned char* s = ring + stage * S::STAGE;
-    const uint32_t to = uint32_t(__cvta_generic_to_shared(s));
-    int* where = reinterpret_cast<int*>(s + S::STAGE - 16);
-    for (int p = 0; p < 4; ++p) {
-      while (at < blocks && (page < 0 || sub == pieces || (at << m.page_shift) + sub * 16 > last)) look();
-      const int start = at < blocks ? (at << m.page_shift) + sub * 16 : -1;
-      if (threadIdx.x == 0) where[p] = start;
-      if (start < 0) continue;
-      const size_t from = ((size_t(page) * a.heads + head) << m.page_shift) + sub * 16;
-      ++sub;
-#pragma unroll
-      for (int i = 0; i < (S::ROW + KV_PROMPT_THREADS - 1) / KV_PROMPT_THREADS; ++i) {
-        const int u = threadIdx.x + i * KV_PROMPT_THREADS, r = u / (S::ROW / 16), x = (u - r * (S::ROW / 16)) * 16, bytes = start + r <= last ? 16 : 0;
-        if (S::ROW % KV_PROMPT_THREADS && u >= S::ROW) break;
-        const uint32_t dst = to + (16 * p + r) * S::PITCH + x;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(a.kp + from * S::ROW + u * 16), "r"(bytes));
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + S::ROWS * S::PITCH), "l"(a.vp + from * S::ROW + u * 16), "r"(bytes));
+  if (warp == 5 || warp == 6) {  // keys, values
+    const bool values = warp == 6;
+    uint64_t* const full = values ? bars->v_full : bars->k_full;
+    uint64_t* const empty = values ? bars->v_empty : bars->k_empty;
+    const unsigned char* const src = values ? a.vp : a.kp;
+    unsigned char* const base = smem + (values ? S::V_AT : S::K_AT);
+    auto hand_over = [&](int i) {  // tile i has arrived
+      if constexpr (KIND == FV_KV_SAME) {
+        if (values) {  // a lane looks at what it has copied
+          unsigned char* const to = base + (i & 1) * S::STAGE;
+          uint32_t found = 0u;
+#pragma unroll 8
+          for (int x = 0; x < S::ROWS * B::UNITS / 32; ++x) {
+            const int n = lane + 32 * x, r = n / B::UNITS;
+            const uint4 v = *reinterpret_cast<const uint4*>(to + B::place(r, n - r * B::UNITS));
+            found = watch<T>(watch<T>(watch<T>(watch<T>(found, v.x), v.y), v.z), v.w);
+          }
+          const bool any = __any_sync(FV_FULL, found != 0u);
+          if (any) {
+            for (int x = 0; x < S::ROWS * B::UNITS / 32; ++x) {
+              const int n = lane + 32 * x, r = n / B::UNITS;
+              uint4* at = reinterpret_cast<uint4*>(to + B::place(r, n - r * B::UNITS));
+              uint4 v = *at;
+              v.x = finite_only<T>(v.x, found), v.y = finite_only<T>(v.y, found), v.z = finite_only<T>(v.z, found), v.w = finite_only<T>(v.w, found);
+              *at = v;
+            }
+          }
+          if (lane == 0) bars->odd[i & 1] = any;
+        }
       }
+      fence_async();
+      mbar_arrive(&full[i & 1]);
+    };
+    for (int i = 0; i < tiles; ++i) {
+      const uint32_t turn = uint32_t(i >> 1) & 1u;  // of the tile's place
+      if (i >= 2 && !__all_sync(FV_FULL, mbar_wait(&empty[i & 1], turn ^ 1u, abort, 32))) break;
+      if constexpr (KIND == FV_KV_SAME) {
+        B::start(a, m, work, i, src, smem_u32(base + (i & 1) * S::STAGE), lane);
+        if (i) {
+          asm volatile("cp.async.wait_group 1;");
+          hand_over(i - 1);
+        }
+      } else {
+        B::convert(a, m, work, i, src, base + (i & 1) * S::STAGE, lane);
+        if (values) {  // the scales of both, which the queries' threads leave together with the values
+          float* const sc = reinterpret_cast<float*>(smem + S::SCALE_AT) + (i & 1) * 2 * S::ROWS;
+          float most = 0.f;
+          for (int r = lane; r < S::ROWS; r += 32) {
+            int begin = 0;
+            size_t from = 0;
+            const bool on = work.piece(a, m, 4 * i + (r >> 4), begin, from) && begin + (r & 15) <= last;
+            const float ks = on ? __ldg(a.k_scale + from + (r & 15)) : 0.f, vs = on ? __ldg(a.v_scale + from + (r & 15)) : 0.f;
+            sc[r] = ks, sc[S::ROWS + r] = vs;
+            most = fmaxf(most, vs);  // leaves NaN out: it reaches the sums through its weight
+          }
+          const int e = int(__reduce_max_sync(FV_FULL, __float_as_uint(most)) >> 23);
+          if (lane == 0) bars->exponent[i & 1] = e;
+        }
+        hand_over(i);
+      }
+    }
+    if constexpr (KIND == FV_KV_SAME) {
+      asm volatile("cp.async.wait_all;");
+      if (tiles) hand_over(tiles - 1);
+    }
+  } else if (warp == 4) {  // products
+    constexpr uint32_t kind_bits = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10));
+    constexpr uint32_t qk = kind_bits | (uint32_t(S::ROWS >> 3) << 17) | (128u >> 4 << 24);
+    constexpr uint32_t pv = kind_bits | (1u << 16) | (uint32_t(D >> 3) << 17) | (128u >> 4 << 24);  // values: components along a row
+    auto scores = [&](int i) {  // of tile i
+      if (!__all_sync(FV_FULL, mbar_wait(&bars->k_full[i & 1], uint32_t(i >> 1) & 1u, abort, 0))) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t q = smem_u32(smem), k = smem_u32(smem + S::K_AT + (i & 1) * S::STAGE);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          const uint32_t at = (s & 3) * 32;
+          tc_mma_f16<false>(tmem + (i & 1) * 64, make_desc(desc_lo(q + (s >> 2) * S::Q_HALF + at), DESC_HI_SW128),
+                            make_desc(desc_lo(k + (s >> 2) * S::HALF + at), DESC_HI_SW128), qk, s > 0);
+        }
+        tc_commit<false>(&bars->k_empty[i & 1]);
+        tc_commit<false>(&bars->s_full[i & 1]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool on = tiles > 0 && scores(0);
+    for (int i = 0; on && i < tiles; ++i) {
+      if (i + 1 < tiles) {
+        // the place of the next scores holds the weights of the tile before this one
+        on = __all_sync(FV_FULL, i == 0 || mbar_wait(&bars->pv_done, uint32_t(i - 1) & 1u, abort, 0));
+        on = on && scores(i + 1);
+        if (!on) break;
+      }
+      on = __all_sync(FV_FULL, mbar_wait(&bars->v_full[i & 1], uint32_t(i >> 1) & 1u, abort, 0) && mbar_wait(&bars->p_full[i & 1], uint32_t(i >> 1) & 1u, abort, 0));
+      if (!on) break;
+      tc_fence_after();
+      if (elect_one()) {
+        // rows of 128 bytes along the components: 8 rows of the cache 1024 bytes apart, 64 components a HALF
+        const uint32_t v = smem_u32(smem + S::V_AT + (i & 1) * S::STAGE);
+#pragma unroll
+        for (int s = 0; s < S::ROWS / 16; ++s) {
+          const uint32_t lo = ((v + s * 2048) >> 4) | (uint32_t(S::HALF >> 4) << 16);
+          tc_mma_ts(tmem + S::O_COL, tmem + (i & 1) * 64 + s * 8, make_desc(lo, DESC_HI_SW128), pv, 1u);
+        }
+        tc_commit<false>(&bars->v_empty[i & 1]);
+        tc_commit<false>(&bars->pv_done);
+        if (i + 1 == tiles) tc_commit<false>(&bars->all_done);
+      }
+      __syncwarp();
+    }
+  } else {  // weights
+    const uint32_t lanes = uint32_t(warp * 32) << 16;
+    const int pos = pos0 + tok;
+    // the list of the thread's row: the entry that is next, and the one behind it on its way
+    const int32_t* const mylist = a.blocks && mine ? a.blocks + (size_t(row0 + tok) * a.heads + head) * a.k : nullptr;
+    int entry = -1, ahead = mylist ? __ldg(mylist) : 0, index = 0;
+    float top = -INFINITY, sum = 0.f;
+    int unit = 0;  // 8 bits: values stand for multiples of 2^(unit - 126)
+    bool on = true;
+    {
+      uint32_t zero[32];
+#pragma unroll
+      for (int z = 0; z < 32; ++z) zero[z] = 0u;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) tc_st32(tmem + lanes + S::O_COL + c, zero);
+      tc_st_wait();
+    }
+    for (int i = 0; i < tiles; ++i) {
+      int seen[4];  // rows of each piece that the query sees
+      bool any = false, whole = true;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        int start = 0;
+        size_t from;
+        const bool there = work.piece(a, m, 4 * i + p, start, from);
+        seen[p] = 0;
+        if (there && mine) {
+          bool sees = start <= pos;
+          if (a.blocks) {
+            const int block = start >> m.page_shift;
+            while (entry < block) {  // entries that are blocks, each above all before it
+              const int e = ahead;
+              ++index;
+              ahead = index < a.k ? __ldg(mylist + index) : 0;
+              if (index > a.k) entry = INT_MAX;
+              else if (e > entry && e < blocks && (e << m.page_shift) <= pos) entry = e;
+            }
+            sees = sees && entry == block;
+          }
+          if (sees) seen[p] = min(16, pos - start + 1);
+        }
+        any = any || seen[p] > 0;
+        whole = whole && (seen[p] == 0 || seen[p] == 16);
+      }
+      const uint32_t turn = uint32_t(i >> 1) & 1u;
+      on = __all_sync(FV_FULL, mbar_wait(&bars->s_full[i & 1], turn, abort, 0) && mbar_wait(&bars->v_full[i & 1], turn, abort, 0));
+      if (!on) break;
+      tc_fence_after();
+      const uint32_t place = tmem + lanes + (i & 1) * 64;
+      uint32_t p[32];
+      bool changed = false;
+      float factor = 1.f;
+      int e = unit;
       if constexpr (KIND != FV_KV_SAME) {
-        if (threadIdx.x < 32) {
-          const int r = threadIdx.x & 15, bytes = start + r <= last ? 4 : 0;
-          const float* src = (threadIdx.x < 16 ? a.k_scale : a.v_scale) + from + r;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 2 * S::ROWS * S::PITCH + ((threadIdx.x >> 4) * S::ROWS + 16 * p + r) * 4), "l"(src), "r"(bytes));
-        }
+        e = max(unit, bars->exponent[i & 1]);
+        factor = __uint_as_float(uint32_t(max(127 + unit - e, 0)) << 23);
+        changed = e != unit;
+        unit = e;
       }
-    }
-    asm volatile("cp.async.commit_group;");
-  };
-  look();  // `after` becomes the first block
-  look();
-#pragma unroll 1
-  for (int i = 0; i < S::STAGES - 1; ++i) fill(i);
-
-  // a lane has the list of one of its warp's rows: the entry that is next, and the one behind it on its way
-  const int32_t* const list = a.blocks ? a.blocks + (size_t(row + (lane < mine ? lane : 0)) * a.heads + head) * a.k : nullptr;
-  int entry = -1, ahead = a.blocks && lane < mine ? __ldg(list) : 0, index = 0;
-
-  float o[2][D / 8][4], top[2][2], l[2][2];  // tiles of 16 columns; of 8 components
-  int unit = 0;  // 8 bits: values stand for multiples of 2^(unit - 126)
+      const bool busy = __any_sync(FV_FULL, any || changed);
+      [[maybe_unused]] const bool odd = KIND == FV_KV_SAME && bars->odd[i & 1] != 0;
+      if (busy) {
+        uint32_t r[64];
+        tc_ld64_issue(place, r);
+        tc_ld64_wait(r);
+        float* s = reinterpret_cast<float*>(r);
+        [[maybe_unused]] const float* const sc = reinterpret_cast<const float*>(smem + S::SCALE_AT) + (i & 1) * 2 * S::ROWS;
+        if constexpr (KIND != FV_KV_SAME) {
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    top[x][0] = top[x][1] = -INFINITY, l[x][0] = l[x][1] = 0.f;
-#pragma unroll
-    for (int u = 0; u < D / 8; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[x][u][i] = 0.f;
-  }
-  const int r8 = lane & 7, second = lane >> 3 & 1, third = lane >> 4;  // which row of which of four 8 x 8 tiles a lane points at
-  const uint32_t q_at = uint32_t(__cvta_generic_to_shared(sq)) + (r8 + second * 8) * S::Q_PITCH + third * 16;
-
-  // 32 rows of the cache, in two pieces that begin at start[0] and start[1] and are seen by who[0] and who[1]; ALL: by every row of
-  // the warp, whole.  ODD: some of their values are not finite.
-  auto take = [&](const unsigned char* s, int pair, const int* start, const unsigned* who, auto all_of, auto odd_of) {
-    constexpr bool ALL = decltype(all_of)::value, ODD = decltype(odd_of)::value;
-    const uint32_t keys = uint32_t(__cvta_generic_to_shared(s)) + 32 * pair * S::PITCH, values = keys + S::ROWS * S::PITCH;
-    [[maybe_unused]] const float* const scales = reinterpret_cast<const float*>(s + 2 * S::ROWS * S::PITCH) + 32 * pair;
-    float sc[2][4][4] = {};  // tiles of columns; of 8 rows of the cache
-    if constexpr (KIND == FV_KV_SAME) {
-      const uint32_t k_at = keys + (r8 + third * 8) * S::PITCH + second * 16;
-#pragma unroll
-      for (int st = 0; st < D / 16; ++st) {
-        uint32_t q[2][4], k[2][4];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) ldmatrix(q[x], q_at + x * 16 * S::Q_PITCH + st * 32), ldmatrix(k[x], k_at + x * 16 * S::PITCH + st * 32);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) mma_16<M>(sc[x][j], q[x][0], q[x][1], q[x][2], q[x][3], k[j >> 1][(j & 1) * 2], k[j >> 1][(j & 1) * 2 + 1]);
-      }
-    } else {
-      const uint32_t k_at = keys + (r8 + second * 8) * S::PITCH + third * 16;
-#pragma unroll
-      for (int st = 0; st < D / 32; ++st) {
-        uint32_t c[2][4];  // 16 rows each: rows 0-7 and 8-15 of 16 components, then of the next 16
-#pragma unroll
-        for (int h = 0; h < 2; ++h) ldmatrix(c[h], k_at + h * 16 * S::PITCH + st * 32);
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          uint32_t q[2][4], k[4][2];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) ldmatrix(q[x], q_at + x * 16 * S::Q_PITCH + (2 * st + z) * 32);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) codes_to_half<KIND>(c[j >> 1][2 * z + (j & 1)], k[j][0], k[j][1]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) mma_16<M>(sc[x][j], q[x][0], q[x][1], q[x][2], q[x][3], k[j][0], k[j][1]);
-        }
-      }
-    }
-    [[maybe_unused]] float vs[4][2];  // of a lane's rows of the cache: 8 j + 2 t + i
-    float grown = 1.f;
-    if constexpr (KIND != FV_KV_SAME) {
-      float most = 0.f;  // leaves NaN out: it reaches the sums through its weight
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 ks = *reinterpret_cast<const float2*>(scales + 8 * j + 2 * t);
-        float2 v = *reinterpret_cast<const float2*>(scales + S::ROWS + 8 * j + 2 * t);
-        if (!ALL && start[j >> 1] < 0) v = make_float2(0.f, 0.f);
-        most = fmaxf(most, fmaxf(v.x, v.y));
-        vs[j][0] = v.x, vs[j][1] = v.y;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) sc[x][j][0] *= ks.x, sc[x][j][1] *= ks.y, sc[x][j][2] *= ks.x, sc[x][j][3] *= ks.y;
-      }
-      const int e = max(unit, int(__reduce_max_sync(FV_FULL, __float_as_uint(most)) >> 23));
-      grown = __uint_as_float(uint32_t(max(127 + unit - e, 0)) << 23);
-      unit = e;
-      const float down = __uint_as_float(uint32_t(max(253 - e, 1)) << 23);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) vs[j][0] *= down, vs[j][1] *= down;
-    }
-    bool moved = grown != 1.f;
-    float to[2][2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float y = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool seen = ALL || (who[j >> 1] >> row_of[x][i] & 1u);
-          const int ahead = pos + row_of[x][i] - start[j >> 1] - 8 * (j & 1) - 2 * t;  // rows of the cache up to the column's own
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            float& v = sc[x][j][2 * i + z];
-            v *= by[x][i];
-            if (!ALL && !(seen && z <= ahead)) v = -INFINITY;
-            y = fmaxf(y, v);
+          for (int j = 0; j < 64; j += 4) {
+            const float4 ks = *reinterpret_cast<const float4*>(sc + j);
+            s[j] *= ks.x, s[j + 1] *= ks.y, s[j + 2] *= ks.z, s[j + 3] *= ks.w;
           }
         }
-        to[x][i] = y;
-        moved = moved || y > top[x][i] + GROWN;  // -inf + GROWN is -inf
-      }
-    if (__any_sync(FV_FULL, moved)) {
+        if (__all_sync(FV_FULL, whole)) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+          for (int j = 0; j < 64; ++j) s[j] = seen[j >> 4] ? s[j] : -INFINITY;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float y = fmaxf(top[x][i], to[x][i]);
-          y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 1));
-          y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 2));
-          const float by_l = y > top[x][i] ? exp2_of(top[x][i] - y) : 1.f, by_o = by_l * grown;
-          top[x][i] = y;
-          l[x][i] *= by_l;
-#pragma unroll
-          for (int u = 0; u < D / 8; ++u) o[x][u][2 * i] *= by_o, o[x][u][2 * i + 1] *= by_o;
+          for (int j = 0; j < 64; ++j) s[j] = (j & 15) < seen[j >> 4] ? s[j] : -INFINITY;
         }
-    }
-    // weights, rounded to 16 bits: tiles of 16 columns by 16 rows of the cache
-    uint32_t p[2][2][4];
+        float y[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float off = top[x][i] == -INFINITY ? 0.f : ONE - top[x][i];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float y[2];
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            y[z] = exp2_of(sc[x][j][2 * i + z] + off);
-            l[x][i] += y[z];
-            if constexpr (KIND != FV_KV_SAME) y[z] = y[z] != 0.f ? y[z] * vs[j][z] : 0.f;
-            if constexpr (ODD) sc[x][j][2 * i + z] = y[z];
-          }
-          p[x][j >> 1][i + 2 * (j & 1)] = Pair<M>::from_float(y[0], y[1]);
-        }
-      }
-    if constexpr (KIND == FV_KV_SAME) {
-      const uint32_t v_at = values + (r8 + second * 8) * S::PITCH + third * 16;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (!ALL && start[h] < 0) continue;  // its place holds anything
-#pragma unroll
-        for (int u = 0; u < D / 8; u += 2) {
-          uint32_t v[4];
-          ldmatrix_t(v, v_at + h * 16 * S::PITCH + u * 16);
-          if constexpr (ODD) {
-#pragma unroll
-            for (int z = 0; z < 4; ++z) v[z] = finite_only<T>(v[z]);
-          }
-#pragma unroll
-          for (int z = 0; z < 2; ++z)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) mma_16<M>(o[x][u + z], p[x][h][0], p[x][h][1], p[x][h][2], p[x][h][3], v[2 * z], v[2 * z + 1]);
-        }
-        if constexpr (ODD) {  // what was left out, to the columns that have a weight for it
-#pragma unroll 1
-          for (int j = 0; j < 16; ++j) {
-            const T* vr = reinterpret_cast<const T*>(s + (S::ROWS + 32 * pair + 16 * h + j) * S::PITCH);
-            float w[2][2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                float y = 0.f;  // tile j / 8 of the piece, lane j / 2 % 4, number j % 2
-#pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                  const float here = __shfl_sync(FV_FULL, sc[x][2 * h + (z >> 1)][2 * i + (z & 1)], (lane & ~3) + (j >> 1 & 3));
-                  if ((j >> 3) == (z >> 1) && (j & 1) == (z & 1)) y = here;
-                }
-                w[x][i] = y;
-              }
-#pragma unroll
-            for (int u = 0; u < D / 8; ++u)
-#pragma unroll
-              for (int z = 0; z < 2; ++z) {
-                const float v = float(vr[8 * u + 2 * t + z]);
-                if (kv_finite(v)) continue;
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                  for (int i = 0; i < 2; ++i)
-                    if (w[x][i] != 0.f) o[x][u][2 * i + z] += w[x][i] * v;
-              }
+        for (int j = 4; j < 64; ++j) y[j & 3] = fmaxf(y[j & 3], s[j]);
+        const float to = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * by;
+        if (to > top + GROWN || top == -INFINITY) {
+          if (to > top) {
+            const float f = exp2_of(top - to);
+            factor *= f, sum *= f;
+            changed = changed || top != -INFINITY;  // without weights so far the query's O is 0
+            top = to;
           }
         }
-      }
-    } else {
-      const uint32_t v_at = values + (r8 + second * 8) * S::PITCH + third * 16;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (!ALL && start[h] < 0) continue;
-#pragma unroll
-        for (int u = 0; u < D / 8; u += 4) {
-          uint32_t c[4];  // rows 0-7 and 8-15 of 16 components, then of the next 16
-          ldmatrix_t(c, v_at + h * 16 * S::PITCH + u * 8);
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            uint32_t v[2][2];  // the even and the odd components of 16, of two neighbouring rows each
-#pragma unroll
-            for (int i = 0; i < 2; ++i) codes_to_half<KIND>(__byte_perm(c[2 * z + i], 0, 0x3120), v[0][i], v[1][i]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int x = 0; x < 2; ++x) mma_16<M>(o[x][u + 2 * z + i], p[x][h][0], p[x][h][1], p[x][h][2], p[x][h][3], v[i][0], v[i][1]);
-          }
-        }
-      }
-    }
-  };
-
-#pragma unroll 1
-  for (int stage = 0;; stage = stage + 1 == S::STAGES ? 0 : stage + 1) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2));
-    unsigned char* const s = ring + stage * S::STAGE;
-    int odd = 0;
-    if constexpr (KIND == FV_KV_SAME) {  // each thread looks at what it has copied
-      uint32_t found = 0u;
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-#pragma unroll
-        for (int i = 0; i < (S::ROW + KV_PROMPT_THREADS - 1) / KV_PROMPT_THREADS; ++i) {
-          const int u = threadIdx.x + i * KV_PROMPT_THREADS, r = u / (S::ROW / 16), x = (u - r * (S::ROW / 16)) * 16;
-          if (S::ROW % KV_PROMPT_THREADS && u >= S::ROW) break;
-          const uint4 v = *reinterpret_cast<const uint4*>(s + (S::ROWS + 16 * p + r) * S::PITCH + x);
-          found = watch<T>(watch<T>(watch<T>(watch<T>(found, v.x), v.y), v.z), v.w);
-        }
-      odd = __syncthreads_or(found != 0u);  // 0 * w is 0 or -0, and 0 + -0 is 0
-    } else {
-      __syncthreads();
-    }
-    const int* const where = reinterpret_cast<const int*>(s + S::STAGE - 16);
-    if (where[0] < 0) break;  // the union is done
-    fill(stage == 0 ? S::STAGES - 1 : stage - 1);  // the stage that everybody has left
-#pragma unroll 1
-    for (int pair = 0; pair < 2; ++pair) {
-      int start[2];
-      unsigned who[2];  // the warp's rows that see the piece
-      bool all = true;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        start[h] = where[2 * pair + h];
-        bool sees = lane < mine && start[h] >= 0 && start[h] <= pos + lane;
-        if (a.blocks) {
-          const int block = start[h] >= 0 ? start[h] >> m.page_shift : -1;
-          while (lane < mine && entry < block) {  // entries that are blocks, each above all before it; blocks: none is left
-            const int e = ahead;
-            ++index;
-            ahead = index < a.k ? __ldg(list + index) : 0;
-            if (index > a.k) entry = INT_MAX;
-            else if (e > entry && e < blocks && (e << m.page_shift) <= pos + lane) entry = e;
-          }
-          sees = sees && entry == block;
-        }
-        who[h] = __ballot_sync(FV_FULL, sees);
-        all = all && who[h] == everyone && start[h] + 15 <= pos;
-      }
-      if ((who[0] | who[1]) == 0u) continue;
-      using Yes = std::true_type;
-      using No = std::false_type;
-      if (KIND == FV_KV_SAME && odd) take(s, pair, start, who, No(), std::integral_constant<bool, KIND == FV_KV_SAME>());
-      else if (all) take(s, pair, start, who, Yes(), No());
-      else take(s, pair, start, who, No(), No());
-    }
-  }
-  asm volatile("cp.async.wait_all;");
-
-  // results: through the place of the warp's own queries, to be written in whole rows
-  const float f = KIND != FV_KV_SAME ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
-  __syncwarp();
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float y = l[x][i];
-      y += __shfl_xor_sync(FV_FULL, y, 1);
-      y += __shfl_xor_sync(FV_FULL, y, 2);
-      const int c = 16 * x + 8 * i + g, tok = c / per;
-      const float down = y == 0.f ? 0.f : f / y;
-      uint32_t* to = reinterpret_cast<uint32_t*>(sq + c * S::Q_PITCH);
-#pragma unroll
-      for (int u = 0; u < D / 8; u += 2) {
-        float v[4] = {o[x][u][2 * i], o[x][u][2 * i + 1], o[x][u + 1][2 * i], o[x][u + 1][2 * i + 1]};
-#pragma unroll
-        for (int z = 0; z < 4; ++z) v[z] = y == 0.f ? 0.f : v[z] * down;
+        const float off = top == -INFINITY ? 0.f : ONE - top;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
         if constexpr (KIND == FV_KV_SAME) {
-          to[4 * u + t] = Pair<T>::from_float(v[0], v[1]), to[4 * u + 4 + t] = Pair<T>::from_float(v[2], v[3]);
-        } else {  // components 4 t, 4 t + 2, 4 t + 1, 4 t + 3 of 16
-          *reinterpret_cast<uint2*>(to + 4 * u + 2 * t) = make_uint2(Pair<T>::from_float(v[0], v[2]), Pair<T>::from_float(v[1], v[3]));
+#pragma unroll
+          for (int j = 0; j < 64; ++j) s[j] = exp2_of(__fmaf_rn(s[j], by, off)), part[j & 3] += s[j];
+        } else {
+          const float down = __uint_as_float(uint32_t(max(253 - e, 1)) << 23);
+#pragma unroll
+          for (int j = 0; j < 64; j += 4) {
+            const float4 vs = *reinterpret_cast<const float4*>(sc + S::ROWS + j);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const float w = exp2_of(__fmaf_rn(s[j + z], by, off));
+              part[z] += w;
+              s[j + z] = w != 0.f ? w * ((&vs.x)[z] * down) : 0.f;
+            }
+          }
         }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) p[j] = Pair<M>::from_float(s[2 * j], s[2 * j + 1]);
+        // O, scaled to the new maximum, and values that were taken out of the product
+        const bool scale_o = __any_sync(FV_FULL, changed);
+        if (KIND == FV_KV_SAME && odd) {
+          on = __all_sync(FV_FULL, i == 0 || mbar_wait(&bars->pv_done, uint32_t(i - 1) & 1u, abort, 0));
+          if (!on) break;
+          tc_fence_after();
+          float w[64];  // where a loop can index them
+#pragma unroll
+          for (int j = 0; j < 64; ++j) w[j] = s[j];
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tc_ld32_issue(tmem + lanes + S::O_COL + c, o);
+            tc_ld_wait(o);
+#pragma unroll
+            for (int z = 0; z < 32; ++z) o[z] = __float_as_uint(__uint_as_float(o[z]) * factor);
+#pragma unroll 1
+            for (int j = 0; j < 64; ++j) {
+              const float weight = w[j];
+              int start = 0;
+              size_t from = 0;
+              if (weight == 0.f || !work.piece(a, m, 4 * i + (j >> 4), start, from)) continue;
+              const unsigned char* row = a.vp + ((from + (j & 15)) * D + c) * 2;
+#pragma unroll
+              for (int z = 0; z < 32; z += 2) {
+                const float2 v = Pair<T>::to_float(__ldg(reinterpret_cast<const uint32_t*>(row) + z / 2));
+                if (!kv_finite(v.x)) o[z] = __float_as_uint(__uint_as_float(o[z]) + weight * v.x);
+                if (!kv_finite(v.y)) o[z + 1] = __float_as_uint(__uint_as_float(o[z + 1]) + weight * v.y);
+              }
+            }
+            tc_st32(tmem + lanes + S::O_COL + c, o);
+          }
+          tc_st_wait();
+        } else if (scale_o) {
+          on = __all_sync(FV_FULL, i == 0 || mbar_wait(&bars->pv_done, uint32_t(i - 1) & 1u, abort, 0));
+          if (!on) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tc_ld32_issue(tmem + lanes + S::O_COL + c, o);
+            tc_ld_wait(o);
+#pragma unroll
+            for (int z = 0; z < 32; ++z) o[z] = __float_as_uint(__uint_as_float(o[z]) * factor);
+            tc_st32(tmem + lanes + S::O_COL + c, o);
+          }
+          tc_st_wait();
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) p[j] = 0u;
       }
-      if (a.lse && t == 0 && c < cols && tok < mine)
-        a.lse[size_t(row + tok) * a.heads * a.group + size_t(head) * a.group + first + c - tok * per] =
-            y == 0.f ? -INFINITY : (top[x][i] - ONE + log2f(y)) * 0.693147180559945309f;
+      tc_st32(place, p);
+      tc_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bars->p_full[i & 1]);
     }
-  __syncwarp();
-  for (int i = lane; i < COLS * (D / 8); i += 32) {
-    const int c = i / (D / 8), x = i - c * (D / 8), tok = c / per;
-    if (c < cols && tok < mine)
-      *reinterpret_cast<uint4*>(a.out + ((size_t(row + tok) * a.heads * a.group + size_t(head) * a.group + first + c - tok * per) * D + x * 8) * 2) =
-          *reinterpret_cast<const uint4*>(sq + c * S::Q_PITCH + x * 16);
+    // (pv_done may lie one or two phases behind here, which its parity does not tell apart)
+    if (on && tiles) on = __all_sync(FV_FULL, mbar_wait(&bars->all_done, 0u, abort, 0));
+    tc_fence_after();
+    const float f = KIND != FV_KV_SAME ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
+    const float down = sum == 0.f ? 0.f : f / sum;
+    const size_t query = (size_t(row0 + tok) * a.heads + head) * a.group + h;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      uint32_t o[32];
+      tc_ld32_issue(tmem + lanes + S::O_COL + c, o);
+      tc_ld_wait(o);
+      uint4 w[4];
+#pragma unroll
+      for (int z = 0; z < 16; ++z) {
+        const float u = __uint_as_float(o[2 * z]) * down, v = __uint_as_float(o[2 * z + 1]) * down;
+        // a wait that ran out leaves no result: NaN
+        reinterpret_cast<uint32_t*>(w)[z] = !on ? 0x7FFF7FFFu : sum == 0.f ? 0u : Pair<T>::from_float(u, v);
+      }
+      if (mine) {
+#pragma unroll
+        for (int z = 0; z < 4; ++z) *reinterpret_cast<uint4*>(a.out + (query * D + c + 8 * z) * 2) = w[z];
+      }
+    }
+    if (mine && a.lse) a.lse[query] = sum == 0.f ? -INFINITY : (top - ONE + log2f(sum)) * 0.693147180559945309f;
   }
+  if (warp == 5 || warp == 6) asm volatile("cp.async.wait_all;");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+}
+
+size_t prompt_entries(const fv_kv_batch* b, int group, bool lists, size_t k) {
+  const size_t most = size_t(KV_PROMPT_COLS / group) * k;
+  return lists && most < b->table_width ? most : b->table_width;
 }
 
 template <class T, int KIND, int D>
 int prompt_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a) {
   using S = Tile<KIND, D>;
-  const int tiles = (a.group + KV_PROMPT_COLS - 1) / KV_PROMPT_COLS, tc = KV_PROMPT_WARPS * (a.group <= KV_PROMPT_COLS ? KV_PROMPT_COLS / a.group : 1);
-  const size_t items = b->cu ? b->rows / tc + b->nseq : b->nseq, smem = S::SMEM + (b->table_width + 31) / 32 * 4;
-  if (size_t(kv->heads) * tiles > 65535) return fail(FV_ERR_UNSUPPORTED, "fv_kv_attend_dev: more than 65535 tiles of query heads");
+  const int tc = KV_PROMPT_COLS / a.group;
+  const size_t items = b->cu ? b->rows / tc + b->nseq : b->nseq;
+  const size_t smem = S::LIST_AT + 8 * prompt_entries(b, a.group, a.blocks != nullptr, a.k);
   FV_TRY((kv_allow_smem<kv_prompt_kernel<T, KIND, D>>(kv->device, smem)));
-  kv_prompt_kernel<T, KIND, D><<<dim3(unsigned(items), unsigned(kv->heads * tiles)), KV_PROMPT_THREADS, smem, s>>>(a, kv_batch(kv, b), tiles);
+  kv_prompt_kernel<T, KIND, D><<<dim3(unsigned(items), kv->heads), KV_PROMPT_THREADS, smem, s>>>(a, kv_batch(kv, b));
   FV_CUDA(cudaGetLastError());
   return FV_OK;
 }
 
 }  // namespace
+
+// Entries of the union that fit beside the largest tiles.
+bool kv_prompt_fits(const fv_kv_batch* b, size_t group, bool lists, size_t k) {
+  return prompt_entries(b, int(group), lists, k) <= (226 * 1024 - size_t(Tile<FV_KV_INT8, 128>::LIST_AT)) / 8 && b->table_width <= (1u << 18);
+}
 
 int kv_prompt_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a) { FV_KV_DISPATCH(kv, prompt_of, kv, s, b, a); }
 
