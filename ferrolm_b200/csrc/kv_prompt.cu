@@ -6,7 +6,7 @@
 //   S = Q K^T (128 x 64) and O += P V (128 x dim): tcgen05.mma from shared memory into tensor memory, P read from there
 //   P = 2^(scale S - max): a thread to a query, which has a whole row of S in its registers: no exchange between lanes
 //
-// Warps 0-3 turn S into P, warp 4 issues the products, warp 5 brings keys and warp 6 values, each two tiles ahead at most; S has
+// Warps 0-3 turn S into P, warp 4 issues the products, two warps bring keys and four values, each two tiles ahead at most; S has
 // two places, so that the next one is worked out while this one becomes P.  P takes the place of its S.  Two CTAs share an SM, and
 // the other one's products and copies fill the time in which the first one's threads compute powers of two: 16 an SM and clock,
 // so 512 clocks for a tile whose products take about 250.  That, and the share of a tile that its rows do not have in
@@ -26,12 +26,16 @@ namespace fv {
 
 namespace {
 
-enum { KV_PROMPT_COLS = 128, KV_PROMPT_WARPS = 7, KV_PROMPT_THREADS = 32 * KV_PROMPT_WARPS };
+// warps 0-3: weights; 4: products; 6-7: keys; 8-11: values
+enum { KV_PROMPT_COLS = 128, KV_PROMPT_THREADS = 384, KV_PROMPT_KEYS = 64, KV_PROMPT_VALUES = 128 };
+// Registers: two CTAs share an SM, so a thread starts with 80; the threads of the weights take over what the others give up.
+enum { KV_PROMPT_REGS = 80, KV_PROMPT_REGS_MORE = 128, KV_PROMPT_REGS_LESS = 56 };
+static_assert(KV_PROMPT_REGS_MORE + 2 * KV_PROMPT_REGS_LESS <= 3 * KV_PROMPT_REGS, "more than a CTA starts with would never come");
 
 struct PromptBars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done, all_done;
   uint32_t tmem;
-  int abort, odd[2], exponent[2], entries;
+  int abort, odd[2][4], exponent[2], entries;
 };
 
 template <int KIND, int D>
@@ -73,13 +77,11 @@ __device__ __forceinline__ void tc_st32(uint32_t to, const uint32_t* r) {
 }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// zeros in the halves that are not finite, and whether there are any
+// zeros in the halves that are not finite
 template <class T>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w, uint32_t& found) {
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
   constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
-  const uint32_t bad = __vcmpeq2(w & e, e);
-  found |= bad;
-  return w & ~bad;
+  return w & ~__vcmpeq2(w & e, e);
 }
 // x + 0 * w in both halves: NaN from the first that is not finite on
 template <class T>
@@ -105,61 +107,130 @@ struct PromptWork {
   }
 };
 
-// One warp brings tile i of the keys (or values) to `to`: rows of 128 bytes, 16-byte pieces exchanged by the row's number as the
+// N threads bring tile i of the keys (or values) to `to`: rows of 128 bytes, 16-byte pieces exchanged by the row's number as the
 // tensor cores read them, zeros for rows that are none.  Piece u of a row of 16 bytes in 16 bits, of 8 codes in 8.
-template <class T, int KIND, int D>
+template <class T, int KIND, int D, int N>
 struct Bring {
   using S = Tile<KIND, D>;
-  static constexpr int UNITS = D / 8;  // 16-byte pieces of a row as it is brought
+  static constexpr int UNITS = D / 8, PIECE = 16 * UNITS, TIMES = (PIECE + N - 1) / N;  // 16-byte pieces of a row, and of 16 rows
   static __device__ __forceinline__ uint32_t place(int r, int u) { return (u >> 3) * S::HALF + r * 128 + (((u & 7) ^ (r & 7)) << 4); }
+  // f(piece of 16 rows, its x-th time, row of the tile, piece of the row, number in the piece), for what thread t has of the tile
+  template <class F>
+  static __device__ __forceinline__ void each(int t, F&& f) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+      for (int x = 0; x < TIMES; ++x) {
+        const int n = t + N * x, r = n / UNITS;
+        if (PIECE % N && n >= PIECE) continue;
+        f(p, x, 16 * p + r, n - r * UNITS, n);
+      }
+  }
 
-  static __device__ __forceinline__ void start(const KvAttend& a, const KvBatch& m, const PromptWork& w, int i, const unsigned char* src, uint32_t to, int lane) {
-    static_assert(KIND == FV_KV_SAME, "");
+  static __device__ __forceinline__ void start(const KvAttend& a, const KvBatch& m, const PromptWork& w, int i, const unsigned char* src, uint32_t to, int t) {
+    const unsigned char* from[4];
+    int seen[4];  // rows of the piece that somebody sees
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       int begin = 0;
-      size_t from = 0;
-      const bool on = w.piece(a, m, 4 * i + p, begin, from);
-#pragma unroll
-      for (int x = 0; x < 16 * UNITS / 32; ++x) {
-        const int n = lane + 32 * x, r = n / UNITS, u = n - r * UNITS;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + place(16 * p + r, u)), "l"(src + (on ? from * (2 * D) + n * 16 : 0)),
-                     "r"(on && begin + r <= w.last ? 16 : 0));
-      }
+      size_t at = 0;
+      seen[p] = w.piece(a, m, 4 * i + p, begin, at) ? w.last - begin + 1 : 0;
+      from[p] = src + (seen[p] ? at * (2 * D) : 0);
     }
+    each(t, [&](int p, int, int r, int u, int n) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + place(r, u)), "l"(from[p] + n * 16), "r"((r & 15) < seen[p] ? 16 : 0));
+    });
     asm volatile("cp.async.commit_group;");
   }
   // 8 bits: through registers, where the codes become fp16
-  static __device__ __forceinline__ void convert(const KvAttend& a, const KvBatch& m, const PromptWork& w, int i, const unsigned char* src, unsigned char* to, int lane) {
+  static __device__ __forceinline__ void convert(const KvAttend& a, const KvBatch& m, const PromptWork& w, int i, const unsigned char* src, unsigned char* to, int t) {
+    uint2 c[4][TIMES];
+    const unsigned char* from[4];
+    int seen[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       int begin = 0;
-      size_t from = 0;
-      const bool on = w.piece(a, m, 4 * i + p, begin, from);
-      uint2 c[16 * UNITS / 32];
-#pragma unroll
-      for (int x = 0; x < 16 * UNITS / 32; ++x) {
-        const int n = lane + 32 * x, r = n / UNITS;
-        c[x] = make_uint2(0, 0);
-        if (on && begin + r <= w.last) c[x] = __ldg(reinterpret_cast<const uint2*>(src + from * D + n * 8));
-      }
-#pragma unroll
-      for (int x = 0; x < 16 * UNITS / 32; ++x) {
-        const int n = lane + 32 * x, r = n / UNITS, u = n - r * UNITS;
-        uint4 y;
-        codes_to_half<KIND>(c[x].x, y.x, y.y);
-        codes_to_half<KIND>(c[x].y, y.z, y.w);
-        *reinterpret_cast<uint4*>(to + place(16 * p + r, u)) = y;
-      }
+      size_t at = 0;
+      seen[p] = w.piece(a, m, 4 * i + p, begin, at) ? w.last - begin + 1 : 0;
+      from[p] = src + (seen[p] ? at * D : 0);
     }
+    each(t, [&](int p, int x, int r, int, int n) {
+      c[p][x] = (r & 15) < seen[p] ? __ldg(reinterpret_cast<const uint2*>(from[p] + n * 8)) : make_uint2(0, 0);
+    });
+    each(t, [&](int p, int x, int r, int u, int) {
+      uint4 y;
+      codes_to_half<KIND>(c[p][x].x, y.x, y.y);
+      codes_to_half<KIND>(c[p][x].y, y.z, y.w);
+      *reinterpret_cast<uint4*>(to + place(r, u)) = y;
+    });
   }
 };
+
+// What brings keys (VALUES: values) to their two places, tile by tile.
+template <class T, int KIND, int D, bool VALUES>
+__device__ __forceinline__ void bring_all(const KvAttend& a, const KvBatch& m, const PromptWork& work, unsigned char* smem, PromptBars* bars, const AbortCtl& abort, int t) {
+  using S = Tile<KIND, D>;
+  using B = Bring<T, KIND, D, VALUES ? KV_PROMPT_VALUES : KV_PROMPT_KEYS>;
+  const int lane = t & 31;
+  uint64_t* const full = VALUES ? bars->v_full : bars->k_full;
+  uint64_t* const empty = VALUES ? bars->v_empty : bars->k_empty;
+  const unsigned char* const src = VALUES ? a.vp : a.kp;
+  unsigned char* const base = smem + (VALUES ? S::V_AT : S::K_AT);
+  for (int i = 0; i < work.tiles; ++i) {
+    const uint32_t turn = uint32_t(i >> 1) & 1u;  // of the tile's place
+    unsigned char* const to = base + (i & 1) * S::STAGE;
+    if (i >= 2 && !__all_sync(FV_FULL, mbar_wait(&empty[i & 1], turn ^ 1u, abort, 32))) break;
+    if constexpr (KIND == FV_KV_SAME) {
+      B::start(a, m, work, i, src, smem_u32(to), t);
+      asm volatile("cp.async.wait_all;");
+      if constexpr (VALUES) {  // a thread looks at what it has copied
+        uint32_t found = 0u;
+        B::each(t, [&](int, int, int r, int u, int) {
+          const uint4 v = *reinterpret_cast<const uint4*>(to + B::place(r, u));
+          found = watch<T>(watch<T>(watch<T>(watch<T>(found, v.x), v.y), v.z), v.w);
+        });
+        const bool any = __any_sync(FV_FULL, found != 0u);
+        if (any) {
+#pragma unroll 1
+          for (int p = 0; p < 4; ++p)
+            for (int n = t; n < B::PIECE; n += KV_PROMPT_VALUES) {
+              const int r = n / B::UNITS;
+              uint4* at = reinterpret_cast<uint4*>(to + B::place(16 * p + r, n - r * B::UNITS));
+              uint4 v = *at;
+              v.x = finite_only<T>(v.x), v.y = finite_only<T>(v.y), v.z = finite_only<T>(v.z), v.w = finite_only<T>(v.w);
+              *at = v;
+            }
+        }
+        if (lane == 0) bars->odd[i & 1][t >> 5] = any;
+      }
+    } else {
+      B::convert(a, m, work, i, src, to, t);
+      if (VALUES && t < 32) {  // the scales of both, which the queries' threads leave together with the values
+        float* const sc = reinterpret_cast<float*>(smem + S::SCALE_AT) + (i & 1) * 2 * S::ROWS;
+        float most = 0.f;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const int r = lane + 32 * z;
+          int begin = 0;
+          size_t from = 0;
+          const bool on = work.piece(a, m, 4 * i + (r >> 4), begin, from) && begin + (r & 15) <= work.last;
+          const float ks = on ? __ldg(a.k_scale + from + (r & 15)) : 0.f, vs = on ? __ldg(a.v_scale + from + (r & 15)) : 0.f;
+          sc[r] = ks, sc[S::ROWS + r] = vs;
+          most = fmaxf(most, vs);  // leaves NaN out: it reaches the sums through its weight
+        }
+        const int e = int(__reduce_max_sync(FV_FULL, __float_as_uint(most)) >> 23);
+        if (lane == 0) bars->exponent[i & 1] = e;
+      }
+    }
+    fence_async();
+    mbar_arrive(&full[i & 1]);
+  }
+}
 
 template <class T, int KIND, int D>
 __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAttend a, KvBatch m) {
   using S = Tile<KIND, D>;
   using M = typename std::conditional<KIND == FV_KV_SAME, T, __half>::type;
-  using B = Bring<T, KIND, D>;
   constexpr bool HALF = std::is_same<M, __half>::value;
   constexpr float ONE = HALF ? 14.f : 0.f;   // log2 of what stands for a weight of 1
   constexpr float GROWN = HALF ? 1.f : 8.f;  // log2 of what a maximum may lag behind by
@@ -184,9 +255,8 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->k_full[i], 32), mbar_init(&bars->k_empty[i], 1), mbar_init(&bars->v_full[i], 32), mbar_init(&bars->v_empty[i], 1);
+      mbar_init(&bars->k_full[i], KV_PROMPT_KEYS), mbar_init(&bars->k_empty[i], 1), mbar_init(&bars->v_full[i], KV_PROMPT_VALUES), mbar_init(&bars->v_empty[i], 1);
       mbar_init(&bars->s_full[i], 1), mbar_init(&bars->p_full[i], KV_PROMPT_COLS);
-      bars->odd[i] = 0;
     }
     mbar_init(&bars->pv_done, 1), mbar_init(&bars->all_done, 1);
     bars->abort = 0;
@@ -276,72 +346,13 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
   const uint32_t tmem = bars->tmem;
   const AbortCtl abort{&bars->abort, WAIT_LIMIT_CYCLES};
 
-  if (warp == 5 || warp == 6) {  // keys, values
-    const bool values = warp == 6;
-    uint64_t* const full = values ? bars->v_full : bars->k_full;
-    uint64_t* const empty = values ? bars->v_empty : bars->k_empty;
-    const unsigned char* const src = values ? a.vp : a.kp;
-    unsigned char* const base = smem + (values ? S::V_AT : S::K_AT);
-    auto hand_over = [&](int i) {  // tile i has arrived
-      if constexpr (KIND == FV_KV_SAME) {
-        if (values) {  // a lane looks at what it has copied
-          unsigned char* const to = base + (i & 1) * S::STAGE;
-          uint32_t found = 0u;
-#pragma unroll 8
-          for (int x = 0; x < S::ROWS * B::UNITS / 32; ++x) {
-            const int n = lane + 32 * x, r = n / B::UNITS;
-            const uint4 v = *reinterpret_cast<const uint4*>(to + B::place(r, n - r * B::UNITS));
-            found = watch<T>(watch<T>(watch<T>(watch<T>(found, v.x), v.y), v.z), v.w);
-          }
-          const bool any = __any_sync(FV_FULL, found != 0u);
-          if (any) {
-            for (int x = 0; x < S::ROWS * B::UNITS / 32; ++x) {
-              const int n = lane + 32 * x, r = n / B::UNITS;
-              uint4* at = reinterpret_cast<uint4*>(to + B::place(r, n - r * B::UNITS));
-              uint4 v = *at;
-              v.x = finite_only<T>(v.x, found), v.y = finite_only<T>(v.y, found), v.z = finite_only<T>(v.z, found), v.w = finite_only<T>(v.w, found);
-              *at = v;
-            }
-          }
-          if (lane == 0) bars->odd[i & 1] = any;
-        }
-      }
-      fence_async();
-      mbar_arrive(&full[i & 1]);
-    };
-    for (int i = 0; i < tiles; ++i) {
-      const uint32_t turn = uint32_t(i >> 1) & 1u;  // of the tile's place
-      if (i >= 2 && !__all_sync(FV_FULL, mbar_wait(&empty[i & 1], turn ^ 1u, abort, 32))) break;
-      if constexpr (KIND == FV_KV_SAME) {
-        B::start(a, m, work, i, src, smem_u32(base + (i & 1) * S::STAGE), lane);
-        if (i) {
-          asm volatile("cp.async.wait_group 1;");
-          hand_over(i - 1);
-        }
-      } else {
-        B::convert(a, m, work, i, src, base + (i & 1) * S::STAGE, lane);
-        if (values) {  // the scales of both, which the queries' threads leave together with the values
-          float* const sc = reinterpret_cast<float*>(smem + S::SCALE_AT) + (i & 1) * 2 * S::ROWS;
-          float most = 0.f;
-          for (int r = lane; r < S::ROWS; r += 32) {
-            int begin = 0;
-            size_t from = 0;
-            const bool on = work.piece(a, m, 4 * i + (r >> 4), begin, from) && begin + (r & 15) <= last;
-            const float ks = on ? __ldg(a.k_scale + from + (r & 15)) : 0.f, vs = on ? __ldg(a.v_scale + from + (r & 15)) : 0.f;
-            sc[r] = ks, sc[S::ROWS + r] = vs;
-            most = fmaxf(most, vs);  // leaves NaN out: it reaches the sums through its weight
-          }
-          const int e = int(__reduce_max_sync(FV_FULL, __float_as_uint(most)) >> 23);
-          if (lane == 0) bars->exponent[i & 1] = e;
-        }
-        hand_over(i);
-      }
-    }
-    if constexpr (KIND == FV_KV_SAME) {
-      asm volatile("cp.async.wait_all;");
-      if (tiles) hand_over(tiles - 1);
-    }
-  } else if (warp == 4) {  // products
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(int(KV_PROMPT_REGS_LESS)));
+    bring_all<T, KIND, D, true>(a, m, work, smem, bars, abort, threadIdx.x - 256);
+  } else if (warp >= 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(int(KV_PROMPT_REGS_LESS)));
+    if (warp >= 6) bring_all<T, KIND, D, false>(a, m, work, smem, bars, abort, threadIdx.x - 192);
+    if (warp == 4) {  // products
     constexpr uint32_t kind_bits = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10));
     constexpr uint32_t qk = kind_bits | (uint32_t(S::ROWS >> 3) << 17) | (128u >> 4 << 24);
     constexpr uint32_t pv = kind_bits | (1u << 16) | (uint32_t(D >> 3) << 17) | (128u >> 4 << 24);  // values: components along a row
@@ -387,7 +398,9 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
       }
       __syncwarp();
     }
+    }
   } else {  // weights
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(int(KV_PROMPT_REGS_MORE)));
     const uint32_t lanes = uint32_t(warp * 32) << 16;
     const int pos = pos0 + tok;
     // the list of the thread's row: the entry that is next, and the one behind it on its way
@@ -447,11 +460,13 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
         unit = e;
       }
       const bool busy = __any_sync(FV_FULL, any || changed);
-      [[maybe_unused]] const bool odd = KIND == FV_KV_SAME && bars->odd[i & 1] != 0;
+      [[maybe_unused]] const bool odd = KIND == FV_KV_SAME && (bars->odd[i & 1][0] | bars->odd[i & 1][1] | bars->odd[i & 1][2] | bars->odd[i & 1][3]);
       if (busy) {
         uint32_t r[64];
-        tc_ld64_issue(place, r);
-        tc_ld64_wait(r);
+        tc_ld32_issue(place, r);
+        tc_ld32_issue(place + 32, r + 32);
+        tc_ld_wait(r);
+        tc_ld_wait(r + 32);
         float* s = reinterpret_cast<float*>(r);
         [[maybe_unused]] const float* const sc = reinterpret_cast<const float*>(smem + S::SCALE_AT) + (i & 1) * 2 * S::ROWS;
         if constexpr (KIND != FV_KV_SAME) {
@@ -583,7 +598,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
     }
     if (mine && a.lse) a.lse[query] = sum == 0.f ? -INFINITY : (top - ONE + log2f(sum)) * 0.693147180559945309f;
   }
-  if (warp == 5 || warp == 6) asm volatile("cp.async.wait_all;");
+  if (warp >= 6) asm volatile("cp.async.wait_all;");
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -602,6 +617,13 @@ int prompt_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAtt
   const size_t items = b->cu ? b->rows / tc + b->nseq : b->nseq;
   const size_t smem = S::LIST_AT + 8 * prompt_entries(b, a.group, a.blocks != nullptr, a.k);
   FV_TRY((kv_allow_smem<kv_prompt_kernel<T, KIND, D>>(kv->device, smem)));
+  static std::atomic<int> regs{0};  // a thread's at launch: the kernel waits for more than they add up to
+  if (regs.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes at;
+    FV_CUDA(cudaFuncGetAttributes(&at, kv_prompt_kernel<T, KIND, D>));
+    regs.store(at.numRegs, std::memory_order_relaxed);
+  }
+  if (regs.load(std::memory_order_relaxed) < KV_PROMPT_REGS) return fail(FV_ERR_UNSUPPORTED, "fv_kv_attend_dev: built with fewer registers than it shares out");
   kv_prompt_kernel<T, KIND, D><<<dim3(unsigned(items), kv->heads), KV_PROMPT_THREADS, smem, s>>>(a, kv_batch(kv, b));
   FV_CUDA(cudaGetLastError());
   return FV_OK;
