@@ -77,6 +77,24 @@ __device__ __forceinline__ void tc_st32(uint32_t to, const uint32_t* r) {
 }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two floats at a time.
+__device__ __forceinline__ void fma2(float* x, float by, float add) {  // x[0..1] * by + add
+  asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%0, %1};\nmov.b64 b, {%2, %2};\nmov.b64 c, {%3, %3};\nfma.rn.f32x2 a, a, b, c;\nmov.b64 {%0, %1}, a;\n}\n"
+      : "+f"(x[0]), "+f"(x[1])
+      : "f"(by), "f"(add));
+}
+__device__ __forceinline__ void mul2(float* x, float y0, float y1) {
+  asm("{\n.reg .b64 a, b;\nmov.b64 a, {%0, %1};\nmov.b64 b, {%2, %3};\nmul.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n" : "+f"(x[0]), "+f"(x[1]) : "f"(y0), "f"(y1));
+}
+__device__ __forceinline__ void add2(float* x, const float* y) {
+  asm("{\n.reg .b64 a, b;\nmov.b64 a, {%0, %1};\nmov.b64 b, {%2, %3};\nadd.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n" : "+f"(x[0]), "+f"(x[1]) : "f"(y[0]), "f"(y[1]));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // zeros in the halves that are not finite
 template <class T>
 __device__ __forceinline__ uint32_t finite_only(uint32_t w) {
@@ -176,6 +194,7 @@ __device__ __forceinline__ void bring_all(const KvAttend& a, const KvBatch& m, c
   uint64_t* const empty = VALUES ? bars->v_empty : bars->k_empty;
   const unsigned char* const src = VALUES ? a.vp : a.kp;
   unsigned char* const base = smem + (VALUES ? S::V_AT : S::K_AT);
+  [[maybe_unused]] int unit = 0;  // 8 bits: values stand for multiples of 2^(unit - 126), whose largest so far is below 1
   for (int i = 0; i < work.tiles; ++i) {
     const uint32_t turn = uint32_t(i >> 1) & 1u;  // of the tile's place
     unsigned char* const to = base + (i & 1) * S::STAGE;
@@ -207,19 +226,22 @@ __device__ __forceinline__ void bring_all(const KvAttend& a, const KvBatch& m, c
       B::convert(a, m, work, i, src, to, t);
       if (VALUES && t < 32) {  // the scales of both, which the queries' threads leave together with the values
         float* const sc = reinterpret_cast<float*>(smem + S::SCALE_AT) + (i & 1) * 2 * S::ROWS;
-        float most = 0.f;
+        float vs[2], most = 0.f;
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           const int r = lane + 32 * z;
           int begin = 0;
           size_t from = 0;
           const bool on = work.piece(a, m, 4 * i + (r >> 4), begin, from) && begin + (r & 15) <= work.last;
-          const float ks = on ? __ldg(a.k_scale + from + (r & 15)) : 0.f, vs = on ? __ldg(a.v_scale + from + (r & 15)) : 0.f;
-          sc[r] = ks, sc[S::ROWS + r] = vs;
-          most = fmaxf(most, vs);  // leaves NaN out: it reaches the sums through its weight
+          sc[r] = on ? __ldg(a.k_scale + from + (r & 15)) : 0.f;
+          vs[z] = on ? __ldg(a.v_scale + from + (r & 15)) : 0.f;
+          most = fmaxf(most, vs[z]);  // leaves NaN out: it reaches the sums through its weight
         }
-        const int e = int(__reduce_max_sync(FV_FULL, __float_as_uint(most)) >> 23);
-        if (lane == 0) bars->exponent[i & 1] = e;
+        unit = max(unit, int(__reduce_max_sync(FV_FULL, __float_as_uint(most)) >> 23));
+        const float down = __uint_as_float(uint32_t(max(253 - unit, 1)) << 23);
+        sc[S::ROWS + lane] = vs[0] * down, sc[S::ROWS + 32 + lane] = vs[1] * down;
+        const bool any = __any_sync(FV_FULL, !kv_finite(vs[0]) || !kv_finite(vs[1]));
+        if (lane == 0) bars->exponent[i & 1] = unit, bars->odd[i & 1][0] = any;
       }
     }
     fence_async();
@@ -419,31 +441,35 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
     }
     for (int i = 0; i < tiles; ++i) {
       int seen[4];  // rows of each piece that the query sees
-      bool any = false, whole = true;
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        int start = 0;
-        size_t from;
-        const bool there = work.piece(a, m, 4 * i + p, start, from);
-        seen[p] = 0;
-        if (there && mine) {
-          bool sees = start <= pos;
-          if (a.blocks) {
-            const int block = start >> m.page_shift;
-            while (entry < block) {  // entries that are blocks, each above all before it
-              const int e = ahead;
-              ++index;
-              ahead = index < a.k ? __ldg(mylist + index) : 0;
-              if (index > a.k) entry = INT_MAX;
-              else if (e > entry && e < blocks && (e << m.page_shift) <= pos) entry = e;
-            }
-            sees = sees && entry == block;
-          }
-          if (sees) seen[p] = min(16, pos - start + 1);
+      auto sees = [&](int2 at, int start) {  // whether the query sees the rows from `start` on, of a block of the union
+        if (!mine || at.y < 0 || start > pos) return false;
+        if (!a.blocks) return true;
+        while (entry < at.x) {  // entries that are blocks, each above all before it
+          const int e = ahead;
+          ++index;
+          ahead = index < a.k ? __ldg(mylist + index) : 0;
+          if (index > a.k) entry = INT_MAX;
+          else if (e > entry && e < blocks && (e << m.page_shift) <= pos) entry = e;
         }
-        any = any || seen[p] > 0;
-        whole = whole && (seen[p] == 0 || seen[p] == 16);
+        return entry == at.x;
+      };
+      if (m.page_shift >= 6) {  // the tile is of one block
+        const int more = m.page_shift - 6;
+        const int2 at = list[i >> more];
+        const int start = (at.x << m.page_shift) + ((i & ((1 << more) - 1)) << 6), n = sees(at, start) ? pos - start + 1 : 0;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) seen[p] = min(max(n - 16 * p, 0), 16);
+      } else {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int piece = 4 * i + p;
+          const int2 at = piece < work.pieces ? list[piece >> per] : make_int2(0, -1);
+          const int start = (at.x << m.page_shift) + ((piece & ((1 << per) - 1)) << 4);
+          seen[p] = sees(at, start) ? min(pos - start + 1, 16) : 0;
+        }
       }
+      const bool any = (seen[0] | seen[1] | seen[2] | seen[3]) != 0, all = (seen[0] & seen[1] & seen[2] & seen[3]) == 16;
+      const bool whole = ((seen[0] | seen[1] | seen[2] | seen[3]) & 15) == 0;
       const uint32_t turn = uint32_t(i >> 1) & 1u;
       on = __all_sync(FV_FULL, mbar_wait(&bars->s_full[i & 1], turn, abort, 0) && mbar_wait(&bars->v_full[i & 1], turn, abort, 0));
       if (!on) break;
@@ -452,15 +478,14 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
       uint32_t p[32];
       bool changed = false;
       float factor = 1.f;
-      int e = unit;
       if constexpr (KIND != FV_KV_SAME) {
-        e = max(unit, bars->exponent[i & 1]);
+        const int e = bars->exponent[i & 1];
         factor = __uint_as_float(uint32_t(max(127 + unit - e, 0)) << 23);
         changed = e != unit;
         unit = e;
       }
       const bool busy = __any_sync(FV_FULL, any || changed);
-      [[maybe_unused]] const bool odd = KIND == FV_KV_SAME && (bars->odd[i & 1][0] | bars->odd[i & 1][1] | bars->odd[i & 1][2] | bars->odd[i & 1][3]);
+      const bool odd = KIND == FV_KV_SAME ? (bars->odd[i & 1][0] | bars->odd[i & 1][1] | bars->odd[i & 1][2] | bars->odd[i & 1][3]) != 0 : bars->odd[i & 1][0] != 0;
       if (busy) {
         uint32_t r[64];
         tc_ld32_issue(place, r);
@@ -473,47 +498,49 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
 #pragma unroll
           for (int j = 0; j < 64; j += 4) {
             const float4 ks = *reinterpret_cast<const float4*>(sc + j);
-            s[j] *= ks.x, s[j + 1] *= ks.y, s[j + 2] *= ks.z, s[j + 3] *= ks.w;
+            mul2(s + j, ks.x, ks.y), mul2(s + j + 2, ks.z, ks.w);
           }
         }
-        if (__all_sync(FV_FULL, whole)) {
+        if (!__all_sync(FV_FULL, all)) {
+          if (__all_sync(FV_FULL, whole)) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) s[j] = seen[j >> 4] ? s[j] : -INFINITY;
-        } else {
+            for (int j = 0; j < 64; ++j) s[j] = seen[j >> 4] ? s[j] : -INFINITY;
+          } else {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) s[j] = (j & 15) < seen[j >> 4] ? s[j] : -INFINITY;
-        }
-        float y[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int j = 4; j < 64; ++j) y[j & 3] = fmaxf(y[j & 3], s[j]);
-        const float to = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) * by;
-        if (to > top + GROWN || top == -INFINITY) {
-          if (to > top) {
-            const float f = exp2_of(top - to);
-            factor *= f, sum *= f;
-            changed = changed || top != -INFINITY;  // without weights so far the query's O is 0
-            top = to;
+            for (int j = 0; j < 64; ++j) s[j] = (j & 15) < seen[j >> 4] ? s[j] : -INFINITY;
           }
+        }
+        float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 64; j += 2) y[j >> 1 & 3] = max3(y[j >> 1 & 3], s[j], s[j + 1]);
+        const float to = fmaxf(max3(y[0], y[1], y[2]), y[3]) * by;
+        if (to > top + GROWN || (top == -INFINITY && to > top)) {
+          const float f = exp2_of(top - to);
+          factor *= f, sum *= f;
+          changed = changed || top != -INFINITY;  // without weights so far the query's O is 0
+          top = to;
         }
         const float off = top == -INFINITY ? 0.f : ONE - top;
         float part[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (KIND == FV_KV_SAME) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) s[j] = exp2_of(__fmaf_rn(s[j], by, off)), part[j & 3] += s[j];
-        } else {
-          const float down = __uint_as_float(uint32_t(max(253 - e, 1)) << 23);
-#pragma unroll
-          for (int j = 0; j < 64; j += 4) {
-            const float4 vs = *reinterpret_cast<const float4*>(sc + S::ROWS + j);
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              const float w = exp2_of(__fmaf_rn(s[j + z], by, off));
-              part[z] += w;
-              s[j + z] = w != 0.f ? w * ((&vs.x)[z] * down) : 0.f;
-            }
-          }
+        for (int j = 0; j < 64; j += 2) {
+          fma2(s + j, by, off);
+          s[j] = exp2_of(s[j]), s[j + 1] = exp2_of(s[j + 1]);
+          add2(part + (j & 2), s + j);
         }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
+        if constexpr (KIND != FV_KV_SAME) {
+          if (!odd) {
+#pragma unroll
+            for (int j = 0; j < 64; j += 4) {
+              const float4 vs = *reinterpret_cast<const float4*>(sc + S::ROWS + j);
+              mul2(s + j, vs.x, vs.y), mul2(s + j + 2, vs.z, vs.w);
+            }
+          } else {  // a scale of NaN reaches the rows that have a weight for it
+#pragma unroll
+            for (int j = 0; j < 64; ++j) s[j] = s[j] != 0.f ? s[j] * sc[S::ROWS + j] : 0.f;
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 32; ++j) p[j] = Pair<M>::from_float(s[2 * j], s[2 * j + 1]);
         // O, scaled to the new maximum, and values that were taken out of the product
