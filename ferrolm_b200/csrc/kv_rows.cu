@@ -88,21 +88,21 @@ __device__ __forceinline__ void write_row(const uint4& raw, bool on, unsigned ch
     if (!fine) most = INFINITY;  // also where it is a NaN, which fmaxf drops
     most = group_max<N>(most);
     const bool ok = most < INFINITY, coded = ok && most > 0.f;
-    const float down = kv_down(most), den = coded ? most * down : 1.f, up = Eight<KIND>::top * down;
+    const float down = kv_down(most), den = coded ? most * down : 1.f, up = coded ? Eight<KIND>::top * down : 0.f, inv = __fdiv_rn(1.f, den);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = coded ? __fdiv_rn(x[i] * up, den) : 0.f;
+    for (int i = 0; i < 8; ++i) x[i] = ok ? x[i] * up : 0.f;  // of a row that is not finite, codes of zero
     if (on) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(Eight<KIND>::pack(x), Eight<KIND>::pack(x + 4));
+      *reinterpret_cast<uint2*>(dst) = make_uint2(Eight<KIND>::pack(x, den, inv), Eight<KIND>::pack(x + 4, den, inv));
       if (first_lane) *scale = ok ? __fdiv_rn(most, Eight<KIND>::top) : __int_as_float(0x7FC00000);
     }
   }
 }
 
-// An item is the part of one block that this call writes, for one head; WARPS of them share an item (4: prompts, 1: a few rows
+// An item is the part of one block that this call writes, for one head; WARPS of them share an item (8: prompts, 1: a few rows
 // for each sequence, four heads to a CTA).  One owner for each block's bounds means no atomics, and the order of the rows does
 // not change a minimum.  N lanes hold a row, 8 values each, so a warp writes 32 / N rows at once.
 template <class T, int KIND, int D, int WARPS>
-__global__ void __launch_bounds__(128) kv_add_kernel(KvPool pool, KvBatch m, KvInput kin, KvInput vin) {
+__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128, WARPS > 1 ? 3 : 1) kv_add_kernel(KvPool pool, KvBatch m, KvInput kin, KvInput vin) {
   constexpr int N = D <= 64 ? 8 : 16, PER = 32 / N, L = D / 8;
   constexpr int ROW = KIND == FV_KV_SAME ? 2 * D : D, VAL = ROW / D;
   __shared__ float s_lo[WARPS > 1 ? WARPS * D : 1], s_hi[WARPS > 1 ? WARPS * D : 1];
@@ -124,27 +124,39 @@ __global__ void __launch_bounds__(128) kv_add_kernel(KvPool pool, KvBatch m, KvI
   float lo[8], hi[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
-  for (int p0 = begin + part * PER; p0 < end; p0 += WARPS * PER) {
-    const int p = p0 + sub, slot = p & (size - 1);
-    const bool on = in_row && p < end;
-    const size_t row = size_t(r0 + (p - pos0));
-    uint4 kr = make_uint4(0, 0, 0, 0), vr = kr;
-    if (on) {
-      kr = *reinterpret_cast<const uint4*>(kin.p + row * kin.row + head * kin.head + l * 16);
-      vr = *reinterpret_cast<const uint4*>(vin.p + row * vin.row + head * vin.head + l * 16);
-      const uint32_t w[4] = {kr.x, kr.y, kr.z, kr.w};
+  constexpr int AHEAD = WARPS > 1 ? 2 : 1;  // rows that a lane has on their way
+  for (int p0 = begin + part * PER; p0 < end; p0 += AHEAD * WARPS * PER) {
+    uint4 kr[AHEAD], vr[AHEAD];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float2 f = Pair<T>::to_float(w[i]);
-        f.x = kv_finite(f.x) ? f.x : 0.f;
-        f.y = kv_finite(f.y) ? f.y : 0.f;
-        lo[2 * i] = fminf(lo[2 * i], f.x), hi[2 * i] = fmaxf(hi[2 * i], f.x);
-        lo[2 * i + 1] = fminf(lo[2 * i + 1], f.y), hi[2 * i + 1] = fmaxf(hi[2 * i + 1], f.y);
+    for (int z = 0; z < AHEAD; ++z) {
+      const int p = p0 + z * WARPS * PER + sub;
+      kr[z] = vr[z] = make_uint4(0, 0, 0, 0);
+      if (in_row && p < end) {
+        const size_t row = size_t(r0 + (p - pos0));
+        kr[z] = __ldg(reinterpret_cast<const uint4*>(kin.p + row * kin.row + head * kin.head + l * 16));
+        vr[z] = __ldg(reinterpret_cast<const uint4*>(vin.p + row * vin.row + head * vin.head + l * 16));
       }
     }
-    const size_t row_at = at * size + slot;
-    write_row<T, KIND, N>(kr, on, pool.k + row_at * ROW + l * 8 * VAL, pool.k_scale + row_at, l == 0);
-    write_row<T, KIND, N>(vr, on, pool.v + row_at * ROW + l * 8 * VAL, pool.v_scale + row_at, l == 0);
+#pragma unroll
+    for (int z = 0; z < AHEAD; ++z) {
+      if (z && p0 + z * WARPS * PER >= end) break;  // whole warps
+      const int p = p0 + z * WARPS * PER + sub, slot = p & (size - 1);
+      const bool on = in_row && p < end;
+      if (on) {
+        const uint32_t w[4] = {kr[z].x, kr[z].y, kr[z].z, kr[z].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float2 f = Pair<T>::to_float(w[i]);
+          f.x = kv_finite(f.x) ? f.x : 0.f;
+          f.y = kv_finite(f.y) ? f.y : 0.f;
+          lo[2 * i] = fminf(lo[2 * i], f.x), hi[2 * i] = fmaxf(hi[2 * i], f.x);
+          lo[2 * i + 1] = fminf(lo[2 * i + 1], f.y), hi[2 * i + 1] = fmaxf(hi[2 * i + 1], f.y);
+        }
+      }
+      const size_t row_at = at * size + slot;
+      write_row<T, KIND, N>(kr[z], on, pool.k + row_at * ROW + l * 8 * VAL, pool.k_scale + row_at, l == 0);
+      write_row<T, KIND, N>(vr[z], on, pool.v + row_at * ROW + l * 8 * VAL, pool.v_scale + row_at, l == 0);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -192,21 +204,22 @@ __global__ void __launch_bounds__(128) kv_add_kernel(KvPool pool, KvBatch m, KvI
   }
   most = group_max<32>(most);
   if (lane < L) {
-    const float down = kv_down(most), den = most > 0.f ? most * down : 1.f, up = 127.f * down;
+    const float down = kv_down(most), den = most > 0.f ? most * down : 1.f, up = 127.f * down, inv = __fdiv_rn(1.f, den);
     int8_t* codes = pool.bound_codes + at * (2 * D) + lane * 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) lo[i] = __fdiv_rn(lo[i] * up, den), hi[i] = __fdiv_rn(hi[i] * up, den);
+    for (int i = 0; i < 8; ++i) lo[i] *= up, hi[i] *= up;
     using E = Eight<FV_KV_INT8>;
-    *reinterpret_cast<uint2*>(codes) = make_uint2(E::pack(lo), E::pack(lo + 4));
-    *reinterpret_cast<uint2*>(codes + D) = make_uint2(E::pack(hi), E::pack(hi + 4));
+    *reinterpret_cast<uint2*>(codes) = make_uint2(E::pack(lo, den, inv), E::pack(lo + 4, den, inv));
+    *reinterpret_cast<uint2*>(codes + D) = make_uint2(E::pack(hi, den, inv), E::pack(hi + 4, den, inv));
     if (lane == 0) pool.bound_scale[at] = __fdiv_rn(most, 127.f);
   }
 }
 
-// ROWS rows of the call for all heads: a thread moves 8 values of a row of a head at a time.  A row's place is looked up once.
+// ROWS rows of the call for all heads: a thread moves 16 bytes of a row of a head at a time, of keys and of values, and has those of
+// four rows on their way.  A row's place is looked up once.
 template <class T, int KIND, int D, int ROWS>
-__global__ void __launch_bounds__(256) kv_vectors_kernel(KvPool pool, KvBatch m, unsigned char* k_out, unsigned char* v_out) {
-  constexpr int L = D / 8, ROW = KIND == FV_KV_SAME ? 2 * D : D, VAL = ROW / D;
+__global__ void __launch_bounds__(256) kv_vectors_kernel(KvPool pool, KvBatch m, unsigned char* k_out, unsigned char* v_out, bool wide) {
+  constexpr int VALUES = KIND == FV_KV_SAME ? 8 : 16, L = D / VALUES, ROW = KIND == FV_KV_SAME ? 2 * D : D, AHEAD = 4;
   __shared__ long long s_at[ROWS];  // page * heads * size + slot: the row in head 0; -1: none
   const int first = blockIdx.x * ROWS;
   if (threadIdx.x < ROWS) {
@@ -232,32 +245,50 @@ __global__ void __launch_bounds__(256) kv_vectors_kernel(KvPool pool, KvBatch m,
     s_at[threadIdx.x] = at;
   }
   __syncthreads();
-  const int per_row = pool.heads * L;
-  for (int r = 0; r < ROWS; ++r) {
-    const long long at0 = s_at[r];
-    if (at0 < 0) continue;
-    for (int i = threadIdx.x; i < per_row; i += 256) {
-      const int head = i / L, l = i - head * L;
+  const unsigned per_row = unsigned(pool.heads) * L, all = per_row * ROWS;
+  for (unsigned i0 = threadIdx.x; i0 < all; i0 += AHEAD * 256) {
+    uint4 in[AHEAD][2];
+    float scale[AHEAD][2];
+    size_t to[AHEAD];
+    bool on[AHEAD];
+#pragma unroll
+    for (int z = 0; z < AHEAD; ++z) {
+      const unsigned i = i0 + z * 256, r = i / per_row, x = i - r * per_row, head = x / L, l = x - head * L;
+      const long long at0 = i < all ? s_at[r] : -1;
+      on[z] = at0 >= 0;
+      if (!on[z]) continue;
       const size_t at = size_t(at0) + (size_t(head) << pool.page_shift);
-      const size_t to = (size_t(first + r) * per_row + i) * 16;
+      to[z] = ((size_t(first) + r) * per_row + x) * (2 * VALUES);
+      in[z][0] = __ldg(reinterpret_cast<const uint4*>(pool.k + at * ROW + l * 16));
+      in[z][1] = __ldg(reinterpret_cast<const uint4*>(pool.v + at * ROW + l * 16));
+      if constexpr (KIND != FV_KV_SAME) scale[z][0] = __ldg(pool.k_scale + at), scale[z][1] = __ldg(pool.v_scale + at);
+    }
+#pragma unroll
+    for (int z = 0; z < AHEAD; ++z) {
+      if (!on[z]) continue;
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
-        const unsigned char* src = (which ? pool.v : pool.k) + at * ROW + l * 8 * VAL;
-        uint4 out;
+        uint4* const out = reinterpret_cast<uint4*>((which ? v_out : k_out) + to[z]);
+        const uint4 c = in[z][which];
         if constexpr (KIND == FV_KV_SAME) {
-          out = *reinterpret_cast<const uint4*>(src);
+          *out = c;
         } else {
-          const uint2 c = *reinterpret_cast<const uint2*>(src);
-          const float s = (which ? pool.v_scale : pool.k_scale)[at];
-          float y[8];
-          Eight<KIND>::unpack(c.x, y);
-          Eight<KIND>::unpack(c.y, y + 4);
-          uint32_t w[4];
+          const float s = scale[z][which];
+          const uint32_t codes[4] = {c.x, c.y, c.z, c.w};
+          uint32_t w[8];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) w[x] = Pair<T>::from_float(y[2 * x] * s, y[2 * x + 1] * s);
-          out = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int x = 0; x < 4; ++x) {
+            float y[4];
+            Eight<KIND>::unpack(codes[x], y);
+            w[2 * x] = Pair<T>::from_float(y[0] * s, y[1] * s), w[2 * x + 1] = Pair<T>::from_float(y[2] * s, y[3] * s);
+          }
+          if (wide)  // the results begin on 32 bytes: one store, where two would each leave half of every sector
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                         "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+          else
+            out[0] = make_uint4(w[0], w[1], w[2], w[3]), out[1] = make_uint4(w[4], w[5], w[6], w[7]);
         }
-        *reinterpret_cast<uint4*>((which ? v_out : k_out) + to) = out;
       }
     }
   }
@@ -268,20 +299,26 @@ int add_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvInput&
   const KvBatch m = kv_batch(kv, b);
   const KvPool pool = kv_pool(kv);
   const size_t items = b->cu ? b->rows / kv->page_size + 2 * b->nseq : b->nseq;
-  // a warp for a block where a sequence brings a few rows, four where it brings a prompt
+  // a warp for a block where a sequence brings a few rows, eight where it brings a prompt
   if (b->rows <= 8 * b->nseq)
     kv_add_kernel<T, KIND, D, 1><<<dim3(unsigned(items), (kv->heads + 3) / 4), 128, 0, s>>>(pool, m, k, v);
   else
-    kv_add_kernel<T, KIND, D, 4><<<dim3(unsigned(items), kv->heads), 128, 0, s>>>(pool, m, k, v);
+    kv_add_kernel<T, KIND, D, 8><<<dim3(unsigned(items), kv->heads), 256, 0, s>>>(pool, m, k, v);
   FV_CUDA(cudaGetLastError());
   return FV_OK;
 }
 
 template <class T, int KIND, int D>
 int vectors_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, void* k, void* v) {
-  constexpr int ROWS = 8;
-  kv_vectors_kernel<T, KIND, D, ROWS><<<unsigned((b->rows + ROWS - 1) / ROWS), 256, 0, s>>>(
-      kv_pool(kv), kv_batch(kv, b), static_cast<unsigned char*>(k), static_cast<unsigned char*>(v));
+  const bool wide = kv_aligned(k, 32) && kv_aligned(v, 32);
+  auto go = [&](auto rows_of) {
+    constexpr int ROWS = decltype(rows_of)::value;
+    kv_vectors_kernel<T, KIND, D, ROWS><<<unsigned((b->rows + ROWS - 1) / ROWS), 256, 0, s>>>(
+        kv_pool(kv), kv_batch(kv, b), static_cast<unsigned char*>(k), static_cast<unsigned char*>(v), wide);
+  };
+  // few rows: a CTA for four of them, so that more SMs have some (24 rows of 8 heads in int8: 5.2 us by sixteens, VECTORS_NOTE)
+  if (b->rows <= 16 * 148) go(std::integral_constant<int, 4>());
+  else go(std::integral_constant<int, 16>());
   FV_CUDA(cudaGetLastError());
   return FV_OK;
 }
