@@ -139,6 +139,7 @@ struct DeviceGuard {
   explicit DeviceGuard(int dev) {
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
     if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
+    else prev = -1;  // nothing to put back
   }
   ~DeviceGuard() {
     if (prev >= 0) cudaSetDevice(prev);

@@ -4,8 +4,8 @@
 //
 // One row has as many queries to a key head as its group has heads, so a key is read for a few products only: the bytes of the
 // blocks bound it.  A warp takes 16 rows of a block at a time, with a running maximum and sum of its own, through stages in shared
-// memory that no other warp waits for.  Many rows get a CTA for each key head; the work of few is cut into equal parts for all
-// warps that the GPU holds, and joined by a second kernel.
+// memory that no other warp waits for.  Many rows, and short lists, get a CTA for each key head; the work of few is cut into equal
+// parts for all warps that the GPU holds, and joined by a second kernel.
 //
 // The products are S^T = K Q^T and O^T = V^T P^T, so that 8 queries fill a tile that would have 16 the other way round.  Sums
 // over components may go in any order, so lane t of four holds neighbouring components where the product would have it
@@ -24,8 +24,18 @@ namespace fv {
 int kv_prompt_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a);  // kv_prompt.cu
 bool kv_prompt_fits(const fv_kv_batch* b, size_t group, bool lists, size_t k);
 
-// up to so many rows and tasks the work is cut into equal parts, for as many warps
-enum { KV_PARTS_ROWS = 2048, KV_PARTS_TASKS = 2048, KV_PARTS_WARPS = 160 * 16 };
+// The work is cut into equal parts, for at most so many warps, where there are fewer tasks than CTAs that the GPU holds and each
+// has enough pieces of 16 rows.  Else a CTA works on each task.  8 key heads of 4 queries, int8, both ways (us, parts first):
+//   pieces    16      40      80      192
+//   64 tasks  10/7.3  11/11   14/17   20/34
+//   320       17/14   24/23   35/39   61/77
+//   512       19/16   32/28   49/46   89/91
+// In 8 bits long lists are worth it up to twice as many tasks: 64 rows of 8 key heads over 192 pieces 93 us in parts, 99 by tasks;
+// in 16 bits, where the copies leave the time, 148 and 126.
+enum { KV_PARTS_TASKS = 400, KV_PARTS_PIECES = 64, KV_PARTS_TASKS_LONG = 1024, KV_PARTS_PIECES_LONG = 192, KV_PARTS_WARPS = 160 * 16 };
+static bool in_parts(int kind, size_t tasks, size_t pieces) {
+  return (tasks < KV_PARTS_TASKS && pieces >= KV_PARTS_PIECES) || (kind != FV_KV_SAME && tasks <= KV_PARTS_TASKS_LONG && pieces >= KV_PARTS_PIECES_LONG);
+}
 
 namespace {
 
@@ -65,7 +75,7 @@ struct Stage {
   static constexpr int PIECES = KIND == FV_KV_SAME ? 1 : 2;
   static constexpr int SIZE = PIECES * PIECE;
   static constexpr int LEAST = 4 / PIECES;  // stages worth a share of their own
-  static constexpr int DEPTH = 16 * 1024 / SIZE < 2 ? 2 : 16 * 1024 / SIZE > 6 ? 6 : 16 * 1024 / SIZE;
+  static constexpr int DEPTH = 16 * 1024 / SIZE < 3 ? 3 : 16 * 1024 / SIZE > 6 ? 6 : 16 * 1024 / SIZE;
 
   static __device__ __forceinline__ int key_at(int step, int t) {  // first of the four
     constexpr int steps = PER_LOAD / 4;
@@ -451,7 +461,7 @@ __device__ __forceinline__ int pieces_of(const KvAttend& a, const KvBatch& m, in
   return a.blocks ? a.k << (m.page_shift - 4) : min((pos >> 4) + 1, m.table_width << (m.page_shift - 4));
 }
 
-// Many rows: a CTA for one row and key head; its warps take turns at the pieces.
+// A CTA for one row and key head; its warps take turns at the pieces.
 template <class T, int KIND, int D, int NT>
 __global__ void __launch_bounds__(32 * KV_TOKEN_WARPS) kv_token_kernel(KvAttend a, KvBatch m, int tiles) {
   constexpr int W = KV_TOKEN_WARPS, COLS = 8 * NT;
@@ -493,7 +503,7 @@ __global__ void __launch_bounds__(32 * KV_TOKEN_WARPS) kv_token_kernel(KvAttend 
   finish<T, KIND, D, NT, W, D / 16>(s, a, row, head, first, 0, warp, lane);
 }
 
-// Few rows: all the pieces of all rows and heads (tasks), in units of a stage, are cut into equal parts, one for each warp that
+// Or: all the pieces of all rows and heads (tasks), in units of a stage, are cut into equal parts, one for each warp that
 // the GPU holds, whatever the lengths.  A warp leaves its share of each task that it meets in `part`: that of warp w of task t at
 // number w + t, since along the units one of the two grows.  A second kernel joins them.
 struct Parts {
@@ -731,8 +741,8 @@ int token_launch(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const Kv
   if (tasks_a_row > 65535) return fail(FV_ERR_UNSUPPORTED, "fv_kv_attend_dev: more than 65535 tiles of query heads");
   const size_t ring = size_t(W) * S::DEPTH * S::SIZE, shares = size_t(W) * H::FLOATS * 4;
   const KvBatch m = kv_batch(kv, b);
-  if (tasks <= KV_PARTS_TASKS && b->rows <= KV_PARTS_ROWS && work) {
-    const size_t smem = ring + 4 * (b->rows + 1), most = ring + 4 * (KV_PARTS_ROWS + 1);
+  if (work && in_parts(KIND, tasks, (a.blocks ? size_t(a.k) : b->table_width) * (kv->page_size / 16))) {
+    const size_t smem = ring + 4 * (b->rows + 1), most = ring + 4 * (KV_PARTS_TASKS_LONG + 1);
     Parts p{int(b->rows), int(tasks_a_row), S::LEAST, 0, static_cast<float*>(work)};
     FV_TRY((kv_allow_smem<kv_parts_kernel<T, KIND, D, NT>>(kv->device, most)));
     FV_TRY((parts_warps<T, KIND, D, NT>(kv->device, ring + 1024, &p.warps)));
@@ -779,11 +789,10 @@ int kv_token_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const
 
 }  // namespace fv
 
-// Shares that are worth their room: beyond that many tasks a CTA for each of them leaves no SM without work for long.
 extern "C" size_t fv_kv_attend_work(const fv_kv* kv, const fv_kv_batch* batch, size_t group) {
-  if (!kv || !batch || group == 0 || group > 128 || batch->rows > fv::KV_PARTS_ROWS) return 0;
-  const size_t cols = group <= 8 ? 8 : 16, tasks = batch->rows * kv->heads * ((group + cols - 1) / cols);
-  return tasks && tasks <= fv::KV_PARTS_TASKS ? (tasks + fv::KV_PARTS_WARPS) * cols * (kv->dim + 2) * 4 : 0;
+  if (!kv || !batch || group == 0 || group > 128 || batch->rows > fv::KV_PARTS_TASKS_LONG) return 0;
+  const size_t cols = group <= 8 ? 8 : 16, tasks = batch->rows * kv->heads * ((group + cols - 1) / cols), pieces = batch->table_width * (kv->page_size / 16);
+  return tasks && fv::in_parts(kv->kind, tasks, pieces) ? (tasks + fv::KV_PARTS_WARPS) * cols * (kv->dim + 2) * 4 : 0;
 }
 
 extern "C" int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* q, size_t q_row, size_t q_head,
