@@ -741,7 +741,8 @@ int token_launch(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const Kv
   if (tasks_a_row > 65535) return fail(FV_ERR_UNSUPPORTED, "fv_kv_attend_dev: more than 65535 tiles of query heads");
   const size_t ring = size_t(W) * S::DEPTH * S::SIZE, shares = size_t(W) * H::FLOATS * 4;
   const KvBatch m = kv_batch(kv, b);
-  if (work && in_parts(KIND, tasks, (a.blocks ? size_t(a.k) : b->table_width) * (kv->page_size / 16))) {
+  const size_t pieces = (a.blocks ? size_t(a.k) : b->table_width) * (kv->page_size / 16);  // of a task, at most
+  if (work && in_parts(KIND, tasks, pieces) && pieces * tasks <= size_t(1) << 30) {
     const size_t smem = ring + 4 * (b->rows + 1), most = ring + 4 * (KV_PARTS_TASKS_LONG + 1);
     Parts p{int(b->rows), int(tasks_a_row), S::LEAST, 0, static_cast<float*>(work)};
     FV_TRY((kv_allow_smem<kv_parts_kernel<T, KIND, D, NT>>(kv->device, most)));

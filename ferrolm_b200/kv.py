@@ -13,7 +13,7 @@ before.  Positions below 0 or in a block that the table has no column for, and b
 cache (-1, say), are skipped: nothing is written or read there and nothing attends to them.
 
 The calls run on the current torch stream of the cache's device and do not wait for it; they can be captured into a CUDA
-graph.  Tensors are used on that stream only.
+graph.  Tensors are used on that stream only.  They know no gradients.
 """
 from __future__ import annotations
 
@@ -82,6 +82,7 @@ class KvCache:
 
         L = lib()
         self._ref, self._i32, self._f32, self._index = C.byref(self._c), torch.int32, torch.float32, self.device.index
+        self._grad = torch.is_grad_enabled
         self._empty_like, self._contiguous = torch.empty_like, torch.contiguous_format
         self._get_stream, self._work_sizes = torch._C._cuda_getCurrentRawStream, {}
         self._add, self._vectors, self._search, self._attend = L.fv_kv_add_dev, L.fv_kv_vectors_dev, L.fv_kv_search_dev, L.fv_kv_attend_dev
@@ -112,6 +113,8 @@ class KvCache:
             _refuse(f"{what} is (rows, heads, dim) with dim {self.dim}" + (f" and {heads} heads" if heads else "") + f": got {tuple(shape)}")
         if x.dtype is not self.dtype or x.device != self.device:
             _refuse(f"{what} is {self.dtype} on {self.device}: got {x.dtype} on {x.device}")
+        if x.requires_grad and self._grad():
+            _refuse(f"{what} wants a gradient, and the cache gives none: call it under torch.no_grad() or with a detached tensor")
         r, h, d = x.stride()
         at = x.data_ptr()
         if d != 1 or (r | h) & 7 or at & 15:
@@ -124,7 +127,7 @@ class KvCache:
     def add(self, k, v, table, lens, cu=None):
         """Writes the call's rows `k` and `v` (rows, heads, dim) into their pages and keeps the bounds of their blocks.
 
-        A page that is written to belongs to one sequence of the call.  A block that gets its first row forgets what its
+        A page that is written to is one block of one sequence of the call.  A block that gets its first row forgets what its
         bounds were; one that is written again from its middle on keeps the bounds of the rows that were there.  Key
         components that are not finite count as zero in the bounds."""
         k, kp, kr, kh, rows = self._rows(k, "k", self.heads)

@@ -302,16 +302,16 @@ int fv_merge_topk_static_dev(int device, void* stream, const fv_neighbor* d_part
  * as NaN; k_scale and v_scale are NULL for FV_KV_SAME.  k, v and bounds begin on 16 bytes, bound_codes on 16, scales on 4.
  * dim is 64, 96 or 128, page_size 16, 32, 64 or 128.
  *
- * The calls take a cudaStream_t of that device (NULL: its default stream), launch one kernel on it and return: they allocate
- * nothing, wait for nothing and may be captured into a graph.  Calls on one cache are ordered by their streams; nothing in
- * the library is shared between them.
+ * The calls take a cudaStream_t of that device (NULL: its default stream), launch a kernel or two on it and return: they
+ * allocate nothing, wait for nothing and may be captured into a graph.  Calls on one cache are ordered by their streams; nothing
+ * in the library is shared between them.
  *
  * A batch: sequence b has its pages in table[b][0..table_width) and lens[b] rows, those of this call among them.  The call
  * is about its last n_b rows: row i of them stands at position lens[b] - n_b + i, and they are rows cu[b] .. cu[b+1] of the
  * call's tensors (cu: nseq + 1 ascending numbers from 0; NULL: one row each, rows = nseq).  Rows from cu[nseq] on are not
  * touched.  Positions below 0 or in a block from table_width on, and blocks whose table entry is not a page of the cache
- * (-1, say), are skipped: nothing is read or written there, and nothing attends to them.  A page that add writes to belongs
- * to one sequence of the call. */
+ * (-1, say), are skipped: nothing is read or written there, and nothing attends to them.  A page that add writes to is one
+ * block of one sequence of the call. */
 enum { FV_KV_BF16 = 0, FV_KV_FP16 = 1 };                 /* dtype */
 enum { FV_KV_SAME = 0, FV_KV_INT8 = 1, FV_KV_E4M3 = 2 }; /* kind */
 typedef struct fv_kv {
@@ -360,7 +360,7 @@ int fv_kv_search_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, co
  * blocks that each row and key head attends to, as fv_kv_search_dev gives them (ascending; an entry that is no block the
  * query can see, or is not above all before it that are, is skipped), or NULL for all of them.  A row with nothing to
  * attend to gets zeros and -inf.  Scores, maxima and sums are 32-bit floats; weights are rounded to 16 bits before they meet the
- * values. */
+ * values.  The waits inside the kernels are bounded (about 2 s); results of one that ran out are NaN. */
 int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* q, size_t q_row, size_t q_head,
                      size_t group, const int32_t* blocks, size_t k, float scale, void* out, float* lse, void* work, size_t work_bytes);
 /* Bytes of device memory that fv_kv_attend_dev wants as `work` (on 16 bytes, the caller's, used until the call's kernels are
