@@ -4,7 +4,9 @@
 //   code = rn(top * x / most),  scale = most / top,  most = max |x| over a row of a head
 //   lo, hi = componentwise min and max over the block's keys; their codes the same way with one scale for both
 //
-// Both are a pass over the data with a handful of operations for each value.
+// Both are a pass over the data with a handful of operations for each value, and bound by the bytes.  94k rows of 8 heads of 128
+// read back from e4m3 (605 MB): 95.5 us, 6.3 TB/s, 97% of the copy rate.  14k rows of prompts added as e4m3 (87 MB): 37 us, 2.4
+// TB/s: a block's rows pass through one CTA, whose rounding and bounds leave its loads waiting.  24 single rows: 3.7 and 3.2 us.
 #include <climits>
 
 #include "kv.cuh"
@@ -316,7 +318,7 @@ int vectors_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, void* k, v
     kv_vectors_kernel<T, KIND, D, ROWS><<<unsigned((b->rows + ROWS - 1) / ROWS), 256, 0, s>>>(
         kv_pool(kv), kv_batch(kv, b), static_cast<unsigned char*>(k), static_cast<unsigned char*>(v), wide);
   };
-  // few rows: a CTA for four of them, so that more SMs have some (24 rows of 8 heads in int8: 5.2 us by sixteens, VECTORS_NOTE)
+  // few rows: a CTA for four of them, so that more SMs have some (24 rows of 8 heads in int8: 3.2 us, 5.2 by sixteens)
   if (b->rows <= 16 * 148) go(std::integral_constant<int, 4>());
   else go(std::integral_constant<int, 16>());
   FV_CUDA(cudaGetLastError());

@@ -12,6 +12,11 @@
 //   score           float(p . hi + n . lo) * bound_scale
 //   result          the first `first` blocks, the last `recent` up to the query's own, then the largest scores (the lower
 //                   block of equals) up to k in all, in ascending order, -1 behind the last
+//
+// The bounds are 2 dim + 4 bytes for a block, so a token's search is a few dependent loads long (the table, the bounds, then the
+// threshold): 10.4 us for one request over 2032 blocks of 8 heads, 4.2 MB, in clusters of 8 (28.7 without); 12.5 us for 48
+// requests.  A prompt's search is bound by what each row does after the products: 92 us for 3.2k rows of 8 heads over up to
+// 512 blocks, about 800 instructions a warp for a row's codes, 1000 for its threshold and list.
 #include <climits>
 
 #include <cooperative_groups.h>
@@ -266,9 +271,9 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int n, int k, int32
 // the components are a sum, so lane t of four may hold 16 neighbouring ones where the product would have it hold 4 of each 16,
 // on both sides.
 template <class T, int D, int NT, int TEAM>
-__global__ void __launch_bounds__(KV_SEARCH_THREADS, TEAM > 1 ? 3 : 2) kv_search_kernel(KvSearch a, KvBatch m, int pitch, int splits) {
+__global__ void __launch_bounds__(KV_SEARCH_THREADS, 3) kv_search_kernel(KvSearch a, KvBatch m, int pitch, int splits) {
   constexpr int R = TEAM > 1 ? 1 : 8 * NT, CHUNKS = 2 * D / 64;
-  constexpr int SHIFT = R == 1 ? 0 : R == 8 ? 3 : R == 16 ? 4 : 5;
+  constexpr int SHIFT = R == 1 ? 0 : R == 8 ? 3 : 4;
   __shared__ __align__(16) int8_t s_codes[8 * NT][2 * D + 16];
   __shared__ int s_team[2 * KV_SEARCH_WARPS];
   __shared__ uint2 s_list[KV_SEARCH_WARPS][TEAM > 1 ? 1 : KV_SEARCH_LIST];
@@ -357,7 +362,8 @@ __global__ void __launch_bounds__(KV_SEARCH_THREADS, TEAM > 1 ? 3 : 2) kv_search
     const uint32_t* mine = keys + size_t(r) * pitch;
     int32_t* out = a.out + (size_t(row + r) * a.heads + head) * a.k;
     if (n <= 8 * 32 * TEAM) choose<TEAM, 8>(mine, n, a.k, out, s_team, s_list[warp]);
-    else if (n <= 20 * 32 * TEAM) choose<TEAM, 20>(mine, n, a.k, out, s_team, s_list[warp]);
+    else if (n <= 16 * 32 * TEAM) choose<TEAM, 16>(mine, n, a.k, out, s_team, s_list[warp]);
+    else if (n <= 24 * 32 * TEAM) choose<TEAM, 24>(mine, n, a.k, out, s_team, s_list[warp]);
     else choose<TEAM, 0>(mine, n, a.k, out, s_team, s_list[warp]);
   };
   if constexpr (TEAM > 1) {
@@ -398,11 +404,11 @@ int search_launch(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const K
 
 template <class T, int D>
 int search_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvSearch& a) {
-  // 8 to 32 rows of a prompt share a read of the bounds, as many as leave room for two CTAs on an SM; where a sequence brings a
-  // few rows, or the table is wide, a CTA works on one row
+  // 16 rows of a prompt share a read of the bounds, or 8 where the keys of 16 do not leave room for two CTAs on an SM (32 of them
+  // leave room for two where 16 leave it for three: 99 us and 92 for 3.2k rows over 512 blocks); where a sequence brings a few
+  // rows, or the table is wide, a CTA works on one row
   const size_t row = size_t(search_pitch(b->table_width)) * 4, most = 100 * 1024;
   if (b->rows <= 4 * b->nseq || 8 * row > 2 * most) return search_launch<T, D, 1, 8>(kv, s, b, a);
-  if (32 * row <= most) return search_launch<T, D, 4, 1>(kv, s, b, a);
   if (16 * row <= most) return search_launch<T, D, 2, 1>(kv, s, b, a);
   return search_launch<T, D, 1, 1>(kv, s, b, a);
 }

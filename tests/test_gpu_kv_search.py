@@ -126,3 +126,47 @@ def test_the_same_blocks_whichever_way_the_rows_are_cut():
         again = c.search_blocks(wide[:, 5:], table, i32([n]).cuda(), 16, cu=i32([0, 200]).cuda())
     s.synchronize()
     assert torch.equal(again, whole)
+
+
+def test_the_longest_table():
+    """As many blocks as one search takes, for a cluster's one row and for rows of a prompt, most of them without a page."""
+    heads, group, dim, page, width = 1, 1, 64, 16, 50_000
+    c, p = pair(700, heads, dim, page, BF, seed=9)
+    table = torch.full((1, width), -1, dtype=torch.int32)
+    at = torch.randperm(width, generator=torch.Generator().manual_seed(2))[:690]
+    table[0, at] = torch.randperm(700, generator=torch.Generator().manual_seed(3))[:690].to(torch.int32)
+    table[0, width - 1], table[0, 0] = 0, 1
+    n = width * page - 2
+    q = queries(6, heads, group, dim, BF, 3)
+    whole = c.search_blocks(q.cuda(), table.cuda(), i32([n]).cuda(), 40, cu=i32([0, 6]).cuda())
+    want = p.search(q[5:], table, [n], 40, None, 1, 2, torch.zeros((1, heads, 40), dtype=torch.int64))
+    assert torch.equal(whole[5:].cpu().long(), want)
+    for i in range(6):
+        assert torch.equal(c.search_blocks(q[i : i + 1].cuda(), table.cuda(), i32([n - 5 + i]).cuda(), 40), whole[i : i + 1])
+
+
+def test_calls_that_are_refused():
+    import ferrolm_b200 as fv
+
+    c = fv.KvCache(8, 2, 64, page_size=16)
+    table, lens = i32([[0, 1, 2]]).cuda(), i32([40]).cuda()
+    q = torch.zeros((1, 4, 64), dtype=BF, device="cuda")
+    for bad in (dict(k=0), dict(k=4097), dict(first=-1), dict(recent=-2), dict(lens=lens.long()), dict(table=table[0]), dict(lens=i32([40, 1]).cuda()),
+                dict(cu=i32([0, 1, 2]).cuda()), dict(cu=i32([0, 1])), dict(q=q.half()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q.cpu()),
+                dict(q=q.expand(2, 4, 64)), dict(q=q.clone().requires_grad_()), dict(out=torch.zeros((1, 2, 5), dtype=torch.int32, device="cuda"))):
+        a = dict(q=q, table=table, lens=lens, k=2) | bad
+        with pytest.raises(fv.FerrovecError):
+            c.search_blocks(a.pop("q"), a.pop("table"), a.pop("lens"), a.pop("k"), **a)
+    k = torch.zeros((1, 2, 64), dtype=BF, device="cuda")
+    for bad in (dict(k=k.half()), dict(v=k[:, :1]), dict(k=k.expand(2, 2, 64)), dict(table=table.cpu()), dict(v=k.clone().requires_grad_())):
+        a = dict(k=k, v=k, table=table, lens=lens) | bad
+        with pytest.raises(fv.FerrovecError):
+            c.add(**a)
+    for bad in (dict(blocks=i32([[[0], [1]]])), dict(blocks=i32([[[0, 1]]]).cuda()), dict(blocks=torch.zeros((1, 2, 0), dtype=torch.int32, device="cuda")),
+                dict(scale=float("nan")), dict(out=q.half()), dict(out=(q, q), return_lse=True)):
+        with pytest.raises(fv.FerrovecError):
+            c.attend(q, table, lens, **bad)
+    with pytest.raises(fv.FerrovecError):
+        c.vectors(table, lens, out=(k, k.half()))
+    with torch.no_grad():  # where no gradient is wanted, a parameter is a tensor like another
+        c.attend(q.clone().requires_grad_(), table, lens)
