@@ -266,6 +266,99 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int n, int k, int32
     for (int i = at + lane; i < k; i += 32) out[i] = -1;
 }
 
+// The least t with at least k of a warp's keys from it on, and exactly k where that can be; there are more than k, fewer than
+// k of them forced.  N keys a lane, 0 for none.
+template <int N>
+__device__ __forceinline__ uint32_t kth(const uint32_t* keys, int k) {
+  uint32_t hi = 0, low = 0;  // largest that is not forced; the largest complement
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (keys[i] != 0xFFFFFFFFu) hi = max(hi, keys[i]);
+    if (keys[i] != 0u) low = max(low, ~keys[i]);
+  }
+  hi = __reduce_max_sync(FV_FULL, hi), low = ~__reduce_max_sync(FV_FULL, low);
+  const uint32_t differ = hi ^ low;
+  int bit = differ ? 31 - __clz(int(differ)) : -1;
+  uint32_t t = bit < 0 ? hi : hi & ~((2u << bit) - 1u);
+  for (; bit >= 0; --bit) {
+    const uint32_t c = t | 1u << bit;
+    int cnt = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) cnt += keys[i] >= c;
+    cnt = __reduce_add_sync(FV_FULL, cnt);
+    if (cnt >= k) t = c;
+    if (cnt == k) break;
+  }
+  return max(t, 1u);
+}
+
+// The same as choose<8, ..> for most searches, with three barriers instead of one for every bit: of the threads' largest keys the
+// k-th is a bound that few more than k keys reach; they are filed in order, and a warp finishes.  False: too many reach it, and
+// nothing is done.
+__device__ __forceinline__ bool choose_few(const uint32_t* keys, int n, int k, int32_t* out, int* s_team, uint32_t* s_tops, uint2* s_list) {
+  constexpr int W = KV_SEARCH_WARPS;
+  const int lane = lane_id(), warp = threadIdx.x >> 5;
+  const int per = ((n + W - 1) / W + 31) / 32 * 32, begin = min(n, warp * per), end = min(n, begin + per);  // a warp's stretch
+  if (k > KV_SEARCH_LIST) return false;
+  uint32_t top = 0;
+  for (int i = begin + lane; i < end; i += 32) top = max(top, keys[i]);
+  s_tops[threadIdx.x] = top;
+  __syncthreads();
+  uint32_t tops[W];
+  int there = 0;  // and forced ones times 2^16; every warp finds the bound for itself
+#pragma unroll
+  for (int i = 0; i < W; ++i) tops[i] = s_tops[32 * i + lane], there += (tops[i] != 0u) + (tops[i] == 0xFFFFFFFFu ? 1 << 16 : 0);
+  there = __reduce_add_sync(FV_FULL, there);
+  if ((there & 0xFFFF) <= k || (there >> 16) >= k) return false;
+  const uint32_t least = kth<W>(tops, k);
+  int count = 0;
+  for (int i0 = begin; i0 < end; i0 += 32) count += __popc(__ballot_sync(FV_FULL, i0 + lane < end && keys[i0 + lane] >= least));
+  if (lane == 0) s_team[warp] = count;
+  __syncthreads();
+  int at = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w < warp) at += s_team[w];
+    all += s_team[w];
+  }
+  if (all > KV_SEARCH_LIST) return false;
+  const unsigned before = (1u << lane) - 1u;
+  for (int i0 = begin; i0 < end; i0 += 32) {
+    const uint32_t x = i0 + lane < end ? keys[i0 + lane] : 0u;
+    const unsigned in = __ballot_sync(FV_FULL, x >= least);
+    if (x >= least) s_list[at + __popc(in & before)] = make_uint2(x, uint32_t(i0 + lane));
+    at += __popc(in);
+  }
+  __syncthreads();
+  if (warp) return true;
+  constexpr int N = KV_SEARCH_LIST / 32;
+  uint32_t few[N], which[N];
+  int forced = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint2 x = 32 * i + lane < all ? s_list[32 * i + lane] : make_uint2(0u, 0u);
+    few[i] = x.x, which[i] = x.y;
+    forced += x.x == 0xFFFFFFFFu;
+  }
+  forced = __reduce_add_sync(FV_FULL, forced);
+  const uint32_t t = all == k ? 1u : forced >= k ? 0xFFFFFFFFu : kth<N>(few, k);
+  int above = 0, from = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) above += few[i] > t, from += few[i] >= t;
+  above = __reduce_add_sync(FV_FULL, above), from = __reduce_add_sync(FV_FULL, from);
+  const int room = from == k ? k : k - above;  // for keys equal to t: all of them, or the first
+  int to = 0, seen = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const unsigned eqs = __ballot_sync(FV_FULL, few[i] == t);
+    const bool take = few[i] > t || (few[i] == t && seen + __popc(eqs & before) < room);
+    const unsigned takes = __ballot_sync(FV_FULL, take);
+    if (take) out[to + __popc(takes & before)] = int(which[i]);
+    to += __popc(takes), seen += __popc(eqs);
+  }
+  return true;
+}
+
 // TEAM = 8: one row of the call to a CTA (a token), or to a cluster of up to 8 where there are few.  TEAM = 1: 8 * NT consecutive rows of one sequence (a prompt), which share
 // what is read of the bounds.  A warp takes 16 blocks at a time straight from memory into the operands of a matrix product:
 // the components are a sum, so lane t of four may hold 16 neighbouring ones where the product would have it hold 4 of each 16,
@@ -276,7 +369,8 @@ __global__ void __launch_bounds__(KV_SEARCH_THREADS, 3) kv_search_kernel(KvSearc
   constexpr int SHIFT = R == 1 ? 0 : R == 8 ? 3 : 4;
   __shared__ __align__(16) int8_t s_codes[8 * NT][2 * D + 16];
   __shared__ int s_team[2 * KV_SEARCH_WARPS];
-  __shared__ uint2 s_list[KV_SEARCH_WARPS][TEAM > 1 ? 1 : KV_SEARCH_LIST];
+  __shared__ uint2 s_list[TEAM > 1 ? 1 : KV_SEARCH_WARPS][KV_SEARCH_LIST];
+  __shared__ uint32_t s_tops[TEAM > 1 ? KV_SEARCH_THREADS : 1];
   uint32_t* const keys = reinterpret_cast<uint32_t*>(dyn_smem());  // [R][pitch]
   const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = lane_id(), g = lane >> 2, t = lane & 3;
   const int rank = TEAM > 1 ? int(blockIdx.x) % splits : 0;
@@ -361,10 +455,15 @@ __global__ void __launch_bounds__(KV_SEARCH_THREADS, 3) kv_search_kernel(KvSearc
   auto pick = [&](int r) {
     const uint32_t* mine = keys + size_t(r) * pitch;
     int32_t* out = a.out + (size_t(row + r) * a.heads + head) * a.k;
-    if (n <= 8 * 32 * TEAM) choose<TEAM, 8>(mine, n, a.k, out, s_team, s_list[warp]);
-    else if (n <= 16 * 32 * TEAM) choose<TEAM, 16>(mine, n, a.k, out, s_team, s_list[warp]);
-    else if (n <= 24 * 32 * TEAM) choose<TEAM, 24>(mine, n, a.k, out, s_team, s_list[warp]);
-    else choose<TEAM, 0>(mine, n, a.k, out, s_team, s_list[warp]);
+    uint2* const list = s_list[TEAM > 1 ? 0 : warp];
+    if constexpr (TEAM > 1) {
+      if (choose_few(mine, n, a.k, out, s_team, s_tops, list)) return;
+      __syncthreads();
+    }
+    if (n <= 8 * 32 * TEAM) choose<TEAM, 8>(mine, n, a.k, out, s_team, list);
+    else if (TEAM == 1 && n <= 16 * 32) choose<TEAM, TEAM == 1 ? 16 : 0>(mine, n, a.k, out, s_team, list);
+    else if (TEAM == 1 && n <= 24 * 32) choose<TEAM, TEAM == 1 ? 24 : 0>(mine, n, a.k, out, s_team, list);
+    else choose<TEAM, 0>(mine, n, a.k, out, s_team, list);
   };
   if constexpr (TEAM > 1) {
     pick(0);
