@@ -648,12 +648,15 @@ __global__ void __launch_bounds__(32 * KV_TOKEN_WARPS) kv_join_kernel(KvAttend a
   const int warp = threadIdx.x >> 5, lane = lane_id(), t = lane & 3;
   const int row = blockIdx.x, task = blockIdx.y, u0 = blockIdx.z * U;
   units_before<Stage<KIND, D>>(a, m, p.rows, before, s_warp);
-  if (place_of(m, row).b < 0) return;
+  const bool none = place_of(m, row).b < 0;
   const int mine = units_a_warp(p, before[p.rows]), units = before[row + 1] - before[row];
   const long long begin = (long long)(before[row]) * p.tasks_a_row + (long long)(task) * units;
   const int w0 = int(begin / mine), w1 = units ? int((begin + units - 1) / mine) : w0 - 1;  // the warps that met the task
   const float* const part = p.part + (size_t(row) * p.tasks_a_row + task) * H::FLOATS;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the shares
+  // For the shares.  Every CTA waits, whether it has some or not: what the stream holds next starts when these are done, and must
+  // not start before the kernel that leaves the shares is.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (none) return;
   float4 o[U][NT];
   float most[NT][2], total[NT][2];
 #pragma unroll

@@ -378,51 +378,51 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(int(KV_PROMPT_REGS_LESS)));
     if (warp >= 6) bring_all<T, KIND, D, false>(a, m, work, smem, bars, abort, threadIdx.x - 192);
     if (warp == 4) {  // products
-    constexpr uint32_t kind_bits = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10));
-    constexpr uint32_t qk = kind_bits | (uint32_t(S::ROWS >> 3) << 17) | (128u >> 4 << 24);
-    constexpr uint32_t pv = kind_bits | (1u << 16) | (uint32_t(D >> 3) << 17) | (128u >> 4 << 24);  // values: components along a row
-    auto scores = [&](int i) {  // of tile i
-      if (!__all_sync(FV_FULL, mbar_wait(&bars->k_full[i & 1], uint32_t(i >> 1) & 1u, abort, 0))) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint32_t q = smem_u32(smem), k = smem_u32(smem + S::K_AT + (i & 1) * S::STAGE);
+      constexpr uint32_t kind_bits = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10));
+      constexpr uint32_t qk = kind_bits | (uint32_t(S::ROWS >> 3) << 17) | (128u >> 4 << 24);
+      constexpr uint32_t pv = kind_bits | (1u << 16) | (uint32_t(D >> 3) << 17) | (128u >> 4 << 24);  // values: components along a row
+      auto scores = [&](int i) {  // of tile i
+        if (!__all_sync(FV_FULL, mbar_wait(&bars->k_full[i & 1], uint32_t(i >> 1) & 1u, abort, 0))) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t q = smem_u32(smem), k = smem_u32(smem + S::K_AT + (i & 1) * S::STAGE);
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          const uint32_t at = (s & 3) * 32;
-          tc_mma_f16<false>(tmem + (i & 1) * 64, make_desc(desc_lo(q + (s >> 2) * S::Q_HALF + at), DESC_HI_SW128),
-                            make_desc(desc_lo(k + (s >> 2) * S::HALF + at), DESC_HI_SW128), qk, s > 0);
+          for (int s = 0; s < D / 16; ++s) {
+            const uint32_t at = (s & 3) * 32;
+            tc_mma_f16<false>(tmem + (i & 1) * 64, make_desc(desc_lo(q + (s >> 2) * S::Q_HALF + at), DESC_HI_SW128),
+                              make_desc(desc_lo(k + (s >> 2) * S::HALF + at), DESC_HI_SW128), qk, s > 0);
+          }
+          tc_commit<false>(&bars->k_empty[i & 1]);
+          tc_commit<false>(&bars->s_full[i & 1]);
         }
-        tc_commit<false>(&bars->k_empty[i & 1]);
-        tc_commit<false>(&bars->s_full[i & 1]);
-      }
-      __syncwarp();
-      return true;
-    };
-    bool on = tiles > 0 && scores(0);
-    for (int i = 0; on && i < tiles; ++i) {
-      if (i + 1 < tiles) {
-        // the place of the next scores holds the weights of the tile before this one
-        on = __all_sync(FV_FULL, i == 0 || mbar_wait(&bars->pv_done, uint32_t(i - 1) & 1u, abort, 0));
-        on = on && scores(i + 1);
+        __syncwarp();
+        return true;
+      };
+      bool on = tiles > 0 && scores(0);
+      for (int i = 0; on && i < tiles; ++i) {
+        if (i + 1 < tiles) {
+          // the place of the next scores holds the weights of the tile before this one
+          on = __all_sync(FV_FULL, i == 0 || mbar_wait(&bars->pv_done, uint32_t(i - 1) & 1u, abort, 0));
+          on = on && scores(i + 1);
+          if (!on) break;
+        }
+        on = __all_sync(FV_FULL, mbar_wait(&bars->v_full[i & 1], uint32_t(i >> 1) & 1u, abort, 0) && mbar_wait(&bars->p_full[i & 1], uint32_t(i >> 1) & 1u, abort, 0));
         if (!on) break;
-      }
-      on = __all_sync(FV_FULL, mbar_wait(&bars->v_full[i & 1], uint32_t(i >> 1) & 1u, abort, 0) && mbar_wait(&bars->p_full[i & 1], uint32_t(i >> 1) & 1u, abort, 0));
-      if (!on) break;
-      tc_fence_after();
-      if (elect_one()) {
-        // rows of 128 bytes along the components: 8 rows of the cache 1024 bytes apart, 64 components a HALF
-        const uint32_t v = smem_u32(smem + S::V_AT + (i & 1) * S::STAGE);
+        tc_fence_after();
+        if (elect_one()) {
+          // rows of 128 bytes along the components: 8 rows of the cache 1024 bytes apart, 64 components a HALF
+          const uint32_t v = smem_u32(smem + S::V_AT + (i & 1) * S::STAGE);
 #pragma unroll
-        for (int s = 0; s < S::ROWS / 16; ++s) {
-          const uint32_t lo = ((v + s * 2048) >> 4) | (uint32_t(S::HALF >> 4) << 16);
-          tc_mma_ts(tmem + S::O_COL, tmem + (i & 1) * 64 + s * 8, make_desc(lo, DESC_HI_SW128), pv, 1u);
+          for (int s = 0; s < S::ROWS / 16; ++s) {
+            const uint32_t lo = ((v + s * 2048) >> 4) | (uint32_t(S::HALF >> 4) << 16);
+            tc_mma_ts(tmem + S::O_COL, tmem + (i & 1) * 64 + s * 8, make_desc(lo, DESC_HI_SW128), pv, 1u);
+          }
+          tc_commit<false>(&bars->v_empty[i & 1]);
+          tc_commit<false>(&bars->pv_done);
+          if (i + 1 == tiles) tc_commit<false>(&bars->all_done);
         }
-        tc_commit<false>(&bars->v_empty[i & 1]);
-        tc_commit<false>(&bars->pv_done);
-        if (i + 1 == tiles) tc_commit<false>(&bars->all_done);
+        __syncwarp();
       }
-      __syncwarp();
-    }
     }
   } else {  // weights
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(int(KV_PROMPT_REGS_MORE)));
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
         for (int z = 0; z < 4; ++z) *reinterpret_cast<uint4*>(a.out + (query * D + c + 8 * z) * 2) = w[z];
       }
     }
-    if (mine && a.lse) a.lse[query] = sum == 0.f ? -INFINITY : (top - ONE + log2f(sum)) * 0.693147180559945309f;
+    if (mine && a.lse) a.lse[query] = !on ? __int_as_float(0x7FC00000) : sum == 0.f ? -INFINITY : (top - ONE + log2f(sum)) * 0.693147180559945309f;
   }
   if (warp >= 6) asm volatile("cp.async.wait_all;");
   tc_fence_before();

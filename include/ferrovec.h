@@ -299,7 +299,7 @@ int fv_merge_topk_static_dev(int device, void* stream, const fv_neighbor* d_part
  * (scales), [pages][heads][2][dim] (bounds: the componentwise minima and maxima of a block's keys; bound_codes: the same in
  * 8 bits), [pages][heads] (bound_scale), contiguous.  k and v hold `dtype` (FV_KV_SAME) or 8 bits: a row is
  * code * scale with scale = max|x| / 127 (int8) or / 448 (e4m3), and a row with a value that is not finite reads back
- * as NaN; k_scale and v_scale are NULL for FV_KV_SAME.  k, v and bounds begin on 16 bytes, bound_codes on 16, scales on 4.
+ * as NaN (its scale; codes are always numbers); k_scale and v_scale are NULL for FV_KV_SAME.  k, v and bounds begin on 16 bytes, bound_codes on 16, scales on 4.
  * dim is 64, 96 or 128, page_size 16, 32, 64 or 128.
  *
  * The calls take a cudaStream_t of that device (NULL: its default stream), launch a kernel or two on it and return: they
