@@ -35,7 +35,7 @@ struct KvSearch {
   int32_t* out;
 };
 
-enum { KV_SEARCH_THREADS = 256, KV_SEARCH_WARPS = 8, KV_SEARCH_LIST = 128 };
+enum { KV_SEARCH_THREADS = 256, KV_SEARCH_WARPS = 8, KV_SEARCH_LIST = 128, KV_SEARCH_WIDTH = 50000 };
 
 // The 2 D codes of one row's group of queries to dst, by a warp: lanes 0 .. D/4-1 have 4 components each.
 template <class T, int D>
@@ -114,14 +114,14 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int n, int k, int32
     }
   };
   int phase = 0;
-  auto total = [&](int x) {  // over the team
+  auto total = [&](unsigned x) {  // over the team
     x = __reduce_add_sync(FV_FULL, x);
     if constexpr (TEAM > 1) {
-      if (lane == 0) s_team[phase * TEAM + warp] = x;
+      if (lane == 0) s_team[phase * TEAM + warp] = int(x);
       __syncthreads();
       x = 0;
 #pragma unroll
-      for (int w = 0; w < TEAM; ++w) x += s_team[phase * TEAM + w];
+      for (int w = 0; w < TEAM; ++w) x += unsigned(s_team[phase * TEAM + w]);
       phase ^= 1;
     }
     return x;
@@ -137,15 +137,16 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int n, int k, int32
     }
     return x;
   };
-  int counts = 0;  // candidates, and forced ones times 2^16
+  unsigned counts = 0;  // candidates, and forced ones times 2^16: there are at most KV_SEARCH_WIDTH of either, so neither leaves its half
+  static_assert(KV_SEARCH_WIDTH < 1 << 16, "two counts share a word");
   uint32_t hi = 0, second = 0;  // a thread's two largest keys that are not forced
   each([&](uint32_t x) {
-    counts += (x != 0u) + (x == 0xFFFFFFFFu ? 1 << 16 : 0);
+    counts += (x != 0u ? 1u : 0u) + (x == 0xFFFFFFFFu ? 1u << 16 : 0u);
     const uint32_t y = x == 0xFFFFFFFFu ? 0u : x;
     second = max(second, min(hi, y)), hi = max(hi, y);
   });
   counts = total(counts);
-  const int there = counts & 0xFFFF, forced = counts >> 16;
+  const int there = int(counts & 0xFFFFu), forced = int(counts >> 16);
   const unsigned before = (1u << lane) - 1u;
   auto bisect = [&](uint32_t lo, uint32_t up, auto&& over, uint32_t& t) {  // the least t with at most k keys from it on, or the k-th key
     const uint32_t differ = up ^ lo;
@@ -155,7 +156,7 @@ __device__ __forceinline__ void choose(const uint32_t* keys, int n, int k, int32
       const uint32_t c = t | 1u << bit;
       int cnt = 0;
       over([&](uint32_t x) { cnt += x >= c; });
-      cnt = total(cnt);
+      cnt = int(total(unsigned(cnt)));
       if (cnt >= k) t = c;
       if (cnt == k) return true;
     }
@@ -527,7 +528,7 @@ extern "C" int fv_kv_search_dev(const fv_kv* kv, void* stream, const fv_kv_batch
   FV_TRY(fv::kv_check(kv, batch, "fv_kv_search_dev"));
   if (group == 0 || group > 128) return fv::fail(FV_ERR_UNSUPPORTED, "fv_kv_search_dev: group is 1 to 128 query heads to a key head");
   if (k == 0 || k > FV_KV_MAX_BLOCKS) return fv::fail(FV_ERR_UNSUPPORTED, "fv_kv_search_dev: k is 1 to 4096 blocks");
-  if (batch->table_width > 50000)
+  if (batch->table_width > fv::KV_SEARCH_WIDTH)
     return fv::fail(FV_ERR_UNSUPPORTED, "fv_kv_search_dev: a table of more than 50000 blocks; use larger pages");
   if (batch->rows == 0 || batch->nseq == 0) return FV_OK;
   if (!q || !out) return fv::fail(FV_ERR_ARG, "fv_kv_search_dev: NULL queries or result");
