@@ -19,7 +19,10 @@
 // A maximum that grows by less than a factor of 2 (fp16) or 256 (bf16) is left as it was: the weights stay within their type, and
 // O, in tensor memory, need not be scaled as often.  Values that are not finite would reach rows that do not see them as
 // 0 * inf: they are taken out on their way in, and added by the threads whose rows see them.  In 8 bits the codes become fp16,
-// exactly, on their way in; a key's scale multiplies its column of S, a value's its weight (kv_attend.cu).
+// exactly, on their way in; a key's scale multiplies its column of S, a value's its weight (kv_attend.cu), relative to a
+// power of two that follows the largest scale that the query itself has seen: what only the others of its tile see costs it no bits.
+// The tile's scales come relative to the same for all that the CTA's queries see, which mostly is the query's own power too; a warp
+// with a query for which it is not takes the scales as they are (int8, dense: 386 us with and without; e4m3, lists: 1182 us of 1164).
 #include <climits>
 
 #include "kv.cuh"
@@ -38,7 +41,8 @@ static_assert(KV_PROMPT_REGS_MORE + 2 * KV_PROMPT_REGS_LESS <= 3 * KV_PROMPT_REG
 struct PromptBars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done, all_done;
   uint32_t tmem;
-  int abort, odd[2][4], exponent[2], entries;
+  int abort, odd[2][4], entries;
+  int2 exponent[2];  // of the largest scale of a value, of the tile and of all tiles up to it
 };
 
 template <int KIND, int D>
@@ -49,7 +53,7 @@ struct Tile {
   static constexpr int STAGE = HALVES * HALF;            // keys or values of one tile
   static constexpr int Q_HALF = KV_PROMPT_COLS * 128;
   static constexpr int Q = HALVES * Q_HALF;
-  static constexpr int SCALES = KIND == FV_KV_SAME ? 0 : 2 * 2 * ROWS * 4;  // [stage][keys, values][ROWS]
+  static constexpr int SCALES = KIND == FV_KV_SAME ? 0 : 2 * 3 * ROWS * 4;  // [stage][keys, values relative to the largest, values][ROWS]
   static constexpr int K_AT = Q, V_AT = Q + 2 * STAGE, SCALE_AT = Q + 4 * STAGE, BARS_AT = SCALE_AT + SCALES;
   static constexpr int LIST_AT = BARS_AT + (int(sizeof(PromptBars)) + 15) / 16 * 16;
   static constexpr int O_COL = 128;  // columns of tensor memory: S or P 0-63, 64-127, O from 128 on
@@ -197,7 +201,7 @@ __device__ __forceinline__ void bring_all(const KvAttend& a, const KvBatch& m, c
   uint64_t* const empty = VALUES ? bars->v_empty : bars->k_empty;
   const unsigned char* const src = VALUES ? a.vp : a.kp;
   unsigned char* const base = smem + (VALUES ? S::V_AT : S::K_AT);
-  [[maybe_unused]] int unit = 0;  // 8 bits: values stand for multiples of 2^(unit - 126), whose largest so far is below 1
+  [[maybe_unused]] int unit = 1;  // 8 bits: scales stand for multiples of 2^(unit - 126), none so far for 2 or more
   for (int i = 0; i < work.tiles; ++i) {
     const uint32_t turn = uint32_t(i >> 1) & 1u;  // of the tile's place
     unsigned char* const to = base + (i & 1) * S::STAGE;
@@ -228,7 +232,7 @@ __device__ __forceinline__ void bring_all(const KvAttend& a, const KvBatch& m, c
     } else {
       B::convert(a, m, work, i, src, to, t);
       if (VALUES && t < 32) {  // the scales of both, which the queries' threads leave together with the values
-        float* const sc = reinterpret_cast<float*>(smem + S::SCALE_AT) + (i & 1) * 2 * S::ROWS;
+        float* const sc = reinterpret_cast<float*>(smem + S::SCALE_AT) + (i & 1) * 3 * S::ROWS;
         float vs[2], most = 0.f;
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
@@ -240,11 +244,13 @@ __device__ __forceinline__ void bring_all(const KvAttend& a, const KvBatch& m, c
           vs[z] = on ? __ldg(a.v_scale + from + (r & 15)) : 0.f;
           most = fmaxf(most, vs[z]);  // leaves NaN out: it reaches the sums through its weight
         }
-        unit = max(unit, int(__reduce_max_sync(FV_FULL, __float_as_uint(most)) >> 23));
+        const int e = int(__reduce_max_sync(FV_FULL, __float_as_uint(most)) >> 23);
+        unit = e > unit + 1 ? e : unit;
         const float down = __uint_as_float(uint32_t(max(253 - unit, 1)) << 23);
         sc[S::ROWS + lane] = vs[0] * down, sc[S::ROWS + 32 + lane] = vs[1] * down;
+        sc[2 * S::ROWS + lane] = vs[0], sc[2 * S::ROWS + 32 + lane] = vs[1];
         const bool any = __any_sync(FV_FULL, !kv_finite(vs[0]) || !kv_finite(vs[1]));
-        if (lane == 0) bars->exponent[i & 1] = unit, bars->odd[i & 1][0] = any;
+        if (lane == 0) bars->exponent[i & 1] = make_int2(e, unit), bars->odd[i & 1][0] = any;
       }
     }
     fence_async();
@@ -258,7 +264,8 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
   using M = typename std::conditional<KIND == FV_KV_SAME, T, __half>::type;
   constexpr bool HALF = std::is_same<M, __half>::value;
   constexpr float ONE = HALF ? 14.f : 0.f;   // log2 of what stands for a weight of 1
-  constexpr float GROWN = HALF ? 1.f : 8.f;  // log2 of what a maximum may lag behind by
+  // log2 of what a maximum may lag behind by; in 8 bits, where the weights meet scales of less than 2, 2^14.9 of them stay in fp16
+  constexpr float GROWN = KIND != FV_KV_SAME ? 0.9f : HALF ? 1.f : 8.f;
   unsigned char* const smem = dyn_smem();
   PromptBars* const bars = reinterpret_cast<PromptBars*>(smem + S::BARS_AT);
   int2* const list = reinterpret_cast<int2*>(smem + S::LIST_AT);
@@ -432,7 +439,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
     const int32_t* const mylist = a.blocks && mine ? a.blocks + (size_t(row0 + tok) * a.heads + head) * a.k : nullptr;
     int entry = -1, ahead = mylist ? __ldg(mylist) : 0, index = 0;
     float top = -INFINITY, sum = 0.f;
-    int unit = 0;  // 8 bits: values stand for multiples of 2^(unit - 126)
+    int unit = 0;  // 8 bits: values stand for multiples of 2^(unit - 126), scales the query has seen are below 2 of it; 0: none seen
     bool on = true;
     {
       uint32_t zero[32];
@@ -481,13 +488,19 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
       uint32_t p[32];
       bool changed = false;
       float factor = 1.f;
+      [[maybe_unused]] const float* const sc = reinterpret_cast<const float*>(smem + S::SCALE_AT) + (i & 1) * 3 * S::ROWS;
+      [[maybe_unused]] bool alike = true;  // the tile's scales are relative to the query's unit
       if constexpr (KIND != FV_KV_SAME) {
-        const int e = bars->exponent[i & 1];
-        factor = __uint_as_float(uint32_t(max(127 + unit - e, 0)) << 23);
-        changed = e != unit;
-        unit = e;
+        const int2 e = bars->exponent[i & 1];
+        if (all && (e.x > unit + 1 || unit == 0)) {  // of a tile that the query sees the whole of
+          const int own = max(e.x, 1);
+          factor = __uint_as_float(uint32_t(max(127 + unit - own, 0)) << 23);
+          changed = unit != 0;  // without weights so far the query's O is 0
+          unit = own;
+        }
+        alike = __all_sync(FV_FULL, !any || unit == e.y);
       }
-      const bool busy = __any_sync(FV_FULL, any || changed);
+      const bool busy = __any_sync(FV_FULL, any);
       const bool odd = KIND == FV_KV_SAME ? (bars->odd[i & 1][0] | bars->odd[i & 1][1] | bars->odd[i & 1][2] | bars->odd[i & 1][3]) != 0 : bars->odd[i & 1][0] != 0;
       if (busy) {
         uint32_t r[64];
@@ -496,7 +509,6 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
         tc_ld_wait(r);
         tc_ld_wait(r + 32);
         float* s = reinterpret_cast<float*>(r);
-        [[maybe_unused]] const float* const sc = reinterpret_cast<const float*>(smem + S::SCALE_AT) + (i & 1) * 2 * S::ROWS;
         if constexpr (KIND != FV_KV_SAME) {
 #pragma unroll
           for (int j = 0; j < 64; j += 4) {
@@ -533,15 +545,28 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
         }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
         if constexpr (KIND != FV_KV_SAME) {
-          if (!odd) {
+          if (!odd && alike) {
 #pragma unroll
             for (int j = 0; j < 64; j += 4) {
               const float4 vs = *reinterpret_cast<const float4*>(sc + S::ROWS + j);
               mul2(s + j, vs.x, vs.y), mul2(s + j + 2, vs.z, vs.w);
             }
-          } else {  // a scale of NaN reaches the rows that have a weight for it
+          } else {
+            const int2 e = bars->exponent[i & 1];
+            if (any && (e.x > unit + 1 || unit == 0)) {  // a scale of the tile is above the query's unit: whether it has a weight
+              float most = 0.f;  // leaves NaN out
 #pragma unroll
-            for (int j = 0; j < 64; ++j) s[j] = s[j] != 0.f ? s[j] * sc[S::ROWS + j] : 0.f;
+              for (int j = 0; j < 64; ++j) most = fmaxf(most, s[j] != 0.f ? sc[2 * S::ROWS + j] : 0.f);
+              const int own = max(int(__float_as_uint(most) >> 23), 1);
+              if (own > unit + 1 || unit == 0) {
+                factor *= __uint_as_float(uint32_t(max(127 + unit - own, 0)) << 23);
+                changed = changed || unit != 0;  // without weights so far the query's O is 0
+                unit = own;
+              }
+            }
+            const float down = __uint_as_float(uint32_t(max(253 - unit, 1)) << 23);
+#pragma unroll  // scales of NaN, and those beyond the query's unit, reach the rows that have a weight for them
+            for (int j = 0; j < 64; ++j) s[j] = s[j] != 0.f ? s[j] * (sc[2 * S::ROWS + j] * down) : 0.f;
           }
         }
 #pragma unroll
