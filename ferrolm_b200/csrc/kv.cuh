@@ -67,6 +67,8 @@ struct KvBatch {
   __device__ __forceinline__ int cu_at(int b) const {  // rows before sequence b, never outside of the call's tensors
     return cu ? min(max(__ldg(cu + b), 0), rows) : min(b, rows);
   }
+  // rows of sequence b.  Less than none are none: a position, n rows before it, stays within 32 bits.
+  __device__ __forceinline__ int len(int b) const { return max(__ldg(lens + b), 0); }
   // page of block j of sequence b, or -1
   __device__ __forceinline__ int page(int b, int j) const {
     if (j < 0 || j >= table_width) return -1;

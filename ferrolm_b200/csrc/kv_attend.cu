@@ -410,7 +410,7 @@ struct Place {
 __device__ __forceinline__ Place place_of(const KvBatch& m, int row) {  // whole warps call it
   const int b = m.cu ? kv_find(m, row, 1, 0) : row;
   if (row < m.cu_at(b) || row >= m.cu_at(b + 1)) return {-1, -1};
-  return {b, __ldg(m.lens + b) - max(m.cu_at(b + 1), row + 1) + row};
+  return {b, m.len(b) - max(m.cu_at(b + 1), row + 1) + row};
 }
 
 // The pieces of one row and key head, 16 rows each, and where they lie: lane i has block and page of the i-th of 32 of the row's
@@ -532,9 +532,9 @@ __device__ __forceinline__ void units_before(const KvAttend& a, const KvBatch& m
         if (m.cu_at(lo + h) <= r) lo += h, n -= h;
         else n = h;
       }
-      if (r < rows && r >= m.cu_at(lo) && r < m.cu_at(lo + 1)) pos = __ldg(m.lens + lo) - max(m.cu_at(lo + 1), r + 1) + r;
+      if (r < rows && r >= m.cu_at(lo) && r < m.cu_at(lo + 1)) pos = m.len(lo) - max(m.cu_at(lo + 1), r + 1) + r;
     } else if (r < rows) {
-      pos = __ldg(m.lens + r) - 1;
+      pos = m.len(r) - 1;
     }
     int x = (pieces_of(a, m, pos) + S::PIECES - 1) / S::PIECES;
 #pragma unroll

@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
   const int r0 = m.cu_at(b), r1 = max(m.cu_at(b + 1), r0);
   const int row0 = m.cu ? r0 + (item - (r0 / tc + b)) * tc : r0, rows = min(tc, r1 - row0);
   if (row0 < r0 || rows <= 0) return;
-  const int pos0 = __ldg(m.lens + b) - r1 + row0, last = pos0 + rows - 1;  // positions of the first and the last row
+  const int pos0 = m.len(b) - r1 + row0, last = pos0 + rows - 1;  // positions of the first and the last row
   const int blocks = min(m.table_width, last < 0 ? 0 : (last >> m.page_shift) + 1);
 
   if (warp == 4) {

@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128, WARPS > 1 ? 3 : 
   if (head >= pool.heads) return;  // whole warps, and with WARPS > 1 whole blocks
   const int shift = pool.page_shift, size = 1 << shift, item = blockIdx.x;
   const int b = m.cu ? kv_find(m, item, size, 2) : item;
-  const int r0 = m.cu_at(b), r1 = max(m.cu_at(b + 1), r0), len = __ldg(m.lens + b);
+  const int r0 = m.cu_at(b), r1 = max(m.cu_at(b + 1), r0), len = m.len(b);
   const int pos0 = len - (r1 - r0);  // of row r0
   const int j = (max(pos0, 0) >> shift) + (m.cu ? item - ((r0 >> shift) + 2 * b) : 0);
   const int begin = max(max(pos0, 0), j << shift), end = min(len, (j + 1) << shift);
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(256) kv_vectors_kernel(KvPool pool, KvBatch m,
       } else {
         lo = r;
       }
-      const int pos = __ldg(m.lens + lo) - max(m.cu_at(lo + 1), r + 1) + r;
+      const int pos = m.len(lo) - max(m.cu_at(lo + 1), r + 1) + r;
       if (pos >= 0) {
         const int page = m.page(lo, pos >> pool.page_shift);
         if (page >= 0) at = ((long long)(page) * pool.heads << pool.page_shift) + (pos & ((1 << pool.page_shift) - 1));

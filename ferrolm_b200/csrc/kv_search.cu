@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(KV_SEARCH_THREADS, 3) kv_search_kernel(KvSearc
     rows = min(R, r1 - row);
     if (row < r0 || rows <= 0) return;  // the same for a whole cluster
   }
-  const int pos0 = __ldg(m.lens + b) - max(m.cu_at(b + 1), row + 1) + row;  // of the first row
+  const int pos0 = m.len(b) - max(m.cu_at(b + 1), row + 1) + row;  // of the first row
   const int n = min(m.table_width, pos0 + rows - 1 < 0 ? 0 : ((pos0 + rows - 1) >> m.page_shift) + 1);
   const int begin = (rank * KV_SEARCH_WARPS + warp) * 16, step = splits * KV_SEARCH_WARPS * 16;
   int ahead[2];  // the pages that are next
