@@ -34,6 +34,7 @@ int kv_check(const fv_kv* kv, const fv_kv_batch* b, const char* who) {
     return fail(FV_ERR_ARG, w + ": scales do not begin on 4 bytes");
   if (b->rows > size_t(INT_MAX) / 2 || b->nseq > size_t(INT_MAX) / 8 || b->table_width > size_t(1) << 24 || b->table_stride > size_t(1) << 40)
     return fail(FV_ERR_UNSUPPORTED, w + ": rows, nseq or table_width is too large");
+  if (b->table_width > size_t(INT_MAX) / kv->page_size) return fail(FV_ERR_UNSUPPORTED, w + ": positions in the table's last block leave 31 bits");
   if (b->rows && b->nseq && (!b->lens || (!b->table && b->table_width))) return fail(FV_ERR_ARG, w + ": NULL table or lens");
   if (!b->cu && b->rows != b->nseq) return fail(FV_ERR_ARG, w + ": without cu there is one row for each sequence");
   if (!kv_aligned(b->table, 4) || !kv_aligned(b->lens, 4) || !kv_aligned(b->cu, 4))

@@ -1,0 +1,13 @@
+"""What the key/value cache's entry points refuse because of its size, and what they say that a call needs; all before any CUDA call."""
+from tests.test_kv_cpu import UNSUPPORTED, batch, cache, calls, fv  # noqa: F401
+
+
+def test_a_table_whose_last_block_ends_behind_31_bits(fv):  # noqa: F811
+    """16,777,216 blocks of 128 rows: the position behind the last row of the last one is 2^31.  One block less, or smaller ones, are fine."""
+    for name, call in calls(fv).items():
+        if name == "fv_kv_search_dev":  # takes 50,000
+            continue
+        assert call(cache(page_size=128), batch(table_width=1 << 24)) == UNSUPPORTED
+        assert fv.kv.lib().fv_last_error().decode().startswith(name)
+        for page, width in ((128, (1 << 24) - 1), (64, 1 << 24)):
+            assert call(cache(page_size=page), batch(table_width=width, nseq=0, rows=0)) == 0
