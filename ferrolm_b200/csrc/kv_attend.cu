@@ -800,6 +800,7 @@ int kv_token_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const
 
 extern "C" size_t fv_kv_attend_work(const fv_kv* kv, const fv_kv_batch* batch, size_t group) {
   if (!kv || !batch || group == 0 || group > 128 || batch->rows > fv::KV_PARTS_TASKS_LONG) return 0;
+  if (fv::is_prompt(batch, group, false, 0)) return 0;  // with lists too: a shorter union fits where the whole table does
   const size_t cols = group <= 8 ? 8 : 16, tasks = batch->rows * kv->heads * ((group + cols - 1) / cols), pieces = batch->table_width * (kv->page_size / 16);
   return tasks && fv::in_parts(kv->kind, tasks, pieces) ? (tasks + fv::KV_PARTS_WARPS) * cols * (kv->dim + 2) * 4 : 0;
 }

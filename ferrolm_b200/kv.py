@@ -216,11 +216,12 @@ class KvCache:
         if return_lse:
             lse_at = lse.data_ptr()
         batch, work_at = self._batch(table, lens, cu, rows), None
-        size = self._work_sizes.get((rows, heads, batch.table_width))  # depends on these alone
+        shape = rows, heads, batch.nseq, batch.table_width
+        size = self._work_sizes.get(shape)  # depends on these alone
         if size is None:
             if len(self._work_sizes) > 4096:
                 self._work_sizes.clear()
-            size = self._work_sizes[rows, heads, batch.table_width] = lib().fv_kv_attend_work(self._ref, batch, group)
+            size = self._work_sizes[shape] = lib().fv_kv_attend_work(self._ref, batch, group)
         if size:
             work = self.bound_scale.new_empty(size >> 2)
             work_at = work.data_ptr()

@@ -364,8 +364,8 @@ int fv_kv_search_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, co
 int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* q, size_t q_row, size_t q_head,
                      size_t group, const int32_t* blocks, size_t k, float scale, void* out, float* lse, void* work, size_t work_bytes);
 /* Bytes of device memory that fv_kv_attend_dev wants as `work` (on 16 bytes, the caller's, used until the call's kernels are
- * done): with it the work of a few rows is cut into equal parts over the whole GPU.  0: none.  Without it (NULL) the call is
- * as right, and slower where there are few rows. */
+ * done): with it the work of a few rows is cut into equal parts over the whole GPU.  0: none, as for prompts.  It is enough for any
+ * lists of blocks; a call over short ones may not use it.  Without it (NULL) the call is as right, and slower where there are few rows. */
 size_t fv_kv_attend_work(const fv_kv* kv, const fv_kv_batch* batch, size_t group);
 
 /* ---- seeded synthetic data for benchmarks and tests: a mixture of `clusters` Gaussians.
