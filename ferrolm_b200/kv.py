@@ -38,6 +38,7 @@ class KvCache:
     The memory is torch's: `k`, `v` (pages, heads, page_size, dim), `k_scale`, `v_scale` (pages, heads, page_size) or None,
     `bounds` (pages, heads, 2, dim: the componentwise minima and maxima of a block's keys), `bound_codes` (the same in 8
     bits) and `bound_scale` (pages, heads).  `buffers`: a dict of them by these names, where the caller has them already.
+    Their contents are anyone's to change; the tensors are the cache's for good, since every call goes to their addresses.
     """
 
     def __init__(self, pages: int, heads: int, dim: int, page_size: int = 64, dtype=None, kind: str = "same", device=None,
@@ -65,9 +66,7 @@ class KvCache:
             x = buffers.get(name)
             if x is None or tuple(x.shape) != shape or x.dtype != t or not x.is_contiguous():
                 _refuse(f"buffers[{name!r}] is a contiguous {t} tensor of {shape}")
-        self.k, self.v, self.bounds = buffers["k"], buffers["v"], buffers["bounds"]
-        self.bound_codes, self.bound_scale = buffers["bound_codes"], buffers["bound_scale"]
-        self.k_scale, self.v_scale = (buffers["k_scale"], buffers["v_scale"]) if kind != "same" else (None, None)
+        self._held = {n: buffers[n] for n in want}
         if not self.k.is_cuda or any(buffers[n].device != self.k.device for n in want):
             _refuse("the buffers of a cache are on one CUDA device")
         self.device = self.k.device
@@ -86,6 +85,9 @@ class KvCache:
         self._empty_like, self._contiguous = torch.empty_like, torch.contiguous_format
         self._get_stream, self._work_sizes = torch._C._cuda_getCurrentRawStream, {}
         self._add, self._vectors, self._search, self._attend = L.fv_kv_add_dev, L.fv_kv_vectors_dev, L.fv_kv_search_dev, L.fv_kv_attend_dev
+
+    k, v, bounds, bound_codes, bound_scale, k_scale, v_scale = (
+        property(lambda self, name=name: self._held.get(name)) for name in ("k", "v", "bounds", "bound_codes", "bound_scale", "k_scale", "v_scale"))
 
     # ---- the batch and the rows of a call
     def _batch(self, table, lens, cu, rows: int):

@@ -82,3 +82,20 @@ def test_lengths_below_zero_are_sequences_without_rows(kind, new, blocks):
             if lists is None:  # the work may be cut in other places: weights and results are rounded twice on both sides, half a step of bf16 each
                 assert (got[new:].float() - want[1].float()).abs().max() <= 4 * 2.0**-8 * want[1].float().abs().max()
                 assert (lse[new:] - want[2]).abs().max() <= 2.0**-12
+
+
+@pytest.mark.parametrize("kind", ["same", "e4m3"])
+def test_the_tensors_of_a_cache_stay(kind):
+    """Another tensor in place of one that every call's address is from would leave the calls with memory that is freed."""
+    import ferrolm_b200 as fv
+
+    c = fv.KvCache(3, 2, 64, page_size=16, kind=kind)
+    for name in ("k", "v", "bounds", "bound_codes", "bound_scale", "k_scale", "v_scale"):
+        x = getattr(c, name)
+        assert (x is None) == (kind == "same" and name.endswith("_scale") and name != "bound_scale")
+        with pytest.raises(AttributeError):
+            setattr(c, name, None if x is None else x.clone())
+        assert getattr(c, name) is x
+    pool = {n: getattr(c, n) for n in ("k", "v", "bounds", "bound_codes", "bound_scale", "k_scale", "v_scale")}
+    again = fv.KvCache(3, 2, 64, page_size=16, kind=kind, buffers=pool)
+    assert all(getattr(again, n) is x for n, x in pool.items())
