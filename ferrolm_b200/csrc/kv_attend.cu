@@ -29,17 +29,38 @@ namespace fv {
 int kv_prompt_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a);  // kv_prompt.cu
 bool kv_prompt_fits(const fv_kv_batch* b, size_t group, bool lists, size_t k);
 
-// The work is cut into equal parts, for at most so many warps, where there are fewer tasks than CTAs that the GPU holds and each
-// has enough pieces of 16 rows.  Else a CTA works on each task.  8 key heads of 4 queries, int8, both ways (us, parts first):
-//   pieces    16      40      80      192
-//   64 tasks  10/7.3  11/11   14/17   20/34
-//   320       17/14   24/23   35/39   61/77
-//   512       19/16   32/28   49/46   89/91
-// In 8 bits long lists are worth it up to twice as many tasks: 64 rows of 8 key heads over 192 pieces 93 us in parts, 99 by tasks;
-// in 16 bits, where the copies leave the time, 148 and 126.
-enum { KV_PARTS_TASKS = 400, KV_PARTS_PIECES = 64, KV_PARTS_TASKS_LONG = 1024, KV_PARTS_PIECES_LONG = 192, KV_PARTS_WARPS = 160 * 16 };
-static bool in_parts(int kind, size_t tasks, size_t pieces) {
-  return (tasks < KV_PARTS_TASKS && pieces >= KV_PARTS_PIECES) || (kind != FV_KV_SAME && tasks <= KV_PARTS_TASKS_LONG && pieces >= KV_PARTS_PIECES_LONG);
+// A CTA works on each task (a row and key head), or the work of all is cut into equal parts for the warps that the GPU holds, whose
+// shares are then joined.  Which of them: lengths are on the device, so from the most pieces of 16 rows that a task can have.  Both
+// sides, 16 to 1024 tasks of 32 to 768 pieces with caches cold, 8 key heads of 4 queries in dim 128, us by tasks / in parts:
+//   whole sequences of 5/16 to 16/16 of the table      lists of blocks: all tasks the same
+//   int8, pieces  64         128        384            64         128        384
+//   64 tasks      14.5/11.7  23.6/16.1  61.5/26.1      15.2/13.1  24.6/17.7  63.7/33.1
+//   248 tasks     20.3/21.5  33.1/30.8  83.6/62.3      21.6/26.1  34.5/39.0  87.1/84.1
+//   304 tasks     25.7/25.2  40.4/36.6  99.7/74.7      37.5/34.8  56.4/48.2  143/101
+//   512 tasks     34.9/34.3  56.2/51.4  142/114        41.8/44.5  66.2/66.9  178/170
+//   1024 tasks    57.1/57.9  92.1/89.2  236/215        70.6/73.7  116/120    346/344
+//   bf16
+//   64 tasks      15.6/12.7  25.6/17.1  66.4/33.6      16.5/14.5  27.2/20.9  69.1/45.8
+//   248 tasks     22.4/25.5  39.7/41.1  106/97.8       28.9/35.4  49.2/56.5  130/139
+//   304 tasks     28.8/31.4  48.2/49.7  123/119        49.9/44.9  77.6/67.8  197/169
+//   512 tasks     38.9/45.6  69.1/75.4  190/191        53.8/64.8  86.9/105   247/283
+// Sequences differ, and a CTA by itself waits for the longest: parts pay from a length on that grows with what is to be joined, and
+// sooner in 8 bits, where bytes are not what bounds a task.  Lists are alike, so tasks go in waves, and parts pay where the places that the
+// last wave leaves empty would have taken more pieces than cutting costs, about 32 of a place and one for every 16 tasks; not
+// where a wave is full to more than 7/8 (e4m3 loses up to 5% there where int8 gains as much).  In 16 bits with one tile of queries fewer
+// CTAs saturate the bytes too: there only what leaves a third of the SMs without one, half of them where rows are 64 long, and a second
+// wave full to at most 0.6 in dim 128, where an SM holds two CTAs (of three or four the others cover for those that are gone).
+// Over 24 shapes and 4000 such points these lines are 0.5% from the better side on average, within 5% for 96% of them, 21% at worst.
+enum { KV_PARTS_TASKS = 1024, KV_PARTS_WARPS = 160 * 16, KV_SMS = 148 };
+constexpr int kv_ctas_an_sm(int kind, int dim) { return dim == 64 ? 4 : dim == 96 && kind == FV_KV_SAME ? 3 : 2; }
+static bool in_parts(int kind, int dim, int group, bool lists, size_t tasks, size_t pieces) {
+  if (tasks == 0 || tasks > KV_PARTS_TASKS) return false;
+  if (!lists) return pieces >= (kind != FV_KV_SAME ? 48 + tasks / 16 : 32 + tasks / 2);
+  const size_t places = size_t(KV_SMS) * kv_ctas_an_sm(kind, dim), waves = (tasks + places - 1) / places, all = waves * places;
+  if ((all - tasks) * pieces < (32 + tasks / 16) * places) return false;
+  if (kind != FV_KV_SAME || group > 8) return 8 * tasks <= 7 * all;
+  if (waves == 1) return tasks <= size_t(KV_SMS * 2 / 3) * (dim == 64 ? 2 : 1);
+  return dim == 128 && 5 * tasks <= 3 * all;
 }
 
 namespace {
@@ -750,8 +771,9 @@ int token_launch(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const Kv
   const size_t ring = size_t(W) * S::DEPTH * S::SIZE, shares = size_t(W) * H::FLOATS * 4;
   const KvBatch m = kv_batch(kv, b);
   const size_t pieces = (a.blocks ? size_t(a.k) : b->table_width) * (kv->page_size / 16);  // of a task, at most
-  if (work && in_parts(KIND, tasks, pieces) && pieces * tasks <= size_t(1) << 30) {
-    const size_t smem = ring + 4 * (b->rows + 1), most = ring + 4 * (KV_PARTS_TASKS_LONG + 1);
+  static_assert(228 * 1024 / (W * S::DEPTH * S::SIZE + 1024) == kv_ctas_an_sm(KIND, D), "the rule counts the CTAs that an SM holds");
+  if (work && in_parts(KIND, D, a.group, a.blocks != nullptr, tasks, pieces) && pieces * tasks <= size_t(1) << 30) {
+    const size_t smem = ring + 4 * (b->rows + 1), most = ring + 4 * (KV_PARTS_TASKS + 1);
     Parts p{int(b->rows), int(tasks_a_row), S::LEAST, 0, static_cast<float*>(work)};
     FV_TRY((kv_allow_smem<kv_parts_kernel<T, KIND, D, NT>>(kv->device, most)));
     FV_TRY((parts_warps<T, KIND, D, NT>(kv->device, ring + 1024, &p.warps)));
@@ -799,10 +821,11 @@ int kv_token_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const
 }  // namespace fv
 
 extern "C" size_t fv_kv_attend_work(const fv_kv* kv, const fv_kv_batch* batch, size_t group) {
-  if (!kv || !batch || group == 0 || group > 128 || batch->rows > fv::KV_PARTS_TASKS_LONG) return 0;
+  if (!kv || !batch || group == 0 || group > 128 || batch->rows > fv::KV_PARTS_TASKS) return 0;
   if (fv::is_prompt(batch, group, false, 0)) return 0;  // with lists too: a shorter union fits where the whole table does
   const size_t cols = group <= 8 ? 8 : 16, tasks = batch->rows * kv->heads * ((group + cols - 1) / cols), pieces = batch->table_width * (kv->page_size / 16);
-  return tasks && fv::in_parts(kv->kind, tasks, pieces) ? (tasks + fv::KV_PARTS_WARPS) * cols * (kv->dim + 2) * 4 : 0;
+  const bool parts = fv::in_parts(kv->kind, int(kv->dim), int(group), false, tasks, pieces) || fv::in_parts(kv->kind, int(kv->dim), int(group), true, tasks, pieces);
+  return parts ? (tasks + fv::KV_PARTS_WARPS) * cols * (kv->dim + 2) * 4 : 0;
 }
 
 extern "C" int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* q, size_t q_row, size_t q_head,
