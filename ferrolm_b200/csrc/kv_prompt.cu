@@ -22,7 +22,7 @@
 // exactly, on their way in; a key's scale multiplies its column of S, a value's its weight (kv_attend.cu), relative to a
 // power of two that follows the largest scale that the query itself has seen: what only the others of its tile see costs it no bits.
 // The tile's scales come relative to the same for all that the CTA's queries see, which mostly is the query's own power too; a warp
-// with a query for which it is not takes the scales as they are (int8, dense: 386 us with and without; e4m3, lists: 1182 us of 1164).
+// with a query for which it is not takes the scales as they are (as fast as one power for all: int8, dense 388 us, e4m3, lists 1160).
 #include <climits>
 
 #include "kv.cuh"
@@ -631,8 +631,9 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
     // (pv_done may lie one or two phases behind here, which its parity does not tell apart)
     if (on && tiles) on = __all_sync(FV_FULL, mbar_wait(&bars->all_done, 0u, abort, 0));
     tc_fence_after();
+    // two factors: their product can be too small for all of its bits where the scales are
     const float f = KIND != FV_KV_SAME ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
-    const float down = sum == 0.f ? 0.f : f / sum;
+    const float down = sum == 0.f ? 0.f : 1.f / sum;
     const size_t query = (size_t(row0 + tok) * a.heads + head) * a.group + h;
 #pragma unroll 1
     for (int c = 0; c < D; c += 32) {
@@ -642,7 +643,8 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
       uint4 w[4];
 #pragma unroll
       for (int z = 0; z < 16; ++z) {
-        const float u = __uint_as_float(o[2 * z]) * down, v = __uint_as_float(o[2 * z + 1]) * down;
+        float u = __uint_as_float(o[2 * z]) * down, v = __uint_as_float(o[2 * z + 1]) * down;
+        if constexpr (KIND != FV_KV_SAME) u *= f, v *= f;
         // a wait that ran out leaves no result: NaN
         reinterpret_cast<uint32_t*>(w)[z] = !on ? 0x7FFF7FFFu : sum == 0.f ? 0u : Pair<T>::from_float(u, v);
       }
