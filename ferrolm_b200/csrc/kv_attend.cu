@@ -12,14 +12,18 @@
 // hold some of each 16: loads are 16 bytes.  V's rows arrive a lane each and are paired by byte permutations, P^T comes from S^T by a
 // transposition in registers.
 //
-// 64 rows of 64 heads over 48 blocks of int8 (417 MB): 91 us, 4.6 TB/s, 0.70 of the copy rate; 32 whole sequences in bf16 (0.9 GB):
-// 162 us, 5.6 TB/s; 12 of 15k rows in e4m3 (271 MB): 61 us, 4.4 TB/s.  A warp's steps from keys to scores to weights depend on one
+// 64 rows of 64 heads over 48 blocks of int8 (417 MB): 93 us, 4.5 TB/s, 0.69 of the copy rate; 32 whole sequences in bf16 (0.9 GB):
+// 162 us, 5.6 TB/s; 12 of 15k rows in e4m3 (271 MB): 57 us, 4.8 TB/s.  A warp's steps from keys to scores to weights depend on one
 // another (about 1160 clocks a piece of bf16 when it is alone); in 8 bits the codes' way to fp16 adds to them.  One request's
-// 32 blocks take 12.4 us, most of it dependent loads: the list, the table, the rows, and the shares that are joined.
+// 32 blocks take 10.2 us in a graph, most of it dependent loads: the list, the table, the rows, and the shares that are joined.
 //
 // In 8 bits the codes are exact in fp16; a key's scale multiplies its score, a value's its weight, relative to the largest
-// power of two of a scale so far.  Weights are rounded to 16 bits for the second product: fp16 with 2^14 for 1, so that none
-// above 2^-28 loses bits, or two bf16 numbers (a weight and what its rounding left), which is as good; the loads leave the time.
+// power of two of a scale that the row has seen.  Weights are rounded to 16 bits for the second product: fp16 with 2^14 for 1, so that
+// none above 2^-28 loses bits, or two bf16 numbers (a weight and what its rounding left), which is as good; the loads leave the time.
+// In 8 bits what is rounded is the weight times its value's relative scale: no bits are lost above 2^-28 of that product, and
+// below it up to 2^-39 of the largest scale times the code, so a row whose scale is 2^20 below the largest one seen keeps all
+// bits for weights above 2^-8.  bf16 queries become fp16 there, times a power of two that brings the largest component to 2^13: a component
+// below 2^-27 of it loses bits, up to 2^-38 of it.  A second number would cost a second product; scores of keys in 8 bits are no better.
 #include <climits>
 
 #include "kv.cuh"

@@ -7,16 +7,21 @@
 //   P = 2^(scale S - max): a thread to a query, which has a whole row of S in its registers: no exchange between lanes
 //
 // Warps 0-3 turn S into P, warp 4 issues the products, two warps bring keys and four values, each two tiles ahead at most; S has
-// two places, so that the next one is worked out while this one becomes P.  P takes the place of its S.  Two CTAs share an SM: the
-// products of a tile take 256 clocks of it and its powers of two 512 (16 an SM and clock), while its threads' own chain of
-// steps, from S to P, takes about 1800 with another CTA beside it.  That chain, and the share of a tile that its rows do not
-// have in common, bounds it.
-//   4096 rows of 32 heads over all rows before them, bf16: 243 us, 565 TFLOP/s (0.34 of the measured rate); int8: 418 us
-//   1687 rows over 16 of up to 266 blocks each: 211 us; 59 blocks on average are in the union of 32 rows' lists
+// two places, so that the next one is worked out while this one becomes P.  P takes the place of its S.  Two CTAs share an SM.
+//   4096 rows of 32 heads over all rows before them, bf16: 239 us, 575 TFLOP/s (0.35 of the measured rate); int8: 388 us
+//   1687 rows over 16 of up to 266 blocks each: 208 us; 59 blocks on average are in the union of 32 rows' lists
+// Where the time of the first goes, by clocks read in the kernel (at 1.8 GHz, which made it 277 us): a tile takes a warp of the weights 2800,
+// with another CTA beside it.  1400 are from S to P, 350 to find the rows that it sees, 290 and 190 to load S and to store P, 150 to scale
+// O, and 460 are waits, 290 of them for S and 170 for the values; the products take 256, the powers of two 512 (16 an SM and clock).
+// A CTA begins in 7800 and ends in 3700, with 98000 between; and a place is empty for 65 of the 277 us: the longest CTAs come first within a
+// head, but one head comes after the other, so the last one's are late.  Over int8 a tile takes 4700, 2400 of them from S to P.  With
+// lists 2900 and 81 us of 234 without work: 432 CTAs go to 296 places.
 // Warps with tiles of their own for every 8 rows, on mma.sync, whose lists have 36 blocks in common but which has a quarter of the
 // rate, took 563 and 525 us.
 //
-// A maximum that grows by less than a factor of 2 (fp16) or 256 (bf16) is left as it was: the weights stay within their type, and
+// P is rounded to the values' type once, in bf16 to 2^-9 of each weight: the error of a result grows by a tenth of what its own
+// rounding leaves (0.0018 of it against 64 bits, 0.0017 with weights in 32), where a second number for the rest would be a second product.
+// A maximum that grows by less than a factor of 2 (fp16; 2^0.9 over 8 bits) or 256 (bf16) is left as it was: the weights stay within their type, and
 // O, in tensor memory, need not be scaled as often.  Values that are not finite would reach rows that do not see them as
 // 0 * inf: they are taken out on their way in, and added by the threads whose rows see them.  In 8 bits the codes become fp16,
 // exactly, on their way in; a key's scale multiplies its column of S, a value's its weight (kv_attend.cu), relative to a
@@ -273,7 +278,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
 
   // which rows of which sequence
   const int tc = KV_PROMPT_COLS / a.group;                // rows of a CTA
-  const int item = int(gridDim.x - 1 - blockIdx.x);       // the rows that see most come first
+  const int item = int(gridDim.x - 1 - blockIdx.x);       // of a head, the rows that see most come first
   const int b = m.cu ? kv_find(m, item, tc, 1) : item;
   const int r0 = m.cu_at(b), r1 = max(m.cu_at(b + 1), r0);
   const int row0 = m.cu ? r0 + (item - (r0 / tc + b)) * tc : r0, rows = min(tc, r1 - row0);

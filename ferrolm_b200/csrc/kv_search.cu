@@ -11,12 +11,17 @@
 //   p, n            sums of the positive and negative codes, then whole(127 p / max(|p|, |n|))
 //   score           float(p . hi + n . lo) * bound_scale
 //   result          the first `first` blocks, the last `recent` up to the query's own, then the largest scores (the lower
-//                   block of equals) up to k in all, in ascending order, -1 behind the last
+//                   block of equals) up to k in all, in ascending order, -1 behind the last; of more than k forced ones the lowest
 //
 // The bounds are 2 dim + 4 bytes for a block, so a token's search is a few dependent loads long (the table, the bounds, then the
-// threshold): 10.4 us for one request over 2032 blocks of 8 heads, 4.2 MB, in clusters of 8 (28.7 without); 12.5 us for 48
-// requests.  A prompt's search is bound by what each row does after the products: 92 us for 3.2k rows of 8 heads over up to
-// 512 blocks, about 800 instructions a warp for a row's codes, 1000 for its threshold and list.
+// threshold): 8.2 us in a graph for one request over 2032 blocks of 8 heads, 4.2 MB, in clusters of 8, and 11.3 us for 48 requests; a
+// call's steps on the host make that 10.5 (28.7 without clusters) and 12.3.  A prompt's search is bound by what each row does
+// besides its products: 89 us for 3.2k rows of 8 heads over up to 512 blocks, about 2400 instructions a warp for a row and head.
+//
+// The score is no bound itself: queries, their sums and bounds are rounded to nearest, with one scale for a group's queries, so
+// that a head below 1/254 of the largest one counts as nothing, and a block's score may miss the unrounded one by about half a
+// step of each (tests/test_gpu_kv_scores.py works it out).  Of the blocks that are not forced 97 to 99 in 100 are the same as
+// without any rounding, on keys with channels that stand out.
 #include <climits>
 
 #include <cooperative_groups.h>

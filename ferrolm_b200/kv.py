@@ -13,7 +13,7 @@ before.  Positions below 0 or in a block that the table has no column for, and b
 cache (-1, say), are skipped: nothing is written or read there and nothing attends to them.
 
 The calls run on the current torch stream of the cache's device and do not wait for it; they can be captured into a CUDA
-graph.  Tensors are used on that stream only.  They know no gradients.
+graph.  Tensors are used on that stream only.  They know no gradients.  A length below 0 counts as 0.
 """
 from __future__ import annotations
 
@@ -170,9 +170,13 @@ class KvCache:
 
         `q` is (rows, heads * group, dim), the query heads of a key head one behind the other.  A block's score is the sum
         over those heads of the largest inner product that the block's bounds allow, worked out in whole numbers, so that
-        it does not depend on how the work is cut; of equal scores the lower block is taken.  The first `first` blocks
-        and the last `recent` ones up to the query's own are always among the `k`, blocks behind the query's position and
-        blocks without a page never."""
+        it does not depend on how the work is cut; of equal scores the lower block is taken.  Queries (with one scale for a
+        key head's group) and bounds are rounded to 8 bits for that, to nearest: a score is close to the bound, not always
+        above it, and a head below 1/254 of its group's largest component counts as nothing.
+
+        The first `first` blocks and the last `recent` ones up to the query's own are among the `k` before any other; of more
+        than `k` such blocks the lowest are the result, and the query's own is not in it: `k` is to be at least
+        `first + recent`.  Blocks behind the query's position and blocks without a page are never among them."""
         q, qp, qr, qh, rows = self._rows(q, "q", 0)
         group = self._group(q)
         if first < 0 or recent < 0 or k < 1:
@@ -195,7 +199,11 @@ class KvCache:
         `blocks`: the blocks that each row and key head attends to, (rows, heads, k) int32 as `search_blocks` gives them;
         without it, all of them.  Entries that are no block the query can see, and entries not above all of those before
         them, are skipped.  A row with nothing to attend to gets zeros and -inf.  `scale` is dim ** -0.5 unless given.
-        `out`: the tensor to write to (with `return_lse` a pair)."""
+        `out`: the tensor to write to (with `return_lse` a pair).
+
+        Calls whose sequences bring more than four rows on average are worked on as prompts, others row by row (as is a
+        prompt whose table has more than about 16,400 columns); a long prompt is faster in a call of its own than among
+        many single rows."""
         q, qp, qr, qh, rows = self._rows(q, "q", 0)
         heads, group, at, k = q.shape[1], self._group(q), None, 0
         if blocks is not None:

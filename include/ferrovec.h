@@ -309,7 +309,7 @@ int fv_merge_topk_static_dev(int device, void* stream, const fv_neighbor* d_part
  * A batch: sequence b has its pages in table[b][0..table_width) and lens[b] rows, those of this call among them.  The call
  * is about its last n_b rows: row i of them stands at position lens[b] - n_b + i, and they are rows cu[b] .. cu[b+1] of the
  * call's tensors (cu: nseq + 1 ascending numbers from 0; NULL: one row each, rows = nseq).  Rows from cu[nseq] on are not
- * touched.  Positions below 0 or in a block from table_width on, and blocks whose table entry is not a page of the cache
+ * touched.  A length below 0 counts as 0; table_width * page_size is less than 2^31.  Positions below 0 or in a block from table_width on, and blocks whose table entry is not a page of the cache
  * (-1, say), are skipped: nothing is read or written there, and nothing attends to them.  A page that add writes to is one
  * block of one sequence of the call. */
 enum { FV_KV_BF16 = 0, FV_KV_FP16 = 1 };                 /* dtype */
@@ -349,9 +349,16 @@ int fv_kv_vectors_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, v
 /* For every row and key head the k blocks that promise its queries the largest inner products: out is [rows][heads][k], block
  * numbers (not pages) ascending, -1 behind the last.  q: [rows][heads * group][dim], query heads group*h .. group*h + group-1
  * belonging to key head h.  The score of a block is the sum over those heads of the largest inner product that its bounds
- * allow, in 8 bits: whole numbers, the same on every path; of equals the lower block is taken.  The first `first` blocks and
- * the last `recent` ones up to the query's own are always among the k.  Blocks behind the query's own position and blocks
- * without a page are never.  k and group are at most 4096 and 128, table_width at most 50000. */
+ * allow, in 8 bits: whole numbers, the same on every path; of equals the lower block is taken.  Queries (with one scale for the group)
+ * and bounds are rounded to nearest, so a score is close to the bound but none itself, and a head below 1/254 of its group's largest
+ * component counts as nothing.  The first `first` blocks and the last `recent` ones up to the query's own are among the k before any
+ * other; if these are more than k, the lowest of them are the result, and the query's own block is not in it.  Blocks behind the
+ * query's own position and blocks without a page are never.  k and group are at most 4096 and 128, table_width at most 50000.
+ *
+ * A call works on prompts (rows that share what is read) where its sequences bring more than four rows on average, rows of padding
+ * among them, and on single rows otherwise; both give the same blocks.  The same holds for fv_kv_attend_dev (unless a prompt's table has
+ * more than about 16,400 columns, or its lists that many entries in common: then rows by themselves).  A batch of single rows and a long
+ * prompt is as right as two calls, and slower. */
 enum { FV_KV_MAX_BLOCKS = 4096 };
 int fv_kv_search_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* q, size_t q_row, size_t q_head,
                      size_t group, size_t k, size_t first, size_t recent, int32_t* out);
@@ -360,7 +367,9 @@ int fv_kv_search_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, co
  * blocks that each row and key head attends to, as fv_kv_search_dev gives them (ascending; an entry that is no block the
  * query can see, or is not above all before it that are, is skipped), or NULL for all of them.  A row with nothing to
  * attend to gets zeros and -inf.  Scores, maxima and sums are 32-bit floats; weights are rounded to 16 bits before they meet the
- * values.  The waits inside the kernels are bounded (about 2 s); results of one that ran out are NaN. */
+ * values.  Over 8 bits a weight is rounded together with its value's scale, relative to the largest scale among the rows that the
+ * query sees, which costs a result up to 2^-38 of that scale times the largest code for each row, and bf16 queries become fp16, which
+ * costs a component up to 2^-38 of the query's largest.  The waits inside the kernels are bounded (about 2 s); results of one that ran out are NaN. */
 int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* q, size_t q_row, size_t q_head,
                      size_t group, const int32_t* blocks, size_t k, float scale, void* out, float* lse, void* work, size_t work_bytes);
 /* Bytes of device memory that fv_kv_attend_dev wants as `work` (on 16 bytes, the caller's, used until the call's kernels are
