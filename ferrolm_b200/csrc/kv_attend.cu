@@ -21,9 +21,9 @@
 // power of two of a scale that the row has seen.  Weights are rounded to 16 bits for the second product: fp16 with 2^14 for 1, so that
 // none above 2^-28 loses bits, or two bf16 numbers (a weight and what its rounding left), which is as good; the loads leave the time.
 // In 8 bits what is rounded is the weight times its value's relative scale: no bits are lost above 2^-28 of that product, and
-// below it up to 2^-39 of the largest scale times the code, so a row whose scale is 2^20 below the largest one seen keeps all
+// below it up to 2^-38 of the largest scale times the code, so a row whose scale is 2^20 below the largest one seen keeps all
 // bits for weights above 2^-8.  bf16 queries become fp16 there, times a power of two that brings the largest component to 2^13: a component
-// below 2^-27 of it loses bits, up to 2^-38 of it.  A second number would cost a second product; scores of keys in 8 bits are no better.
+// below 2^-30 of it loses bits, up to 2^-38 of it.  A second number would cost a second product; scores of keys in 8 bits are no better.
 #include <climits>
 
 #include "kv.cuh"
