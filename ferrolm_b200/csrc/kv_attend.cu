@@ -49,7 +49,8 @@ bool kv_prompt_fits(const fv_kv_batch* b, size_t group, bool lists, size_t k);
 //   304 tasks     28.8/31.4  48.2/49.7  123/119        49.9/44.9  77.6/67.8  197/169
 //   512 tasks     38.9/45.6  69.1/75.4  190/191        53.8/64.8  86.9/105   247/283
 // Sequences differ, and a CTA by itself waits for the longest: parts pay from a length on that grows with what is to be joined, and
-// sooner in 8 bits, where bytes are not what bounds a task.  Lists are alike, so tasks go in waves, and parts pay where the places that the
+// sooner in 8 bits, where bytes are not what bounds a task.  So do lists that reach over more than a quarter of the table: sequences that
+// are shorter have fewer blocks than k.  Other lists are alike, so tasks go in waves, and parts pay where the places that the
 // last wave leaves empty would have taken more pieces than cutting costs, about 32 of a place and one for every 16 tasks; not
 // where a wave is full to more than 7/8 (e4m3 loses up to 5% there where int8 gains as much).  In 16 bits with one tile of queries fewer
 // CTAs saturate the bytes too: there only what leaves a third of the SMs without one, half of them where rows are 64 long, and a second
@@ -57,9 +58,9 @@ bool kv_prompt_fits(const fv_kv_batch* b, size_t group, bool lists, size_t k);
 // Over 24 shapes and 4000 such points these lines are 0.5% from the better side on average, within 5% for 96% of them, 21% at worst.
 enum { KV_PARTS_TASKS = 1024, KV_PARTS_WARPS = 160 * 16, KV_SMS = 148 };
 constexpr int kv_ctas_an_sm(int kind, int dim) { return dim == 64 ? 4 : dim == 96 && kind == FV_KV_SAME ? 3 : 2; }
-static bool in_parts(int kind, int dim, int group, bool lists, size_t tasks, size_t pieces) {
+static bool in_parts(int kind, int dim, int group, bool alike, size_t tasks, size_t pieces) {
   if (tasks == 0 || tasks > KV_PARTS_TASKS) return false;
-  if (!lists) return pieces >= (kind != FV_KV_SAME ? 48 + tasks / 16 : 32 + tasks / 2);
+  if (!alike) return pieces >= (kind != FV_KV_SAME ? 48 + tasks / 16 : 32 + tasks / 2);
   const size_t places = size_t(KV_SMS) * kv_ctas_an_sm(kind, dim), waves = (tasks + places - 1) / places, all = waves * places;
   if ((all - tasks) * pieces < (32 + tasks / 16) * places) return false;
   if (kind != FV_KV_SAME || group > 8) return 8 * tasks <= 7 * all;
@@ -775,8 +776,9 @@ int token_launch(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const Kv
   const size_t ring = size_t(W) * S::DEPTH * S::SIZE, shares = size_t(W) * H::FLOATS * 4;
   const KvBatch m = kv_batch(kv, b);
   const size_t pieces = (a.blocks ? size_t(a.k) : b->table_width) * (kv->page_size / 16);  // of a task, at most
+  const bool alike = a.blocks && size_t(a.k) * 4 <= b->table_width;
   static_assert(228 * 1024 / (W * S::DEPTH * S::SIZE + 1024) == kv_ctas_an_sm(KIND, D), "the rule counts the CTAs that an SM holds");
-  if (work && in_parts(KIND, D, a.group, a.blocks != nullptr, tasks, pieces) && pieces * tasks <= size_t(1) << 30) {
+  if (work && in_parts(KIND, D, a.group, alike, tasks, pieces) && pieces * tasks <= size_t(1) << 30) {
     const size_t smem = ring + 4 * (b->rows + 1), most = ring + 4 * (KV_PARTS_TASKS + 1);
     Parts p{int(b->rows), int(tasks_a_row), S::LEAST, 0, static_cast<float*>(work)};
     FV_TRY((kv_allow_smem<kv_parts_kernel<T, KIND, D, NT>>(kv->device, most)));
