@@ -99,3 +99,81 @@ def test_the_tensors_of_a_cache_stay(kind):
     pool = {n: getattr(c, n) for n in ("k", "v", "bounds", "bound_codes", "bound_scale", "k_scale", "v_scale")}
     again = fv.KvCache(3, 2, 64, page_size=16, kind=kind, buffers=pool)
     assert all(getattr(again, n) is x for n, x in pool.items())
+
+
+@pytest.mark.parametrize("kind,dtype", [("same", BF), ("same", torch.float16), ("int8", BF), ("e4m3", torch.float16)])
+@pytest.mark.parametrize("group", [100, 128])
+def test_the_largest_groups(kind, dtype, group):
+    """One row to a tile of a prompt, several tiles of queries to a row by itself, and the largest sums of a search."""
+    from tests.test_gpu_kv_attend import check, lists, pair, queries
+    from tests.test_gpu_kv_search import check as check_search
+
+    heads, dim, page = 2, 64, 16
+    c, p = pair(30, heads, dim, page, dtype, kind)
+    table = torch.randperm(30, generator=torch.Generator().manual_seed(1))[:28].view(2, 14).to(torch.int32)
+    for news, lens in (([7, 6], [14 * page - 3, 40]), ([1, 1], [100, 9 * page])):
+        cu, n = i32([0, news[0], sum(news)]), sum(news)
+        q = queries(n, heads, group, dim, dtype, 3)
+        check(c, p, q, table, lens, cu, None)
+        check(c, p, q, table, lens, cu, lists(n, heads, 5, 9, 4))
+    x = torch.randint(-127, 128, p.bound_codes.shape, generator=torch.Generator().manual_seed(2))
+    p.bound_codes.copy_(x), c.bound_codes.copy_(x.to(torch.int8))
+    p.bound_scale.fill_(0.25), c.bound_scale.fill_(0.25)
+    q = torch.full((13, heads * group, dim), 3.0, dtype=dtype)  # all codes 127: sums of 127 * group
+    q[5:, ::2] = -3.0
+    q[9:, :, ::3] = 0.01
+    check_search(c, p, q, table, [14 * page - 3, 9 * page], 4, i32([0, 7, 13]))
+
+
+@pytest.mark.parametrize("kind", ["same", "int8"])
+@pytest.mark.parametrize("new", [1, 9])
+def test_nothing_to_look_at(kind, new):
+    """No column in the table, no page in the cache, no entry that is a page, no row that belongs to a sequence: zeros, -inf and -1 for rows
+    of sequences, and rows of none are left alone."""
+    import ferrolm_b200 as fv
+
+    heads, group, dim, page, B = 3, 4, 96, 32, 2
+    rows = torch.randn((B * new + 3, heads * (group + 2), dim), device="cuda").to(BF)
+    q, k, v = rows.split([heads * group, heads, heads], 1)
+    lens, cu, none = i32([500, 700]).cuda(), i32([0, new, 2 * new]).cuda(), i32([0, 0, 0]).cuda()
+    full = torch.arange(40, dtype=torch.int32, device="cuda").view(B, 20)
+    for pages, table, at in ((40, full[:, :0], cu), (0, full, cu), (40, torch.full_like(full, -1), cu), (40, full, none), (0, full[:, :0], none)):
+        c = fv.KvCache(pages, heads, dim, page_size=page, kind=kind)
+        c.add(k, v, table, lens, cu=at)
+        assert not c.k.any() and not c.bounds.any()
+        out = torch.full((2, len(q), heads, dim), 7.5, dtype=BF, device="cuda")
+        c.vectors(table, lens, cu=at, out=tuple(out.unbind(0)))
+        assert at is none or (out == 7.5).all()
+        found = torch.full((len(q), heads, 6), -9, dtype=torch.int32, device="cuda")
+        c.search_blocks(q, table, lens, 6, cu=at, out=found)
+        live = 0 if at is none else 2 * new
+        assert (found[:live] == -1).all() and (found[live:] == -9).all()
+        for lists in (None, torch.arange(6, dtype=torch.int32, device="cuda").expand(len(q), heads, 6).contiguous()):
+            y, lse = torch.full_like(q, 7.5).contiguous(), torch.full((len(q), heads * group), 7.5, device="cuda")
+            c.attend(q, table, lens, cu=at, blocks=lists, return_lse=True, out=(y, lse))
+            assert (y[:live] == 0).all() and (lse[:live] == -torch.inf).all() and (y[live:] == 7.5).all() and (lse[live:] == 7.5).all()
+
+
+@pytest.mark.parametrize("kind,dtype", [("same", BF), ("int8", torch.float16)])
+@pytest.mark.parametrize("piece", [50, 70])
+def test_single_rows_and_a_piece_of_a_prompt_in_one_call(kind, dtype, piece):
+    """20 sequences of a row each around one that brings 50 rows (all of them go by themselves) or 70 (all go as prompts)."""
+    from tests.test_gpu_kv_attend import check, lists, pair, queries
+    from tests.test_gpu_kv_search import check as check_search
+
+    heads, group, dim, page, B = 2, 4, 64, 16, 21
+    c, p = pair(B * 8, heads, dim, page, dtype, kind)
+    g = torch.Generator().manual_seed(piece)
+    table = torch.randperm(B * 8, generator=g).view(B, 8).to(torch.int32)
+    news = [1] * 9 + [piece] + [1] * 11
+    lens = [int(torch.randint(1, 8 * page, (1,), generator=g)) for _ in news]
+    lens[9], lens[3], lens[15] = 8 * page - 1, 1, 0
+    cu = i32([0] + torch.tensor(news).cumsum(0).tolist())
+    n = int(cu[-1])
+    q = queries(n, heads, group, dim, dtype, 3)
+    check(c, p, q, table, lens, cu, None)
+    check(c, p, q, table, lens, cu, lists(n, heads, 4, 8, 4))
+    x = torch.randint(-127, 128, p.bound_codes.shape, generator=g)
+    p.bound_codes.copy_(x), c.bound_codes.copy_(x.to(torch.int8))
+    p.bound_scale.fill_(0.25), c.bound_scale.fill_(0.25)
+    check_search(c, p, q, table, lens, 4, cu)
