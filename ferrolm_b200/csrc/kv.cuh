@@ -16,6 +16,9 @@ namespace fv {
 // host side
 int kv_check(const fv_kv* kv, const fv_kv_batch* batch, const char* who);  // kv_rows.cu
 inline bool kv_aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+// bytes of a row of a head, and of its scales
+inline size_t kv_row_bytes(const fv_kv* kv) { return kv->kind == FV_KV_SAME ? 2 * kv->dim : kv->kind == FV_KV_INT4X32 ? kv->dim / 2 : kv->dim; }
+inline size_t kv_scale_bytes(const fv_kv* kv) { return kv->kind == FV_KV_SAME ? 0 : kv->kind == FV_KV_INT4X32 ? kv->dim / 32 : 4; }
 
 // Returns fn<type, kind, dim>(...) for what the cache holds.  kv_check has looked at the three.
 #define FV_KV_DISPATCH(kv, fn, ...)                                                                                     \
@@ -27,7 +30,8 @@ inline bool kv_aligned(const void* p, size_t to) { return (reinterpret_cast<uint
   {                                                                                 \
     if (_k == FV_KV_SAME) FV_KV_DIM_(T, FV_KV_SAME, fn, __VA_ARGS__)                \
     else if (_k == FV_KV_INT8) FV_KV_DIM_(T, FV_KV_INT8, fn, __VA_ARGS__)           \
-    else FV_KV_DIM_(T, FV_KV_E4M3, fn, __VA_ARGS__)                                 \
+    else if (_k == FV_KV_E4M3) FV_KV_DIM_(T, FV_KV_E4M3, fn, __VA_ARGS__)           \
+    else FV_KV_DIM_(T, FV_KV_INT4X32, fn, __VA_ARGS__)                              \
   }
 #define FV_KV_DIM_(T, K, fn, ...)                      \
   {                                                    \
@@ -184,6 +188,47 @@ struct Eight<FV_KV_E4M3> {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"(uint16_t(w >> 16)));
     const float2 x = Pair<__half>::to_float(a), z = Pair<__half>::to_float(b);
     y[0] = x.x, y[1] = x.y, y[2] = z.x, y[3] = z.y;
+  }
+};
+
+// ---------------------------------------------------------------------------------------------
+// 4-bit values.  A group of 32 neighbouring components has a scale of 5 exponent and 3 mantissa bits without a sign, fp16's upper byte
+// moved down by one bit, so fp16 = byte << 7: the smallest one that 7 times is not below any component, at most 9216 (7 times it is
+// in fp16's range).  code = rn(x / scale) + 8, from 1 to 15.  scale * (code - 8) has seven significant bits at most and no bit below 2^-17: it is
+// exact in fp16, and in bf16.  A quotient of 11 and 4 bits is the border of two codes exactly or further from it than half a
+// step of 32 bits, as is a seventh of 11 bits from a scale.
+// A row is 8 * groups pieces of 16 bits, four neighbouring components each, the lowest in the lowest bits: first the groups' first
+// pieces, then their second ones, and so on.  A quarter of a row has eight neighbours of every group that way, an eighth has four.
+struct Four {
+  static constexpr float LARGEST = 9216.f;
+  static constexpr uint32_t NAN_SCALE = 255;
+  static __device__ __forceinline__ uint32_t scale_of(float most) {  // its byte; `most` is finite
+    const float t = __fdiv_rn(most, 7.f);
+    if (t < 0x1p-14f) return uint32_t(ceilf(t * 0x1p17f));
+    return (min(__float_as_uint(t) + 0xFFFFFu, __float_as_uint(LARGEST)) >> 20) - ((127 - 15) << 3);
+  }
+  static __device__ __forceinline__ float value(uint32_t byte) { return __half2float(__ushort_as_half(uint16_t(byte << 7))); }
+  // eight codes of neighbouring components, the first in the lowest bits, from values of at most 7 scales; inv = 1 / scale
+  static __device__ __forceinline__ uint32_t pack(const float* x, float scale, float inv) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= uint32_t(kv_whole(x[i], scale, inv) + 8) << (4 * i);
+    return w;
+  }
+  // the eight codes of group g in the NG words of a quarter of a row
+  template <int NG>
+  static __device__ __forceinline__ uint32_t group(const uint32_t* w, int g) {
+    return __byte_perm(w[g / 2], w[(NG + g) / 2], (g & 1 ? 0x32 : 0x10) | ((NG + g) & 1 ? 0x7600 : 0x5400));
+  }
+  // Eight codes to the pairs (0, 4), (1, 5), (2, 6), (3, 7) of fp16, exactly: a code is added to 1024, or 16 times it to 1024, by its place.
+  static __device__ __forceinline__ void halves(uint32_t w, uint32_t* to) {
+    const __half2 low = __half2half2(__ushort_as_half(0x6408)), high = __half2half2(__ushort_as_half(0x5480));  // 1032, 72
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t y = i ? w >> 8 : w, x0 = (y & 0x000F000Fu) | 0x64006400u, x1 = (y & 0x00F000F0u) | 0x54005400u;
+      const __half2 u = __hsub2(*reinterpret_cast<const __half2*>(&x0), low), v = __hsub2(*reinterpret_cast<const __half2*>(&x1), high);
+      to[2 * i] = *reinterpret_cast<const uint32_t*>(&u), to[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&v);
+    }
   }
 };
 

@@ -57,7 +57,7 @@ bool kv_prompt_fits(const fv_kv_batch* b, size_t group, bool lists, size_t k);
 // wave full to at most 0.6 in dim 128, where an SM holds two CTAs (of three or four the others cover for those that are gone).
 // Over 24 shapes and 4000 such points these lines are 0.5% from the better side on average, within 5% for 96% of them, 21% at worst.
 enum { KV_PARTS_TASKS = 1024, KV_PARTS_WARPS = 160 * 16, KV_SMS = 148 };
-constexpr int kv_ctas_an_sm(int kind, int dim) { return dim == 64 ? 4 : dim == 96 && kind == FV_KV_SAME ? 3 : 2; }
+constexpr int kv_ctas_an_sm(int kind, int dim) { return kind == FV_KV_INT4X32 ? 4 : dim == 64 ? 4 : dim == 96 && kind == FV_KV_SAME ? 3 : 2; }
 static bool in_parts(int kind, int dim, int group, bool alike, size_t tasks, size_t pieces) {
   if (tasks == 0 || tasks > KV_PARTS_TASKS) return false;
   if (!alike) return pieces >= (kind != FV_KV_SAME ? 48 + tasks / 16 : 32 + tasks / 2);
@@ -160,12 +160,62 @@ struct Stage {
   static __device__ __forceinline__ int seen(const unsigned char* s) { return *reinterpret_cast<const int*>(s + 2 * 16 * ROW + SCALES); }
 };
 
+// The same in 4 bits.  A row is a quarter of 16 bits' bytes, so a lane takes a quarter of a key, eight components of each of NG groups,
+// and an eighth of a value, four of each, in one piece where NG is even.  32-byte pieces of values change places by
+// the row's number, where rows of 16 bytes' lanes would meet in the same banks.
+template <int D>
+struct Stage<FV_KV_INT4X32, D> {
+  static constexpr int NG = D / 32, ROW = D / 2, SCALE = 16 * NG;     // SCALE: bytes of 16 rows' scales
+  static constexpr int PIECE = 2 * 16 * ROW + 2 * SCALE + 16;          // keys, values, scales, how many of the rows are seen
+  static constexpr int PIECES = 2;
+  static constexpr int SIZE = PIECES * PIECE;
+  static constexpr int LEAST = 4 / PIECES;
+  static constexpr int DEPTH = 13 * 1024 / SIZE < 2 ? 2 : 13 * 1024 / SIZE > 6 ? 6 : 13 * 1024 / SIZE;
+
+  static __device__ __forceinline__ int value_at(int e, int g) { return 32 * (e >> 2) + 4 * g + (e & 3); }
+  static __device__ __forceinline__ int value_byte(int r, int at) {
+    if (ROW == 64) return (r >> 1) * 128 + ((((r & 1) * 2 + (at >> 5)) ^ (r >> 1 & 3)) << 5) + (at & 31);
+    if (ROW == 32) return (r >> 1) * 64 + (((r ^ r >> 2) & 1) << 5) + at;
+    return r * ROW + at;
+  }
+  static __device__ __forceinline__ void fill(unsigned char* s, const KvAttend& a, int page, int head, int page_shift, int slot, int seen, int lane) {
+    if (lane == 0) *reinterpret_cast<int*>(s + 2 * 16 * ROW + 2 * SCALE) = min(seen, 16);
+    if (seen <= 0) return;
+    const size_t at = ((size_t(page) * a.heads + head) << page_shift) + slot;
+    const unsigned char *kr = a.kp + at * ROW, *vr = a.vp + at * ROW;
+    const uint32_t to = uint32_t(__cvta_generic_to_shared(s));
+#pragma unroll
+    for (int i = 0; i < (ROW + 31) / 32; ++i) {
+      const int n = (lane + 32 * i) * 16, r = n / ROW;
+      if (ROW % 32 && n >= 16 * ROW) continue;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + n), "l"(kr + n));
+      // zeros in place of values that are not seen
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 16 * ROW + value_byte(r, n - r * ROW)), "l"(vr + n), "r"(r < seen ? 16 : 0));
+    }
+    if (lane < 2 * NG) {
+      const bool values = lane >= NG;
+      const int n = (values ? lane - NG : lane) * 16;
+      const unsigned char* from = reinterpret_cast<const unsigned char*>(values ? a.v_scale : a.k_scale) + at * NG + n;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 2 * 16 * ROW + lane * 16), "l"(from), "r"(min(max(seen * NG - n, 0), 16)));
+    }
+  }
+  static __device__ __forceinline__ int seen(const unsigned char* s) { return *reinterpret_cast<const int*>(s + 2 * 16 * ROW + 2 * SCALE); }
+  // The scales of a row, a byte each, as fp16: groups 0 and 2, then 1 and 3.
+  static __device__ __forceinline__ void scales(const unsigned char* s, int r, uint32_t* to) {
+    uint32_t w;
+    if constexpr (NG == 4) w = *reinterpret_cast<const uint32_t*>(s + 4 * r);
+    else if constexpr (NG == 2) w = *reinterpret_cast<const uint16_t*>(s + 2 * r);
+    else w = s[3 * r] | uint32_t(s[3 * r + 1]) << 8 | uint32_t(s[3 * r + 2]) << 16;
+    to[0] = (w & 0x00FF00FFu) << 7, to[1] = (w & 0xFF00FF00u) >> 1;
+  }
+};
+
 // A warp's share of a row's attention: NT tiles of 8 queries.  A lane's queries are 8 x + 2 t and the next one.
 template <class T, int KIND, int D, int NT>
 struct Share {
   using M = typename std::conditional<KIND == FV_KV_SAME, T, __half>::type;
   using L = Stage<KIND, D>;
-  static constexpr bool TWO = std::is_same<M, __nv_bfloat16>::value;
+  static constexpr bool TWO = std::is_same<M, __nv_bfloat16>::value, FOUR = KIND == FV_KV_INT4X32, SCALED = KIND != FV_KV_SAME && !FOUR;
   static constexpr float ONE = TWO ? 0.f : 14.f;  // log2 of what stands for a weight of 1
   uint32_t q[D / 16][NT][2];
   float by[NT][2];  // scale of a lane's queries
@@ -182,8 +232,18 @@ struct Share {
       float most = 0.f;
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
-        w[s][0] = w[s][1] = 0u;
-        if (on) load_words<2>(w[s], src + 2 * L::key_at(s, t));
+        if (!FOUR || s % 2 == 0) w[s][0] = w[s][1] = 0u;
+        if (FOUR && s % 2 == 0) w[s + 1][0] = w[s + 1][1] = 0u;
+        if constexpr (FOUR) {  // of eight neighbouring components two steps take the pairs (0, 4), (1, 5) and (2, 6), (3, 7)
+          if (on && s % 2 == 0) {
+            uint32_t e[4];
+            load_words<4>(e, src + 2 * (16 * s + 8 * t));
+            w[s][0] = __byte_perm(e[0], e[2], 0x5410), w[s][1] = __byte_perm(e[0], e[2], 0x7632);
+            w[s + 1][0] = __byte_perm(e[1], e[3], 0x5410), w[s + 1][1] = __byte_perm(e[1], e[3], 0x7632);
+          }
+        } else {
+          if (on) load_words<2>(w[s], src + 2 * L::key_at(s, t));
+        }
         if constexpr (!std::is_same<M, T>::value) {
           const float2 u = Pair<T>::to_float(w[s][0]), v = Pair<T>::to_float(w[s][1]);
           most = fmaxf(most, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(v.x), fabsf(v.y))));
@@ -221,6 +281,135 @@ struct Share {
   }
 
   __device__ __forceinline__ void take(const unsigned char* stage, int g, int t) {
+    if constexpr (FOUR) take_four(stage, g, t);
+    else take_rows(stage, g, t);
+  }
+
+  // 4 bits: codes are exact in fp16.  A key's scales multiply the sums over their groups; a value is multiplied by its scale, exactly, before
+  // its product.
+  __device__ __forceinline__ void take_four(const unsigned char* stage, int g, int t) {
+    constexpr int P = L::PIECES, NG = D / 32;
+    int visible[P], any = 0;
+#pragma unroll
+    for (int h = 0; h < P; ++h) visible[h] = L::seen(stage + h * L::PIECE), any = max(any, visible[h]);
+    if (any <= 0) return;
+    float s[P][NT][4];
+#pragma unroll
+    for (int h = 0; h < P; ++h) {
+      const unsigned char* const keys = stage + h * L::PIECE;
+      uint32_t k[2][NG], sc[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const unsigned char* from = keys + (g + 8 * i) * L::ROW + t * 4 * NG;
+        if constexpr (NG == 3) load_words<1>(k[i], from), load_words<1>(k[i] + 1, from + 4), load_words<1>(k[i] + 2, from + 8);
+        else load_words<NG>(k[i], from);
+        L::scales(keys + 2 * 16 * L::ROW, g + 8 * i, sc[i]);
+      }
+#pragma unroll
+      for (int x = 0; x < NT; ++x) s[h][x][0] = s[h][x][1] = s[h][x][2] = s[h][x][3] = 0.f;
+#pragma unroll
+      for (int y = 0; y < NG; ++y) {
+        uint32_t a[2][4];
+        Four::halves(Four::group<NG>(k[0], y), a[0]);
+        Four::halves(Four::group<NG>(k[1], y), a[1]);
+        float ks[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 f = Pair<__half>::to_float(sc[i][y & 1]);
+          ks[i] = y < 2 ? f.x : f.y;
+        }
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_16<M>(c, a[0][0], a[1][0], a[0][1], a[1][1], q[2 * y][x][0], q[2 * y][x][1]);
+          mma_16<M>(c, a[0][2], a[1][2], a[0][3], a[1][3], q[2 * y + 1][x][0], q[2 * y + 1][x][1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[h][x][i] = __fmaf_rn(c[i], ks[i >> 1], s[h][x][i]);
+        }
+      }
+    }
+    bool moved = false;
+    float to[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+#pragma unroll
+      for (int h = 0; h < P; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[h][x][i] = g + (i & 2) * 4 < visible[h] ? s[h][x][i] * by[x][i & 1] : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        to[x][i] = fmaxf(fmaxf(s[0][x][i], s[0][x][i + 2]), fmaxf(s[P - 1][x][i], s[P - 1][x][i + 2]));
+        moved = moved || to[x][i] > m[x][i];
+      }
+    }
+    if (__any_sync(FV_FULL, moved)) {  // seldom, after the first pieces
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float y = fmaxf(m[x][i], to[x][i]);
+          y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 4));
+          y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 8));
+          y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 16));
+          const float down = y > m[x][i] ? exp2_of(m[x][i] - y) : 1.f;
+          m[x][i] = y;
+          l[x][i] *= down;
+#pragma unroll
+          for (int u = 0; u < D / 16; ++u) o[u][x][i] *= down, o[u][x][i + 2] *= down;
+        }
+    }
+    uint32_t b[P][NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int h = 0; h < P; ++h) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = exp2_of(s[h][x][i] - (m[x][i & 1] == -INFINITY ? 0.f : m[x][i & 1]) + ONE);
+          l[x][i & 1] += p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) b[h][x][i] = transposed(Pair<M>::from_float(p[2 * i], p[2 * i + 1]));
+      }
+#pragma unroll
+    for (int h = 0; h < P; ++h) {
+      if (visible[h] <= 0) continue;  // its values are anything
+      const unsigned char *const values = stage + h * L::PIECE + 16 * L::ROW, *const scales = stage + h * L::PIECE + 2 * 16 * L::ROW + L::SCALE;
+      uint32_t v[4][(NG + 1) / 2], sc[4][2];  // of rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9: four components of every group
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 2 * t + (i & 1) + (i & 2) * 4;
+        if constexpr (NG == 3) {
+          const uint16_t* from = reinterpret_cast<const uint16_t*>(values + L::value_byte(r, g * 6));
+          v[i][0] = from[0] | uint32_t(from[1]) << 16, v[i][1] = from[2];
+        } else {
+          load_words<NG / 2>(v[i], values + L::value_byte(r, g * 2 * NG));
+        }
+        L::scales(scales, r, sc[i]);
+      }
+#pragma unroll
+      for (int y = 0; y < NG; ++y) {
+        uint32_t a[2][4];  // [rows 2 t, or 2 t + 8, and the next one][component]
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          Four::halves(__byte_perm(v[2 * z][y / 2], v[2 * z + 1][y / 2], y & 1 ? 0x7632 : 0x5410), a[z]);
+          const uint32_t w = __byte_perm(sc[2 * z][y & 1], sc[2 * z + 1][y & 1], y < 2 ? 0x5410 : 0x7632);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const __half2 f = __hmul2(*reinterpret_cast<const __half2*>(&a[z][e]), *reinterpret_cast<const __half2*>(&w));
+            a[z][e] = *reinterpret_cast<const uint32_t*>(&f);
+          }
+        }
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+#pragma unroll
+          for (int x = 0; x < NT; ++x) mma_16<M>(o[2 * y + z][x], a[0][2 * z], a[0][2 * z + 1], a[1][2 * z], a[1][2 * z + 1], b[h][x][0], b[h][x][1]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void take_rows(const unsigned char* stage, int g, int t) {
     constexpr int P = L::PIECES;
     int visible[P], any = 0;
 #pragma unroll
@@ -366,7 +555,7 @@ struct Share {
   static constexpr int FLOATS = 8 * NT * (D + 2);
   __device__ __forceinline__ void store(float* to, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    const float f = KIND != FV_KV_SAME ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
+    const float f = SCALED ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
 #pragma unroll

@@ -43,6 +43,9 @@ enum { KV_PROMPT_COLS = 128, KV_PROMPT_THREADS = 384, KV_PROMPT_KEYS = 64, KV_PR
 enum { KV_PROMPT_REGS = 80, KV_PROMPT_REGS_MORE = 128, KV_PROMPT_REGS_LESS = 56 };
 static_assert(KV_PROMPT_REGS_MORE + 2 * KV_PROMPT_REGS_LESS <= 3 * KV_PROMPT_REGS, "more than a CTA starts with would never come");
 
+// Rows have one scale each, which multiplies scores and weights; in 4 bits the groups' scales go into the fp16 values.
+constexpr bool kv_scaled(int kind) { return kind == FV_KV_INT8 || kind == FV_KV_E4M3; }
+
 struct PromptBars {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done, all_done;
   uint32_t tmem;
@@ -58,7 +61,7 @@ struct Tile {
   static constexpr int STAGE = HALVES * HALF;            // keys or values of one tile
   static constexpr int Q_HALF = KV_PROMPT_COLS * 128;
   static constexpr int Q = HALVES * Q_HALF;
-  static constexpr int SCALES = KIND == FV_KV_SAME ? 0 : 2 * 3 * ROWS * 4;  // [stage][keys, values relative to the largest, values][ROWS]
+  static constexpr int SCALES = !kv_scaled(KIND) ? 0 : 2 * 3 * ROWS * 4;  // [stage][keys, values relative to the largest, values][ROWS]
   static constexpr int K_AT = Q, V_AT = Q + 2 * STAGE, SCALE_AT = Q + 4 * STAGE, BARS_AT = SCALE_AT + SCALES;
   static constexpr int LIST_AT = BARS_AT + (int(sizeof(PromptBars)) + 15) / 16 * 16;
   static constexpr int O_COL = 128;  // columns of tensor memory: S or P 0-63, 64-127, O from 128 on
@@ -196,6 +199,67 @@ struct Bring {
   }
 };
 
+// 4 bits: N threads bring a tile as fp16, code times scale, exactly.  A thread has a quarter of a row, eight neighbouring components of every
+// group, in the order 0 4 1 5 2 6 3 7 that the codes come apart in; queries and results are put into it and out of it again.
+// Eight lanes that store at one time have rows four apart, whose pieces lie in different banks.  VALUES: a group whose scale is no
+// number becomes zeros; whether there was one is returned.
+template <int D, int N, bool VALUES>
+struct BringFour {
+  using S = Tile<FV_KV_INT4X32, D>;
+  static constexpr int NG = D / 32, TIMES = 256 / N;
+  static __device__ __forceinline__ bool convert(const KvAttend& a, const KvBatch& m, const PromptWork& w, int i, unsigned char* to, int t) {
+    const unsigned char* const src = VALUES ? a.vp : a.kp;
+    const uint8_t* const scales = reinterpret_cast<const uint8_t*>(VALUES ? a.v_scale : a.k_scale);
+    const int quarter = t & 3, r16 = (t >> 5 & 1) * 8 + (t >> 2 & 1) * 4 + (t >> 3 & 3);  // row of the piece
+    uint32_t c[TIMES][NG], sc[TIMES];
+#pragma unroll
+    for (int x = 0; x < TIMES; ++x) {
+      const int p = x * (N / 64) + (t >> 6);
+      int begin = 0;
+      size_t at = 0;
+      sc[x] = 0u;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) c[x][g] = 0u;
+      if (!w.piece(a, m, 4 * i + p, begin, at) || begin + r16 > w.last) continue;  // zeros for rows that nobody sees
+      const unsigned char* from = src + (at + r16) * (D / 2) + quarter * (4 * NG);
+      const uint8_t* s = scales + (at + r16) * NG;
+      if constexpr (NG == 4) {
+        const uint4 y = __ldg(reinterpret_cast<const uint4*>(from));
+        c[x][0] = y.x, c[x][1] = y.y, c[x][2] = y.z, c[x][3] = y.w;
+        sc[x] = __ldg(reinterpret_cast<const uint32_t*>(s));
+      } else if constexpr (NG == 2) {
+        const uint2 y = __ldg(reinterpret_cast<const uint2*>(from));
+        c[x][0] = y.x, c[x][1] = y.y;
+        sc[x] = __ldg(reinterpret_cast<const uint16_t*>(s));
+      } else {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) c[x][g] = __ldg(reinterpret_cast<const uint32_t*>(from) + g), sc[x] |= uint32_t(__ldg(s + g)) << (8 * g);
+      }
+    }
+    bool odd = false;
+#pragma unroll
+    for (int x = 0; x < TIMES; ++x) {
+      const int r = 16 * (x * (N / 64) + (t >> 6)) + r16;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        uint32_t byte = sc[x] >> (8 * g) & 255u;
+        if (VALUES && byte >= 248u) odd = true, byte = 0u;
+        const __half2 by = __half2half2(__ushort_as_half(uint16_t(byte << 7)));
+        uint32_t y[4];
+        Four::halves(Four::group<NG>(c[x], g), y);
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const __half2 f = __hmul2(*reinterpret_cast<const __half2*>(&y[z]), by);
+          y[z] = *reinterpret_cast<const uint32_t*>(&f);
+        }
+        const int u = 4 * g + quarter;
+        *reinterpret_cast<uint4*>(to + (u >> 3) * S::HALF + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+      }
+    }
+    return odd;
+  }
+};
+
 // What brings keys (VALUES: values) to their two places, tile by tile.
 template <class T, int KIND, int D, bool VALUES>
 __device__ __forceinline__ void bring_all(const KvAttend& a, const KvBatch& m, const PromptWork& work, unsigned char* smem, PromptBars* bars, const AbortCtl& abort, int t) {
@@ -234,6 +298,12 @@ __device__ __forceinline__ void bring_all(const KvAttend& a, const KvBatch& m, c
         }
         if (lane == 0) bars->odd[i & 1][t >> 5] = any;
       }
+    } else if constexpr (KIND == FV_KV_INT4X32) {
+      const bool odd = BringFour<D, VALUES ? KV_PROMPT_VALUES : KV_PROMPT_KEYS, VALUES>::convert(a, m, work, i, to, t);
+      if constexpr (VALUES) {
+        const bool any = __any_sync(FV_FULL, odd);
+        if (lane == 0) bars->odd[i & 1][t >> 5] = any;
+      }
     } else {
       B::convert(a, m, work, i, src, to, t);
       if (VALUES && t < 32) {  // the scales of both, which the queries' threads leave together with the values
@@ -267,10 +337,10 @@ template <class T, int KIND, int D>
 __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAttend a, KvBatch m) {
   using S = Tile<KIND, D>;
   using M = typename std::conditional<KIND == FV_KV_SAME, T, __half>::type;
-  constexpr bool HALF = std::is_same<M, __half>::value;
+  constexpr bool HALF = std::is_same<M, __half>::value, FOUR = KIND == FV_KV_INT4X32, SCALED = kv_scaled(KIND);
   constexpr float ONE = HALF ? 14.f : 0.f;   // log2 of what stands for a weight of 1
   // log2 of what a maximum may lag behind by; in 8 bits, where the weights meet scales of less than 2, 2^14.9 of them stay in fp16
-  constexpr float GROWN = KIND != FV_KV_SAME ? 0.9f : HALF ? 1.f : 8.f;
+  constexpr float GROWN = SCALED ? 0.9f : HALF ? 1.f : 8.f;
   unsigned char* const smem = dyn_smem();
   PromptBars* const bars = reinterpret_cast<PromptBars*>(smem + S::BARS_AT);
   int2* const list = reinterpret_cast<int2*>(smem + S::LIST_AT);
@@ -359,6 +429,8 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
         }
         w[z] = (w[z] ^ sign) & keep;
       }
+      if constexpr (FOUR)
+        x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
       const int r = threadIdx.x;
       *reinterpret_cast<uint4*>(smem + (u >> 3) * S::Q_HALF + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = x;
     }
@@ -495,7 +567,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
       float factor = 1.f;
       [[maybe_unused]] const float* const sc = reinterpret_cast<const float*>(smem + S::SCALE_AT) + (i & 1) * 3 * S::ROWS;
       [[maybe_unused]] bool alike = true;  // the tile's scales are relative to the query's unit
-      if constexpr (KIND != FV_KV_SAME) {
+      if constexpr (SCALED) {
         const int2 e = bars->exponent[i & 1];
         if (all && (e.x > unit + 1 || unit == 0)) {  // of a tile that the query sees the whole of
           const int own = max(e.x, 1);
@@ -506,7 +578,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
         alike = __all_sync(FV_FULL, !any || unit == e.y);
       }
       const bool busy = __any_sync(FV_FULL, any);
-      const bool odd = KIND == FV_KV_SAME ? (bars->odd[i & 1][0] | bars->odd[i & 1][1] | bars->odd[i & 1][2] | bars->odd[i & 1][3]) != 0 : bars->odd[i & 1][0] != 0;
+      const bool odd = !SCALED ? (bars->odd[i & 1][0] | bars->odd[i & 1][1] | bars->odd[i & 1][2] | bars->odd[i & 1][3]) != 0 : bars->odd[i & 1][0] != 0;
       if (busy) {
         uint32_t r[64];
         tc_ld32_issue(place, r);
@@ -514,7 +586,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
         tc_ld_wait(r);
         tc_ld_wait(r + 32);
         float* s = reinterpret_cast<float*>(r);
-        if constexpr (KIND != FV_KV_SAME) {
+        if constexpr (SCALED) {
 #pragma unroll
           for (int j = 0; j < 64; j += 4) {
             const float4 ks = *reinterpret_cast<const float4*>(sc + j);
@@ -549,7 +621,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
           add2(part + (j & 2), s + j);
         }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
-        if constexpr (KIND != FV_KV_SAME) {
+        if constexpr (SCALED) {
           if (!odd && alike) {
 #pragma unroll
             for (int j = 0; j < 64; j += 4) {
@@ -578,7 +650,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
         for (int j = 0; j < 32; ++j) p[j] = Pair<M>::from_float(s[2 * j], s[2 * j + 1]);
         // O, scaled to the new maximum, and values that were taken out of the product
         const bool scale_o = __any_sync(FV_FULL, changed);
-        if (KIND == FV_KV_SAME && odd) {
+        if (!SCALED && odd) {
           on = __all_sync(FV_FULL, i == 0 || mbar_wait(&bars->pv_done, uint32_t(i - 1) & 1u, abort, 0));
           if (!on) break;
           tc_fence_after();
@@ -598,6 +670,14 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
               int start = 0;
               size_t from = 0;
               if (weight == 0.f || !work.piece(a, m, 4 * i + (j >> 4), start, from)) continue;
+              if constexpr (FOUR) {  // 32 components are a group
+                const uint32_t byte = __ldg(reinterpret_cast<const uint8_t*>(a.v_scale) + (from + (j & 15)) * (D / 32) + (c >> 5));
+                if (byte >= 248u) {
+#pragma unroll
+                  for (int z = 0; z < 32; ++z) o[z] = 0x7FFFFFFFu;
+                }
+                continue;
+              }
               const unsigned char* row = a.vp + ((from + (j & 15)) * D + c) * 2;
 #pragma unroll
               for (int z = 0; z < 32; z += 2) {
@@ -637,7 +717,7 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
     if (on && tiles) on = __all_sync(FV_FULL, mbar_wait(&bars->all_done, 0u, abort, 0));
     tc_fence_after();
     // two factors: their product can be too small for all of its bits where the scales are
-    const float f = KIND != FV_KV_SAME ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
+    const float f = SCALED ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
     const float down = sum == 0.f ? 0.f : 1.f / sum;
     const size_t query = (size_t(row0 + tok) * a.heads + head) * a.group + h;
 #pragma unroll 1
@@ -648,8 +728,10 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
       uint4 w[4];
 #pragma unroll
       for (int z = 0; z < 16; ++z) {
-        float u = __uint_as_float(o[2 * z]) * down, v = __uint_as_float(o[2 * z + 1]) * down;
-        if constexpr (KIND != FV_KV_SAME) u *= f, v *= f;
+        constexpr int order[4] = {0, 4, 1, 5};
+        const int z0 = FOUR ? (z & ~3) * 2 + order[z & 3] : 2 * z, z1 = FOUR ? z0 + 2 : 2 * z + 1;
+        float u = __uint_as_float(o[z0]) * down, v = __uint_as_float(o[z1]) * down;
+        if constexpr (SCALED) u *= f, v *= f;
         // a wait that ran out leaves no result: NaN
         reinterpret_cast<uint32_t*>(w)[z] = !on ? 0x7FFF7FFFu : sum == 0.f ? 0u : Pair<T>::from_float(u, v);
       }

@@ -17,7 +17,8 @@ int kv_check(const fv_kv* kv, const fv_kv_batch* b, const char* who) {
   const std::string w(who);
   if (!kv || !b) return fail(FV_ERR_ARG, w + ": NULL cache or batch");
   if (kv->dtype != FV_KV_BF16 && kv->dtype != FV_KV_FP16) return fail(FV_ERR_UNSUPPORTED, w + ": dtype is bf16 or fp16");
-  if (kv->kind < FV_KV_SAME || kv->kind > FV_KV_E4M3) return fail(FV_ERR_UNSUPPORTED, w + ": kind is same, int8 or e4m3");
+  const bool four = kv->kind == FV_KV_INT4X32;
+  if (!four && (kv->kind < FV_KV_SAME || kv->kind > FV_KV_E4M3)) return fail(FV_ERR_UNSUPPORTED, w + ": kind is same, int8, e4m3 or int4x32");
   if (kv->dim != 64 && kv->dim != 96 && kv->dim != 128) return fail(FV_ERR_UNSUPPORTED, w + ": dim is 64, 96 or 128");
   if (kv->page_size != 16 && kv->page_size != 32 && kv->page_size != 64 && kv->page_size != 128)
     return fail(FV_ERR_UNSUPPORTED, w + ": page_size is 16, 32, 64 or 128");
@@ -30,8 +31,8 @@ int kv_check(const fv_kv* kv, const fv_kv_batch* b, const char* who) {
   if (!coded && (kv->k_scale || kv->v_scale)) return fail(FV_ERR_ARG, w + ": a cache of 16 bits has no scales");
   if (!kv_aligned(kv->k, 16) || !kv_aligned(kv->v, 16) || !kv_aligned(kv->bounds, 16) || !kv_aligned(kv->bound_codes, 16))
     return fail(FV_ERR_ARG, w + ": a buffer of the cache does not begin on 16 bytes");
-  if (!kv_aligned(kv->k_scale, 4) || !kv_aligned(kv->v_scale, 4) || !kv_aligned(kv->bound_scale, 4))
-    return fail(FV_ERR_ARG, w + ": scales do not begin on 4 bytes");
+  if (!kv_aligned(kv->k_scale, four ? 16 : 4) || !kv_aligned(kv->v_scale, four ? 16 : 4) || !kv_aligned(kv->bound_scale, 4))
+    return fail(FV_ERR_ARG, w + ": scales do not begin on 4 bytes (those of 4-bit rows on 16)");
   if (b->rows > size_t(INT_MAX) / 2 || b->nseq > size_t(INT_MAX) / 8 || b->table_width > size_t(1) << 24 || b->table_stride > size_t(1) << 40)
     return fail(FV_ERR_UNSUPPORTED, w + ": rows, nseq or table_width is too large");
   if (b->table_width > size_t(INT_MAX) / kv->page_size) return fail(FV_ERR_UNSUPPORTED, w + ": positions in the table's last block leave 31 bits");
@@ -46,7 +47,7 @@ namespace {
 
 struct KvPool {
   unsigned char *k, *v;
-  float *k_scale, *v_scale;
+  float *k_scale, *v_scale;  // of 4-bit rows: bytes
   unsigned char* bounds;
   int8_t* bound_codes;
   float* bound_scale;
@@ -70,12 +71,38 @@ __device__ __forceinline__ float group_max(float x) {  // over N neighbouring la
   return x;
 }
 
-// One row of 8 values a lane over N lanes: codes (or the 16 bits as they are) to dst, the scale to *scale.  `on`: the lane
-// has values of a row that is written.
-template <class T, int KIND, int N>
-__device__ __forceinline__ void write_row(const uint4& raw, bool on, unsigned char* dst, float* scale, bool first_lane) {
+// One row of 8 values a lane over N lanes, lane l's from 8 l on: codes (or the 16 bits as they are) to row `at` of dst, the scales to those
+// of that row.  `on`: the lane has values of a row that is written.  Whole warps call it.
+template <class T, int KIND, int D, int N>
+__device__ __forceinline__ void write_row(const uint4& raw, bool on, unsigned char* dst, float* scale, size_t at, int l) {
   if constexpr (KIND == FV_KV_SAME) {
-    if (on) *reinterpret_cast<uint4*>(dst) = raw;
+    if (on) *reinterpret_cast<uint4*>(dst + at * (2 * D) + l * 16) = raw;
+  } else if constexpr (KIND == FV_KV_INT4X32) {
+    constexpr int NG = D / 32;
+    float x[8], most = 0.f;
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Pair<T>::to_float(w[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      fine = fine && kv_finite(f.x) && kv_finite(f.y);
+      most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+    }
+    most = group_max<4>(fine ? most : INFINITY);  // of the group's four lanes; infinite also where it is a NaN, which fmaxf drops
+    const bool ok = most < INFINITY;
+    const uint32_t byte = ok ? Four::scale_of(most) : Four::NAN_SCALE;
+    const float s = ok ? Four::value(byte) : 0.f, top = 7.f * s, den = s > 0.f ? s : 1.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = ok ? fminf(fmaxf(x[i], -top), top) : 0.f;
+    const uint32_t code = Four::pack(x, den, __fdiv_rn(1.f, den));
+    // lane l writes pieces 2 l and 2 l + 1: piece n is the (n / NG)-th four of group n % NG, half of what lane 4 (n % NG) + n / NG / 2 has
+    const int n0 = 2 * l, n1 = n0 + 1, u0 = n0 / NG, u1 = n1 / NG;
+    const uint32_t a = __shfl_sync(FV_FULL, code, 4 * (n0 - u0 * NG) + (u0 >> 1), N), b = __shfl_sync(FV_FULL, code, 4 * (n1 - u1 * NG) + (u1 >> 1), N);
+    if (on) {
+      *reinterpret_cast<uint32_t*>(dst + at * (D / 2) + l * 4) = __byte_perm(a, b, (u0 & 1 ? 0x32 : 0x10) | (u1 & 1 ? 0x7600 : 0x5400));
+      if ((l & 3) == 0) reinterpret_cast<uint8_t*>(scale)[at * NG + l / 4] = uint8_t(byte);
+    }
   } else {
     float x[8];
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -95,8 +122,8 @@ __device__ __forceinline__ void write_row(const uint4& raw, bool on, unsigned ch
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = ok ? x[i] * up : 0.f;  // of a row that is not finite, codes of zero
     if (on) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(Eight<KIND>::pack(x, den, inv), Eight<KIND>::pack(x + 4, den, inv));
-      if (first_lane) *scale = ok ? __fdiv_rn(most, Eight<KIND>::top) : __int_as_float(0x7FC00000);
+      *reinterpret_cast<uint2*>(dst + at * D + l * 8) = make_uint2(Eight<KIND>::pack(x, den, inv), Eight<KIND>::pack(x + 4, den, inv));
+      if (l == 0) scale[at] = ok ? __fdiv_rn(most, Eight<KIND>::top) : __int_as_float(0x7FC00000);
     }
   }
 }
@@ -107,7 +134,6 @@ __device__ __forceinline__ void write_row(const uint4& raw, bool on, unsigned ch
 template <class T, int KIND, int D, int WARPS>
 __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128, WARPS > 1 ? 3 : 1) kv_add_kernel(KvPool pool, KvBatch m, KvInput kin, KvInput vin) {
   constexpr int N = D <= 64 ? 8 : 16, PER = 32 / N, L = D / 8;
-  constexpr int ROW = KIND == FV_KV_SAME ? 2 * D : D, VAL = ROW / D;
   __shared__ float s_lo[WARPS > 1 ? WARPS * D : 1], s_hi[WARPS > 1 ? WARPS * D : 1];
   const int warp = threadIdx.x >> 5, lane = lane_id();
   const int head = WARPS > 1 ? int(blockIdx.y) : int(blockIdx.y) * 4 + warp, part = WARPS > 1 ? warp : 0;
@@ -157,8 +183,8 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128, WARPS > 1 ? 3 : 
         }
       }
       const size_t row_at = at * size + slot;
-      write_row<T, KIND, N>(kr[z], on, pool.k + row_at * ROW + l * 8 * VAL, pool.k_scale + row_at, l == 0);
-      write_row<T, KIND, N>(vr[z], on, pool.v + row_at * ROW + l * 8 * VAL, pool.v_scale + row_at, l == 0);
+      write_row<T, KIND, D, N>(kr[z], on, pool.k, pool.k_scale, row_at, l);
+      write_row<T, KIND, D, N>(vr[z], on, pool.v, pool.v_scale, row_at, l);
     }
   }
 #pragma unroll
@@ -222,7 +248,9 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128, WARPS > 1 ? 3 : 
 // four rows on their way.  A row's place is looked up once.
 template <class T, int KIND, int D, int ROWS>
 __global__ void __launch_bounds__(256) kv_vectors_kernel(KvPool pool, KvBatch m, unsigned char* k_out, unsigned char* v_out, bool wide) {
-  constexpr int VALUES = KIND == FV_KV_SAME ? 8 : 16, L = D / VALUES, ROW = KIND == FV_KV_SAME ? 2 * D : D, AHEAD = 4;
+  constexpr bool FOUR = KIND == FV_KV_INT4X32;
+  constexpr int NG = D / 32;  // 4 bits: a thread has a quarter of a row, eight components of each of NG groups
+  constexpr int VALUES = FOUR ? 8 * NG : KIND == FV_KV_SAME ? 8 : 16, L = D / VALUES, ROW = FOUR ? D / 2 : KIND == FV_KV_SAME ? 2 * D : D, AHEAD = 4;
   __shared__ long long s_at[ROWS];  // page * heads * size + slot: the row in head 0; -1: none
   const int first = blockIdx.x * ROWS;
   if (threadIdx.x < ROWS) {
@@ -251,7 +279,7 @@ __global__ void __launch_bounds__(256) kv_vectors_kernel(KvPool pool, KvBatch m,
   const unsigned per_row = unsigned(pool.heads) * L, all = per_row * ROWS;
   for (unsigned i0 = threadIdx.x; i0 < all; i0 += AHEAD * 256) {
     uint4 in[AHEAD][2];
-    float scale[AHEAD][2];
+    float scale[AHEAD][2];  // 4 bits: NG bytes
     size_t to[AHEAD];
     bool on[AHEAD];
 #pragma unroll
@@ -261,6 +289,24 @@ __global__ void __launch_bounds__(256) kv_vectors_kernel(KvPool pool, KvBatch m,
       on[z] = at0 >= 0;
       if (!on[z]) continue;
       const size_t at = size_t(at0) + (size_t(head) << pool.page_shift);
+      if constexpr (FOUR) {
+        to[z] = ((size_t(first) + r) * pool.heads + head) * (2 * D) + l * 16;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+          const unsigned char* from = (which ? pool.v : pool.k) + at * ROW + l * (4 * NG);
+          uint4& w = in[z][which];
+          if constexpr (NG == 4) w = __ldg(reinterpret_cast<const uint4*>(from));
+          else if constexpr (NG == 2) reinterpret_cast<uint2&>(w) = __ldg(reinterpret_cast<const uint2*>(from));
+          else w.x = __ldg(reinterpret_cast<const uint32_t*>(from)), w.y = __ldg(reinterpret_cast<const uint32_t*>(from) + 1), w.z = __ldg(reinterpret_cast<const uint32_t*>(from) + 2);
+          const uint8_t* sc = reinterpret_cast<const uint8_t*>(which ? pool.v_scale : pool.k_scale) + at * NG;
+          uint32_t bytes = 0;
+          if constexpr (NG == 4) bytes = __ldg(reinterpret_cast<const uint32_t*>(sc));
+          else if constexpr (NG == 2) bytes = __ldg(reinterpret_cast<const uint16_t*>(sc));
+          else bytes = __ldg(sc) | uint32_t(__ldg(sc + 1)) << 8 | uint32_t(__ldg(sc + 2)) << 16;
+          scale[z][which] = __uint_as_float(bytes);
+        }
+        continue;
+      }
       to[z] = ((size_t(first) + r) * per_row + x) * (2 * VALUES);
       in[z][0] = __ldg(reinterpret_cast<const uint4*>(pool.k + at * ROW + l * 16));
       in[z][1] = __ldg(reinterpret_cast<const uint4*>(pool.v + at * ROW + l * 16));
@@ -275,6 +321,18 @@ __global__ void __launch_bounds__(256) kv_vectors_kernel(KvPool pool, KvBatch m,
         const uint4 c = in[z][which];
         if constexpr (KIND == FV_KV_SAME) {
           *out = c;
+        } else if constexpr (FOUR) {
+          const uint32_t words[4] = {c.x, c.y, c.z, c.w}, bytes = __float_as_uint(scale[z][which]);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const uint32_t codes = Four::group<NG>(words, g);
+            const float s = Four::value(bytes >> (8 * g) & 255);
+            uint32_t w[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              w[x] = Pair<T>::from_float(float(int(codes >> (8 * x) & 15) - 8) * s, float(int(codes >> (8 * x + 4) & 15) - 8) * s);
+            out[4 * g] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
         } else {
           const float s = scale[z][which];
           const uint32_t codes[4] = {c.x, c.y, c.z, c.w};

@@ -21,7 +21,7 @@ import ctypes as C
 
 from ._lib import FV_ERR_ARG, FerrovecError, check, fv_kv, fv_kv_batch, lib
 
-KINDS = ("same", "int8", "e4m3")
+KINDS = {"same": 0, "int8": 1, "e4m3": 2, "int4x32": 4}
 
 
 def _refuse(text: str):
@@ -33,9 +33,13 @@ class KvCache:
 
     `kind`: "same" keeps rows as they come (`dtype`: torch.bfloat16 or torch.float16); "int8" and "e4m3" round every row
     of a head to 8 bits with a scale of its own (max |x| / 127 or / 448).  A row with a value that is not finite reads
-    back as NaN from an 8-bit cache.  `page_size`: 16, 32, 64 or 128 rows.
+    back as NaN from an 8-bit cache.  "int4x32" rounds to 4 bits, whole numbers from -7 to 7, with a scale for every 32
+    neighbouring components: max |x| / 7 rounded up to a number of 4 significant bits, from 2**-17 to 9216, so that what a row
+    holds is exact in `dtype`; components beyond 64512 become that, and a group with a value that is not finite reads back
+    as NaN.  `page_size`: 16, 32, 64 or 128 rows.
 
-    The memory is torch's: `k`, `v` (pages, heads, page_size, dim), `k_scale`, `v_scale` (pages, heads, page_size) or None,
+    The memory is torch's: `k`, `v` (pages, heads, page_size, dim), `k_scale`, `v_scale` (pages, heads, page_size) or None (of
+    "int4x32" bytes: (..., dim / 2), two codes each, and (..., dim / 32); `include/ferrovec.h` says which component is where),
     `bounds` (pages, heads, 2, dim: the componentwise minima and maxima of a block's keys), `bound_codes` (the same in 8
     bits) and `bound_scale` (pages, heads).  `buffers`: a dict of them by these names, where the caller has them already.
     Their contents are anyone's to change; the tensors are the cache's for good, since every call goes to their addresses.
@@ -53,12 +57,14 @@ class KvCache:
         if pages < 0 or heads < 1 or dim not in (64, 96, 128) or page_size not in (16, 32, 64, 128):
             _refuse(f"pages >= 0, heads >= 1, dim 64, 96 or 128, page_size 16, 32, 64 or 128: got {pages}, {heads}, {dim}, {page_size}")
         self.pages, self.heads, self.dim, self.page_size, self.dtype, self.kind = pages, heads, dim, page_size, dtype, kind
-        held = {"same": dtype, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}[kind]
-        rows, scales = (pages, heads, page_size, dim), (pages, heads, page_size)
+        held = {"same": dtype, "int8": torch.int8, "e4m3": torch.float8_e4m3fn, "int4x32": torch.uint8}[kind]
+        rows, scales, scale = (pages, heads, page_size, dim), (pages, heads, page_size), torch.float32
+        if kind == "int4x32":
+            rows, scales, scale = (pages, heads, page_size, dim // 2), (pages, heads, page_size, dim // 32), torch.uint8
         want = {"k": (rows, held), "v": (rows, held), "bounds": ((pages, heads, 2, dim), dtype),
                 "bound_codes": ((pages, heads, 2, dim), torch.int8), "bound_scale": ((pages, heads), torch.float32)}
         if kind != "same":
-            want |= {"k_scale": (scales, torch.float32), "v_scale": (scales, torch.float32)}
+            want |= {"k_scale": (scales, scale), "v_scale": (scales, scale)}
         if buffers is None:
             device = torch.device("cuda" if device is None else device)
             buffers = {n: torch.zeros(s, dtype=t, device=device) for n, (s, t) in want.items()}
@@ -71,7 +77,7 @@ class KvCache:
             _refuse("the buffers of a cache are on one CUDA device")
         self.device = self.k.device
         at = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
-        self._c = fv_kv(self.device.index, int(dtype == torch.float16), KINDS.index(kind), page_size, heads, dim, pages, at(self.k),
+        self._c = fv_kv(self.device.index, int(dtype == torch.float16), KINDS[kind], page_size, heads, dim, pages, at(self.k),
                         at(self.v), at(self.k_scale), at(self.v_scale), at(self.bounds), at(self.bound_codes), at(self.bound_scale))
         self._ready()
 

@@ -300,6 +300,14 @@ int fv_merge_topk_static_dev(int device, void* stream, const fv_neighbor* d_part
  * 8 bits), [pages][heads] (bound_scale), contiguous.  k and v hold `dtype` (FV_KV_SAME) or 8 bits: a row is
  * code * scale with scale = max|x| / 127 (int8) or / 448 (e4m3), and a row with a value that is not finite reads back
  * as NaN (its scale; codes are always numbers); k_scale and v_scale are NULL for FV_KV_SAME.  k, v and bounds begin on 16 bytes, bound_codes on 16, scales on 4.
+ *
+ * FV_KV_INT4X32: k and v are [pages][heads][page_size][dim / 2] bytes, the scales (k_scale and v_scale point to bytes, on 16)
+ * [pages][heads][page_size][dim / 32], one for every 32 neighbouring components.  A scale byte is the number 2^(e - 18) (8 + m), e its upper
+ * five bits and m its lower three, or 2^-17 m where e is 0 (fp16's bits, moved down by seven); 255: not a number.  It is the
+ * smallest that is not below max|x| / 7, and at most 9216.  A code of 4 bits is 8 + rn(x / scale), from 1 to 15 (x beyond 7 scales
+ * as 7 scales), and (code - 8) * scale is exact in fp16 and in bf16.  A row is dim / 4 numbers of 16 bits, each four neighbouring components, the
+ * lowest in its lowest bits: number u * dim / 32 + g holds components 32 g + 4 u to 32 g + 4 u + 3.  A group with a value that
+ * is not finite reads back as NaN.
  * dim is 64, 96 or 128, page_size 16, 32, 64 or 128.
  *
  * The calls take a cudaStream_t of that device (NULL: its default stream), launch a kernel or two on it and return: they
@@ -313,7 +321,7 @@ int fv_merge_topk_static_dev(int device, void* stream, const fv_neighbor* d_part
  * (-1, say), are skipped: nothing is read or written there, and nothing attends to them.  A page that add writes to is one
  * block of one sequence of the call. */
 enum { FV_KV_BF16 = 0, FV_KV_FP16 = 1 };                 /* dtype */
-enum { FV_KV_SAME = 0, FV_KV_INT8 = 1, FV_KV_E4M3 = 2 }; /* kind */
+enum { FV_KV_SAME = 0, FV_KV_INT8 = 1, FV_KV_E4M3 = 2, FV_KV_INT4X32 = 4 }; /* kind */
 typedef struct fv_kv {
   int device;
   int dtype;
