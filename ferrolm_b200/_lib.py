@@ -65,8 +65,26 @@ class fv_kv_batch(C.Structure):
                 ("cu", C.c_void_p), ("nseq", C.c_size_t), ("rows", C.c_size_t)]
 
 
+class fv_rotary(C.Structure):
+    _fields_ = [("device", C.c_int), ("dtype", C.c_int), ("dim", C.c_uint32), ("part", C.c_uint32), ("layout", C.c_int), ("amplitude", C.c_float),
+                ("turns", C.c_void_p)]
+
+
+class fv_rotary_rows(C.Structure):
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("in_row", C.c_size_t), ("in_head", C.c_size_t), ("out_row", C.c_size_t),
+                ("out_head", C.c_size_t), ("heads", C.c_size_t)]
+
+
+class fv_pages(C.Structure):
+    _fields_ = [("device", C.c_int), ("page_size", C.c_uint32), ("pages", C.c_uint64), ("refs", C.c_void_p)]
+
+
+class fv_table(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("stride", C.c_size_t), ("width", C.c_size_t), ("nseq", C.c_size_t)]
+
+
 _vp, _sz, _i, _u32, _u64 = C.c_void_p, C.c_size_t, C.c_int, C.c_uint32, C.c_uint64
-_pp, _kvb = C.POINTER(C.c_void_p), C.POINTER(fv_kv_batch)
+_pp, _kvb, _tab = C.POINTER(C.c_void_p), C.POINTER(fv_kv_batch), C.POINTER(fv_table)
 
 # every symbol include/ferrovec.h declares: name -> (restype, argtypes)
 SIGNATURES = {
@@ -155,6 +173,15 @@ SIGNATURES = {
     "fv_kv_search_dev": (_i, [_vp, _vp, _kvb, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _vp]),
     "fv_kv_attend_dev": (_i, [_vp, _vp, _kvb, _vp, _sz, _sz, _sz, _vp, _sz, C.c_float, _vp, _vp, _vp, _sz]),
     "fv_kv_attend_work": (_sz, [_vp, _kvb, _sz]),
+    "fv_kv_copy_pages_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _vp]),
+    "fv_rotate_dev": (_i, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _sz, _vp, _i]),
+    "fv_pages_fork_dev": (_i, [_vp, _vp, _tab, _vp, _vp, _tab]),
+    "fv_pages_free_dev": (_i, [_vp, _vp, _tab, _vp]),
+    "fv_pages_extend_dev": (_i, [_vp, _vp, _vp, _sz, _tab, _vp, _vp, _vp, _vp, _sz]),
+    "fv_pages_extend_work": (_sz, [_vp, _tab]),
+    "fv_pages_compact_dev": (_i, [_vp, _vp, _vp, _sz, _vp, _vp, _vp, _sz]),
+    "fv_pages_compact_work": (_sz, [_vp]),
+    "fv_pages_remap_dev": (_i, [_vp, _vp, _vp, _tab]),
     "fv_datagen_dev": (_i, [_vp, _u64, _sz, _sz, _sz, _sz, _vp]),
 }
 

@@ -1,0 +1,509 @@
+// Which pages of a cache are in use, and their copies.
+//
+// refs[p] counts the table entries that hold page p; 0: it is free.  fork and free are a pass over the table with an addition for each entry.
+// extend and compact have to number things in order (the free pages, the blocks that want one), so each is planned by one CTA whose
+// threads meet at its barriers, and what it decides to copy is copied by all SMs in a second kernel.  Nothing depends on the order of
+// atomics: additions commute, and a page's last holder is found by the smallest number.
+#include <climits>
+
+#include "kv.cuh"
+
+namespace fv {
+namespace {
+
+enum { PAGES_THREADS = 1024, PAGES_WARPS = 32, PAGES_SEQS = 2048, COPY_THREADS = 256, COPY_SLICE = 32 * 1024, COPY_PARTS = 7 };
+
+struct Pages {
+  int32_t* refs;
+  int pages, page_shift;
+};
+struct Table {
+  int32_t* at;
+  size_t stride;
+  int width, nseq;
+};
+
+// Sum over the CTA up to this thread, exclusive; *all: over everybody.  s: PAGES_WARPS + 1 ints, in use until the next barrier.
+__device__ __forceinline__ int sum_before(int x, int* s, int* all) {
+  const int warp = threadIdx.x >> 5, lane = lane_id();
+  int up = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(FV_FULL, up, o);
+    if (lane >= o) up += y;
+  }
+  if (lane == 31) s[warp] = up;
+  __syncthreads();
+  const int mine = lane < PAGES_WARPS ? s[lane] : 0;
+  int w = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(FV_FULL, w, o);
+    if (lane >= o) w += y;
+  }
+  *all = __shfl_sync(FV_FULL, w, 31);
+  const int before = __shfl_sync(FV_FULL, w - mine, warp);
+  __syncthreads();
+  return before + up - x;
+}
+
+// The warp's part of the pages: f(page, whether it is one, count) for 128 pages at a time, four neighbours a lane.
+template <class F>
+__device__ __forceinline__ void each_page(const Pages& p, F&& f) {
+  const int warp = threadIdx.x >> 5, lane = lane_id();
+  const int share = ((p.pages + PAGES_WARPS - 1) / PAGES_WARPS + 127) & ~127;
+  const int begin = int(min((long long)(warp) * share, (long long)(p.pages))), end = int(min((long long)(begin) + share, (long long)(p.pages)));
+  const bool wide = (reinterpret_cast<uintptr_t>(p.refs) & 15) == 0;
+#pragma unroll 4
+  for (int i = begin; i < end; i += 128) {
+    const int at = i + 4 * lane;
+    int4 r = make_int4(-1, -1, -1, -1);  // behind the last page
+    if (wide && at + 4 <= p.pages) {
+      r = __ldcg(reinterpret_cast<const int4*>(p.refs + at));
+    } else {
+      int* x = reinterpret_cast<int*>(&r);
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+        if (at + z < p.pages) x[z] = __ldcg(p.refs + at + z);
+    }
+    if (!f(at, r)) break;  // for whole warps
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+struct Extend {
+  const int32_t *lens, *more;
+  int32_t* missing;
+  int32_t *count, *before, *free, *src, *dst;  // in the caller's work
+};
+
+// Entry e of the blocks that rows come to: sequence b's are before[b] .. before[b + 1], from block `first` on.
+__device__ __forceinline__ int32_t* entry_at(const Pages& p, const Table& t, const Extend& x, const int* before, int e) {
+  int lo = 0, n = t.nseq;
+  while (n > 1) {  // the last sequence that begins at or before e
+    const int h = n / 2;
+    if (before[lo + h] <= e) lo += h, n -= h;
+    else n = h;
+  }
+  const int first = max(__ldg(x.lens + lo), 0) >> p.page_shift;
+  return t.at + size_t(lo) * t.stride + first + (e - before[lo]);
+}
+
+// What a table entry says while this runs: a page; -1: it wants one; -2 - q: it wants one and a copy of page q.
+__global__ void __launch_bounds__(PAGES_THREADS) pages_extend_kernel(Pages p, Table t, Extend x) {
+  __shared__ int s_sum[PAGES_WARPS + 1], s_before[PAGES_SEQS + 1], s_count;
+  const int tid = threadIdx.x;
+  int* const before = t.nseq <= PAGES_SEQS ? s_before : x.before;
+  if (tid == 0) s_count = 0, before[0] = 0;
+  int entries = 0;
+  for (int b0 = 0; b0 < t.nseq; b0 += PAGES_THREADS) {
+    const int b = b0 + tid;
+    int n = 0, all;
+    if (b < t.nseq) {
+      const int len = max(__ldg(x.lens + b), 0), more = max(__ldg(x.more + b), 0);
+      const long long end = ((long long)(len) + more + (1 << p.page_shift) - 1) >> p.page_shift;
+      if (more) n = max(int(min(end, (long long)(t.width))) - (len >> p.page_shift), 0);
+    }
+    const int up = sum_before(n, s_sum, &all);
+    if (b < t.nseq) before[b + 1] = entries + up + n;
+    entries += all;
+  }
+  __syncthreads();
+  // who wants a page
+  bool shared = false;
+  int wants = 0;
+  for (int e = tid; e < entries; e += PAGES_THREADS) {
+    int32_t* at = entry_at(p, t, x, before, e);
+    const int q = __ldcg(at);
+    if (unsigned(q) >= unsigned(p.pages)) __stcg(at, -1), ++wants;
+    else if (__ldcg(p.refs + q) > 1) __stcg(at, -2 - q), shared = true, ++wants;
+  }
+  if (__syncthreads_or(shared)) {
+    // who holds a page with others gives it up; where nobody is left, refs becomes the smallest number of those who did, far below 0, and
+    // that one keeps it
+    for (int e = tid; e < entries; e += PAGES_THREADS) {
+      const int q = -2 - __ldcg(entry_at(p, t, x, before, e));
+      if (q >= 0) atomicSub(p.refs + q, 1);
+    }
+    __syncthreads();
+    for (int e = tid; e < entries; e += PAGES_THREADS) {
+      const int q = -2 - __ldcg(entry_at(p, t, x, before, e));
+      if (q >= 0 && __ldcg(p.refs + q) <= 0) atomicMin(p.refs + q, INT_MIN + e);
+    }
+    __syncthreads();
+    for (int e = tid; e < entries; e += PAGES_THREADS) {
+      int32_t* at = entry_at(p, t, x, before, e);
+      const int q = -2 - __ldcg(at);
+      if (q >= 0 && __ldcg(p.refs + q) == INT_MIN + e) __stcg(at, q), --wants;
+    }
+    __syncthreads();
+    for (int e = tid; e < entries; e += PAGES_THREADS) {
+      const int q = __ldcg(entry_at(p, t, x, before, e));
+      if (q >= 0 && __ldcg(p.refs + q) < 0) __stcg(p.refs + q, 1);
+    }
+  }
+  int all;
+  sum_before(wants, s_sum, &all);
+  wants = all;
+  if (wants) {
+    // the free pages, as many as are wanted
+    int n = 0;
+    each_page(p, [&](int, const int4& r) { return n += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0), true; });
+    int rank = sum_before(n, s_sum, &all);  // of a lane: its pages are not neighbours, only the warp's sum counts
+    if (all < wants) {  // nothing is changed
+      for (int e = tid; e < entries; e += PAGES_THREADS) {
+        int32_t* at = entry_at(p, t, x, before, e);
+        const int q = -2 - __ldcg(at);
+        if (q >= 0) atomicAdd(p.refs + q, 1), __stcg(at, q);
+      }
+      if (tid == 0) *x.missing = wants - all, *x.count = 0;
+      return;
+    }
+    rank = __shfl_sync(FV_FULL, rank, 0);
+    each_page(p, [&](int at, const int4& r) {
+      const int c = (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
+      int up = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(FV_FULL, up, o);
+        if (int(lane_id()) >= o) up += y;
+      }
+      int i = rank + up - c;
+      if (r.x == 0 && i < wants) x.free[i] = at;
+      i += r.x == 0;
+      if (r.y == 0 && i < wants) x.free[i] = at + 1;
+      i += r.y == 0;
+      if (r.z == 0 && i < wants) x.free[i] = at + 2;
+      i += r.z == 0;
+      if (r.w == 0 && i < wants) x.free[i] = at + 3;
+      rank += __shfl_sync(FV_FULL, up, 31);
+      return rank < wants;
+    });
+    __syncthreads();
+    int given = 0;
+    for (int e0 = 0; e0 < entries; e0 += PAGES_THREADS) {
+      const int e = e0 + tid;
+      int32_t* at = e < entries ? entry_at(p, t, x, before, e) : nullptr;
+      const int q = at ? __ldcg(at) : 0;
+      const int i = given + sum_before(q < 0, s_sum, &all);
+      given += all;
+      if (q < 0) {
+        const int page = __ldcg(x.free + i);
+        *at = page;
+        p.refs[page] = 1;
+        if (q < -1) {
+          const int c = atomicAdd(&s_count, 1);
+          x.src[c] = -2 - q, x.dst[c] = page;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (tid == 0) *x.missing = 0, *x.count = s_count;
+}
+
+__global__ void __launch_bounds__(256) pages_fork_kernel(Pages p, Table from, const int32_t* lens, const int32_t* parents, Table to) {
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= to.width) return;
+  for (int i = blockIdx.y; i < to.nseq; i += gridDim.y) {
+    const int b = __ldg(parents + i);
+    int q = -1;
+    if (unsigned(b) < unsigned(from.nseq) && j < from.width) {
+      const int len = lens ? max(__ldg(lens + b), 0) : INT_MAX;
+      if ((long long)(j) << p.page_shift < len) q = __ldg(from.at + size_t(b) * from.stride + j);
+      if (unsigned(q) >= unsigned(p.pages)) q = -1;
+    }
+    to.at[size_t(i) * to.stride + j] = q;
+    if (q >= 0) atomicAdd(p.refs + q, 1);
+  }
+}
+
+__global__ void __launch_bounds__(256) pages_free_kernel(Pages p, Table t, const int32_t* lens) {
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= t.width) return;
+  for (int b = blockIdx.y; b < t.nseq; b += gridDim.y) {
+    const int len = lens ? max(__ldg(lens + b), 0) : 0;
+    if ((long long)(j) << p.page_shift < len) continue;
+    int32_t* at = t.at + size_t(b) * t.stride + j;
+    const int q = *at;
+    if (q == -1) continue;
+    *at = -1;
+    if (unsigned(q) < unsigned(p.pages) && atomicSub(p.refs + q, 1) <= 0) atomicAdd(p.refs + q, 1);  // it was free already
+  }
+}
+
+__global__ void __launch_bounds__(256) pages_remap_kernel(const int32_t* map, int pages, Table t) {
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= t.width) return;
+  for (int b = blockIdx.y; b < t.nseq; b += gridDim.y) {
+    int32_t* at = t.at + size_t(b) * t.stride + j;
+    const int q = *at;
+    if (unsigned(q) < unsigned(pages)) *at = __ldg(map + q);
+  }
+}
+
+__global__ void __launch_bounds__(PAGES_THREADS) pages_compact_kernel(Pages p, int32_t* map, int32_t* used, int32_t* count, int32_t* src, int32_t* dst) {
+  __shared__ int s_sum[PAGES_WARPS + 1];
+  const int lane = lane_id();
+  int n = 0, all;
+  each_page(p, [&](int, const int4& r) { return n += (r.x > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0), true; });
+  sum_before(n, s_sum, &all);
+  const int live = all;
+  // a page below `live` that is free is a hole; one from there on that is not moves to the hole of its number
+  int holes = 0, movers = 0;
+  each_page(p, [&](int at, const int4& r) {
+    const int* c = reinterpret_cast<const int*>(&r);
+#pragma unroll
+    for (int z = 0; z < 4; ++z) holes += at + z < live && c[z] <= 0, movers += at + z >= live && at + z < p.pages && c[z] > 0;
+    return true;
+  });
+  int hole = sum_before(holes, s_sum, &all);
+  const int moved = all;
+  int mover = sum_before(movers, s_sum, &all);
+  hole = __shfl_sync(FV_FULL, hole, 0), mover = __shfl_sync(FV_FULL, mover, 0);
+  each_page(p, [&](int at, const int4& r) {
+    const int* c = reinterpret_cast<const int*>(&r);
+    int own = 0;  // a hole, or from `live` on a mover: a lane's four are counted together, 128 pages lie on both sides of `live` at most once
+#pragma unroll
+    for (int z = 0; z < 4; ++z) own += at + z < live ? c[z] <= 0 : at + z < p.pages && c[z] > 0 ? 1 << 16 : 0;
+    int up = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(FV_FULL, up, o);
+      if (lane >= o) up += y;
+    }
+    int h = hole + ((up - own) & 0xFFFF), m = mover + ((up - own) >> 16);
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      if (at + z >= p.pages) continue;
+      if (at + z < live && c[z] <= 0) dst[h++] = at + z;
+      if (at + z >= live && c[z] > 0) src[m++] = at + z;
+      map[at + z] = c[z] > 0 ? at + z : -1;
+    }
+    const int sum = __shfl_sync(FV_FULL, up, 31);
+    hole += sum & 0xFFFF, mover += sum >> 16;
+    return true;
+  });
+  __syncthreads();
+  for (int i = threadIdx.x; i < moved; i += PAGES_THREADS) {
+    const int from = __ldcg(src + i), to = __ldcg(dst + i);
+    map[from] = to;
+    p.refs[to] = __ldcg(p.refs + from);
+    p.refs[from] = 0;
+  }
+  if (threadIdx.x == 0) *used = live, *count = moved;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Copies of pages: a page's part of each of the cache's buffers, in slices of 32 KB.  A CTA has 8 loads of 16 bytes a thread on their way.
+struct CopyPart {
+  unsigned char* at;
+  unsigned bytes, slices;  // of a page
+  bool wide;               // whole 16 bytes
+};
+struct Copy {
+  CopyPart part[COPY_PARTS];
+  const int32_t *src, *dst, *count;
+  long long n;
+  unsigned pages, slices;
+};
+
+__global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(Copy c) {
+  constexpr int AHEAD = COPY_SLICE / 16 / COPY_THREADS;
+  const long long pairs = c.count ? min(c.n, (long long)(max(__ldcg(c.count), 0))) : c.n, items = pairs * c.slices;
+  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+    const long long pair = item / c.slices;
+    unsigned slice = unsigned(item - pair * c.slices);
+    const int from = __ldcg(c.src + pair), to = __ldcg(c.dst + pair);
+    if (unsigned(from) >= c.pages || unsigned(to) >= c.pages) continue;
+    unsigned char* at = nullptr;
+    unsigned bytes = 0;
+    bool wide = true;
+#pragma unroll
+    for (int i = 0; i < COPY_PARTS; ++i) {
+      if (!at && slice < c.part[i].slices) at = c.part[i].at, bytes = c.part[i].bytes, wide = c.part[i].wide;
+      else if (!at) slice -= c.part[i].slices;
+    }
+    const unsigned char* const in = at + size_t(from) * bytes + size_t(slice) * COPY_SLICE;
+    unsigned char* const out = at + size_t(to) * bytes + size_t(slice) * COPY_SLICE;
+    const unsigned n = min(bytes - slice * COPY_SLICE, unsigned(COPY_SLICE));
+    if (wide) {
+      uint4 x[AHEAD];
+#pragma unroll
+      for (int z = 0; z < AHEAD; ++z) {
+        const unsigned i = (threadIdx.x + z * COPY_THREADS) * 16;
+        if (i < n) x[z] = __ldcs(reinterpret_cast<const uint4*>(in + i));
+      }
+#pragma unroll
+      for (int z = 0; z < AHEAD; ++z) {
+        const unsigned i = (threadIdx.x + z * COPY_THREADS) * 16;
+        if (i < n) __stcs(reinterpret_cast<uint4*>(out + i), x[z]);
+      }
+    } else {
+      for (unsigned i = threadIdx.x * 4; i < n; i += COPY_THREADS * 4) *reinterpret_cast<uint32_t*>(out + i) = *reinterpret_cast<const uint32_t*>(in + i);
+    }
+  }
+}
+
+int copy_pages(const fv_kv* kv, cudaStream_t s, const int32_t* src, const int32_t* dst, size_t n, const int32_t* count) {
+  if (n == 0 || kv->pages == 0) return FV_OK;
+  const size_t rows = size_t(kv->heads) * kv->page_size, row = kv_row_bytes(kv), scale = kv_scale_bytes(kv), bounds = size_t(kv->heads) * 2 * kv->dim;
+  void* const at[COPY_PARTS] = {kv->k, kv->v, kv->bounds, kv->bound_codes, kv->k_scale, kv->v_scale, kv->bound_scale};
+  const size_t bytes[COPY_PARTS] = {rows * row, rows * row, 2 * bounds, bounds, rows * scale, rows * scale, 4 * size_t(kv->heads)};
+  Copy c = {};
+  for (int i = 0; i < COPY_PARTS; ++i) {
+    if (bytes[i] >= size_t(1) << 31) return fail(FV_ERR_UNSUPPORTED, "copies of pages: a page of 2 GB or more");
+    c.part[i] = {static_cast<unsigned char*>(at[i]), unsigned(bytes[i]), unsigned((bytes[i] + COPY_SLICE - 1) / COPY_SLICE), kv_aligned(at[i], 16) && bytes[i] % 16 == 0};
+    c.slices += c.part[i].slices;
+  }
+  c.src = src, c.dst = dst, c.count = count, c.n = (long long)(n), c.pages = unsigned(kv->pages);
+  const size_t items = n * c.slices, most = 148 * 8;
+  pages_copy_kernel<<<unsigned(items < most ? items : most), COPY_THREADS, 0, s>>>(c);
+  FV_CUDA(cudaGetLastError());
+  return FV_OK;
+}
+
+int pages_check(const fv_pages* p, const std::string& w) {
+  if (!p) return fail(FV_ERR_ARG, w + ": NULL pages");
+  if (p->page_size != 16 && p->page_size != 32 && p->page_size != 64 && p->page_size != 128)
+    return fail(FV_ERR_UNSUPPORTED, w + ": page_size is 16, 32, 64 or 128");
+  if (p->pages > size_t(INT_MAX) - 256) return fail(FV_ERR_UNSUPPORTED, w + ": pages does not fit 31 bits");
+  if (p->device < 0) return fail(FV_ERR_ARG, w + ": device index out of range");
+  if (p->pages && !p->refs) return fail(FV_ERR_ARG, w + ": NULL refs");
+  if (!kv_aligned(p->refs, 4)) return fail(FV_ERR_ARG, w + ": refs does not begin on 4 bytes");
+  return FV_OK;
+}
+int table_check(const fv_pages* p, const fv_table* t, const std::string& w) {
+  if (!t) return fail(FV_ERR_ARG, w + ": NULL table");
+  if (t->nseq > size_t(INT_MAX) / 8 || t->width > size_t(1) << 24 || t->stride > size_t(1) << 40) return fail(FV_ERR_UNSUPPORTED, w + ": nseq or width is too large");
+  if (t->width > size_t(INT_MAX) / p->page_size) return fail(FV_ERR_UNSUPPORTED, w + ": positions in the table's last block leave 31 bits");
+  if (t->nseq && t->width && !t->table) return fail(FV_ERR_ARG, w + ": NULL table");
+  if (t->nseq > 1 && t->stride < t->width) return fail(FV_ERR_ARG, w + ": rows of the table overlap");
+  if (!kv_aligned(t->table, 4)) return fail(FV_ERR_ARG, w + ": table does not begin on 4 bytes");
+  return FV_OK;
+}
+int caches_check(const fv_pages* p, const fv_kv* const* caches, size_t n, const char* who) {
+  const std::string w(who);
+  if (n && !caches) return fail(FV_ERR_ARG, w + ": NULL caches");
+  const fv_kv_batch none = {};
+  for (size_t i = 0; i < n; ++i) {
+    FV_TRY(kv_check(caches[i], &none, who));
+    if (caches[i]->device != p->device || caches[i]->pages != p->pages || caches[i]->page_size != p->page_size)
+      return fail(FV_ERR_ARG, w + ": a cache has other pages, or is on another device");
+  }
+  return FV_OK;
+}
+Pages pages_of(const fv_pages* p) { return Pages{p->refs, int(p->pages), __builtin_ctz(p->page_size)}; }
+Table table_of(const fv_table* t) { return Table{t->table, t->stride, int(t->width), int(t->nseq)}; }
+dim3 table_grid(const fv_table* t) { return dim3(unsigned((t->width + 255) / 256), unsigned(t->nseq < 65535 ? t->nseq : 65535)); }
+
+// pages that a call can give or move
+size_t most_pages(const fv_pages* p, const fv_table* t) {
+  const size_t entries = t->nseq * t->width;
+  return entries < p->pages ? entries : p->pages;
+}
+
+}  // namespace
+}  // namespace fv
+
+extern "C" int fv_kv_copy_pages_dev(const fv_kv* kv, void* stream, const int32_t* src, const int32_t* dst, size_t n, const int32_t* count) {
+  const fv_kv_batch none = {};
+  FV_TRY(fv::kv_check(kv, &none, "fv_kv_copy_pages_dev"));
+  if (n == 0 || kv->pages == 0) return FV_OK;
+  if (n > size_t(INT_MAX)) return fv::fail(FV_ERR_UNSUPPORTED, "fv_kv_copy_pages_dev: n does not fit 31 bits");
+  if (!src || !dst) return fv::fail(FV_ERR_ARG, "fv_kv_copy_pages_dev: NULL src or dst");
+  if (!fv::kv_aligned(src, 4) || !fv::kv_aligned(dst, 4) || !fv::kv_aligned(count, 4)) return fv::fail(FV_ERR_ARG, "fv_kv_copy_pages_dev: src, dst or count does not begin on 4 bytes");
+  fv::DeviceGuard g(kv->device);
+  if (!g.ok) return fv::fail(FV_ERR_CUDA, "cudaSetDevice failed (there is no CPU path)");
+  return fv::copy_pages(kv, static_cast<cudaStream_t>(stream), src, dst, n, count);
+}
+
+extern "C" int fv_pages_fork_dev(const fv_pages* p, void* stream, const fv_table* from, const int32_t* lens, const int32_t* parents, const fv_table* out) {
+  const char* w = "fv_pages_fork_dev";
+  FV_TRY(fv::pages_check(p, w));
+  FV_TRY(fv::table_check(p, from, w));
+  FV_TRY(fv::table_check(p, out, w));
+  if (out->nseq == 0 || out->width == 0) return FV_OK;
+  if (!parents || !fv::kv_aligned(parents, 4) || !fv::kv_aligned(lens, 4)) return fv::fail(FV_ERR_ARG, std::string(w) + ": parents is not there, or it or lens does not begin on 4 bytes");
+  if (from->table == out->table) return fv::fail(FV_ERR_ARG, std::string(w) + ": out is the table");
+  fv::DeviceGuard g(p->device);
+  if (!g.ok) return fv::fail(FV_ERR_CUDA, "cudaSetDevice failed (there is no CPU path)");
+  fv::pages_fork_kernel<<<fv::table_grid(out), 256, 0, static_cast<cudaStream_t>(stream)>>>(fv::pages_of(p), fv::table_of(from), lens, parents, fv::table_of(out));
+  FV_CUDA(cudaGetLastError());
+  return FV_OK;
+}
+
+extern "C" int fv_pages_free_dev(const fv_pages* p, void* stream, const fv_table* t, const int32_t* lens) {
+  const char* w = "fv_pages_free_dev";
+  FV_TRY(fv::pages_check(p, w));
+  FV_TRY(fv::table_check(p, t, w));
+  if (!fv::kv_aligned(lens, 4)) return fv::fail(FV_ERR_ARG, std::string(w) + ": lens does not begin on 4 bytes");
+  if (t->nseq == 0 || t->width == 0) return FV_OK;
+  fv::DeviceGuard g(p->device);
+  if (!g.ok) return fv::fail(FV_ERR_CUDA, "cudaSetDevice failed (there is no CPU path)");
+  fv::pages_free_kernel<<<fv::table_grid(t), 256, 0, static_cast<cudaStream_t>(stream)>>>(fv::pages_of(p), fv::table_of(t), lens);
+  FV_CUDA(cudaGetLastError());
+  return FV_OK;
+}
+
+// work: the number of copies, where sequences' entries begin, the free pages, sources and places of copies
+extern "C" size_t fv_pages_extend_work(const fv_pages* p, const fv_table* t) {
+  if (!p || !t) return 0;
+  return 4 * (4 + (t->nseq + 4) / 4 * 4 + 3 * ((fv::most_pages(p, t) + 3) / 4 * 4));
+}
+
+extern "C" int fv_pages_extend_dev(const fv_pages* p, void* stream, const fv_kv* const* caches, size_t ncaches, const fv_table* t, const int32_t* lens,
+                                   const int32_t* more, int32_t* missing, void* work, size_t work_bytes) {
+  const char* w = "fv_pages_extend_dev";
+  FV_TRY(fv::pages_check(p, w));
+  FV_TRY(fv::table_check(p, t, w));
+  FV_TRY(fv::caches_check(p, caches, ncaches, w));
+  if (t->nseq && (!lens || !more)) return fv::fail(FV_ERR_ARG, std::string(w) + ": NULL lens or more");
+  if (!missing || !fv::kv_aligned(missing, 4) || !fv::kv_aligned(lens, 4) || !fv::kv_aligned(more, 4))
+    return fv::fail(FV_ERR_ARG, std::string(w) + ": missing is not there, or it, lens or more does not begin on 4 bytes");
+  if (!work || !fv::kv_aligned(work, 16) || work_bytes < fv_pages_extend_work(p, t)) return fv::fail(FV_ERR_ARG, std::string(w) + ": work is smaller than fv_pages_extend_work says, or does not begin on 16 bytes");
+  if (t->nseq * t->width > size_t(1) << 30) return fv::fail(FV_ERR_UNSUPPORTED, std::string(w) + ": the table has more than 2^30 entries");
+  fv::DeviceGuard g(p->device);
+  if (!g.ok) return fv::fail(FV_ERR_CUDA, "cudaSetDevice failed (there is no CPU path)");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const size_t most = fv::most_pages(p, t), room = (most + 3) / 4 * 4;
+  int32_t* const at = static_cast<int32_t*>(work);
+  fv::Extend x{lens, more, missing, at, at + 4, nullptr, nullptr, nullptr};
+  x.free = x.before + (t->nseq + 4) / 4 * 4, x.src = x.free + room, x.dst = x.src + room;
+  fv::pages_extend_kernel<<<1, fv::PAGES_THREADS, 0, s>>>(fv::pages_of(p), fv::table_of(t), x);
+  FV_CUDA(cudaGetLastError());
+  for (size_t i = 0; i < ncaches; ++i) FV_TRY(fv::copy_pages(caches[i], s, x.src, x.dst, most, x.count));
+  return FV_OK;
+}
+
+extern "C" size_t fv_pages_compact_work(const fv_pages* p) { return p ? 4 * (4 + 2 * ((p->pages + 3) / 4 * 4)) : 0; }
+
+extern "C" int fv_pages_compact_dev(const fv_pages* p, void* stream, const fv_kv* const* caches, size_t ncaches, int32_t* used, int32_t* map, void* work, size_t work_bytes) {
+  const char* w = "fv_pages_compact_dev";
+  FV_TRY(fv::pages_check(p, w));
+  FV_TRY(fv::caches_check(p, caches, ncaches, w));
+  if (!used || (!map && p->pages) || !fv::kv_aligned(used, 4) || !fv::kv_aligned(map, 4)) return fv::fail(FV_ERR_ARG, std::string(w) + ": used or map is not there or does not begin on 4 bytes");
+  if (!work || !fv::kv_aligned(work, 16) || work_bytes < fv_pages_compact_work(p)) return fv::fail(FV_ERR_ARG, std::string(w) + ": work is smaller than fv_pages_compact_work says, or does not begin on 16 bytes");
+  fv::DeviceGuard g(p->device);
+  if (!g.ok) return fv::fail(FV_ERR_CUDA, "cudaSetDevice failed (there is no CPU path)");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int32_t* const at = static_cast<int32_t*>(work);
+  int32_t *const src = at + 4, *const dst = src + (p->pages + 3) / 4 * 4;
+  fv::pages_compact_kernel<<<1, fv::PAGES_THREADS, 0, s>>>(fv::pages_of(p), map, used, at, src, dst);
+  FV_CUDA(cudaGetLastError());
+  for (size_t i = 0; i < ncaches; ++i) FV_TRY(fv::copy_pages(caches[i], s, src, dst, size_t(p->pages), at));
+  return FV_OK;
+}
+
+extern "C" int fv_pages_remap_dev(const fv_pages* p, void* stream, const int32_t* map, const fv_table* t) {
+  const char* w = "fv_pages_remap_dev";
+  FV_TRY(fv::pages_check(p, w));
+  FV_TRY(fv::table_check(p, t, w));
+  if (t->nseq == 0 || t->width == 0 || p->pages == 0) return FV_OK;
+  if (!map || !fv::kv_aligned(map, 4)) return fv::fail(FV_ERR_ARG, std::string(w) + ": map is not there or does not begin on 4 bytes");
+  fv::DeviceGuard g(p->device);
+  if (!g.ok) return fv::fail(FV_ERR_CUDA, "cudaSetDevice failed (there is no CPU path)");
+  fv::pages_remap_kernel<<<fv::table_grid(t), 256, 0, static_cast<cudaStream_t>(stream)>>>(map, int(p->pages), fv::table_of(t));
+  FV_CUDA(cudaGetLastError());
+  return FV_OK;
+}

@@ -91,6 +91,7 @@ class KvCache:
         self._empty_like, self._contiguous = torch.empty_like, torch.contiguous_format
         self._get_stream, self._work_sizes = torch._C._cuda_getCurrentRawStream, {}
         self._add, self._vectors, self._search, self._attend = L.fv_kv_add_dev, L.fv_kv_vectors_dev, L.fv_kv_search_dev, L.fv_kv_attend_dev
+        self._copy = L.fv_kv_copy_pages_dev
 
     k, v, bounds, bound_codes, bound_scale, k_scale, v_scale = (
         property(lambda self, name=name: self._held.get(name)) for name in ("k", "v", "bounds", "bound_codes", "bound_scale", "k_scale", "v_scale"))
@@ -164,6 +165,16 @@ class KvCache:
         if status:
             check(status)
         return k, v
+
+    def copy_pages(self, src, dst):
+        """Copies page `src[i]` to `dst[i]`, rows, scales and bounds (int32 tensors of one length).  No page is twice in `dst`, or in both; pairs
+        with a number that is no page are skipped.  `KvPages` does this where sequences share pages."""
+        for x in (src, dst):
+            if x.dtype is not self._i32 or x.device != self.device or x.dim() != 1 or not x.is_contiguous() or len(x) != len(src):
+                _refuse(f"src and dst are contiguous int32 tensors of one length on {self.device}")
+        status = self._copy(self._ref, self._get_stream(self._index), src.data_ptr(), dst.data_ptr(), len(src), None)
+        if status:
+            check(status)
 
     def _check_out(self, x, shape):
         if tuple(x.shape) != shape or x.dtype is not self.dtype or x.device != self.device or not x.is_contiguous() or x.data_ptr() & 15:

@@ -385,6 +385,74 @@ int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, co
  * lists of blocks; a call over short ones may not use it.  Without it (NULL) the call is as right, and slower where there are few rows. */
 size_t fv_kv_attend_work(const fv_kv* kv, const fv_kv_batch* batch, size_t group);
 
+/* ---- rotary positions (no counterpart in src/vector): queries and keys turned by their rows' positions, before they are added to a
+ * cache and attended to.  Of `dim` components the first `part` are turned in pairs, component i with i + part/2 (half) or 2 i with 2 i + 1
+ * (pairs): y_i = amplitude (x_i cos t - x_j sin t), y_j = amplitude (x_j cos t + x_i sin t), t = 2 pi * position * turns[i] / 2^64.
+ * `turns` (device memory, part/2 numbers) is what a pair turns by at each position, as a fraction of 2^64 of a whole turn, so that far
+ * positions are as exact as near ones.  dim and part are multiples of 16, dim at most 1024.  `back`: the transposed turn (sin t -> -sin t),
+ * which gradients take and which, but for the amplitude's square, undoes the other.
+ *
+ * Row i of a call has the position that fv_kv_batch gives it (lens, cu), or positions[i].  Rows of no sequence and positions below 0
+ * are skipped: nothing is read or written there.  One call turns up to four tensors of the same rows ([rows][heads][dim], strides in
+ * elements, multiples of 8).  `out` may be `in` with the same strides; otherwise they do not overlap. */
+enum { FV_ROTARY_HALF = 0, FV_ROTARY_PAIRS = 1 }; /* layout */
+typedef struct fv_rotary {
+  int device;
+  int dtype; /* FV_KV_BF16 or FV_KV_FP16 */
+  uint32_t dim;
+  uint32_t part;
+  int layout;
+  float amplitude;
+  const uint64_t* turns;
+} fv_rotary;
+typedef struct fv_rotary_rows {
+  const void* in;
+  void* out;
+  size_t in_row, in_head, out_row, out_head;
+  size_t heads;
+} fv_rotary_rows;
+int fv_rotate_dev(const fv_rotary* r, void* stream, const fv_rotary_rows* x, size_t count, size_t rows, const int32_t* lens,
+                  const int32_t* cu, size_t nseq, const int32_t* positions, int back);
+
+/* ---- which pages of caches are in use (no counterpart in src/vector): refs[p] is how many entries of tables hold page p, 0: it is free.
+ * Sequences may share pages.  All memory is the caller's, on `device`; the calls launch on the stream, do not wait, allocate nothing and may be
+ * captured; those of one set of pages are ordered by their streams.  `caches`: the caches whose rows lie in these pages (the layers of
+ * a model), all of `pages` pages of `page_size` rows.  A table entry outside 0 .. pages-1 is none.
+ *
+ * fork: row i of `out` becomes row parents[i] of the table, up to the block of its lens' last row (NULL: all of it), and every page in it counts
+ * one more; -1 behind them, and everywhere where parents[i] is no row.  out is not the table.
+ * free: entries from the first block behind lens (NULL: all) on become -1, and their pages count one less (never below 0).
+ * extend: room for more[b] rows behind lens[b]: of the blocks that those rows come to, one without a page gets a free one, and one
+ * whose page others hold as well gets a free one with a copy of its rows; where all who hold a page are among these blocks, the first
+ * in the table's order keeps it.  Free pages are taken in ascending order, for blocks in the table's order.  Blocks behind the table's width
+ * get none.  If there are fewer free pages than blocks to fill nothing is changed (entries that were none may have become -1), and *missing is how many
+ * are lacking; otherwise it is 0.
+ * compact: of the n pages in use those from n on move to the free ones below n, ascending to ascending; *used = n; map[p] is where
+ * page p lies now (-1: free).  remap: entries of a table become map of what they were. */
+typedef struct fv_pages {
+  int device;
+  uint32_t page_size;
+  uint64_t pages;
+  int32_t* refs;
+} fv_pages;
+typedef struct fv_table {
+  int32_t* table; /* [nseq][width] */
+  size_t stride;  /* from one row to the next */
+  size_t width;
+  size_t nseq;
+} fv_table;
+int fv_pages_fork_dev(const fv_pages* p, void* stream, const fv_table* from, const int32_t* lens, const int32_t* parents, const fv_table* out);
+int fv_pages_free_dev(const fv_pages* p, void* stream, const fv_table* t, const int32_t* lens);
+int fv_pages_extend_dev(const fv_pages* p, void* stream, const fv_kv* const* caches, size_t ncaches, const fv_table* t, const int32_t* lens,
+                        const int32_t* more, int32_t* missing, void* work, size_t work_bytes);
+size_t fv_pages_extend_work(const fv_pages* p, const fv_table* t); /* bytes of `work`, on 16 bytes */
+int fv_pages_compact_dev(const fv_pages* p, void* stream, const fv_kv* const* caches, size_t ncaches, int32_t* used, int32_t* map, void* work, size_t work_bytes);
+size_t fv_pages_compact_work(const fv_pages* p);
+int fv_pages_remap_dev(const fv_pages* p, void* stream, const int32_t* map, const fv_table* t);
+/* Copies page src[i] of a cache to dst[i], for i below n and, where `count` (device memory) is given, below *count.  Pairs with a number
+ * that is no page are skipped.  No page is twice in dst, or in both. */
+int fv_kv_copy_pages_dev(const fv_kv* kv, void* stream, const int32_t* src, const int32_t* dst, size_t n, const int32_t* count);
+
 /* ---- seeded synthetic data for benchmarks and tests: a mixture of `clusters` Gaussians.
  * kind 0: centres uniform in [0,255]^dim, sigma 30, clipped to [0,255] and rounded (SIFT-like integers);
  * kind 1: centres normal*3, sigma 1, rows then scaled to unit length (embedding-like).
