@@ -221,11 +221,19 @@ struct Four {
     return __byte_perm(w[g / 2], w[(NG + g) / 2], (g & 1 ? 0x32 : 0x10) | ((NG + g) & 1 ? 0x7600 : 0x5400));
   }
   // Eight codes to the pairs (0, 4), (1, 5), (2, 6), (3, 7) of fp16, exactly: a code is added to 1024, or 16 times it to 1024, by its place.
-  static __device__ __forceinline__ void halves(uint32_t w, uint32_t* to) {
+  // (One instruction masks and adds where one of its two constants is in a register; the compiler, which knows both, would take two.)
+  static __device__ __forceinline__ uint32_t magic(uint32_t x) {
+    uint32_t y;
+    asm volatile("mov.b32 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+  }
+  static __device__ __forceinline__ void halves(uint32_t w, uint32_t* to, uint32_t by_1024, uint32_t by_64) {  // magic(0x64006400), magic(0x54005400)
     const __half2 low = __half2half2(__ushort_as_half(0x6408)), high = __half2half2(__ushort_as_half(0x5480));  // 1032, 72
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t y = i ? w >> 8 : w, x0 = (y & 0x000F000Fu) | 0x64006400u, x1 = (y & 0x00F000F0u) | 0x54005400u;
+      uint32_t x0, x1;
+      asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(x0) : "r"(i ? w >> 8 : w), "r"(by_1024));
+      asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(x1) : "r"(i ? w >> 8 : w), "r"(by_64));
       const __half2 u = __hsub2(*reinterpret_cast<const __half2*>(&x0), low), v = __hsub2(*reinterpret_cast<const __half2*>(&x1), high);
       to[2 * i] = *reinterpret_cast<const uint32_t*>(&u), to[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&v);
     }
@@ -258,6 +266,12 @@ __device__ __forceinline__ void mma_16(float* c, uint32_t a0, uint32_t a1, uint3
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = a b in fp16
+__device__ __forceinline__ void mma_16_of(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 // Four 8-bit codes as two pairs of fp16, exactly: (0, 1) and (2, 3).
 template <int KIND>

@@ -27,6 +27,7 @@
 #include <climits>
 
 #include "kv.cuh"
+#include "tc.cuh"
 
 namespace fv {
 
@@ -84,6 +85,33 @@ __device__ __forceinline__ void load_words(uint32_t* to, const void* from) {
   } else {
     to[0] = *static_cast<const uint32_t*>(from);
   }
+}
+
+// N words, or bytes, from an address in shared memory.
+template <int N>
+__device__ __forceinline__ void shared_words(uint32_t* to, uint32_t from) {
+  if constexpr (N == 4) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(to[0]), "=r"(to[1]), "=r"(to[2]), "=r"(to[3]) : "r"(from));
+  else if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(to[0]), "=r"(to[1]) : "r"(from));
+  else
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(to[i]) : "r"(from + 4 * i));
+}
+template <int N>
+__device__ __forceinline__ uint32_t shared_bytes(uint32_t from) {
+  uint32_t x, y;
+  if constexpr (N == 4) {
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(from));
+  } else if constexpr (N == 2) {
+    asm volatile("{\n.reg .u16 h;\nld.shared.u16 h, [%1];\ncvt.u32.u16 %0, h;\n}\n" : "=r"(x) : "r"(from));
+  } else {
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(from));
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+      asm volatile("ld.shared.u8 %0, [%1];" : "=r"(y) : "r"(from + i));
+      x |= y << (8 * i);
+    }
+  }
+  return x;
 }
 
 // Pieces of 16 rows of one block on their way through a warp's part of shared memory, and which components a lane takes from
@@ -160,55 +188,26 @@ struct Stage {
   static __device__ __forceinline__ int seen(const unsigned char* s) { return *reinterpret_cast<const int*>(s + 2 * 16 * ROW + SCALES); }
 };
 
-// The same in 4 bits.  A row is a quarter of 16 bits' bytes, so a lane takes a quarter of a key, eight components of each of NG groups,
-// and an eighth of a value, four of each, in one piece where NG is even.  32-byte pieces of values change places by
-// the row's number, where rows of 16 bytes' lanes would meet in the same banks.
+// The same in 4 bits: a few lanes start a bulk copy each, of two pieces' keys, values and scales, and a barrier of the stage counts their
+// bytes, so that the others' instructions go to the products.  A lane takes a quarter of a key, eight components of each of NG groups, and
+// an eighth of a value, four of each.  The products' rows are the tokens with every second pair the other way round: for keys, two
+// rows of 64 bytes that are read at one time lie next to each other, and of the four rows of values two do.
 template <int D>
 struct Stage<FV_KV_INT4X32, D> {
-  static constexpr int NG = D / 32, ROW = D / 2, SCALE = 16 * NG;     // SCALE: bytes of 16 rows' scales
-  static constexpr int PIECE = 2 * 16 * ROW + 2 * SCALE + 16;          // keys, values, scales, how many of the rows are seen
+  static constexpr int NG = D / 32, ROW = D / 2, SCALE = 16 * NG;  // SCALE: bytes of 16 rows' scales
   static constexpr int PIECES = 2;
-  static constexpr int SIZE = PIECES * PIECE;
+  static constexpr int VALUES = PIECES * 16 * ROW, KEY_SCALES = 2 * VALUES, VALUE_SCALES = KEY_SCALES + PIECES * SCALE;  // where they lie: each of both pieces
+  static constexpr int SEEN = VALUE_SCALES + PIECES * SCALE, SIZE = SEEN + 16;                                           // how many of the rows are seen
   static constexpr int LEAST = 4 / PIECES;
   static constexpr int DEPTH = 13 * 1024 / SIZE < 2 ? 2 : 13 * 1024 / SIZE > 6 ? 6 : 13 * 1024 / SIZE;
 
   static __device__ __forceinline__ int value_at(int e, int g) { return 32 * (e >> 2) + 4 * g + (e & 3); }
-  static __device__ __forceinline__ int value_byte(int r, int at) {
-    if (ROW == 64) return (r >> 1) * 128 + ((((r & 1) * 2 + (at >> 5)) ^ (r >> 1 & 3)) << 5) + (at & 31);
-    if (ROW == 32) return (r >> 1) * 64 + (((r ^ r >> 2) & 1) << 5) + at;
-    return r * ROW + at;
-  }
-  static __device__ __forceinline__ void fill(unsigned char* s, const KvAttend& a, int page, int head, int page_shift, int slot, int seen, int lane) {
-    if (lane == 0) *reinterpret_cast<int*>(s + 2 * 16 * ROW + 2 * SCALE) = min(seen, 16);
-    if (seen <= 0) return;
-    const size_t at = ((size_t(page) * a.heads + head) << page_shift) + slot;
-    const unsigned char *kr = a.kp + at * ROW, *vr = a.vp + at * ROW;
-    const uint32_t to = uint32_t(__cvta_generic_to_shared(s));
-#pragma unroll
-    for (int i = 0; i < (ROW + 31) / 32; ++i) {
-      const int n = (lane + 32 * i) * 16, r = n / ROW;
-      if (ROW % 32 && n >= 16 * ROW) continue;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + n), "l"(kr + n));
-      // zeros in place of values that are not seen
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 16 * ROW + value_byte(r, n - r * ROW)), "l"(vr + n), "r"(r < seen ? 16 : 0));
-    }
-    if (lane < 2 * NG) {
-      const bool values = lane >= NG;
-      const int n = (values ? lane - NG : lane) * 16;
-      const unsigned char* from = reinterpret_cast<const unsigned char*>(values ? a.v_scale : a.k_scale) + at * NG + n;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 2 * 16 * ROW + lane * 16), "l"(from), "r"(min(max(seen * NG - n, 0), 16)));
-    }
-  }
-  static __device__ __forceinline__ int seen(const unsigned char* s) { return *reinterpret_cast<const int*>(s + 2 * 16 * ROW + 2 * SCALE); }
-  // The scales of a row, a byte each, as fp16: groups 0 and 2, then 1 and 3.
-  static __device__ __forceinline__ void scales(const unsigned char* s, int r, uint32_t* to) {
-    uint32_t w;
-    if constexpr (NG == 4) w = *reinterpret_cast<const uint32_t*>(s + 4 * r);
-    else if constexpr (NG == 2) w = *reinterpret_cast<const uint16_t*>(s + 2 * r);
-    else w = s[3 * r] | uint32_t(s[3 * r + 1]) << 8 | uint32_t(s[3 * r + 2]) << 16;
-    to[0] = (w & 0x00FF00FFu) << 7, to[1] = (w & 0xFF00FF00u) >> 1;
-  }
+  static __device__ __forceinline__ int token(int row) { return row ^ (row >> 1 & 1); }
+  // The bytes of a row's scales as fp16: groups 0 and 2, then 1 and 3.
+  static __device__ __forceinline__ void halves_of(uint32_t w, uint32_t* to) { to[0] = (w & 0x00FF00FFu) << 7, to[1] = (w & 0xFF00FF00u) >> 1; }
 };
+
+constexpr float KV_LAG = 6.f;  // 4 bits: log2 of what a maximum may lag behind by
 
 // A warp's share of a row's attention: NT tiles of 8 queries.  A lane's queries are 8 x + 2 t and the next one.
 template <class T, int KIND, int D, int NT>
@@ -216,11 +215,13 @@ struct Share {
   using M = typename std::conditional<KIND == FV_KV_SAME, T, __half>::type;
   using L = Stage<KIND, D>;
   static constexpr bool TWO = std::is_same<M, __nv_bfloat16>::value, FOUR = KIND == FV_KV_INT4X32, SCALED = KIND != FV_KV_SAME && !FOUR;
-  static constexpr float ONE = TWO ? 0.f : 14.f;  // log2 of what stands for a weight of 1
+  static constexpr float ONE = TWO ? 0.f : FOUR ? 7.f : 14.f;  // log2 of what stands for a weight of 1
   uint32_t q[D / 16][NT][2];
   float by[NT][2];  // scale of a lane's queries
   float o[D / 16][NT][4], m[NT][2], l[NT][2];
-  int unit;  // 8 bits: values stand for multiples of 2^(unit - 126)
+  uint32_t by_1024, by_64;  // 4 bits: what codes are added to
+  int unit;  // 8 bits: values stand for multiples of 2^(unit - 126); 4 bits: 2^(ONE - unit) for a weight of 1
+  float far[NT][2];  // 4 bits: a maximum is replaced by one above this
 
   __device__ __forceinline__ void begin(const KvAttend& a, int row, int head, int first, int g, int t) {
 #pragma unroll
@@ -270,7 +271,7 @@ struct Share {
       for (int i = 0; i < 2; ++i) by[x][i] = a.scale / __shfl_sync(FV_FULL, f, (2 * t + i) * 4);
     }
 #pragma unroll
-    for (int x = 0; x < NT; ++x) m[x][0] = m[x][1] = -INFINITY, l[x][0] = l[x][1] = 0.f;
+    for (int x = 0; x < NT; ++x) m[x][0] = m[x][1] = far[x][0] = far[x][1] = -INFINITY, l[x][0] = l[x][1] = 0.f;
 #pragma unroll
     for (int u = 0; u < D / 16; ++u)
 #pragma unroll
@@ -278,40 +279,44 @@ struct Share {
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[u][x][i] = 0.f;
     unit = 0;
+    if constexpr (FOUR) by_1024 = Four::magic(0x64006400u), by_64 = Four::magic(0x54005400u);
   }
 
-  __device__ __forceinline__ void take(const unsigned char* stage, int g, int t) {
-    if constexpr (FOUR) take_four(stage, g, t);
-    else take_rows(stage, g, t);
+  __device__ __forceinline__ void take_all(uint32_t stage, int g, int t) {
+    if constexpr (NT == 1) take_four<L::PIECES>(stage, 0, g, t);
+    else  // one piece at a time: the registers
+#pragma unroll 1
+      for (int h = 0; h < L::PIECES; ++h) take_four<1>(stage, h, g, t);
   }
 
-  // 4 bits: codes are exact in fp16.  A key's scales multiply the sums over their groups; a value is multiplied by its scale, exactly, before
-  // its product.
-  __device__ __forceinline__ void take_four(const unsigned char* stage, int g, int t) {
-    constexpr int P = L::PIECES, NG = D / 32;
+  // 4 bits: codes are exact in fp16.  A key's scales multiply the sums over their groups; a value's multiply the weights, in fp16.  For
+  // these to stay in range a weight of 1 is 2^(ONE - unit), where unit grows with scales of 2 and more, and a maximum that grows by
+  // less than 2^KV_LAG is left as it was: with few pieces to a warp, most of them have a new one (two thirds of the time went there).
+  // (Codes below fp16's normal numbers, masked out of their words and not subtracted from, would be less work; the tensor cores
+  // keep ten bits less of a sum of such products.)
+  template <int P>
+  __device__ __forceinline__ void take_four(uint32_t stage, int first, int g, int t) {
+    constexpr int NG = D / 32;
     int visible[P], any = 0;
 #pragma unroll
-    for (int h = 0; h < P; ++h) visible[h] = L::seen(stage + h * L::PIECE), any = max(any, visible[h]);
+    for (int h = 0; h < P; ++h) visible[h] = int(shared_bytes<4>(stage + L::SEEN + 4 * (first + h))), any = max(any, visible[h]);
     if (any <= 0) return;
+    const uint32_t keys = stage + (16 * first + L::token(g)) * L::ROW + t * 4 * NG, key_scales = stage + L::KEY_SCALES + (16 * first + L::token(g)) * NG;
+    const uint32_t values = stage + L::VALUES + 16 * first * L::ROW + g * 2 * NG, value_scales = stage + L::VALUE_SCALES + 16 * first * NG;
     float s[P][NT][4];
 #pragma unroll
     for (int h = 0; h < P; ++h) {
-      const unsigned char* const keys = stage + h * L::PIECE;
       uint32_t k[2][NG], sc[2][2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const unsigned char* from = keys + (g + 8 * i) * L::ROW + t * 4 * NG;
-        if constexpr (NG == 3) load_words<1>(k[i], from), load_words<1>(k[i] + 1, from + 4), load_words<1>(k[i] + 2, from + 8);
-        else load_words<NG>(k[i], from);
-        L::scales(keys + 2 * 16 * L::ROW, g + 8 * i, sc[i]);
+        shared_words<NG>(k[i], keys + (16 * h + 8 * i) * L::ROW);
+        L::halves_of(shared_bytes<NG>(key_scales + (16 * h + 8 * i) * NG), sc[i]);
       }
-#pragma unroll
-      for (int x = 0; x < NT; ++x) s[h][x][0] = s[h][x][1] = s[h][x][2] = s[h][x][3] = 0.f;
 #pragma unroll
       for (int y = 0; y < NG; ++y) {
         uint32_t a[2][4];
-        Four::halves(Four::group<NG>(k[0], y), a[0]);
-        Four::halves(Four::group<NG>(k[1], y), a[1]);
+        Four::halves(Four::group<NG>(k[0], y), a[0], by_1024, by_64);
+        Four::halves(Four::group<NG>(k[1], y), a[1], by_1024, by_64);
         float ks[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -320,29 +325,64 @@ struct Share {
         }
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-          float c[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_16<M>(c, a[0][0], a[1][0], a[0][1], a[1][1], q[2 * y][x][0], q[2 * y][x][1]);
+          float c[4];
+          mma_16_of(c, a[0][0], a[1][0], a[0][1], a[1][1], q[2 * y][x][0], q[2 * y][x][1]);
           mma_16<M>(c, a[0][2], a[1][2], a[0][3], a[1][3], q[2 * y + 1][x][0], q[2 * y + 1][x][1]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[h][x][i] = __fmaf_rn(c[i], ks[i >> 1], s[h][x][i]);
+          for (int i = 0; i < 4; ++i) s[h][x][i] = y ? __fmaf_rn(c[i], ks[i >> 1], s[h][x][i]) : c[i] * ks[i >> 1];
         }
       }
     }
-    bool moved = false;
+    uint32_t vs[P][4], high = 0u;  // scales of rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9
+#pragma unroll
+    for (int h = 0; h < P; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        vs[h][i] = shared_bytes<NG>(value_scales + L::token(2 * t + (i & 1)) * NG + (16 * h + (i & 2) * 4) * NG);
+      }
+#pragma unroll
+    for (int h = 0; h < P; ++h) {
+      if (visible[h] < 16) {  // of rows that are not seen the scales are anything
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vs[h][i] = L::token(2 * t + (i & 1)) + (i & 2) * 4 < visible[h] ? vs[h][i] : 0u;
+      }
+      high |= (vs[h][0] | vs[h][1]) | (vs[h][2] | vs[h][3]);
+    }
+    bool moved = (high & 0x80808080u) != 0u, odd = false;  // a scale of 2 or more
     float to[NT][2];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
 #pragma unroll
       for (int h = 0; h < P; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[h][x][i] = g + (i & 2) * 4 < visible[h] ? s[h][x][i] * by[x][i & 1] : -INFINITY;
+        for (int i = 0; i < 4; ++i) s[h][x][i] *= by[x][i & 1];
+#pragma unroll
+      for (int h = 0; h < P; ++h)
+        if (visible[h] < 16) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[h][x][i] = L::token(g) + (i & 2) * 4 < visible[h] ? s[h][x][i] : -INFINITY;
+        }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        to[x][i] = fmaxf(fmaxf(s[0][x][i], s[0][x][i + 2]), fmaxf(s[P - 1][x][i], s[P - 1][x][i + 2]));
-        moved = moved || to[x][i] > m[x][i];
+        to[x][i] = fmaxf(s[0][x][i], s[0][x][i + 2]);
+        if constexpr (P > 1) to[x][i] = fmaxf(to[x][i], fmaxf(s[P - 1][x][i], s[P - 1][x][i + 2]));
+        moved = moved || to[x][i] > far[x][i];
       }
     }
     if (__any_sync(FV_FULL, moved)) {  // seldom, after the first pieces
+      uint32_t most = 0;  // of the scales that are numbers
+#pragma unroll
+      for (int h = 0; h < P; ++h)
+#pragma unroll
+        for (int i = 0; i < 4 * NG; ++i) {
+          const uint32_t byte = vs[h][i / NG] >> (8 * (i % NG)) & 255u;
+          if (byte < 248u) most = max(most, byte);
+          odd = odd || byte >= 248u;
+        }
+      odd = __any_sync(FV_FULL, odd);
+      const int up = max(unit, int(__reduce_max_sync(FV_FULL, most) >> 3) - 16);  // below 2^(e - 14) = 2^(2 + unit)
+      const float less = __uint_as_float(uint32_t(127 + unit - up) << 23);
+      unit = up;
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -351,65 +391,102 @@ struct Share {
           y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 4));
           y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 8));
           y = fmaxf(y, __shfl_xor_sync(FV_FULL, y, 16));
-          const float down = y > m[x][i] ? exp2_of(m[x][i] - y) : 1.f;
-          m[x][i] = y;
+          y = y > far[x][i] ? y : m[x][i];
+          const float down = (y > m[x][i] ? exp2_of(m[x][i] - y) : 1.f) * less;
+          m[x][i] = y, far[x][i] = y == -INFINITY ? y : y + KV_LAG;
           l[x][i] *= down;
 #pragma unroll
           for (int u = 0; u < D / 16; ++u) o[u][x][i] *= down, o[u][x][i + 2] *= down;
         }
     }
     uint32_t b[P][NT][2];
+    const float one = ONE - float(unit);
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
+    for (int x = 0; x < NT; ++x) {
+      const float off[2] = {one - (m[x][0] == -INFINITY ? 0.f : m[x][0]), one - (m[x][1] == -INFINITY ? 0.f : m[x][1])};
 #pragma unroll
       for (int h = 0; h < P; ++h) {
         float p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[i] = exp2_of(s[h][x][i] - (m[x][i & 1] == -INFINITY ? 0.f : m[x][i & 1]) + ONE);
+          p[i] = exp2_of(s[h][x][i] + off[i & 1]);
           l[x][i & 1] += p[i];
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) b[h][x][i] = transposed(Pair<M>::from_float(p[2 * i], p[2 * i + 1]));
       }
+    }
+    if (odd) {  // scales that are no numbers: theirs are the groups' results for queries that have a weight for them; in the products they are zeros
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t bad = 0u;  // bit y: group y's result
+#pragma unroll
+          for (int h = 0; h < P; ++h)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t w = shared_bytes<NG>(value_scales + L::token(g) * NG + (16 * h + 8 * r) * NG);
+              const bool weight = exp2_of(s[h][x][2 * r + i] + one - (m[x][i] == -INFINITY ? 0.f : m[x][i])) != 0.f;
+#pragma unroll
+              for (int y = 0; y < NG; ++y) bad |= L::token(g) + 8 * r < visible[h] && weight && (w >> (8 * y) & 255u) >= 248u ? 1u << y : 0u;
+            }
+          bad |= __shfl_xor_sync(FV_FULL, bad, 4);
+          bad |= __shfl_xor_sync(FV_FULL, bad, 8);
+          bad |= __shfl_xor_sync(FV_FULL, bad, 16);
+#pragma unroll
+          for (int u = 0; u < D / 16; ++u)
+            if (bad >> (u / 2) & 1u) o[u][x][i] = o[u][x][i + 2] = __int_as_float(0x7FC00000);
+        }
+#pragma unroll
+      for (int h = 0; h < P; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int y = 0; y < NG; ++y)
+            if ((vs[h][i] >> (8 * y) & 255u) >= 248u) vs[h][i] &= ~(255u << (8 * y));
+    }
 #pragma unroll
     for (int h = 0; h < P; ++h) {
       if (visible[h] <= 0) continue;  // its values are anything
-      const unsigned char *const values = stage + h * L::PIECE + 16 * L::ROW, *const scales = stage + h * L::PIECE + 2 * 16 * L::ROW + L::SCALE;
-      uint32_t v[4][(NG + 1) / 2], sc[4][2];  // of rows 2 t, 2 t + 1, 2 t + 8 and 2 t + 9: four components of every group
+      uint32_t v[4][(NG + 1) / 2], sc[2][NG];  // four components of every group; the groups' scales of two rows
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = 2 * t + (i & 1) + (i & 2) * 4;
-        if constexpr (NG == 3) {
-          const uint16_t* from = reinterpret_cast<const uint16_t*>(values + L::value_byte(r, g * 6));
-          v[i][0] = from[0] | uint32_t(from[1]) << 16, v[i][1] = from[2];
-        } else {
-          load_words<NG / 2>(v[i], values + L::value_byte(r, g * 2 * NG));
-        }
-        L::scales(scales, r, sc[i]);
+        const uint32_t from = values + L::token(2 * t + (i & 1)) * L::ROW + (16 * h + (i & 2) * 4) * L::ROW;
+        if constexpr (NG == 3) v[i][0] = shared_bytes<2>(from) | shared_bytes<2>(from + 2) << 16, v[i][1] = shared_bytes<2>(from + 4);
+        else shared_words<NG / 2>(v[i], from);
       }
 #pragma unroll
+      for (int z = 0; z < 2; ++z)
+#pragma unroll
+        for (int y = 0; y < NG; y += 2) {
+          uint32_t two[2];
+          L::halves_of(__byte_perm(vs[h][2 * z], vs[h][2 * z + 1], y ? 0x7632 : 0x5410), two);
+          sc[z][y] = two[0];
+          if (y + 1 < NG) sc[z][y + 1] = two[1];
+        }
+#pragma unroll
       for (int y = 0; y < NG; ++y) {
-        uint32_t a[2][4];  // [rows 2 t, or 2 t + 8, and the next one][component]
+        uint32_t a[2][4], w[NT][2];  // [rows 2 t, or 2 t + 8, and the next one][component]
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          Four::halves(__byte_perm(v[2 * z][y / 2], v[2 * z + 1][y / 2], y & 1 ? 0x7632 : 0x5410), a[z]);
-          const uint32_t w = __byte_perm(sc[2 * z][y & 1], sc[2 * z + 1][y & 1], y < 2 ? 0x5410 : 0x7632);
+          Four::halves(__byte_perm(v[2 * z][y / 2], v[2 * z + 1][y / 2], y & 1 ? 0x7632 : 0x5410), a[z], by_1024, by_64);
+          const uint32_t f = sc[z][y];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const __half2 f = __hmul2(*reinterpret_cast<const __half2*>(&a[z][e]), *reinterpret_cast<const __half2*>(&w));
-            a[z][e] = *reinterpret_cast<const uint32_t*>(&f);
+          for (int x = 0; x < NT; ++x) {
+            const __half2 c = __hmul2(*reinterpret_cast<const __half2*>(&b[h][x][z]), *reinterpret_cast<const __half2*>(&f));
+            w[x][z] = *reinterpret_cast<const uint32_t*>(&c);
           }
         }
 #pragma unroll
-        for (int z = 0; z < 2; ++z)
+        for (int x = 0; x < NT; ++x)
 #pragma unroll
-          for (int x = 0; x < NT; ++x) mma_16<M>(o[2 * y + z][x], a[0][2 * z], a[0][2 * z + 1], a[1][2 * z], a[1][2 * z + 1], b[h][x][0], b[h][x][1]);
+          for (int z = 0; z < 2; ++z) mma_16<M>(o[2 * y + z][x], a[0][2 * z], a[0][2 * z + 1], a[1][2 * z], a[1][2 * z + 1], w[x][0], w[x][1]);
       }
     }
   }
 
-  __device__ __forceinline__ void take_rows(const unsigned char* stage, int g, int t) {
+  __device__ __forceinline__ void take(const unsigned char* stage, int g, int t) {
     constexpr int P = L::PIECES;
     int visible[P], any = 0;
 #pragma unroll
@@ -550,14 +627,21 @@ struct Share {
     }
   }
 
+  // Results of a wait that ran out are no numbers.
+  __device__ __forceinline__ void spoil() {
+#pragma unroll
+    for (int x = 0; x < NT; ++x) m[x][0] = m[x][1] = l[x][0] = l[x][1] = __int_as_float(0x7FC00000);
+  }
+
   // The share as it lies in registers: for every two components u and tile x a float4 of each lane, then the maxima and the sums
   // of weights of the 8 NT queries.  A value's unit is multiplied in.
   static constexpr int FLOATS = 8 * NT * (D + 2);
   __device__ __forceinline__ void store(float* to, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    const float f = SCALED ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
+    const float f = SCALED ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : FOUR ? __uint_as_float(uint32_t(127 + unit) << 23) : 1.f;
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
+      if constexpr (FOUR) l[x][0] *= f, l[x][1] *= f;
 #pragma unroll
       for (int u = 0; u < D / 16; ++u)
         reinterpret_cast<float4*>(to)[(u * NT + x) * 32 + lane] = make_float4(o[u][x][0] * f, o[u][x][1] * f, o[u][x][2] * f, o[u][x][3] * f);
@@ -675,6 +759,78 @@ struct Pieces {
   }
 };
 
+// 4 bits: a warp's stages in shared memory, their barriers behind those of all warps.  Lanes 0 to 3 copy keys, values, and scales of
+// either, of both pieces where they are of one block, and with pages of 16 rows lanes 4 to 7 those of the second piece (each copy is some
+// 15 instructions: lanes take turns at it).  Where a page's are, from the first page's on, a lane knows for the head at hand.
+template <int D>
+struct BulkRing {
+  using S = Stage<FV_KV_INT4X32, D>;
+  uint32_t ring, bars;  // addresses in shared memory
+  uint32_t turns;       // bit i: of stage i's barrier
+  bool failed;          // a wait ran out
+  uint32_t to, bytes, row, page;  // of the lane: where its part of a stage is, its bytes, and those of a row and of a page
+  const unsigned char* from;
+  __device__ __forceinline__ void begin(const KvAttend& a, const KvBatch& m, int warp) {
+    const int lane = lane_id(), part = lane & 3;
+    ring = smem_u32(dyn_smem()) + warp * (S::DEPTH * S::SIZE);
+    bars = smem_u32(dyn_smem()) + KV_TOKEN_WARPS * S::DEPTH * S::SIZE + warp * (S::DEPTH * 8);
+    turns = 0u, failed = false;
+    row = part < 2 ? S::ROW : S::NG, page = (uint32_t(a.heads) * row) << m.page_shift;
+    const bool single = m.page_shift == 4;  // pieces are of different blocks
+    bytes = (single ? 16 : 32) * row;
+    to = ring + (part < 2 ? part * S::VALUES : S::KEY_SCALES + (part - 2) * (S::PIECES * S::SCALE)) + (lane >> 2 & 1) * 16 * row;
+    if (lane < S::DEPTH) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bars + lane * 8), "r"(single ? 8u : 4u));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+  }
+  __device__ __forceinline__ void head(const KvAttend& a, const KvBatch& m, int h) {  // the pieces from now on are of key head h
+    const int part = lane_id() & 3;
+    from = part == 0 ? a.kp : part == 1 ? a.vp : reinterpret_cast<const unsigned char*>(part == 2 ? a.k_scale : a.v_scale);
+    from += (size_t(h) * row) << m.page_shift;
+  }
+  // Starts the copies of pieces c and c + 1 (c is even) to stage `at`.
+  __device__ __forceinline__ void fill(Pieces& p, const KvAttend& a, const KvBatch& m, int at, int c) {
+    const int lane = lane_id(), per = m.page_shift - 4, mine = c + (lane >> 2 & 1), i = mine >> per;
+    if (c >> per >= p.base + 32) p.look(a, m, c >> per);
+    const int block = __shfl_sync(FV_FULL, p.block, i & 31), q = __shfl_sync(FV_FULL, p.page, i & 31);
+    if (lane < 8) {
+      const int slot = (mine & ((1 << per) - 1)) << 4, seen = q >= 0 ? p.pos - ((block << m.page_shift) + slot) + 1 : 0;
+      const uint32_t bar = bars + at * 8;
+      if ((lane & 3) == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(ring + at * S::SIZE + S::SEEN + lane), "r"(min(seen, 16)) : "memory");
+      if (per == 0 || lane < 4) {
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(seen > 0 ? bytes : 0u) : "memory");
+        if (seen > 0)
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to + at * S::SIZE),
+                       "l"(from + size_t(uint32_t(q)) * page + uint32_t(slot) * row), "r"(bytes), "r"(bar)
+                       : "memory");
+      }
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ bool landed(int at) const {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bars + at * 8), "r"(turns >> at & 1u)
+        : "memory");
+    return ok != 0u;
+  }
+  __device__ __forceinline__ uint32_t wait(int at) {
+    if (!__all_sync(FV_FULL, landed(at))) {
+      const long long t0 = clock64();
+      while (!__all_sync(FV_FULL, landed(at)))
+        if (__any_sync(FV_FULL, clock64() - t0 > WAIT_LIMIT_CYCLES)) {
+          failed = true;
+          break;
+        }
+    }
+    turns ^= 1u << at;
+    return ring + at * S::SIZE;
+  }
+};
+constexpr int kv_bar_bytes(int kind, int depth) { return kind == FV_KV_INT4X32 ? KV_TOKEN_WARPS * depth * 8 : 0; }
+
 // Pieces of a row: those of its list, or all up to its own position.
 __device__ __forceinline__ int pieces_of(const KvAttend& a, const KvBatch& m, int pos) {
   if (pos < 0) return 0;
@@ -682,8 +838,11 @@ __device__ __forceinline__ int pieces_of(const KvAttend& a, const KvBatch& m, in
 }
 
 // A CTA for one row and key head; its warps take turns at the pieces.
+// 4 bits, one tile of queries: as many CTAs as shared memory holds
+constexpr int kv_least_ctas(int kind, int nt) { return kind == FV_KV_INT4X32 && nt == 1 ? 4 : 0; }
+
 template <class T, int KIND, int D, int NT>
-__global__ void __launch_bounds__(32 * KV_TOKEN_WARPS) kv_token_kernel(KvAttend a, KvBatch m, int tiles) {
+__global__ void __launch_bounds__(32 * KV_TOKEN_WARPS, kv_least_ctas(KIND, NT)) kv_token_kernel(KvAttend a, KvBatch m, int tiles) {
   constexpr int W = KV_TOKEN_WARPS, COLS = 8 * NT;
   using S = Stage<KIND, D>;
   const int warp = threadIdx.x >> 5, lane = lane_id(), g = lane >> 2, t = lane & 3;
@@ -694,6 +853,33 @@ __global__ void __launch_bounds__(32 * KV_TOKEN_WARPS) kv_token_kernel(KvAttend 
   if (pieces.b < 0) return;
   const int n = pieces_of(a, m, pieces.pos), step = W * S::PIECES;
   int next = warp * S::PIECES, at = 0;
+  if constexpr (KIND == FV_KV_INT4X32) {
+    BulkRing<D> stages;
+    stages.begin(a, m, warp);
+    stages.head(a, m, head);
+    for (int i = 0; i < S::DEPTH; ++i, next += step)
+      if (next < n) stages.fill(pieces, a, m, i, next);
+    Share<T, KIND, D, NT> share;
+    share.begin(a, row, head, first, g, t);
+#pragma unroll 1
+    for (int c = warp * S::PIECES; c < n && c < next; c += step) {  // behind `next` there is nothing on its way
+      const uint32_t stage = stages.wait(at);
+      if (!stages.failed) {
+        share.take_all(stage, g, t);
+        __syncwarp();
+        if (next < n) stages.fill(pieces, a, m, at, next);
+        next += step;
+      }
+      at = at + 1 == S::DEPTH ? 0 : at + 1;
+    }
+    if (stages.failed) share.spoil();
+    __syncthreads();  // the stages become the shares' place
+    float* s = reinterpret_cast<float*>(dyn_smem());
+    share.store(s + warp * Share<T, KIND, D, NT>::FLOATS, lane);
+    __syncthreads();
+    finish<T, KIND, D, NT, W, D / 16>(s, a, row, head, first, 0, warp, lane);
+    return;
+  } else {
   auto fill = [&](int to) {
     if (next < n) {
 #pragma unroll
@@ -721,6 +907,7 @@ __global__ void __launch_bounds__(32 * KV_TOKEN_WARPS) kv_token_kernel(KvAttend 
   share.store(s + warp * Share<T, KIND, D, NT>::FLOATS, lane);
   __syncthreads();
   finish<T, KIND, D, NT, W, D / 16>(s, a, row, head, first, 0, warp, lane);
+  }
 }
 
 // Or: all the pieces of all rows and heads (tasks), in units of a stage, are cut into equal parts, one for each warp that
@@ -779,7 +966,7 @@ __device__ __forceinline__ int units_a_warp(const Parts& p, int all) {
 }
 
 template <class T, int KIND, int D, int NT>
-__global__ void __launch_bounds__(32 * KV_TOKEN_WARPS) kv_parts_kernel(KvAttend a, KvBatch m, Parts p, int tiles, int before_at) {
+__global__ void __launch_bounds__(32 * KV_TOKEN_WARPS, kv_least_ctas(KIND, NT)) kv_parts_kernel(KvAttend a, KvBatch m, Parts p, int tiles, int before_at) {
   constexpr int W = KV_TOKEN_WARPS, COLS = 8 * NT;
   using S = Stage<KIND, D>;
   using H = Share<T, KIND, D, NT>;
@@ -824,6 +1011,36 @@ __global__ void __launch_bounds__(32 * KV_TOKEN_WARPS) kv_parts_kernel(KvAttend 
   Pieces pieces;
   pieces.begin(a, m, in.row, in.task / tiles);
   int filled = 0;
+  if constexpr (KIND == FV_KV_INT4X32) {
+    BulkRing<D> stages;
+    stages.begin(a, m, warp);
+    stages.head(a, m, in.task / tiles);
+    auto fill = [&](int to) {
+      if (filled >= n || stages.failed) return;
+      stages.fill(pieces, a, m, to, in.unit * S::PIECES);
+      if (++filled < n && in.step(before, p.tasks_a_row)) pieces.begin(a, m, in.row, in.task / tiles), stages.head(a, m, in.task / tiles);
+    };
+    for (int i = 0; i < S::DEPTH; ++i) fill(i);
+    H share;
+    share.begin(a, out.row, out.task / tiles, out.task % tiles * COLS, g, t);
+    int at = 0;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      if (i < filled) {  // all of them, unless a wait ran out
+        const uint32_t stage = stages.wait(at);
+        if (!stages.failed) share.take_all(stage, g, t);
+      }
+      if (stages.failed) share.spoil();
+      __syncwarp();
+      fill(at);
+      at = at + 1 == S::DEPTH ? 0 : at + 1;
+      const size_t number = size_t(w) + size_t(out.row) * p.tasks_a_row + out.task;
+      const bool last = i + 1 == n, other = !last && out.step(before, p.tasks_a_row);
+      if (last || other) share.store(p.part + number * H::FLOATS, lane);
+      if (other) share.begin(a, out.row, out.task / tiles, out.task % tiles * COLS, g, t);
+    }
+    return;
+  } else {
   auto fill = [&](int to) {
     if (filled < n) {
 #pragma unroll
@@ -849,6 +1066,7 @@ __global__ void __launch_bounds__(32 * KV_TOKEN_WARPS) kv_parts_kernel(KvAttend 
     const bool last = i + 1 == n, other = !last && out.step(before, p.tasks_a_row);
     if (last || other) share.store(p.part + number * H::FLOATS, lane);
     if (other) share.begin(a, out.row, out.task / tiles, out.task % tiles * COLS, g, t);
+  }
   }
 }
 
@@ -962,11 +1180,11 @@ int token_launch(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const Kv
   const int tiles = (a.group + COLS - 1) / COLS;
   const size_t tasks_a_row = size_t(kv->heads) * tiles, tasks = b->rows * tasks_a_row;
   if (tasks_a_row > 65535) return fail(FV_ERR_UNSUPPORTED, "fv_kv_attend_dev: more than 65535 tiles of query heads");
-  const size_t ring = size_t(W) * S::DEPTH * S::SIZE, shares = size_t(W) * H::FLOATS * 4;
+  const size_t ring = size_t(W) * S::DEPTH * S::SIZE + kv_bar_bytes(KIND, S::DEPTH), shares = size_t(W) * H::FLOATS * 4;
   const KvBatch m = kv_batch(kv, b);
   const size_t pieces = (a.blocks ? size_t(a.k) : b->table_width) * (kv->page_size / 16);  // of a task, at most
   const bool alike = a.blocks && size_t(a.k) * 4 <= b->table_width;
-  static_assert(228 * 1024 / (W * S::DEPTH * S::SIZE + 1024) == kv_ctas_an_sm(KIND, D), "the rule counts the CTAs that an SM holds");
+  static_assert(228 * 1024 / (W * S::DEPTH * S::SIZE + kv_bar_bytes(KIND, S::DEPTH) + 1024) == kv_ctas_an_sm(KIND, D), "the rule counts the CTAs that an SM holds");
   if (work && in_parts(KIND, D, a.group, alike, tasks, pieces) && pieces * tasks <= size_t(1) << 30) {
     const size_t smem = ring + 4 * (b->rows + 1), most = ring + 4 * (KV_PARTS_TASKS + 1);
     Parts p{int(b->rows), int(tasks_a_row), S::LEAST, 0, static_cast<float*>(work)};

@@ -237,6 +237,7 @@ struct BringFour {
       }
     }
     bool odd = false;
+    const uint32_t by_1024 = Four::magic(0x64006400u), by_64 = Four::magic(0x54005400u);
 #pragma unroll
     for (int x = 0; x < TIMES; ++x) {
       const int r = 16 * (x * (N / 64) + (t >> 6)) + r16;
@@ -246,7 +247,7 @@ struct BringFour {
         if (VALUES && byte >= 248u) odd = true, byte = 0u;
         const __half2 by = __half2half2(__ushort_as_half(uint16_t(byte << 7)));
         uint32_t y[4];
-        Four::halves(Four::group<NG>(c[x], g), y);
+        Four::halves(Four::group<NG>(c[x], g), y, by_1024, by_64);
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
           const __half2 f = __hmul2(*reinterpret_cast<const __half2*>(&y[z]), by);

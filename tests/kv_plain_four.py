@@ -38,23 +38,35 @@ def packed4(codes):
 
 
 class PlainFour(PlainCache):
-    """k and v hold the values that the codes stand for."""
+    """k and v hold the values that the codes stand for, k_scale and v_scale the largest of a row's scales that is a number."""
 
     def __init__(self, pages, heads, dim, page_size, dtype):
         super().__init__(pages, heads, dim, page_size, dtype, "same")
 
+    def hold(self, name, codes, n):
+        """All rows of k or v."""
+        getattr(self, name).copy_(values4(codes, n))
+        getattr(self, name + "_scale").copy_(torch.where(n == 255, 0.0, SCALES[n.clamp(max=len(SCALES) - 1)]).amax(-1))
+
     def add(self, k, v, table, lens, cu=None):
-        rounded = [values4(*coded4(x.double())) for x in (k, v)]
+        coded = [coded4(x.double()) for x in (k, v)]
+        rounded, scale = [values4(*x) for x in coded], [torch.where(n == 255, 0.0, SCALES[n.clamp(max=len(SCALES) - 1)]).amax(-1) for _, n in coded]
         super().add(k, v, table, lens, cu)  # bounds are those of the rows as they came
         for r, b, pos in self.places(table, lens, cu):
             page = self.page(table, b, pos // self.page_size) if pos >= 0 else -1
             if page >= 0:
-                self.k[page, :, pos % self.page_size], self.v[page, :, pos % self.page_size] = rounded[0][r], rounded[1][r]
+                slot = pos % self.page_size
+                self.k[page, :, slot], self.v[page, :, slot] = rounded[0][r], rounded[1][r]
+                self.k_scale[page, :, slot], self.v_scale[page, :, slot] = scale[0][r], scale[1][r]
 
     def attend(self, q, table, lens, cu, blocks, scale, out, lse):
-        """As the plain cache's, with the tolerances of rows that are exact in fp16: a weight is rounded once, to 2^-11 of itself or 2^-39 of
-        the largest; sums of products have 8 more steps than components (groups are added up one by one); queries of bf16
-        become fp16 relative to their largest component, whose components lose at most 2^-38 of it."""
+        """As the plain cache's, with tolerances of its own; s is a row's largest scale.
+
+        Scores: sums of exact products, of which the groups' are added up one by one: 8 steps more than in the plain cache.  bf16
+        queries become fp16 relative to their largest component, and components lose at most 2^-38 of it.
+        Weights: rounded to fp16, 2^-11 of themselves, and once more as the product with a scale.  2^(7 - unit) stands for a weight of 1,
+        where 2^unit is 1 or at most half the largest scale, and the step of the smallest numbers is 2^-24: each is off by 2^-32 max(1, s / 2),
+        which meets 7 s, and its product by as much, which meets 7.  Values: n products in 32 bits."""
         group, half = q.shape[1] // self.heads, torch.finfo(self.dtype).eps / 2
         tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
         for r, b, pos in self.places(table, lens, cu):
@@ -73,6 +85,7 @@ class PlainFour(PlainCache):
                     out[r, sl], lse[r, sl] = 0, -math.inf
                     continue
                 k, v, x = self.k[pages, h, slots], self.v[pages, h, slots], q[r, sl].double()
+                vs = self.v_scale[pages, h, slots]
                 s = x @ k.T * scale
                 off = abs(scale) * ((self.dim + 8) * 2.0**-24 * float((x.abs() @ k.abs().T).nan_to_num(posinf=0).max())
                                     + self.dim * 2.0**-38 * float(x.abs().max().nan_to_num(posinf=0) * k.abs().nan_to_num().max()))
@@ -81,8 +94,9 @@ class PlainFour(PlainCache):
                 p = w / w.sum(-1, keepdim=True)
                 out[r, sl] = torch.where(p[..., None] > 0, p[..., None] * v, torch.where(p.isnan(), torch.nan, 0.0)[..., None]).sum(1)
                 lse[r, sl] = torch.logsumexp(s, -1)
-                weight = 2.0**-11 + 2 * off + 2 * n * 2.0**-24 + 2.0**-20
-                tol[r, sl] = (p @ v.abs().nan_to_num()) * weight + out[r, sl].abs().nan_to_num(posinf=0) * half * 1.001 + n * 2.0**-38 * v.abs().nan_to_num().max()
+                weight = 2.0**-10 + 2 * off + 2 * n * 2.0**-24 + 2.0**-20
+                tol[r, sl] = (p @ v.abs().nan_to_num()) * weight + out[r, sl].abs().nan_to_num(posinf=0) * half * 1.001
+                tol[r, sl] += n * 2.0**-32 * max(1.0, float(vs.max()) / 2) * 7 * (float(vs.max()) + 1)
                 tol[r, sl] += torch.finfo(self.dtype).smallest_normal * half
                 ltol[r, sl] = off + n * 2.0**-24 + lse[r, sl].abs() * 2.0**-22 + 2.0**-20
         return out, lse, tol, ltol

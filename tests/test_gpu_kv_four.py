@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.kv_plain_four import PlainFour, SCALES, coded4, packed4, values4
+from tests.kv_plain_four import PlainFour, SCALES, coded4, packed4
 from tests.test_gpu_kv_attend import check, lists, queries
 from tests.test_gpu_kv_rows import batch, cuda, i32
 
@@ -27,7 +27,7 @@ def pair(pages, heads, dim, page, dtype, seed=0):
         n = torch.randint(110, 132, codes.shape[:-1], generator=g)  # 2^-5 to 3
         getattr(c, name).copy_(packed4(codes))
         getattr(c, name + "_scale").copy_(n.to(torch.uint8))
-        getattr(p, name).copy_(values4(codes, n))
+        p.hold(name, codes, n)
     return c, p
 
 
@@ -181,7 +181,7 @@ def test_scales_at_both_ends(new):
     for name, choice in (("k", [1, 2, 9, 100, 120]), ("v", [0, 1, 3, 7, 8, 15, 120, 216, 225])):
         n = torch.tensor(choice)[torch.randint(0, len(choice), (12, 1, page, 4), generator=g)]
         codes = torch.randint(-7, 8, (12, 1, page, 4, 32), generator=g).double()
-        getattr(c, name).copy_(packed4(codes)), getattr(c, name + "_scale").copy_(n.to(torch.uint8)), getattr(p, name).copy_(values4(codes, n))
+        getattr(c, name).copy_(packed4(codes)), getattr(c, name + "_scale").copy_(n.to(torch.uint8)), p.hold(name, codes, n)
     table, lens = batch(2, 6, 12, 2), [190, 150]
     cu = None if new == 1 else i32([0, new, 2 * new])
     for by in (1.0, 2.0**-60, 64.0):
