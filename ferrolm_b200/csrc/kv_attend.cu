@@ -188,7 +188,7 @@ struct Stage {
   static __device__ __forceinline__ int seen(const unsigned char* s) { return *reinterpret_cast<const int*>(s + 2 * 16 * ROW + SCALES); }
 };
 
-// The same in 4 bits: a few lanes start a bulk copy each, of two pieces' keys, values and scales, and a barrier of the stage counts their
+// The same in 4 bits: one lane starts bulk copies of two pieces' keys, values and scales, and a barrier of the stage counts their
 // bytes, so that the others' instructions go to the products.  A lane takes a quarter of a key, eight components of each of NG groups, and
 // an eighth of a value, four of each.  The products' rows are the tokens with every second pair the other way round: for keys, two
 // rows of 64 bytes that are read at one time lie next to each other, and of the four rows of values two do.
@@ -759,51 +759,53 @@ struct Pieces {
   }
 };
 
-// 4 bits: a warp's stages in shared memory, their barriers behind those of all warps.  Lanes 0 to 3 copy keys, values, and scales of
-// either, of both pieces where they are of one block, and with pages of 16 rows lanes 4 to 7 those of the second piece (each copy is some
-// 15 instructions: lanes take turns at it).  Where a page's are, from the first page's on, a lane knows for the head at hand.
+// 4 bits: a warp's stages in shared memory, their barriers behind those of all warps.  One lane copies keys, values, and scales of
+// either, of both pieces at once where they are of one block.  (The copies' operands are the warp's: four lanes with one each take turns
+// and need twice the instructions.)
 template <int D>
 struct BulkRing {
   using S = Stage<FV_KV_INT4X32, D>;
   uint32_t ring, bars;  // addresses in shared memory
   uint32_t turns;       // bit i: of stage i's barrier
   bool failed;          // a wait ran out
-  uint32_t to, bytes, row, page;  // of the lane: where its part of a stage is, its bytes, and those of a row and of a page
-  const unsigned char* from;
-  __device__ __forceinline__ void begin(const KvAttend& a, const KvBatch& m, int warp) {
-    const int lane = lane_id(), part = lane & 3;
+  __device__ __forceinline__ void begin(int warp) {
     ring = smem_u32(dyn_smem()) + warp * (S::DEPTH * S::SIZE);
     bars = smem_u32(dyn_smem()) + KV_TOKEN_WARPS * S::DEPTH * S::SIZE + warp * (S::DEPTH * 8);
     turns = 0u, failed = false;
-    row = part < 2 ? S::ROW : S::NG, page = (uint32_t(a.heads) * row) << m.page_shift;
-    const bool single = m.page_shift == 4;  // pieces are of different blocks
-    bytes = (single ? 16 : 32) * row;
-    to = ring + (part < 2 ? part * S::VALUES : S::KEY_SCALES + (part - 2) * (S::PIECES * S::SCALE)) + (lane >> 2 & 1) * 16 * row;
-    if (lane < S::DEPTH) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bars + lane * 8), "r"(single ? 8u : 4u));
+    if (lane_id() < S::DEPTH) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + lane_id() * 8));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncwarp();
   }
-  __device__ __forceinline__ void head(const KvAttend& a, const KvBatch& m, int h) {  // the pieces from now on are of key head h
-    const int part = lane_id() & 3;
-    from = part == 0 ? a.kp : part == 1 ? a.vp : reinterpret_cast<const unsigned char*>(part == 2 ? a.k_scale : a.v_scale);
-    from += (size_t(h) * row) << m.page_shift;
+  static __device__ __forceinline__ void copy(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+  }
+  // n pieces of one block from `slot` of `page` on to stage `to`, the first of them number h there.
+  static __device__ __forceinline__ void copies(const Pieces& p, const KvAttend& a, const KvBatch& m, uint32_t to, uint32_t bar, int page, int slot, int h, int n) {
+    const size_t at = size_t(uint32_t(page)) * (uint32_t(a.heads) << m.page_shift) + uint32_t((p.head << m.page_shift) + slot);
+    copy(to + h * 16 * S::ROW, a.kp + at * S::ROW, n * 16 * S::ROW, bar);
+    copy(to + S::VALUES + h * 16 * S::ROW, a.vp + at * S::ROW, n * 16 * S::ROW, bar);
+    copy(to + S::KEY_SCALES + h * S::SCALE, reinterpret_cast<const unsigned char*>(a.k_scale) + at * S::NG, n * S::SCALE, bar);
+    copy(to + S::VALUE_SCALES + h * S::SCALE, reinterpret_cast<const unsigned char*>(a.v_scale) + at * S::NG, n * S::SCALE, bar);
   }
   // Starts the copies of pieces c and c + 1 (c is even) to stage `at`.
   __device__ __forceinline__ void fill(Pieces& p, const KvAttend& a, const KvBatch& m, int at, int c) {
-    const int lane = lane_id(), per = m.page_shift - 4, mine = c + (lane >> 2 & 1), i = mine >> per;
-    if (c >> per >= p.base + 32) p.look(a, m, c >> per);
-    const int block = __shfl_sync(FV_FULL, p.block, i & 31), q = __shfl_sync(FV_FULL, p.page, i & 31);
-    if (lane < 8) {
-      const int slot = (mine & ((1 << per) - 1)) << 4, seen = q >= 0 ? p.pos - ((block << m.page_shift) + slot) + 1 : 0;
-      const uint32_t bar = bars + at * 8;
-      if ((lane & 3) == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(ring + at * S::SIZE + S::SEEN + lane), "r"(min(seen, 16)) : "memory");
-      if (per == 0 || lane < 4) {
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(seen > 0 ? bytes : 0u) : "memory");
-        if (seen > 0)
-          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to + at * S::SIZE),
-                       "l"(from + size_t(uint32_t(q)) * page + uint32_t(slot) * row), "r"(bytes), "r"(bar)
-                       : "memory");
-      }
+    const int per = m.page_shift - 4, i = c >> per, slot = (c & ((1 << per) - 1)) << 4;
+    if (i >= p.base + 32) p.look(a, m, i);
+    const int block = __shfl_sync(FV_FULL, p.block, i & 31), page = __shfl_sync(FV_FULL, p.page, i & 31);
+    const uint32_t to = ring + at * S::SIZE, bar = bars + at * 8;
+    int seen = page >= 0 ? p.pos - ((block << m.page_shift) + slot) + 1 : 0, more = seen - 16, other = 0;
+    if (per == 0) {  // pages of one piece
+      const int next = __shfl_sync(FV_FULL, p.block, (i & 31) + 1);
+      other = __shfl_sync(FV_FULL, p.page, (i & 31) + 1);
+      more = other >= 0 ? p.pos - (next << 4) + 1 : 0;
+    }
+    if (elect_one()) {
+      constexpr uint32_t BYTES = 2 * (16 * S::ROW + S::SCALE);  // of a piece
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + S::SEEN), "r"(min(seen, 16)), "r"(min(more, 16)) : "memory");
+      const uint32_t all = per == 0 ? (seen > 0 ? BYTES : 0u) + (more > 0 ? BYTES : 0u) : seen > 0 ? 2 * BYTES : 0u;
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(all) : "memory");
+      if (seen > 0) copies(p, a, m, to, bar, page, slot, 0, per == 0 ? 1 : 2);
+      if (per == 0 && more > 0) copies(p, a, m, to, bar, other, 0, 1, 1);
     }
     __syncwarp();
   }
@@ -855,8 +857,7 @@ __global__ void __launch_bounds__(32 * KV_TOKEN_WARPS, kv_least_ctas(KIND, NT)) 
   int next = warp * S::PIECES, at = 0;
   if constexpr (KIND == FV_KV_INT4X32) {
     BulkRing<D> stages;
-    stages.begin(a, m, warp);
-    stages.head(a, m, head);
+    stages.begin(warp);
     for (int i = 0; i < S::DEPTH; ++i, next += step)
       if (next < n) stages.fill(pieces, a, m, i, next);
     Share<T, KIND, D, NT> share;
@@ -1013,12 +1014,11 @@ __global__ void __launch_bounds__(32 * KV_TOKEN_WARPS, kv_least_ctas(KIND, NT)) 
   int filled = 0;
   if constexpr (KIND == FV_KV_INT4X32) {
     BulkRing<D> stages;
-    stages.begin(a, m, warp);
-    stages.head(a, m, in.task / tiles);
+    stages.begin(warp);
     auto fill = [&](int to) {
       if (filled >= n || stages.failed) return;
       stages.fill(pieces, a, m, to, in.unit * S::PIECES);
-      if (++filled < n && in.step(before, p.tasks_a_row)) pieces.begin(a, m, in.row, in.task / tiles), stages.head(a, m, in.task / tiles);
+      if (++filled < n && in.step(before, p.tasks_a_row)) pieces.begin(a, m, in.row, in.task / tiles);
     };
     for (int i = 0; i < S::DEPTH; ++i) fill(i);
     H share;
