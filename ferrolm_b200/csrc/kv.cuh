@@ -202,17 +202,25 @@ struct Eight<FV_KV_E4M3> {
 struct Four {
   static constexpr float LARGEST = 9216.f;
   static constexpr uint32_t NAN_SCALE = 255;
-  static __device__ __forceinline__ uint32_t scale_of(float most) {  // its byte; `most` is finite
-    const float t = __fdiv_rn(most, 7.f);
+  // Its byte, of a finite `most`.  A seventh of 11 bits is a scale or further from one than 2^-14 of itself: what is made smaller by 2^-20, and
+  // is off by less than that, is rounded up to the same.
+  static __device__ __forceinline__ uint32_t scale_of(float most) {
+    const float t = most * 0.14285700f;
     if (t < 0x1p-14f) return uint32_t(ceilf(t * 0x1p17f));
     return (min(__float_as_uint(t) + 0xFFFFFu, __float_as_uint(LARGEST)) >> 20) - ((127 - 15) << 3);
   }
   static __device__ __forceinline__ float value(uint32_t byte) { return __half2float(__ushort_as_half(uint16_t(byte << 7))); }
-  // eight codes of neighbouring components, the first in the lowest bits, from values of at most 7 scales; inv = 1 / scale
-  static __device__ __forceinline__ uint32_t pack(const float* x, float scale, float inv) {
-    uint32_t w = 0;
+  // Eight codes of neighbouring components, the first in the lowest bits, inv = 1 / scale to within 2^-22 of itself.  A quotient x / scale of
+  // 11 and 4 bits from 1/2 on is half a whole number or 2^-13 and more from it, so it is rounded to a multiple of 2^-14 first and then
+  // to a whole number, halves to the even one: both by adding a number whose last place that is.  The sum's bits are a constant and
+  // the code, and the constants of all eight are taken off together.
+  static __device__ __forceinline__ uint32_t pack(const float* x, float inv) {
+    uint32_t w = 0u - (0x4B400000u + (0x4B400000u << 4) + (0x4B400000u << 8));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= uint32_t(kv_whole(x[i], scale, inv) + 8) << (4 * i);
+    for (int i = 0; i < 8; ++i) {
+      const float q = (x[i] * inv + 0x1.8p9f) - 0x1.8p9f;
+      w += __float_as_uint(q + (0x1.8p23f + 8.f)) << (4 * i);
+    }
     return w;
   }
   // the eight codes of group g in the NG words of a quarter of a row

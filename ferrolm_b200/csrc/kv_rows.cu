@@ -79,23 +79,30 @@ __device__ __forceinline__ void write_row(const uint4& raw, bool on, unsigned ch
     if (on) *reinterpret_cast<uint4*>(dst + at * (2 * D) + l * 16) = raw;
   } else if constexpr (KIND == FV_KV_INT4X32) {
     constexpr int NG = D / 32;
-    float x[8], most = 0.f;
+    constexpr uint32_t NOT_FINITE = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;  // and above, without the sign
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    bool fine = true;
+    uint32_t top = 0u;  // the largest without its sign: the bits are ordered as the numbers, and what is no number is above them
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __vmaxu2(top, w[i] & 0x7FFF7FFFu);
+    top = __vmaxu2(top, __shfl_xor_sync(FV_FULL, top, 1));
+    top = __vmaxu2(top, __shfl_xor_sync(FV_FULL, top, 2));
+    top = max(top & 0xFFFFu, top >> 16);
+    const bool ok = top < NOT_FINITE;
+    const float most = Pair<T>::to_float(top).x;
+    const uint32_t byte = ok ? Four::scale_of(most) : Four::NAN_SCALE;
+    const float s = ok ? Four::value(byte) : 0.f;
+    float inv = 0.f, x[8];  // without a scale all codes are those of zero
+    if (s > 0.f) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 f = Pair<T>::to_float(w[i]);
       x[2 * i] = f.x, x[2 * i + 1] = f.y;
-      fine = fine && kv_finite(f.x) && kv_finite(f.y);
-      most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
     }
-    most = group_max<4>(fine ? most : INFINITY);  // of the group's four lanes; infinite also where it is a NaN, which fmaxf drops
-    const bool ok = most < INFINITY;
-    const uint32_t byte = ok ? Four::scale_of(most) : Four::NAN_SCALE;
-    const float s = ok ? Four::value(byte) : 0.f, top = 7.f * s, den = s > 0.f ? s : 1.f;
+    if (!ok || most > 7.f * Four::LARGEST) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = ok ? fminf(fmaxf(x[i], -top), top) : 0.f;
-    const uint32_t code = Four::pack(x, den, __fdiv_rn(1.f, den));
+      for (int i = 0; i < 8; ++i) x[i] = ok ? fminf(fmaxf(x[i], -7.f * Four::LARGEST), 7.f * Four::LARGEST) : 0.f;
+    }
+    const uint32_t code = Four::pack(x, inv);
     // lane l writes pieces 2 l and 2 l + 1: piece n is the (n / NG)-th four of group n % NG, half of what lane 4 (n % NG) + n / NG / 2 has
     const int n0 = 2 * l, n1 = n0 + 1, u0 = n0 / NG, u1 = n1 / NG;
     const uint32_t a = __shfl_sync(FV_FULL, code, 4 * (n0 - u0 * NG) + (u0 >> 1), N), b = __shfl_sync(FV_FULL, code, 4 * (n1 - u1 * NG) + (u1 >> 1), N);
