@@ -129,6 +129,28 @@ struct Pair<__half> {
   }
 };
 
+// zeros in the halves that are not finite
+template <class T>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+  return w & ~__vcmpeq2(w & e, e);
+}
+// The smaller and the larger of each half; none of them a NaN.
+template <class T>
+__device__ __forceinline__ uint32_t min2(uint32_t x, uint32_t y) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  else asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+template <class T>
+__device__ __forceinline__ uint32_t max2(uint32_t x, uint32_t y) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  else asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+
 // ---------------------------------------------------------------------------------------------
 // 8-bit values.  A code is top * x / most rounded to nearest even, and most, x of 8 or 11 significant bits make the quotient
 // either the border of two codes exactly or further from it than half a step of 32 bits: with a correctly rounded division

@@ -110,12 +110,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// zeros in the halves that are not finite
-template <class T>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
-  return w & ~__vcmpeq2(w & e, e);
-}
 // x + 0 * w in both halves: NaN from the first that is not finite on
 template <class T>
 __device__ __forceinline__ uint32_t watch(uint32_t x, uint32_t w) {

@@ -72,9 +72,9 @@ __device__ __forceinline__ float group_max(float x) {  // over N neighbouring la
 }
 
 // One row of 8 values a lane over N lanes, lane l's from 8 l on: codes (or the 16 bits as they are) to row `at` of dst, the scales to those
-// of that row.  `on`: the lane has values of a row that is written.  Whole warps call it.
+// of that row.  `on`: the lane has values of a row that is written.  Whole warps call it.  False: (4 bits) some of the group's are not finite.
 template <class T, int KIND, int D, int N>
-__device__ __forceinline__ void write_row(const uint4& raw, bool on, unsigned char* dst, float* scale, size_t at, int l) {
+__device__ __forceinline__ bool write_row(const uint4& raw, bool on, unsigned char* dst, float* scale, size_t at, int l) {
   if constexpr (KIND == FV_KV_SAME) {
     if (on) *reinterpret_cast<uint4*>(dst + at * (2 * D) + l * 16) = raw;
   } else if constexpr (KIND == FV_KV_INT4X32) {
@@ -110,6 +110,7 @@ __device__ __forceinline__ void write_row(const uint4& raw, bool on, unsigned ch
       *reinterpret_cast<uint32_t*>(dst + at * (D / 2) + l * 4) = __byte_perm(a, b, (u0 & 1 ? 0x32 : 0x10) | (u1 & 1 ? 0x7600 : 0x5400));
       if ((l & 3) == 0) reinterpret_cast<uint8_t*>(scale)[at * NG + l / 4] = uint8_t(byte);
     }
+    return ok;
   } else {
     float x[8];
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -133,6 +134,7 @@ __device__ __forceinline__ void write_row(const uint4& raw, bool on, unsigned ch
       if (l == 0) scale[at] = ok ? __fdiv_rn(most, Eight<KIND>::top) : __int_as_float(0x7FC00000);
     }
   }
+  return true;
 }
 
 // An item is the part of one block that this call writes, for one head; WARPS of them share an item (8: prompts, 1: a few rows
@@ -160,6 +162,9 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128, WARPS > 1 ? 3 : 
   float lo[8], hi[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+  constexpr bool FOUR = KIND == FV_KV_INT4X32;
+  constexpr uint32_t INF2 = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+  [[maybe_unused]] uint32_t lo2[4] = {INF2, INF2, INF2, INF2}, hi2[4] = {INF2 | 0x80008000u, INF2 | 0x80008000u, INF2 | 0x80008000u, INF2 | 0x80008000u};  // 4 bits: in pairs
   constexpr int AHEAD = WARPS > 1 ? 2 : 1;  // rows that a lane has on their way
   for (int p0 = begin + part * PER; p0 < end; p0 += AHEAD * WARPS * PER) {
     uint4 kr[AHEAD], vr[AHEAD];
@@ -178,7 +183,7 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128, WARPS > 1 ? 3 : 
       if (z && p0 + z * WARPS * PER >= end) break;  // whole warps
       const int p = p0 + z * WARPS * PER + sub, slot = p & (size - 1);
       const bool on = in_row && p < end;
-      if (on) {
+      if (on && !FOUR) {
         const uint32_t w[4] = {kr[z].x, kr[z].y, kr[z].z, kr[z].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -190,8 +195,26 @@ __global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128, WARPS > 1 ? 3 : 
         }
       }
       const size_t row_at = at * size + slot;
-      write_row<T, KIND, D, N>(kr[z], on, pool.k, pool.k_scale, row_at, l);
+      const bool fine = write_row<T, KIND, D, N>(kr[z], on, pool.k, pool.k_scale, row_at, l);
+      if constexpr (FOUR) {
+        uint32_t w[4] = {kr[z].x, kr[z].y, kr[z].z, kr[z].w};
+        if (!fine) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = finite_only<T>(w[i]);
+        }
+        if (on) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) lo2[i] = min2<T>(lo2[i], w[i]), hi2[i] = max2<T>(hi2[i], w[i]);
+        }
+      }
       write_row<T, KIND, D, N>(vr[z], on, pool.v, pool.v_scale, row_at, l);
+    }
+  }
+  if constexpr (FOUR) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = Pair<T>::to_float(lo2[i]), c = Pair<T>::to_float(hi2[i]);
+      lo[2 * i] = a.x, lo[2 * i + 1] = a.y, hi[2 * i] = c.x, hi[2 * i + 1] = c.y;
     }
   }
 #pragma unroll
