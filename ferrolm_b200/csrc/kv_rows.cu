@@ -137,11 +137,15 @@ __device__ __forceinline__ bool write_row(const uint4& raw, bool on, unsigned ch
   return true;
 }
 
-// An item is the part of one block that this call writes, for one head; WARPS of them share an item (8: prompts, 1: a few rows
+// CTAs of the kernel below that an SM is to hold.  4 bits: rounding and bounds leave loads waiting, and more CTAs cover that better than
+// more loads on their way (14k rows of 8 heads of 128: 31.6 us with three CTAs of eight warps, 27.9 with four, 25.2 with eight of four).
+constexpr int kv_add_ctas(int kind, int warps) { return warps == 1 ? 1 : kind != FV_KV_INT4X32 ? 3 : warps == 4 ? 8 : 4; }
+
+// An item is the part of one block that this call writes, for one head; WARPS of them share an item (8, or 4: prompts, 1: a few rows
 // for each sequence, four heads to a CTA).  One owner for each block's bounds means no atomics, and the order of the rows does
 // not change a minimum.  N lanes hold a row, 8 values each, so a warp writes 32 / N rows at once.
 template <class T, int KIND, int D, int WARPS>
-__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128, WARPS > 1 ? 3 : 1) kv_add_kernel(KvPool pool, KvBatch m, KvInput kin, KvInput vin) {
+__global__ void __launch_bounds__(WARPS > 1 ? 32 * WARPS : 128, kv_add_ctas(KIND, WARPS)) kv_add_kernel(KvPool pool, KvBatch m, KvInput kin, KvInput vin) {
   constexpr int N = D <= 64 ? 8 : 16, PER = 32 / N, L = D / 8;
   __shared__ float s_lo[WARPS > 1 ? WARPS * D : 1], s_hi[WARPS > 1 ? WARPS * D : 1];
   const int warp = threadIdx.x >> 5, lane = lane_id();
@@ -391,10 +395,18 @@ int add_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvInput&
   const KvPool pool = kv_pool(kv);
   const size_t items = b->cu ? b->rows / kv->page_size + 2 * b->nseq : b->nseq;
   // a warp for a block where a sequence brings a few rows, eight where it brings a prompt
-  if (b->rows <= 8 * b->nseq)
+  if (b->rows <= 8 * b->nseq) {
     kv_add_kernel<T, KIND, D, 1><<<dim3(unsigned(items), (kv->heads + 3) / 4), 128, 0, s>>>(pool, m, k, v);
-  else
-    kv_add_kernel<T, KIND, D, 8><<<dim3(unsigned(items), kv->heads), 256, 0, s>>>(pool, m, k, v);
+    FV_CUDA(cudaGetLastError());
+    return FV_OK;
+  }
+  if constexpr (KIND == FV_KV_INT4X32)
+    if (items * kv->heads > 2 * 148) {  // fewer leave SMs empty: 88 items 5.9 us with eight warps each, 7.5 with four; 552 items 6.3 and 5.6
+      kv_add_kernel<T, KIND, D, 4><<<dim3(unsigned(items), kv->heads), 128, 0, s>>>(pool, m, k, v);
+      FV_CUDA(cudaGetLastError());
+      return FV_OK;
+    }
+  kv_add_kernel<T, KIND, D, 8><<<dim3(unsigned(items), kv->heads), 256, 0, s>>>(pool, m, k, v);
   FV_CUDA(cudaGetLastError());
   return FV_OK;
 }
