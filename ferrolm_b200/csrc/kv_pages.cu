@@ -11,7 +11,7 @@
 namespace fv {
 namespace {
 
-enum { PAGES_THREADS = 1024, PAGES_WARPS = 32, PAGES_SEQS = 2048, COPY_THREADS = 256, COPY_SLICE = 32 * 1024, COPY_PARTS = 7 };
+enum { PAGES_THREADS = 1024, PAGES_WARPS = 32, PAGES_SEQS = 2048, COPY_THREADS = 256, COPY_SLICE = 32 * 1024, COPY_PARTS = 7, COPY_CACHES = 8 };
 
 struct Pages {
   int32_t* refs;
@@ -47,28 +47,47 @@ __device__ __forceinline__ int sum_before(int x, int* s, int* all) {
   return before + up - x;
 }
 
-// The warp's part of the pages: f(page, whether it is one, count) for 128 pages at a time, four neighbours a lane.
-template <class F>
-__device__ __forceinline__ void each_page(const Pages& p, F&& f) {
-  const int warp = threadIdx.x >> 5, lane = lane_id();
-  const int share = ((p.pages + PAGES_WARPS - 1) / PAGES_WARPS + 127) & ~127;
-  const int begin = int(min((long long)(warp) * share, (long long)(p.pages))), end = int(min((long long)(begin) + share, (long long)(p.pages)));
-  const bool wide = (reinterpret_cast<uintptr_t>(p.refs) & 15) == 0;
-#pragma unroll 4
-  for (int i = begin; i < end; i += 128) {
-    const int at = i + 4 * lane;
-    int4 r = make_int4(-1, -1, -1, -1);  // behind the last page
-    if (wide && at + 4 <= p.pages) {
-      r = __ldcg(reinterpret_cast<const int4*>(p.refs + at));
-    } else {
-      int* x = reinterpret_cast<int*>(&r);
+// The warp's part of the pages, four neighbours a lane.  Counts of up to 1024 pages a warp stay in registers from the first look on, so that the
+// passes over them do not wait for memory again, and the first look may be long before.
+struct PageShare {
+  enum { AHEAD = 8 };
+  int begin, end;  // of the warp's pages
+  bool kept;
+  int4 r[AHEAD];
+  __device__ __forceinline__ void load(const Pages& p, int from) {
+    const bool wide = (reinterpret_cast<uintptr_t>(p.refs) & 15) == 0;
 #pragma unroll
-      for (int z = 0; z < 4; ++z)
-        if (at + z < p.pages) x[z] = __ldcg(p.refs + at + z);
+    for (int z = 0; z < AHEAD; ++z) {
+      const int at = from + 128 * z + 4 * int(lane_id());
+      r[z] = make_int4(-1, -1, -1, -1);  // behind the last page
+      if (from + 128 * z >= end) continue;
+      if (wide && at + 4 <= p.pages) {
+        r[z] = __ldcg(reinterpret_cast<const int4*>(p.refs + at));
+      } else {
+        if (at < p.pages) r[z].x = __ldcg(p.refs + at);
+        if (at + 1 < p.pages) r[z].y = __ldcg(p.refs + at + 1);
+        if (at + 2 < p.pages) r[z].z = __ldcg(p.refs + at + 2);
+        if (at + 3 < p.pages) r[z].w = __ldcg(p.refs + at + 3);
+      }
     }
-    if (!f(at, r)) break;  // for whole warps
   }
-}
+  __device__ __forceinline__ void look(const Pages& p) {
+    const long long warp = threadIdx.x >> 5, share = ((p.pages + PAGES_WARPS - 1) / PAGES_WARPS + 127) & ~127;
+    begin = int(min(warp * share, (long long)(p.pages))), end = int(min(warp * share + share, (long long)(p.pages)));
+    kept = share <= 128 * AHEAD;
+    load(p, begin);
+  }
+  // f(first of four pages, their counts) for whole warps, in ascending order, as long as it says so
+  template <class F>
+  __device__ __forceinline__ void each(const Pages& p, F&& f) {
+    for (int i = begin; i < end; i += 128 * AHEAD) {
+      if (!kept) load(p, i);
+#pragma unroll
+      for (int z = 0; z < AHEAD; ++z)
+        if (i + 128 * z < end && !f(i + 128 * z + 4 * int(lane_id()), r[z])) return;
+    }
+  }
+};
 
 // ---------------------------------------------------------------------------------------------
 struct Extend {
@@ -89,10 +108,13 @@ __device__ __forceinline__ int32_t* entry_at(const Pages& p, const Table& t, con
   return t.at + size_t(lo) * t.stride + first + (e - before[lo]);
 }
 
-// What a table entry says while this runs: a page; -1: it wants one; -2 - q: it wants one and a copy of page q.
+// What a table entry says while this runs: a page; -1: it wants one; -2 - q: it wants one and a copy of page q.  A thread's first entry is
+// in its registers.
 __global__ void __launch_bounds__(PAGES_THREADS) pages_extend_kernel(Pages p, Table t, Extend x) {
   __shared__ int s_sum[PAGES_WARPS + 1], s_before[PAGES_SEQS + 1], s_count;
   const int tid = threadIdx.x;
+  PageShare share;
+  share.look(p);  // those that are free now: counts that come to nothing below are given back
   int* const before = t.nseq <= PAGES_SEQS ? s_before : x.before;
   if (tid == 0) s_count = 0, before[0] = 0;
   int entries = 0;
@@ -109,87 +131,92 @@ __global__ void __launch_bounds__(PAGES_THREADS) pages_extend_kernel(Pages p, Ta
     entries += all;
   }
   __syncthreads();
+  int32_t* const at0 = tid < entries ? entry_at(p, t, x, before, tid) : nullptr;
+  int q0 = at0 ? __ldcg(at0) : 0;
+  auto get = [&](int e) { return e == tid ? q0 : __ldcg(entry_at(p, t, x, before, e)); };
+  auto put = [&](int e, int q) {
+    if (e == tid) q0 = q;
+    else __stcg(entry_at(p, t, x, before, e), q);
+  };
   // who wants a page
   bool shared = false;
-  int wants = 0;
+  int wants = 0, all;
   for (int e = tid; e < entries; e += PAGES_THREADS) {
-    int32_t* at = entry_at(p, t, x, before, e);
-    const int q = __ldcg(at);
-    if (unsigned(q) >= unsigned(p.pages)) __stcg(at, -1), ++wants;
-    else if (__ldcg(p.refs + q) > 1) __stcg(at, -2 - q), shared = true, ++wants;
+    const int q = get(e);
+    if (unsigned(q) >= unsigned(p.pages)) put(e, -1), ++wants;
+    else if (__ldcg(p.refs + q) > 1) put(e, -2 - q), shared = true, ++wants;
   }
   if (__syncthreads_or(shared)) {
     // who holds a page with others gives it up; where nobody is left, refs becomes the smallest number of those who did, far below 0, and
     // that one keeps it
     for (int e = tid; e < entries; e += PAGES_THREADS) {
-      const int q = -2 - __ldcg(entry_at(p, t, x, before, e));
+      const int q = -2 - get(e);
       if (q >= 0) atomicSub(p.refs + q, 1);
     }
     __syncthreads();
     for (int e = tid; e < entries; e += PAGES_THREADS) {
-      const int q = -2 - __ldcg(entry_at(p, t, x, before, e));
+      const int q = -2 - get(e);
       if (q >= 0 && __ldcg(p.refs + q) <= 0) atomicMin(p.refs + q, INT_MIN + e);
     }
     __syncthreads();
+    bool keeps0 = false;  // the thread's first entry keeps its page
     for (int e = tid; e < entries; e += PAGES_THREADS) {
-      int32_t* at = entry_at(p, t, x, before, e);
-      const int q = -2 - __ldcg(at);
-      if (q >= 0 && __ldcg(p.refs + q) == INT_MIN + e) __stcg(at, q), --wants;
+      const int q = -2 - get(e);
+      if (q >= 0 && __ldcg(p.refs + q) == INT_MIN + e) put(e, q), --wants, keeps0 = keeps0 || e == tid;
     }
     __syncthreads();
     for (int e = tid; e < entries; e += PAGES_THREADS) {
-      const int q = __ldcg(entry_at(p, t, x, before, e));
-      if (q >= 0 && __ldcg(p.refs + q) < 0) __stcg(p.refs + q, 1);
+      const int q = get(e);
+      if (e == tid ? keeps0 : q >= 0 && __ldcg(p.refs + q) < 0) __stcg(p.refs + q, 1);
     }
   }
-  int all;
   sum_before(wants, s_sum, &all);
   wants = all;
   if (wants) {
     // the free pages, as many as are wanted
     int n = 0;
-    each_page(p, [&](int, const int4& r) { return n += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0), true; });
+    share.each(p, [&](int, const int4& r) { return n += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0), true; });
     int rank = sum_before(n, s_sum, &all);  // of a lane: its pages are not neighbours, only the warp's sum counts
     if (all < wants) {  // nothing is changed
       for (int e = tid; e < entries; e += PAGES_THREADS) {
-        int32_t* at = entry_at(p, t, x, before, e);
-        const int q = -2 - __ldcg(at);
-        if (q >= 0) atomicAdd(p.refs + q, 1), __stcg(at, q);
+        const int q = -2 - get(e);
+        if (q >= 0) atomicAdd(p.refs + q, 1), put(e, q);
       }
+      if (at0) *at0 = q0;
       if (tid == 0) *x.missing = wants - all, *x.count = 0;
       return;
     }
     rank = __shfl_sync(FV_FULL, rank, 0);
-    each_page(p, [&](int at, const int4& r) {
-      const int c = (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
-      int up = c;
+    if (rank < wants) {
+      share.each(p, [&](int at, const int4& r) {
+        const int c = (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
+        int up = c;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(FV_FULL, up, o);
-        if (int(lane_id()) >= o) up += y;
-      }
-      int i = rank + up - c;
-      if (r.x == 0 && i < wants) x.free[i] = at;
-      i += r.x == 0;
-      if (r.y == 0 && i < wants) x.free[i] = at + 1;
-      i += r.y == 0;
-      if (r.z == 0 && i < wants) x.free[i] = at + 2;
-      i += r.z == 0;
-      if (r.w == 0 && i < wants) x.free[i] = at + 3;
-      rank += __shfl_sync(FV_FULL, up, 31);
-      return rank < wants;
-    });
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(FV_FULL, up, o);
+          if (int(lane_id()) >= o) up += y;
+        }
+        int i = rank + up - c;
+        if (r.x == 0 && i < wants) x.free[i] = at;
+        i += r.x == 0;
+        if (r.y == 0 && i < wants) x.free[i] = at + 1;
+        i += r.y == 0;
+        if (r.z == 0 && i < wants) x.free[i] = at + 2;
+        i += r.z == 0;
+        if (r.w == 0 && i < wants) x.free[i] = at + 3;
+        rank += __shfl_sync(FV_FULL, up, 31);
+        return rank < wants;
+      });
+    }
     __syncthreads();
     int given = 0;
     for (int e0 = 0; e0 < entries; e0 += PAGES_THREADS) {
-      const int e = e0 + tid;
-      int32_t* at = e < entries ? entry_at(p, t, x, before, e) : nullptr;
-      const int q = at ? __ldcg(at) : 0;
+      const int e = e0 + tid, q = e < entries ? get(e) : 0;
       const int i = given + sum_before(q < 0, s_sum, &all);
       given += all;
       if (q < 0) {
         const int page = __ldcg(x.free + i);
-        *at = page;
+        put(e, page);
         p.refs[page] = 1;
         if (q < -1) {
           const int c = atomicAdd(&s_count, 1);
@@ -199,6 +226,7 @@ __global__ void __launch_bounds__(PAGES_THREADS) pages_extend_kernel(Pages p, Ta
     }
     __syncthreads();
   }
+  if (at0) *at0 = q0;
   if (tid == 0) *x.missing = 0, *x.count = s_count;
 }
 
@@ -245,13 +273,15 @@ __global__ void __launch_bounds__(256) pages_remap_kernel(const int32_t* map, in
 __global__ void __launch_bounds__(PAGES_THREADS) pages_compact_kernel(Pages p, int32_t* map, int32_t* used, int32_t* count, int32_t* src, int32_t* dst) {
   __shared__ int s_sum[PAGES_WARPS + 1];
   const int lane = lane_id();
+  PageShare share;
+  share.look(p);
   int n = 0, all;
-  each_page(p, [&](int, const int4& r) { return n += (r.x > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0), true; });
+  share.each(p, [&](int, const int4& r) { return n += (r.x > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0), true; });
   sum_before(n, s_sum, &all);
   const int live = all;
   // a page below `live` that is free is a hole; one from there on that is not moves to the hole of its number
   int holes = 0, movers = 0;
-  each_page(p, [&](int at, const int4& r) {
+  share.each(p, [&](int at, const int4& r) {
     const int* c = reinterpret_cast<const int*>(&r);
 #pragma unroll
     for (int z = 0; z < 4; ++z) holes += at + z < live && c[z] <= 0, movers += at + z >= live && at + z < p.pages && c[z] > 0;
@@ -261,7 +291,7 @@ __global__ void __launch_bounds__(PAGES_THREADS) pages_compact_kernel(Pages p, i
   const int moved = all;
   int mover = sum_before(movers, s_sum, &all);
   hole = __shfl_sync(FV_FULL, hole, 0), mover = __shfl_sync(FV_FULL, mover, 0);
-  each_page(p, [&](int at, const int4& r) {
+  share.each(p, [&](int at, const int4& r) {
     const int* c = reinterpret_cast<const int*>(&r);
     int own = 0;  // a hole, or from `live` on a mover: a lane's four are counted together, 128 pages lie on both sides of `live` at most once
 #pragma unroll
@@ -278,88 +308,101 @@ __global__ void __launch_bounds__(PAGES_THREADS) pages_compact_kernel(Pages p, i
       if (at + z >= p.pages) continue;
       if (at + z < live && c[z] <= 0) dst[h++] = at + z;
       if (at + z >= live && c[z] > 0) src[m++] = at + z;
-      map[at + z] = c[z] > 0 ? at + z : -1;
+      map[at + z] = c[z] > 0 ? at + z : -1;  // those that move are put right as they do
     }
     const int sum = __shfl_sync(FV_FULL, up, 31);
     hole += sum & 0xFFFF, mover += sum >> 16;
     return true;
   });
-  __syncthreads();
-  for (int i = threadIdx.x; i < moved; i += PAGES_THREADS) {
-    const int from = __ldcg(src + i), to = __ldcg(dst + i);
-    map[from] = to;
-    p.refs[to] = __ldcg(p.refs + from);
-    p.refs[from] = 0;
-  }
   if (threadIdx.x == 0) *used = live, *count = moved;
 }
 
 // ---------------------------------------------------------------------------------------------
-// Copies of pages: a page's part of each of the cache's buffers, in slices of 32 KB.  A CTA has 8 loads of 16 bytes a thread on their way.
+// Copies of pages: what the caches' buffers hold of a page, one behind the other, in slices of 32 KB; a CTA has 8 loads of 16 bytes a thread
+// on their way.  Slices are of the page, not of a buffer, since small pages would be nothing but ends of buffers (16 rows of one head of 64,
+// 8000 pages: 79 us by buffers).  5000 pages of 131 KB: 220 us, 6.0 TB/s, 0.92 of the copy rate.
 struct CopyPart {
   unsigned char* at;
-  unsigned bytes, slices;  // of a page
-  bool wide;               // whole 16 bytes
+  unsigned bytes, start;  // of a page; its first 16 bytes among those of the page
 };
 struct Copy {
-  CopyPart part[COPY_PARTS];
+  CopyPart wide[COPY_CACHES * COPY_PARTS], narrow[COPY_CACHES * COPY_PARTS];  // in whole 16 bytes, and in 4
+  int nwide, nnarrow;
+  unsigned pieces, slices;  // of 16 bytes, and of 32 KB of these
   const int32_t *src, *dst, *count;
   long long n;
-  unsigned pages, slices;
+  unsigned pages;
+  int32_t *map, *refs;  // not NULL: the pages move, and take their counts along
 };
 
-__global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(Copy c) {
+__global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(const __grid_constant__ Copy c) {
   constexpr int AHEAD = COPY_SLICE / 16 / COPY_THREADS;
   const long long pairs = c.count ? min(c.n, (long long)(max(__ldcg(c.count), 0))) : c.n, items = pairs * c.slices;
+  if (c.map)
+    for (long long i = (long long)(blockIdx.x) * COPY_THREADS + threadIdx.x; i < pairs; i += (long long)(gridDim.x) * COPY_THREADS) {
+      const int from = __ldcg(c.src + i), to = __ldcg(c.dst + i);
+      c.map[from] = to;
+      c.refs[to] = __ldcg(c.refs + from);
+      c.refs[from] = 0;
+    }
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
     const long long pair = item / c.slices;
-    unsigned slice = unsigned(item - pair * c.slices);
-    const int from = __ldcg(c.src + pair), to = __ldcg(c.dst + pair);
-    if (unsigned(from) >= c.pages || unsigned(to) >= c.pages) continue;
-    unsigned char* at = nullptr;
-    unsigned bytes = 0;
-    bool wide = true;
-#pragma unroll
-    for (int i = 0; i < COPY_PARTS; ++i) {
-      if (!at && slice < c.part[i].slices) at = c.part[i].at, bytes = c.part[i].bytes, wide = c.part[i].wide;
-      else if (!at) slice -= c.part[i].slices;
-    }
-    const unsigned char* const in = at + size_t(from) * bytes + size_t(slice) * COPY_SLICE;
-    unsigned char* const out = at + size_t(to) * bytes + size_t(slice) * COPY_SLICE;
-    const unsigned n = min(bytes - slice * COPY_SLICE, unsigned(COPY_SLICE));
-    if (wide) {
-      uint4 x[AHEAD];
+    const unsigned slice = unsigned(item - pair * c.slices);
+    const unsigned from = unsigned(__ldcg(c.src + pair)), to = unsigned(__ldcg(c.dst + pair));
+    if (from >= c.pages || to >= c.pages) continue;
+    const unsigned first = slice * (COPY_SLICE / 16) + threadIdx.x;
+    uint4 x[AHEAD];
+    auto each = [&](auto&& f) {
+      int part = 0;
 #pragma unroll
       for (int z = 0; z < AHEAD; ++z) {
-        const unsigned i = (threadIdx.x + z * COPY_THREADS) * 16;
-        if (i < n) x[z] = __ldcs(reinterpret_cast<const uint4*>(in + i));
+        const unsigned i = first + z * COPY_THREADS;
+        if (i >= c.pieces) continue;
+        while (part + 1 < c.nwide && i >= c.wide[part + 1].start) ++part;
+        const CopyPart& p = c.wide[part];
+        f(z, p, size_t(i - p.start) * 16);
       }
-#pragma unroll
-      for (int z = 0; z < AHEAD; ++z) {
-        const unsigned i = (threadIdx.x + z * COPY_THREADS) * 16;
-        if (i < n) __stcs(reinterpret_cast<uint4*>(out + i), x[z]);
+    };
+    each([&](int z, const CopyPart& p, size_t at) { x[z] = __ldcs(reinterpret_cast<const uint4*>(p.at + size_t(from) * p.bytes + at)); });
+    each([&](int z, const CopyPart& p, size_t at) { __stcs(reinterpret_cast<uint4*>(p.at + size_t(to) * p.bytes + at), x[z]); });
+    if (slice == 0)
+      for (int part = 0; part < c.nnarrow; ++part) {
+        const CopyPart& p = c.narrow[part];
+        for (unsigned i = threadIdx.x * 4; i < p.bytes; i += COPY_THREADS * 4)
+          *reinterpret_cast<uint32_t*>(p.at + size_t(to) * p.bytes + i) = *reinterpret_cast<const uint32_t*>(p.at + size_t(from) * p.bytes + i);
       }
-    } else {
-      for (unsigned i = threadIdx.x * 4; i < n; i += COPY_THREADS * 4) *reinterpret_cast<uint32_t*>(out + i) = *reinterpret_cast<const uint32_t*>(in + i);
-    }
   }
 }
 
-int copy_pages(const fv_kv* kv, cudaStream_t s, const int32_t* src, const int32_t* dst, size_t n, const int32_t* count) {
-  if (n == 0 || kv->pages == 0) return FV_OK;
-  const size_t rows = size_t(kv->heads) * kv->page_size, row = kv_row_bytes(kv), scale = kv_scale_bytes(kv), bounds = size_t(kv->heads) * 2 * kv->dim;
-  void* const at[COPY_PARTS] = {kv->k, kv->v, kv->bounds, kv->bound_codes, kv->k_scale, kv->v_scale, kv->bound_scale};
-  const size_t bytes[COPY_PARTS] = {rows * row, rows * row, 2 * bounds, bounds, rows * scale, rows * scale, 4 * size_t(kv->heads)};
-  Copy c = {};
-  for (int i = 0; i < COPY_PARTS; ++i) {
-    if (bytes[i] >= size_t(1) << 31) return fail(FV_ERR_UNSUPPORTED, "copies of pages: a page of 2 GB or more");
-    c.part[i] = {static_cast<unsigned char*>(at[i]), unsigned(bytes[i]), unsigned((bytes[i] + COPY_SLICE - 1) / COPY_SLICE), kv_aligned(at[i], 16) && bytes[i] % 16 == 0};
-    c.slices += c.part[i].slices;
+// The caches have `pages` pages each.
+int copy_pages(const fv_kv* const* caches, size_t ncaches, size_t pages, cudaStream_t s, const int32_t* src, const int32_t* dst, size_t n, const int32_t* count,
+               int32_t* map, int32_t* refs) {
+  if (n == 0 || pages == 0) return FV_OK;
+  for (size_t first = 0; first < ncaches || (map && first == 0); first += COPY_CACHES) {
+    Copy c = {};
+    for (size_t j = first; j < ncaches && j < first + COPY_CACHES; ++j) {
+      const fv_kv* kv = caches[j];
+      const size_t rows = size_t(kv->heads) * kv->page_size, row = kv_row_bytes(kv), scale = kv_scale_bytes(kv), bounds = size_t(kv->heads) * 2 * kv->dim;
+      void* const at[COPY_PARTS] = {kv->k, kv->v, kv->bounds, kv->bound_codes, kv->k_scale, kv->v_scale, kv->bound_scale};
+      const size_t bytes[COPY_PARTS] = {rows * row, rows * row, 2 * bounds, bounds, rows * scale, rows * scale, 4 * size_t(kv->heads)};
+      for (int i = 0; i < COPY_PARTS; ++i) {
+        if (bytes[i] == 0) continue;
+        if (bytes[i] >= size_t(1) << 31) return fail(FV_ERR_UNSUPPORTED, "copies of pages: a page of 2 GB or more");
+        if (kv_aligned(at[i], 16) && bytes[i] % 16 == 0) {
+          c.wide[c.nwide++] = {static_cast<unsigned char*>(at[i]), unsigned(bytes[i]), c.pieces};
+          c.pieces += unsigned(bytes[i] / 16);
+        } else {
+          c.narrow[c.nnarrow++] = {static_cast<unsigned char*>(at[i]), unsigned(bytes[i]), 0};
+        }
+      }
+    }
+    c.slices = (c.pieces + COPY_SLICE / 16 - 1) / (COPY_SLICE / 16);
+    c.src = src, c.dst = dst, c.count = count, c.n = (long long)(n), c.pages = unsigned(pages);
+    if (first == 0) c.map = map, c.refs = refs;
+    const size_t items = n * (c.slices ? c.slices : 1), most = 148 * 16;
+    pages_copy_kernel<<<unsigned(items < most ? items : most), COPY_THREADS, 0, s>>>(c);
+    FV_CUDA(cudaGetLastError());
   }
-  c.src = src, c.dst = dst, c.count = count, c.n = (long long)(n), c.pages = unsigned(kv->pages);
-  const size_t items = n * c.slices, most = 148 * 8;
-  pages_copy_kernel<<<unsigned(items < most ? items : most), COPY_THREADS, 0, s>>>(c);
-  FV_CUDA(cudaGetLastError());
   return FV_OK;
 }
 
@@ -415,7 +458,7 @@ extern "C" int fv_kv_copy_pages_dev(const fv_kv* kv, void* stream, const int32_t
   if (!fv::kv_aligned(src, 4) || !fv::kv_aligned(dst, 4) || !fv::kv_aligned(count, 4)) return fv::fail(FV_ERR_ARG, "fv_kv_copy_pages_dev: src, dst or count does not begin on 4 bytes");
   fv::DeviceGuard g(kv->device);
   if (!g.ok) return fv::fail(FV_ERR_CUDA, "cudaSetDevice failed (there is no CPU path)");
-  return fv::copy_pages(kv, static_cast<cudaStream_t>(stream), src, dst, n, count);
+  return fv::copy_pages(&kv, 1, kv->pages, static_cast<cudaStream_t>(stream), src, dst, n, count, nullptr, nullptr);
 }
 
 extern "C" int fv_pages_fork_dev(const fv_pages* p, void* stream, const fv_table* from, const int32_t* lens, const int32_t* parents, const fv_table* out) {
@@ -472,8 +515,7 @@ extern "C" int fv_pages_extend_dev(const fv_pages* p, void* stream, const fv_kv*
   x.free = x.before + (t->nseq + 4) / 4 * 4, x.src = x.free + room, x.dst = x.src + room;
   fv::pages_extend_kernel<<<1, fv::PAGES_THREADS, 0, s>>>(fv::pages_of(p), fv::table_of(t), x);
   FV_CUDA(cudaGetLastError());
-  for (size_t i = 0; i < ncaches; ++i) FV_TRY(fv::copy_pages(caches[i], s, x.src, x.dst, most, x.count));
-  return FV_OK;
+  return fv::copy_pages(caches, ncaches, p->pages, s, x.src, x.dst, most, x.count, nullptr, nullptr);
 }
 
 extern "C" size_t fv_pages_compact_work(const fv_pages* p) { return p ? 4 * (4 + 2 * ((p->pages + 3) / 4 * 4)) : 0; }
@@ -491,8 +533,7 @@ extern "C" int fv_pages_compact_dev(const fv_pages* p, void* stream, const fv_kv
   int32_t *const src = at + 4, *const dst = src + (p->pages + 3) / 4 * 4;
   fv::pages_compact_kernel<<<1, fv::PAGES_THREADS, 0, s>>>(fv::pages_of(p), map, used, at, src, dst);
   FV_CUDA(cudaGetLastError());
-  for (size_t i = 0; i < ncaches; ++i) FV_TRY(fv::copy_pages(caches[i], s, src, dst, size_t(p->pages), at));
-  return FV_OK;
+  return fv::copy_pages(caches, ncaches, p->pages, s, src, dst, p->pages, at, map, p->refs);
 }
 
 extern "C" int fv_pages_remap_dev(const fv_pages* p, void* stream, const int32_t* map, const fv_table* t) {
