@@ -266,9 +266,15 @@ struct Share {
             const float2 u = Pair<T>::to_float(w[s][i]);
             q[s][x][i] = Pair<M>::from_float(u.x * f, u.y * f);
           }
+          // 4 bits: a score times the scale stands in one instruction with the maximum, and is -inf where it is not seen: the scale is above 0
+          if constexpr (FOUR) q[s][x][i] = a.scale == 0.f ? 0u : q[s][x][i] ^ (a.scale < 0.f ? 0x80008000u : 0u);
         }
 #pragma unroll
       for (int i = 0; i < 2; ++i) by[x][i] = a.scale / __shfl_sync(FV_FULL, f, (2 * t + i) * 4);
+      if constexpr (FOUR) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) by[x][i] = a.scale == 0.f ? 1.f : fmaxf(fabsf(by[x][i]), __uint_as_float(1u));
+      }
     }
 #pragma unroll
     for (int x = 0; x < NT; ++x) m[x][0] = m[x][1] = far[x][0] = far[x][1] = -INFINITY, l[x][0] = l[x][1] = 0.f;
@@ -337,38 +343,32 @@ struct Share {
 #pragma unroll
     for (int h = 0; h < P; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        vs[h][i] = shared_bytes<NG>(value_scales + L::token(2 * t + (i & 1)) * NG + (16 * h + (i & 2) * 4) * NG);
-      }
+      for (int i = 0; i < 4; ++i) vs[h][i] = shared_bytes<NG>(value_scales + L::token(2 * t + (i & 1)) * NG + (16 * h + (i & 2) * 4) * NG);
+    int least = visible[0];
+    if constexpr (P > 1) least = min(least, visible[P - 1]);
+    if (least < 16) {  // of rows that are not seen scores and scales are anything
 #pragma unroll
-    for (int h = 0; h < P; ++h) {
-      if (visible[h] < 16) {  // of rows that are not seen the scales are anything
+      for (int h = 0; h < P; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vs[h][i] = L::token(2 * t + (i & 1)) + (i & 2) * 4 < visible[h] ? vs[h][i] : 0u;
-      }
-      high |= (vs[h][0] | vs[h][1]) | (vs[h][2] | vs[h][3]);
+        for (int i = 0; i < 4; ++i) {
+          vs[h][i] = L::token(2 * t + (i & 1)) + (i & 2) * 4 < visible[h] ? vs[h][i] : 0u;
+#pragma unroll
+          for (int x = 0; x < NT; ++x) s[h][x][i] = L::token(g) + (i & 2) * 4 < visible[h] ? s[h][x][i] : -INFINITY;
+        }
     }
+#pragma unroll
+    for (int h = 0; h < P; ++h) high |= (vs[h][0] | vs[h][1]) | (vs[h][2] | vs[h][3]);
     bool moved = (high & 0x80808080u) != 0u, odd = false;  // a scale of 2 or more
     float to[NT][2];
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-#pragma unroll
-      for (int h = 0; h < P; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[h][x][i] *= by[x][i & 1];
-#pragma unroll
-      for (int h = 0; h < P; ++h)
-        if (visible[h] < 16) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[h][x][i] = L::token(g) + (i & 2) * 4 < visible[h] ? s[h][x][i] : -INFINITY;
-        }
+    for (int x = 0; x < NT; ++x)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         to[x][i] = fmaxf(s[0][x][i], s[0][x][i + 2]);
         if constexpr (P > 1) to[x][i] = fmaxf(to[x][i], fmaxf(s[P - 1][x][i], s[P - 1][x][i + 2]));
+        to[x][i] *= by[x][i];
         moved = moved || to[x][i] > far[x][i];
       }
-    }
     if (__any_sync(FV_FULL, moved)) {  // seldom, after the first pieces
       uint32_t most = 0;  // of the scales that are numbers
 #pragma unroll
@@ -409,7 +409,7 @@ struct Share {
         float p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[i] = exp2_of(s[h][x][i] + off[i & 1]);
+          p[i] = exp2_of(__fmaf_rn(s[h][x][i], by[x][i & 1], off[i & 1]));
           l[x][i & 1] += p[i];
         }
 #pragma unroll
@@ -427,7 +427,7 @@ struct Share {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const uint32_t w = shared_bytes<NG>(value_scales + L::token(g) * NG + (16 * h + 8 * r) * NG);
-              const bool weight = exp2_of(s[h][x][2 * r + i] + one - (m[x][i] == -INFINITY ? 0.f : m[x][i])) != 0.f;
+              const bool weight = exp2_of(__fmaf_rn(s[h][x][2 * r + i], by[x][i], one - (m[x][i] == -INFINITY ? 0.f : m[x][i]))) != 0.f;
 #pragma unroll
               for (int y = 0; y < NG; ++y) bad |= L::token(g) + 8 * r < visible[h] && weight && (w >> (8 * y) & 255u) >= 248u ? 1u << y : 0u;
             }
@@ -448,7 +448,6 @@ struct Share {
     }
 #pragma unroll
     for (int h = 0; h < P; ++h) {
-      if (visible[h] <= 0) continue;  // its values are anything
       uint32_t v[4][(NG + 1) / 2], sc[2][NG];  // four components of every group; the groups' scales of two rows
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
