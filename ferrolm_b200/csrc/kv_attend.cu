@@ -295,14 +295,17 @@ struct Share {
       for (int h = 0; h < L::PIECES; ++h) take_four<1>(stage, h, g, t);
   }
 
-  // 4 bits: codes are exact in fp16.  A key's scales multiply the sums over their groups; a value's multiply the weights, in fp16.  For
-  // these to stay in range a weight of 1 is 2^(ONE - unit), where unit grows with scales of 2 and more, and a maximum that grows by
-  // less than 2^KV_LAG is left as it was: with few pieces to a warp, most of them have a new one (two thirds of the time went there).
+  // 4 bits: codes are exact in fp16.  A key's scales multiply the sums over their groups.  A value's multiply the weights, in fp16, which rounds
+  // them once more; for these to stay in range a weight of 1 is 2^(ONE - unit), where unit grows with scales of 2 and more.  Results in
+  // fp16 would show that (0.00036 of them against 64 bits, where one rounding leaves 0.00028 and their own 0.00021): there scales
+  // multiply the codes, exactly, at 4 % of the time.  A maximum that grows by less than 2^KV_LAG is left as it was: with few pieces to a
+  // warp, most of them have a new one (a fifth of the instructions were for that).
   // (Codes below fp16's normal numbers, masked out of their words and not subtracted from, would be less work; the tensor cores
   // keep ten bits less of a sum of such products.)
   template <int P>
   __device__ __forceinline__ void take_four(uint32_t stage, int first, int g, int t) {
     constexpr int NG = D / 32;
+    constexpr bool ONCE = std::is_same<T, __half>::value;
     int visible[P], any = 0;
 #pragma unroll
     for (int h = 0; h < P; ++h) visible[h] = int(shared_bytes<4>(stage + L::SEEN + 4 * (first + h))), any = max(any, visible[h]);
@@ -380,7 +383,7 @@ struct Share {
           odd = odd || byte >= 248u;
         }
       odd = __any_sync(FV_FULL, odd);
-      const int up = max(unit, int(__reduce_max_sync(FV_FULL, most) >> 3) - 16);  // below 2^(e - 14) = 2^(2 + unit)
+      const int up = ONCE ? 0 : max(unit, int(__reduce_max_sync(FV_FULL, most) >> 3) - 16);  // below 2^(e - 14) = 2^(2 + unit)
       const float less = __uint_as_float(uint32_t(127 + unit - up) << 23);
       unit = up;
 #pragma unroll
@@ -471,8 +474,19 @@ struct Share {
         for (int z = 0; z < 2; ++z) {
           Four::halves(__byte_perm(v[2 * z][y / 2], v[2 * z + 1][y / 2], y & 1 ? 0x7632 : 0x5410), a[z], by_1024, by_64);
           const uint32_t f = sc[z][y];
+          if constexpr (ONCE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __half2 c = __hmul2(*reinterpret_cast<const __half2*>(&a[z][e]), *reinterpret_cast<const __half2*>(&f));
+              a[z][e] = *reinterpret_cast<const uint32_t*>(&c);
+            }
+          }
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
+            if constexpr (ONCE) {
+              w[x][z] = b[h][x][z];
+              continue;
+            }
             const __half2 c = __hmul2(*reinterpret_cast<const __half2*>(&b[h][x][z]), *reinterpret_cast<const __half2*>(&f));
             w[x][z] = *reinterpret_cast<const uint32_t*>(&c);
           }

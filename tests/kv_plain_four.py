@@ -64,7 +64,7 @@ class PlainFour(PlainCache):
 
         Scores: sums of exact products, of which the groups' are added up one by one: 8 steps more than in the plain cache.  bf16
         queries become fp16 relative to their largest component, and components lose at most 2^-38 of it.
-        Weights: rounded to fp16, 2^-11 of themselves, and once more as the product with a scale.  2^(7 - unit) stands for a weight of 1,
+        Weights: rounded to fp16, 2^-11 of themselves, and for results in bf16 once more as the product with a scale.  2^(7 - unit) stands for a weight of 1,
         where 2^unit is 1 or at most half the largest scale, and the step of the smallest numbers is 2^-24: each is off by 2^-32 max(1, s / 2),
         which meets 7 s, and its product by as much, which meets 7.  Values: n products in 32 bits."""
         group, half = q.shape[1] // self.heads, torch.finfo(self.dtype).eps / 2
@@ -94,7 +94,7 @@ class PlainFour(PlainCache):
                 p = w / w.sum(-1, keepdim=True)
                 out[r, sl] = torch.where(p[..., None] > 0, p[..., None] * v, torch.where(p.isnan(), torch.nan, 0.0)[..., None]).sum(1)
                 lse[r, sl] = torch.logsumexp(s, -1)
-                weight = 2.0**-10 + 2 * off + 2 * n * 2.0**-24 + 2.0**-20
+                weight = (2.0**-11 if self.dtype == torch.float16 else 2.0**-10) + 2 * off + 2 * n * 2.0**-24 + 2.0**-20
                 tol[r, sl] = (p @ v.abs().nan_to_num()) * weight + out[r, sl].abs().nan_to_num(posinf=0) * half * 1.001
                 tol[r, sl] += n * 2.0**-32 * max(1.0, float(vs.max()) / 2) * 7 * (float(vs.max()) + 1)
                 tol[r, sl] += torch.finfo(self.dtype).smallest_normal * half
