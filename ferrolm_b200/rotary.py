@@ -76,8 +76,9 @@ class Rotary:
         else:
             tr, th, td = out.stride() if out.dim() == 3 else (0, 0, 0)
             to = out.data_ptr()
-            if out.shape != shape or out.dtype is not dtype or out.device != self.device or td != 1 or (tr | th) & 7 or to & 15:
-                _refuse(f"what is written to is {dtype} of {tuple(shape)} on {self.device}, its rows on 16 bytes")
+            apart = (tr >= self.dim or shape[0] < 2) and (th >= self.dim or shape[1] < 2)
+            if out.shape != shape or out.dtype is not dtype or out.device != self.device or td != 1 or (tr | th) & 7 or to & 15 or not apart:
+                _refuse(f"what is written to is {dtype} of {tuple(shape)} on {self.device}, its rows on 16 bytes and apart from one another")
         if d != 1 or (r | h) & 7 or at & 15:
             x = x.clone(memory_format=self._contiguous)
             r, h, d = x.stride()

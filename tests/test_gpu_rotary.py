@@ -183,7 +183,7 @@ def test_refusals():
                  lambda: r.rotate(x, lens=pos[:2]), lambda: r.rotate(x), lambda: r.rotate(x, lens=pos, positions=pos), lambda: r.rotate(x, lens=pos, cu=pos),
                  lambda: r.rotate(x[..., :32], positions=pos), lambda: r.rotate(x, x[:2], positions=pos), lambda: r.rotate(x, x.half(), positions=pos),
                  lambda: r.rotate(x.cpu(), positions=pos), lambda: r.rotate(x, positions=pos, out=x[:2]), lambda: r.rotate(x, positions=pos, out=x.half()),
-                 lambda: r.rotate(x[0], positions=pos), lambda: r.rotate(x.clone().requires_grad_(), positions=pos)):
+                 lambda: r.rotate(x[0], positions=pos), lambda: r.rotate(x, positions=pos, out=x[:, :1].expand(3, 2, 64)), lambda: r.rotate(x.clone().requires_grad_(), positions=pos)):
         with pytest.raises(fv.FerrovecError):
             call()
     with torch.no_grad():
