@@ -35,7 +35,8 @@
 
 namespace fv {
 
-int kv_prompt_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a);  // kv_prompt.cu
+int kv_prompt_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a, void* work, size_t work_bytes);  // kv_prompt.cu
+size_t kv_prompt_work(const fv_kv* kv, const fv_kv_batch* b, size_t group);
 bool kv_prompt_fits(const fv_kv_batch* b, size_t group, bool lists, size_t k);
 
 // A CTA works on each task (a row and key head), or the work of all is cut into equal parts for the warps that the GPU holds, whose
@@ -1251,8 +1252,9 @@ int kv_token_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const
 }  // namespace fv
 
 extern "C" size_t fv_kv_attend_work(const fv_kv* kv, const fv_kv_batch* batch, size_t group) {
-  if (!kv || !batch || group == 0 || group > 128 || batch->rows > fv::KV_PARTS_TASKS) return 0;
-  if (fv::is_prompt(batch, group, false, 0)) return 0;  // with lists too: a shorter union fits where the whole table does
+  if (!kv || !batch || group == 0 || group > 128) return 0;
+  if (fv::is_prompt(batch, group, false, 0)) return fv::kv_prompt_work(kv, batch, group);  // with lists too: a shorter union fits where the whole table does
+  if (batch->rows > fv::KV_PARTS_TASKS) return 0;
   const size_t cols = group <= 8 ? 8 : 16, tasks = batch->rows * kv->heads * ((group + cols - 1) / cols), pieces = batch->table_width * (kv->page_size / 16);
   const bool parts = fv::in_parts(kv->kind, int(kv->dim), int(group), false, tasks, pieces) || fv::in_parts(kv->kind, int(kv->dim), int(group), true, tasks, pieces);
   return parts ? (tasks + fv::KV_PARTS_WARPS) * cols * (kv->dim + 2) * 4 : 0;
@@ -1274,6 +1276,6 @@ extern "C" int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch
                        scale * 1.44269504088896341f, static_cast<const unsigned char*>(kv->k), static_cast<const unsigned char*>(kv->v),
                        kv->k_scale, kv->v_scale, static_cast<unsigned char*>(out), lse};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (kv->pages && fv::is_prompt(batch, group, blocks != nullptr, k)) return fv::kv_prompt_attend(kv, s, batch, a);
+  if (kv->pages && fv::is_prompt(batch, group, blocks != nullptr, k)) return fv::kv_prompt_attend(kv, s, batch, a, work, work_bytes);
   return fv::kv_token_attend(kv, s, batch, a, work, work_bytes);
 }

@@ -125,9 +125,11 @@ __device__ __forceinline__ uint32_t watch(uint32_t x, uint32_t w) {
 // What all warps of a CTA know about its work.
 struct PromptWork {
   int head, last, pieces, tiles;  // position of the last row; pieces of 16 rows of the cache, tiles of four of them
+  int first;                      // 4 bits: tile of the union that is this CTA's first
   const int2* list;               // (block, page) of the union, ascending
-  // piece p: where it begins, and its first row in the pages; false: it is none, or has no page
+  // piece p of the CTA's: where it begins, and its first row in the pages; false: it is none, or has no page
   __device__ __forceinline__ bool piece(const KvAttend& a, const KvBatch& m, int p, int& start, size_t& from) const {
+    p += 4 * first;
     if (p >= pieces) return false;
     const int per = m.page_shift - 4, sub = (p & ((1 << per) - 1)) << 4;
     const int2 at = list[p >> per];
@@ -331,8 +333,16 @@ __device__ __forceinline__ void bring_all(const KvAttend& a, const KvBatch& m, c
   }
 }
 
+// 4 bits: the tiles of a CTA's union are shared out to `count` CTAs where there are few of them, at least KV_PROMPT_LEAST to each, whose
+// results [count][rows * heads * group][D] and logarithms to the base of 2 a second kernel joins.
+struct PromptParts {
+  int count;
+  float *out, *lse;
+};
+enum { KV_PROMPT_LEAST = 6, KV_PROMPT_PLACES = 2 * 148, KV_PROMPT_PARTS = 64 };
+
 template <class T, int KIND, int D>
-__global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAttend a, KvBatch m) {
+__global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAttend a, KvBatch m, PromptParts parts) {
   using S = Tile<KIND, D>;
   using M = typename std::conditional<KIND == FV_KV_SAME, T, __half>::type;
   constexpr bool HALF = std::is_same<M, __half>::value, FOUR = KIND == FV_KV_INT4X32, SCALED = kv_scaled(KIND);
@@ -449,6 +459,14 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
   // of the last block only the pieces up to the last row
   work.pieces = entries ? ((entries - 1) << per) + min(1 << per, ((last - (list[entries - 1].x << m.page_shift)) >> 4) + 1) : 0;
   work.tiles = (work.pieces + 3) / 4;
+  work.first = 0;
+  if constexpr (FOUR) {
+    if (parts.count > 1) {
+      const int each = max((work.tiles + parts.count - 1) / parts.count, int(KV_PROMPT_LEAST));
+      work.first = int(blockIdx.z) * each;
+      work.tiles = min(max(work.tiles - work.first, 0), each);
+    }
+  }
   const int tiles = work.tiles;
   const uint32_t tmem = bars->tmem;
   const AbortCtl abort{&bars->abort, WAIT_LIMIT_CYCLES};
@@ -540,14 +558,15 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
       };
       if (m.page_shift >= 6) {  // the tile is of one block
         const int more = m.page_shift - 6;
-        const int2 at = list[i >> more];
-        const int start = (at.x << m.page_shift) + ((i & ((1 << more) - 1)) << 6), n = sees(at, start) ? pos - start + 1 : 0;
+        const int tile = FOUR ? i + work.first : i;
+        const int2 at = list[tile >> more];
+        const int start = (at.x << m.page_shift) + ((tile & ((1 << more) - 1)) << 6), n = sees(at, start) ? pos - start + 1 : 0;
 #pragma unroll
         for (int p = 0; p < 4; ++p) seen[p] = min(max(n - 16 * p, 0), 16);
       } else {
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          const int piece = 4 * i + p;
+          const int piece = 4 * (FOUR ? i + work.first : i) + p;
           const int2 at = piece < work.pieces ? list[piece >> per] : make_int2(0, -1);
           const int start = (at.x << m.page_shift) + ((piece & ((1 << per) - 1)) << 4);
           seen[p] = sees(at, start) ? min(pos - start + 1, 16) : 0;
@@ -718,11 +737,24 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
     const float f = SCALED ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
     const float down = sum == 0.f ? 0.f : 1.f / sum;
     const size_t query = (size_t(row0 + tok) * a.heads + head) * a.group + h;
+    const bool part = FOUR && parts.count > 1;
+    const size_t place = part ? size_t(blockIdx.z) * (size_t(m.rows) * a.heads * a.group) + query : 0;
 #pragma unroll 1
     for (int c = 0; c < D; c += 32) {
       uint32_t o[32];
       tc_ld32_issue(tmem + lanes + S::O_COL + c, o);
       tc_ld_wait(o);
+      if constexpr (FOUR) {
+        if (part) {  // one to be joined: as 32-bit numbers
+#pragma unroll
+          for (int z = 0; z < 8; ++z) {  // of every eight in their order 0 4 1 5 2 6 3 7
+            const int b = 8 * (z >> 1) + (z & 1 ? 1 : 0);
+            const float4 x = make_float4(__uint_as_float(o[b]) * down, __uint_as_float(o[b + 2]) * down, __uint_as_float(o[b + 4]) * down, __uint_as_float(o[b + 6]) * down);
+            if (mine && sum != 0.f) *reinterpret_cast<float4*>(parts.out + place * D + c + 4 * z) = x;
+          }
+          continue;
+        }
+      }
       uint4 w[4];
 #pragma unroll
       for (int z = 0; z < 16; ++z) {
@@ -738,7 +770,8 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
         for (int z = 0; z < 4; ++z) *reinterpret_cast<uint4*>(a.out + (query * D + c + 8 * z) * 2) = w[z];
       }
     }
-    if (mine && a.lse) a.lse[query] = !on ? __int_as_float(0x7FC00000) : sum == 0.f ? -INFINITY : (top - ONE + log2f(sum)) * 0.693147180559945309f;
+    if (part && mine) parts.lse[place] = !on ? __int_as_float(0x7FC00000) : sum == 0.f ? -INFINITY : top - ONE + log2f(sum);
+    if (!part && mine && a.lse) a.lse[query] = !on ? __int_as_float(0x7FC00000) : sum == 0.f ? -INFINITY : (top - ONE + log2f(sum)) * 0.693147180559945309f;
   }
   if (warp >= 6) asm volatile("cp.async.wait_all;");
   tc_fence_before();
@@ -747,16 +780,77 @@ __global__ void __launch_bounds__(KV_PROMPT_THREADS, 2) kv_prompt_kernel(KvAtten
   if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
 }
 
+// Joins the parts of a query: a warp to each.
+template <class T, int D>
+__global__ void __launch_bounds__(256) kv_prompt_join_kernel(KvAttend a, KvBatch m, PromptParts parts) {
+  const int lane = lane_id(), heads = a.heads * a.group, row = blockIdx.x;
+  const int b = m.cu ? kv_find(m, row, 1, 0) : row;
+  if (row < m.cu_at(b) || row >= m.cu_at(b + 1)) return;  // of no sequence
+  const size_t all = size_t(m.rows) * heads;
+  for (int h = blockIdx.y * 8 + (threadIdx.x >> 5); h < heads; h += gridDim.y * 8) {
+    const size_t query = size_t(row) * heads + h;
+    float l[2], most = -INFINITY;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      l[z] = lane + 32 * z < parts.count ? parts.lse[(lane + 32 * z) * all + query] : -INFINITY;
+      most = fmaxf(most, l[z]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(FV_FULL, most, o));
+    float total = 0.f;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) l[z] = l[z] == -INFINITY ? 0.f : exp2_of(l[z] - (most == -INFINITY ? 0.f : most)), total += l[z];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FV_FULL, total, o);
+    float sum[D / 32] = {};
+    for (int z = 0; z < parts.count; ++z) {
+      const float w = __shfl_sync(FV_FULL, z < 32 ? l[0] : l[1], z & 31);
+      if (w == 0.f) continue;  // nothing seen there: its results are anything
+      const float* from = parts.out + (size_t(z) * all + query) * D;
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const float2 x = *reinterpret_cast<const float2*>(from + 64 * i + 2 * lane);
+        sum[2 * i] = __fmaf_rn(w, x.x, sum[2 * i]), sum[2 * i + 1] = __fmaf_rn(w, x.y, sum[2 * i + 1]);
+      }
+      if constexpr (D % 64 != 0) sum[D / 32 - 1] = __fmaf_rn(w, from[D - 32 + lane], sum[D / 32 - 1]);
+    }
+    const float down = total == 0.f ? 0.f : 1.f / total;
+    unsigned char* const to = a.out + query * (2 * D);
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i)
+      *reinterpret_cast<uint32_t*>(to + 128 * i + 4 * lane) = total == 0.f ? 0u : Pair<T>::from_float(sum[2 * i] * down, sum[2 * i + 1] * down);
+    if constexpr (D % 64 != 0) {
+      const uint32_t w = total == 0.f ? 0u : Pair<T>::from_float(sum[D / 32 - 1] * down, 0.f);
+      *reinterpret_cast<uint16_t*>(to + 2 * (D - 32 + lane)) = uint16_t(w);
+    }
+    if (a.lse && lane == 0) a.lse[query] = total == 0.f ? -INFINITY : (most + log2f(total)) * 0.693147180559945309f;
+  }
+}
+
 size_t prompt_entries(const fv_kv_batch* b, int group, bool lists, size_t k) {
   const size_t most = size_t(KV_PROMPT_COLS / group) * k;
   return lists && most < b->table_width ? most : b->table_width;
 }
 
+size_t prompt_items(const fv_kv_batch* b, int group) {
+  const int tc = KV_PROMPT_COLS / group;
+  return b->cu ? b->rows / tc + b->nseq : b->nseq;
+}
+
+// CTAs that the tiles of one's union are shared out to: as many as fill the places that are there for all, by the most tiles that a union can have.
+int prompt_parts(const fv_kv* kv, const fv_kv_batch* b, int group, bool lists, size_t k) {
+  const size_t ctas = prompt_items(b, group) * kv->heads, tiles = prompt_entries(b, group, lists, k) * kv->page_size / 64;
+  if (kv->kind != FV_KV_INT4X32 || ctas == 0) return 1;
+  size_t n = KV_PROMPT_PLACES / ctas;
+  if (n > tiles / KV_PROMPT_LEAST) n = tiles / KV_PROMPT_LEAST;
+  return int(n < 1 ? 1 : n > KV_PROMPT_PARTS ? KV_PROMPT_PARTS : n);
+}
+size_t part_floats(const fv_kv* kv, const fv_kv_batch* b, int group) { return b->rows * kv->heads * group * (kv->dim + 1); }
+
 template <class T, int KIND, int D>
-int prompt_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a) {
+int prompt_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a, void* work, size_t work_bytes) {
   using S = Tile<KIND, D>;
-  const int tc = KV_PROMPT_COLS / a.group;
-  const size_t items = b->cu ? b->rows / tc + b->nseq : b->nseq;
+  const size_t items = prompt_items(b, a.group);
   const size_t smem = S::LIST_AT + 8 * prompt_entries(b, a.group, a.blocks != nullptr, a.k);
   FV_TRY((kv_allow_smem<kv_prompt_kernel<T, KIND, D>>(kv->device, smem)));
   static std::atomic<int> regs{0};  // a thread's at launch: the kernel waits for more than they add up to
@@ -766,8 +860,20 @@ int prompt_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAtt
     regs.store(at.numRegs, std::memory_order_relaxed);
   }
   if (regs.load(std::memory_order_relaxed) < KV_PROMPT_REGS) return fail(FV_ERR_UNSUPPORTED, "fv_kv_attend_dev: built with fewer registers than it shares out");
-  kv_prompt_kernel<T, KIND, D><<<dim3(unsigned(items), kv->heads), KV_PROMPT_THREADS, smem, s>>>(a, kv_batch(kv, b));
+  PromptParts parts{1, nullptr, nullptr};
+  if constexpr (KIND == FV_KV_INT4X32) {
+    const size_t floats = part_floats(kv, b, a.group), room = work ? work_bytes / 4 / floats : 0;
+    const int n = prompt_parts(kv, b, a.group, a.blocks != nullptr, a.k);
+    parts.count = room < 2 ? 1 : size_t(n) < room ? n : int(room);
+    parts.out = static_cast<float*>(work), parts.lse = parts.out + size_t(parts.count) * (floats - floats / (D + 1));
+  }
+  kv_prompt_kernel<T, KIND, D><<<dim3(unsigned(items), kv->heads, parts.count), KV_PROMPT_THREADS, smem, s>>>(a, kv_batch(kv, b), parts);
   FV_CUDA(cudaGetLastError());
+  if constexpr (KIND == FV_KV_INT4X32)
+    if (parts.count > 1) {
+      kv_prompt_join_kernel<T, D><<<dim3(unsigned(b->rows), unsigned((kv->heads * a.group + 7) / 8)), 256, 0, s>>>(a, kv_batch(kv, b), parts);
+      FV_CUDA(cudaGetLastError());
+    }
   return FV_OK;
 }
 
@@ -778,6 +884,14 @@ bool kv_prompt_fits(const fv_kv_batch* b, size_t group, bool lists, size_t k) {
   return prompt_entries(b, int(group), lists, k) <= (226 * 1024 - size_t(Tile<FV_KV_INT8, 128>::LIST_AT)) / 8 && b->table_width <= (1u << 18);
 }
 
-int kv_prompt_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a) { FV_KV_DISPATCH(kv, prompt_of, kv, s, b, a); }
+// Bytes of work that a call's parts want, whatever its lists.
+size_t kv_prompt_work(const fv_kv* kv, const fv_kv_batch* b, size_t group) {
+  const int n = prompt_parts(kv, b, int(group), false, 0);  // lists have at most as many tiles
+  return n > 1 ? 4 * size_t(n) * part_floats(kv, b, int(group)) : 0;
+}
+
+int kv_prompt_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a, void* work, size_t work_bytes) {
+  FV_KV_DISPATCH(kv, prompt_of, kv, s, b, a, work, work_bytes);
+}
 
 }  // namespace fv

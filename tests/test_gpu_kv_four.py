@@ -152,6 +152,34 @@ def test_prompts(dtype, heads, group, dim, page):
     check(c, p, q, table[:, :2], lens, cu, None)  # rows behind the table's last column
 
 
+@pytest.mark.parametrize("dtype,heads,group,dim,page", [(BF, 1, 4, 128, 16), (FP, 2, 7, 96, 64), (BF, 1, 16, 64, 128), (FP, 1, 2, 128, 32)])
+@pytest.mark.parametrize("news,lens", [([6], [2500]), ([9, 5, 0, 7], [1900, 3, 700, 1025]), ([40, 6], [600, 1700])])
+def test_few_rows_over_long_sequences(dtype, heads, group, dim, page, news, lens):
+    """Rows of a sequence whose keys are shared out to many CTAs, some of which see nothing; with a result's place given and without,
+    with and without the logarithms, rows of no sequence left as they were; and the same without room for it."""
+    import ferrolm_b200 as fv
+
+    width = -(-max(lens) // page) + 3
+    c, p = pair(width * len(news) + 1, heads, dim, page, dtype, seed=len(news))
+    table = batch(len(news), width, c.pages, 2)
+    table[0, 2] = -1
+    cu = i32([0] + torch.tensor(news).cumsum(0).tolist())
+    n = int(cu[-1]) + 2
+    q = queries(n, heads, group, dim, dtype, 3)
+    got = check(c, p, q, table, lens, cu, None)
+    check(c, p, q, table, lens, cu, lists(n, heads, 60, width, 4))
+    at = q.cuda(), table.cuda(), i32(lens).cuda(), cuda(cu)
+    alone = c.attend(*at[:3], cu=at[3])
+    assert torch.equal(alone[: int(cu[-1])], got[0][: int(cu[-1])])
+    # the entry point without work: one CTA for each tile of queries
+    whole, lse = torch.zeros_like(got[0]), torch.zeros_like(got[1])
+    b = c._batch(at[1], at[2], at[3], n)
+    assert fv.kv.lib().fv_kv_attend_work(c._ref, b, group) > 0
+    fv.kv.check(c._attend(c._ref, torch.cuda.current_stream().cuda_stream, b, at[0].data_ptr(), at[0].stride(0), at[0].stride(1), group, None, 0, dim**-0.5, whole.data_ptr(), lse.data_ptr(), None, 0))
+    want = p.attend(q, table, lens, cu, None, dim**-0.5, torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape[:2], dtype=torch.float64))
+    assert ((whole.cpu().double() - want[0]).abs() <= want[2]).all()
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("news", [[1, 1, 1], [90, 20, 30]])
 def test_groups_that_are_no_numbers(dtype, news):
