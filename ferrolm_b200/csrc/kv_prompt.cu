@@ -837,13 +837,21 @@ size_t prompt_items(const fv_kv_batch* b, int group) {
   return b->cu ? b->rows / tc + b->nseq : b->nseq;
 }
 
-// CTAs that the tiles of one's union are shared out to: as many as fill the places that are there for all, by the most tiles that a union can have.
+// CTAs that the tiles of one's union are shared out to, by the most tiles that a union can have: those that go in the fewest waves of places for
+// their size, a part's beginning and end counted as a 25th of the whole.  Where all places are taken anyway CTAs of unequal lengths follow one
+// another, and parts only cost (4 groups of 8 key heads, dim 128, us by parts 1/2/3/4/5/8):
+//   104 CTAs, 400 rows over 16,000    304/236/251/208/210/219      216 CTAs, 400 rows over 20,000    543/503/512/460/496/517
+//   256 CTAs, 1000 rows over 8000     224/246/259/259/279/330      648 CTAs, 3000 rows over 6000     445/506/552/599/649/793
 int prompt_parts(const fv_kv* kv, const fv_kv_batch* b, int group, bool lists, size_t k) {
   const size_t ctas = prompt_items(b, group) * kv->heads, tiles = prompt_entries(b, group, lists, k) * kv->page_size / 64;
-  if (kv->kind != FV_KV_INT4X32 || ctas == 0) return 1;
-  size_t n = KV_PROMPT_PLACES / ctas;
-  if (n > tiles / KV_PROMPT_LEAST) n = tiles / KV_PROMPT_LEAST;
-  return int(n < 1 ? 1 : n > KV_PROMPT_PARTS ? KV_PROMPT_PARTS : n);
+  if (kv->kind != FV_KV_INT4X32 || ctas == 0 || ctas >= KV_PROMPT_PLACES) return 1;
+  int best = 1;
+  double least = 1e30;
+  for (size_t n = 1; n <= KV_PROMPT_PARTS && (n == 1 || n * KV_PROMPT_LEAST <= tiles); ++n) {
+    const double cost = double((ctas * n + KV_PROMPT_PLACES - 1) / KV_PROMPT_PLACES) * (1.0 / double(n) + 0.04);
+    if (cost < least) least = cost, best = int(n);
+  }
+  return best;
 }
 size_t part_floats(const fv_kv* kv, const fv_kv_batch* b, int group) { return b->rows * kv->heads * group * (kv->dim + 1); }
 
