@@ -14,7 +14,7 @@
 namespace fv {
 namespace {
 
-enum { PAGES_THREADS = 1024, PAGES_WARPS = 32, PAGES_SEQS = 2048, COPY_THREADS = 256, COPY_SLICE = 32 * 1024, COPY_PARTS = 7, COPY_CACHES = 8 };
+enum { PAGES_THREADS = 1024, PAGES_WARPS = 32, PAGES_SEQS = 2048, COPY_THREADS = 256, COPY_SLICE = 32 * 1024, COPY_PARTS = 7, COPY_CACHES = 8, PAGES_WINDOW = 32 * 1024 };
 
 struct Pages {
   int32_t* refs;
@@ -50,45 +50,36 @@ __device__ __forceinline__ int sum_before(int x, int* s, int* all) {
   return before + up - x;
 }
 
-// The warp's part of the pages, four neighbours a lane.  Counts of up to 1024 pages a warp stay in registers from the first look on, so that the
-// passes over them do not wait for memory again, and the first look may be long before.
-struct PageShare {
-  enum { AHEAD = 8 };
-  int begin, end;  // of the warp's pages
-  bool kept;
+// The counts of a window of pages in a CTA's registers: a warp has 1024 of them in ascending order, a lane four neighbours at a time.  So passes over
+// them do not wait for memory again, and the look may be long before.
+struct PageWindow {
+  enum { AHEAD = PAGES_WINDOW / PAGES_WARPS / 128 };
+  int begin;  // of the warp's pages
   int4 r[AHEAD];
-  __device__ __forceinline__ void load(const Pages& p, int from) {
+  __device__ __forceinline__ void look(const Pages& p, int base) {
     const bool wide = (reinterpret_cast<uintptr_t>(p.refs) & 15) == 0;
+    begin = base + int(threadIdx.x >> 5) * (128 * AHEAD);
 #pragma unroll
     for (int z = 0; z < AHEAD; ++z) {
-      const int at = from + 128 * z + 4 * int(lane_id());
+      const int at = begin + 128 * z + 4 * int(lane_id());
       r[z] = make_int4(-1, -1, -1, -1);  // behind the last page
-      if (from + 128 * z >= end) continue;
+      if (at >= p.pages) continue;
       if (wide && at + 4 <= p.pages) {
         r[z] = __ldcg(reinterpret_cast<const int4*>(p.refs + at));
       } else {
-        if (at < p.pages) r[z].x = __ldcg(p.refs + at);
+        r[z].x = __ldcg(p.refs + at);
         if (at + 1 < p.pages) r[z].y = __ldcg(p.refs + at + 1);
         if (at + 2 < p.pages) r[z].z = __ldcg(p.refs + at + 2);
         if (at + 3 < p.pages) r[z].w = __ldcg(p.refs + at + 3);
       }
     }
   }
-  __device__ __forceinline__ void look(const Pages& p) {
-    const long long warp = threadIdx.x >> 5, share = ((p.pages + PAGES_WARPS - 1) / PAGES_WARPS + 127) & ~127;
-    begin = int(min(warp * share, (long long)(p.pages))), end = int(min(warp * share + share, (long long)(p.pages)));
-    kept = share <= 128 * AHEAD;
-    load(p, begin);
-  }
   // f(first of four pages, their counts) for whole warps, in ascending order, as long as it says so
   template <class F>
-  __device__ __forceinline__ void each(const Pages& p, F&& f) {
-    for (int i = begin; i < end; i += 128 * AHEAD) {
-      if (!kept) load(p, i);
+  __device__ __forceinline__ void each(const Pages& p, F&& f) const {
 #pragma unroll
-      for (int z = 0; z < AHEAD; ++z)
-        if (i + 128 * z < end && !f(i + 128 * z + 4 * int(lane_id()), r[z])) return;
-    }
+    for (int z = 0; z < AHEAD; ++z)
+      if (begin + 128 * z < p.pages && !f(begin + 128 * z + 4 * int(lane_id()), r[z])) return;
   }
 };
 
@@ -116,8 +107,8 @@ __device__ __forceinline__ int32_t* entry_at(const Pages& p, const Table& t, con
 __global__ void __launch_bounds__(PAGES_THREADS) pages_extend_kernel(Pages p, Table t, Extend x) {
   __shared__ int s_sum[PAGES_WARPS + 1], s_before[PAGES_SEQS + 1], s_count;
   const int tid = threadIdx.x;
-  PageShare share;
-  share.look(p);  // those that are free now: counts that come to nothing below are given back
+  PageWindow window;
+  window.look(p, 0);  // those that are free now: counts that come to nothing below are given back
   int* const before = t.nseq <= PAGES_SEQS ? s_before : x.before;
   if (tid == 0) s_count = 0, before[0] = 0;
   int entries = 0;
@@ -177,39 +168,46 @@ __global__ void __launch_bounds__(PAGES_THREADS) pages_extend_kernel(Pages p, Ta
   wants = all;
   if (wants) {
     // the free pages, as many as are wanted
-    int n = 0;
-    share.each(p, [&](int, const int4& r) { return n += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0), true; });
-    int rank = sum_before(n, s_sum, &all);  // of a lane: its pages are not neighbours, only the warp's sum counts
-    if (all < wants) {  // nothing is changed
+    int found = 0;
+    for (int base = 0;;) {
+      int n = 0;
+      window.each(p, [&](int, const int4& r) { return n += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0), true; });
+      int rank = found + sum_before(n, s_sum, &all);  // of a lane: its pages are not neighbours, only the warp's sum counts
+      rank = __shfl_sync(FV_FULL, rank, 0);
+      found += all;
+      if (rank < wants) {
+        window.each(p, [&](int at, const int4& r) {
+          const int c = (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
+          int up = c;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(FV_FULL, up, o);
+            if (int(lane_id()) >= o) up += y;
+          }
+          int i = rank + up - c;
+          if (r.x == 0 && i < wants) x.free[i] = at;
+          i += r.x == 0;
+          if (r.y == 0 && i < wants) x.free[i] = at + 1;
+          i += r.y == 0;
+          if (r.z == 0 && i < wants) x.free[i] = at + 2;
+          i += r.z == 0;
+          if (r.w == 0 && i < wants) x.free[i] = at + 3;
+          rank += __shfl_sync(FV_FULL, up, 31);
+          return rank < wants;
+        });
+      }
+      if (found >= wants || p.pages - base <= PAGES_WINDOW) break;
+      base += PAGES_WINDOW;
+      window.look(p, base);
+    }
+    if (found < wants) {  // nothing is changed
       for (int e = tid; e < entries; e += PAGES_THREADS) {
         const int q = -2 - get(e);
         if (q >= 0) atomicAdd(p.refs + q, 1), put(e, q);
       }
       if (at0) *at0 = q0;
-      if (tid == 0) *x.missing = wants - all, *x.count = 0;
+      if (tid == 0) *x.missing = wants - found, *x.count = 0;
       return;
-    }
-    rank = __shfl_sync(FV_FULL, rank, 0);
-    if (rank < wants) {
-      share.each(p, [&](int at, const int4& r) {
-        const int c = (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
-        int up = c;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(FV_FULL, up, o);
-          if (int(lane_id()) >= o) up += y;
-        }
-        int i = rank + up - c;
-        if (r.x == 0 && i < wants) x.free[i] = at;
-        i += r.x == 0;
-        if (r.y == 0 && i < wants) x.free[i] = at + 1;
-        i += r.y == 0;
-        if (r.z == 0 && i < wants) x.free[i] = at + 2;
-        i += r.z == 0;
-        if (r.w == 0 && i < wants) x.free[i] = at + 3;
-        rank += __shfl_sync(FV_FULL, up, 31);
-        return rank < wants;
-      });
     }
     __syncthreads();
     int given = 0;
@@ -273,28 +271,61 @@ __global__ void __launch_bounds__(256) pages_remap_kernel(const int32_t* map, in
   }
 }
 
-__global__ void __launch_bounds__(PAGES_THREADS) pages_compact_kernel(Pages p, int32_t* map, int32_t* used, int32_t* count, int32_t* src, int32_t* dst) {
+// Pages in use in each window.
+__global__ void __launch_bounds__(PAGES_THREADS) pages_count_kernel(Pages p, int32_t* counts) {
   __shared__ int s_sum[PAGES_WARPS + 1];
-  const int lane = lane_id();
-  PageShare share;
-  share.look(p);
+  PageWindow window;
+  window.look(p, int(blockIdx.x) * PAGES_WINDOW);
   int n = 0, all;
-  share.each(p, [&](int, const int4& r) { return n += (r.x > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0), true; });
+  window.each(p, [&](int, const int4& r) { return n += (r.x > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0), true; });
   sum_before(n, s_sum, &all);
-  const int live = all;
-  // a page below `live` that is free is a hole; one from there on that is not moves to the hole of its number
+  if (threadIdx.x == 0) counts[blockIdx.x] = all;
+}
+
+// With n pages in use a free one below n is a hole, and one in use from there on moves to the hole of its number.  A CTA lists the holes and movers
+// of its window; how many there are before it follows from the windows' counts and, where one lies on both sides of n, a look at that.
+__global__ void __launch_bounds__(PAGES_THREADS) pages_compact_kernel(Pages p, const int32_t* counts, int32_t* map, int32_t* used, int32_t* count, int32_t* src, int32_t* dst) {
+  __shared__ int s_sum[PAGES_WARPS + 1];
+  const int lane = lane_id(), windows = gridDim.x, mine = blockIdx.x;
+  PageWindow window;
+  window.look(p, mine * PAGES_WINDOW);
+  int n = 0, live, all;
+  if (windows == 1) {
+    window.each(p, [&](int, const int4& r) { return n += (r.x > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0), true; });
+  } else {
+    for (int i = threadIdx.x; i < windows; i += PAGES_THREADS) n += __ldcg(counts + i);
+  }
+  sum_before(n, s_sum, &live);
+  // holes and movers of the windows before
+  int hole = 0, mover = 0, moved = 0;
+  if (windows > 1) {
+    const int border = live / PAGES_WINDOW;
+    int below = 0;  // in use in the border's window, in front of the border
+    for (int i = border * PAGES_WINDOW + threadIdx.x; i < live; i += PAGES_THREADS) below += __ldcg(p.refs + i) > 0;
+    sum_before(below, s_sum, &below);
+    int h = 0, m = 0, t = 0;
+    for (int i = threadIdx.x; i < windows; i += PAGES_THREADS) {
+      const int c = __ldcg(counts + i);
+      const int holes = i < border ? PAGES_WINDOW - c : i == border ? live - border * PAGES_WINDOW - below : 0;
+      t += holes;
+      if (i < mine) h += holes, m += i < border ? 0 : i == border ? c - below : c;
+    }
+    sum_before(h, s_sum, &hole);
+    sum_before(m, s_sum, &mover);
+    sum_before(t, s_sum, &moved);
+  }
   int holes = 0, movers = 0;
-  share.each(p, [&](int at, const int4& r) {
+  window.each(p, [&](int at, const int4& r) {
     const int* c = reinterpret_cast<const int*>(&r);
 #pragma unroll
     for (int z = 0; z < 4; ++z) holes += at + z < live && c[z] <= 0, movers += at + z >= live && at + z < p.pages && c[z] > 0;
     return true;
   });
-  int hole = sum_before(holes, s_sum, &all);
-  const int moved = all;
-  int mover = sum_before(movers, s_sum, &all);
+  hole += sum_before(holes, s_sum, &all);
+  if (windows == 1) moved = all;
+  mover += sum_before(movers, s_sum, &all);
   hole = __shfl_sync(FV_FULL, hole, 0), mover = __shfl_sync(FV_FULL, mover, 0);
-  share.each(p, [&](int at, const int4& r) {
+  window.each(p, [&](int at, const int4& r) {
     const int* c = reinterpret_cast<const int*>(&r);
     int own = 0;  // a hole, or from `live` on a mover: a lane's four are counted together, 128 pages lie on both sides of `live` at most once
 #pragma unroll
@@ -317,7 +348,7 @@ __global__ void __launch_bounds__(PAGES_THREADS) pages_compact_kernel(Pages p, i
     hole += sum & 0xFFFF, mover += sum >> 16;
     return true;
   });
-  if (threadIdx.x == 0) *used = live, *count = moved;
+  if (mine == 0 && threadIdx.x == 0) *used = live, *count = moved;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -521,7 +552,9 @@ extern "C" int fv_pages_extend_dev(const fv_pages* p, void* stream, const fv_kv*
   return fv::copy_pages(caches, ncaches, p->pages, s, x.src, x.dst, most, x.count, nullptr, nullptr);
 }
 
-extern "C" size_t fv_pages_compact_work(const fv_pages* p) { return p ? 4 * (4 + 2 * ((p->pages + 3) / 4 * 4)) : 0; }
+// work: the number of moves, their sources and places, and the windows' counts
+static size_t page_windows(const fv_pages* p) { return p->pages > fv::PAGES_WINDOW ? (p->pages + fv::PAGES_WINDOW - 1) / fv::PAGES_WINDOW : 1; }
+extern "C" size_t fv_pages_compact_work(const fv_pages* p) { return p ? 4 * (4 + 2 * ((p->pages + 3) / 4 * 4) + (page_windows(p) + 3) / 4 * 4) : 0; }
 
 extern "C" int fv_pages_compact_dev(const fv_pages* p, void* stream, const fv_kv* const* caches, size_t ncaches, int32_t* used, int32_t* map, void* work, size_t work_bytes) {
   const char* w = "fv_pages_compact_dev";
@@ -533,8 +566,13 @@ extern "C" int fv_pages_compact_dev(const fv_pages* p, void* stream, const fv_kv
   if (!g.ok) return fv::fail(FV_ERR_CUDA, "cudaSetDevice failed (there is no CPU path)");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int32_t* const at = static_cast<int32_t*>(work);
-  int32_t *const src = at + 4, *const dst = src + (p->pages + 3) / 4 * 4;
-  fv::pages_compact_kernel<<<1, fv::PAGES_THREADS, 0, s>>>(fv::pages_of(p), map, used, at, src, dst);
+  int32_t *const src = at + 4, *const dst = src + (p->pages + 3) / 4 * 4, *const counts = dst + (p->pages + 3) / 4 * 4;
+  const unsigned windows = unsigned(page_windows(p));
+  if (windows > 1) {
+    fv::pages_count_kernel<<<windows, fv::PAGES_THREADS, 0, s>>>(fv::pages_of(p), counts);
+    FV_CUDA(cudaGetLastError());
+  }
+  fv::pages_compact_kernel<<<windows, fv::PAGES_THREADS, 0, s>>>(fv::pages_of(p), counts, map, used, at, src, dst);
   FV_CUDA(cudaGetLastError());
   return fv::copy_pages(caches, ncaches, p->pages, s, src, dst, p->pages, at, map, p->refs);
 }

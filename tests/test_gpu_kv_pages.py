@@ -163,7 +163,7 @@ def test_too_few_pages_change_nothing():
     same_rows(caches, moved(rows, plain.copied))
 
 
-@pytest.mark.parametrize("pages,live", [(1, 0), (1, 1), (127, 60), (128, 128), (4097, 1), (5000, 2500), (5000, 4990), (40001, 15000)])
+@pytest.mark.parametrize("pages,live", [(1, 0), (1, 1), (127, 60), (128, 128), (4097, 1), (5000, 2500), (5000, 4990), (32768, 20000), (32769, 32768), (40001, 15000), (40001, 36000), (150000, 65536), (150000, 100000), (150000, 300), (131072, 131072)])
 def test_compaction(pages, live):
     g = torch.Generator().manual_seed(pages + live)
     caches, p, plain = make(pages, 16, ((1, 64, BF, "int4x32"),))
@@ -177,6 +177,20 @@ def test_compaction(pages, live):
     same_rows(caches, moved(rows, plain.copied))
     p.compact(), p.compact(table[:0])
     same(table, p, want, plain)
+
+
+@pytest.mark.parametrize("free", [[100_000, 7], [32_767, 32_768, 65_535, 65_536, 99_999], [99_998]])
+def test_room_far_behind(free):
+    """Free pages in windows behind the first, and fewer of them than are wanted."""
+    caches, p, plain = make(100_001, 16, ((1, 64, BF, "int4x32"),))
+    p.refs.fill_(1)
+    p.refs[torch.tensor(free).cuda()] = 0
+    plain.refs = p.refs.tolist()
+    table, want = torch.full((3, 4), -1, dtype=torch.int32, device="cuda"), [[-1] * 4 for _ in range(3)]
+    for more in ([17, 0, 0], [17, 1, 30], [40, 40, 40]):
+        p.extend(table, i32([0, 0, 0]).cuda(), i32(more).cuda()), plain.extend(want, [0, 0, 0], more)
+        assert int(p.missing) == plain.missing
+        same(table, p, want, plain)
 
 
 def test_tables_that_are_parts_of_others():
