@@ -1,11 +1,11 @@
 // Which pages of a cache are in use, and their copies.
 //
-// 256 sequences of up to 130 blocks among 30,000 pages: forked in 2.2 us, given back in 2.2, given room in 9.4 and their pages copied in 5.8; 24 us of
-// a step's 54, whose rest is the host's.  20,000 pages, half of them in use: planned in 13 us, 660 MB moved in 213 (6.2 TB/s).
+// 256 sequences of up to 130 blocks among 30,000 pages: forked in 2.2 us, given back in 2.2, given room in 9.4 and their pages copied in 5.8; 25 us of
+// a step's 55, whose rest is the host's.  20,000 pages, half of them in use: planned in 13 us, 660 MB moved in 213 (6.2 TB/s).
 //
 // refs[p] counts the table entries that hold page p; 0: it is free.  fork and free are a pass over the table with an addition for each entry.
 // extend and compact have to number things in order (the free pages, the blocks that want one), so each is planned by one CTA whose
-// threads meet at its barriers, and what it decides to copy is copied by all SMs in a second kernel.  Nothing depends on the order of
+// threads meet at its barriers (compact: one to every 32,768 pages), and what is to be copied is copied by all SMs in a second kernel.  Nothing depends on the order of
 // atomics: additions commute, and a page's last holder is found by the smallest number.
 #include <climits>
 
@@ -50,20 +50,21 @@ __device__ __forceinline__ int sum_before(int x, int* s, int* all) {
   return before + up - x;
 }
 
-// The counts of a window of pages in a CTA's registers: a warp has 1024 of them in ascending order, a lane four neighbours at a time.  So passes over
+// The counts of a window of pages in a CTA's registers: a warp has up to 1024 of them in ascending order, a lane four neighbours at a time.  So passes over
 // them do not wait for memory again, and the look may be long before.
 struct PageWindow {
   enum { AHEAD = PAGES_WINDOW / PAGES_WARPS / 128 };
-  int begin;  // of the warp's pages
+  int begin, end;  // of the warp's pages
   int4 r[AHEAD];
   __device__ __forceinline__ void look(const Pages& p, int base) {
     const bool wide = (reinterpret_cast<uintptr_t>(p.refs) & 15) == 0;
-    begin = base + int(threadIdx.x >> 5) * (128 * AHEAD);
+    const int all = min(p.pages - base, int(PAGES_WINDOW)), share = ((all + PAGES_WARPS - 1) / PAGES_WARPS + 127) & ~127;
+    begin = base + int(threadIdx.x >> 5) * share, end = min(begin + share, base + all);
 #pragma unroll
     for (int z = 0; z < AHEAD; ++z) {
       const int at = begin + 128 * z + 4 * int(lane_id());
       r[z] = make_int4(-1, -1, -1, -1);  // behind the last page
-      if (at >= p.pages) continue;
+      if (at >= end) continue;
       if (wide && at + 4 <= p.pages) {
         r[z] = __ldcg(reinterpret_cast<const int4*>(p.refs + at));
       } else {
@@ -79,7 +80,7 @@ struct PageWindow {
   __device__ __forceinline__ void each(const Pages& p, F&& f) const {
 #pragma unroll
     for (int z = 0; z < AHEAD; ++z)
-      if (begin + 128 * z < p.pages && !f(begin + 128 * z + 4 * int(lane_id()), r[z])) return;
+      if (begin + 128 * z < end && !f(begin + 128 * z + 4 * int(lane_id()), r[z])) return;
   }
 };
 
@@ -369,9 +370,12 @@ struct Copy {
   int32_t *map, *refs;  // not NULL: the pages move, and take their counts along
 };
 
+// SMALL: pages of less than a quarter of a slice (8000 of 4.5 KB: 23.6 us, 34.5 with a CTA to each; of 13.8 KB: slower), of which an item has several, so that every thread has something to copy.
+template <bool SMALL>
 __global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(const __grid_constant__ Copy c) {
   constexpr int AHEAD = COPY_SLICE / 16 / COPY_THREADS;
-  const long long pairs = c.count ? min(c.n, (long long)(max(__ldcg(c.count), 0))) : c.n, items = pairs * c.slices;
+  const long long pairs = c.count ? min(c.n, (long long)(max(__ldcg(c.count), 0))) : c.n;
+  const long long items = SMALL ? (pairs * c.pieces + COPY_SLICE / 16 - 1) / (COPY_SLICE / 16) : pairs * c.slices;
   if (c.map)
     for (long long i = (long long)(blockIdx.x) * COPY_THREADS + threadIdx.x; i < pairs; i += (long long)(gridDim.x) * COPY_THREADS) {
       const int from = __ldcg(c.src + i), to = __ldcg(c.dst + i);
@@ -380,6 +384,38 @@ __global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(const __grid_c
       c.refs[from] = 0;
     }
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+    if constexpr (SMALL) {
+      const long long begin = item * (COPY_SLICE / 16), first = begin / c.pieces;
+      const unsigned rest = unsigned(begin - first * c.pieces) + threadIdx.x;
+      uint4 x[AHEAD];
+      unsigned char* out[AHEAD];
+#pragma unroll
+      for (int z = 0; z < AHEAD; ++z) {
+        const unsigned l = rest + z * COPY_THREADS, n = l / c.pieces, i = l - n * c.pieces;
+        out[z] = nullptr;
+        if (first + n >= pairs) continue;
+        const unsigned from = unsigned(__ldcg(c.src + first + n)), to = unsigned(__ldcg(c.dst + first + n));
+        if (from >= c.pages || to >= c.pages) continue;
+        int part = 0;
+        while (part + 1 < c.nwide && i >= c.wide[part + 1].start) ++part;
+        const CopyPart& p = c.wide[part];
+        const size_t at = size_t(i - p.start) * 16;
+        out[z] = p.at + size_t(to) * p.bytes + at;
+        x[z] = __ldcs(reinterpret_cast<const uint4*>(p.at + size_t(from) * p.bytes + at));
+        if (i < 32) {  // the first threads of a page have its odd ends too
+          const unsigned threads = min(c.pieces, 32u);
+          for (int e = 0; e < c.nnarrow; ++e) {
+            const CopyPart& y = c.narrow[e];
+            for (unsigned b = i * 4; b < y.bytes; b += threads * 4)
+              *reinterpret_cast<uint32_t*>(y.at + size_t(to) * y.bytes + b) = *reinterpret_cast<const uint32_t*>(y.at + size_t(from) * y.bytes + b);
+          }
+        }
+      }
+#pragma unroll
+      for (int z = 0; z < AHEAD; ++z)
+        if (out[z]) __stcs(reinterpret_cast<uint4*>(out[z]), x[z]);
+      continue;
+    }
     const long long pair = item / c.slices;
     const unsigned slice = unsigned(item - pair * c.slices);
     const unsigned from = unsigned(__ldcg(c.src + pair)), to = unsigned(__ldcg(c.dst + pair));
@@ -434,7 +470,9 @@ int copy_pages(const fv_kv* const* caches, size_t ncaches, size_t pages, cudaStr
     c.src = src, c.dst = dst, c.count = count, c.n = (long long)(n), c.pages = unsigned(pages);
     if (first == 0) c.map = map, c.refs = refs;
     const size_t items = n * (c.slices ? c.slices : 1), most = 148 * 16;
-    pages_copy_kernel<<<unsigned(items < most ? items : most), COPY_THREADS, 0, s>>>(c);
+    const unsigned ctas = unsigned(items < most ? items : most);
+    if (c.pieces && c.pieces < COPY_SLICE / 64) pages_copy_kernel<true><<<ctas, COPY_THREADS, 0, s>>>(c);
+    else pages_copy_kernel<false><<<ctas, COPY_THREADS, 0, s>>>(c);
     FV_CUDA(cudaGetLastError());
   }
   return FV_OK;
@@ -444,7 +482,7 @@ int pages_check(const fv_pages* p, const std::string& w) {
   if (!p) return fail(FV_ERR_ARG, w + ": NULL pages");
   if (p->page_size != 16 && p->page_size != 32 && p->page_size != 64 && p->page_size != 128)
     return fail(FV_ERR_UNSUPPORTED, w + ": page_size is 16, 32, 64 or 128");
-  if (p->pages > size_t(INT_MAX) - 256) return fail(FV_ERR_UNSUPPORTED, w + ": pages does not fit 31 bits");
+  if (p->pages > size_t(INT_MAX) - 2 * PAGES_WINDOW) return fail(FV_ERR_UNSUPPORTED, w + ": pages does not fit 31 bits");
   if (p->device < 0) return fail(FV_ERR_ARG, w + ": device index out of range");
   if (p->pages && !p->refs) return fail(FV_ERR_ARG, w + ": NULL refs");
   if (!kv_aligned(p->refs, 4)) return fail(FV_ERR_ARG, w + ": refs does not begin on 4 bytes");
