@@ -117,9 +117,9 @@ __global__ void __launch_bounds__(PAGES_THREADS) pages_extend_kernel(Pages p, Ta
     const int b = b0 + tid;
     int n = 0, all;
     if (b < t.nseq) {
-      const int len = max(__ldg(x.lens + b), 0), more = max(__ldg(x.more + b), 0);
+      const int len = max(__ldg(x.lens + b), 0), more = __ldg(x.more + b);
       const long long end = ((long long)(len) + more + (1 << p.page_shift) - 1) >> p.page_shift;
-      if (more) n = max(int(min(end, (long long)(t.width))) - (len >> p.page_shift), 0);
+      if (more >= 0) n = max(int(min(end, (long long)(t.width))) - (len >> p.page_shift), 0);
     }
     const int up = sum_before(n, s_sum, &all);
     if (b < t.nseq) before[b + 1] = entries + up + n;

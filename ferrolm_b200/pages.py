@@ -97,8 +97,9 @@ class KvPages:
     def extend(self, table, lens, more):
         """Room for `more[b]` rows behind the `lens[b]` that sequence b has, in the table itself.
 
-        Of the blocks that those rows come to, one without a page gets a free one, and one whose page others hold as well gets a
-        free one with a copy of its rows, in every cache; where all who hold it are in this call, the first of them keeps it.  Free pages
+        Of the blocks from the one on that the first of those rows comes to, one without a page gets a free one, and one whose page others
+        hold as well gets a free one with a copy of its rows, in every cache (a begun block also where `more[b]` is 0; below 0: the
+        sequence is left as it is); where all who hold it are in this call, the first of them keeps it.  Free pages
         are taken in ascending order, for blocks in the table's order; a block that has a page of its own keeps it, so a call may be
         repeated.  Blocks behind the table's width get none.  If there are not enough free pages, nothing is changed and `missing`
         says how many were lacking."""

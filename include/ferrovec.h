@@ -424,8 +424,9 @@ int fv_rotate_dev(const fv_rotary* r, void* stream, const fv_rotary_rows* x, siz
  * fork: row i of `out` becomes row parents[i] of the table, up to the block of its lens' last row (NULL: all of it), and every page in it counts
  * one more; -1 behind them, and everywhere where parents[i] is no row.  out is not the table.
  * free: entries from the first block behind lens (NULL: all) on become -1, and their pages count one less (never below 0).
- * extend: room for more[b] rows behind lens[b]: of the blocks that those rows come to, one without a page gets a free one, and one
- * whose page others hold as well gets a free one with a copy of its rows; where all who hold a page are among these blocks, the first
+ * extend: room for more[b] rows behind lens[b]: of the blocks lens[b] / page_size up to the last that they come to, one without a page gets
+ * a free one, and one whose page others hold as well gets a free one with a copy of its rows (a begun block also where more[b] is 0; where it
+ * is below 0 the sequence is left as it is); where all who hold a page are among these blocks, the first
  * in the table's order keeps it.  Free pages are taken in ascending order, for blocks in the table's order.  Blocks behind the table's width
  * get none.  If there are fewer free pages than blocks to fill nothing is changed (entries that were none may have become -1), and *missing is how many
  * are lacking; otherwise it is 0.

@@ -34,8 +34,8 @@ class PlainPages:
         self.copied, self.missing = [], 0
         at = []
         for b, row in enumerate(table):
-            n, m = max(lens[b], 0), max(more[b], 0)
-            at += [(b, j) for j in range(n // self.page, min(-(-(n + m) // self.page), len(row))) if m]
+            n, m = max(lens[b], 0), more[b]
+            at += [(b, j) for j in range(n // self.page, min(-(-(n + m) // self.page), len(row))) if m >= 0]
         holders = {}
         for b, j in at:
             q = table[b][j]

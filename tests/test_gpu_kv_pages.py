@@ -147,6 +147,23 @@ def test_sequences_that_share_pages(seed, layers):
     assert int(p.refs.sum()) == 0
 
 
+@pytest.mark.parametrize("more", [[0, 0, 0], [0, -1, 0], [-1, -1, 5], [0, 3, -7]])
+def test_begun_blocks_where_no_rows_come(more):
+    """A begun block that is shared becomes the sequence's own with `more` 0 too; with less the sequence is left alone."""
+    caches, p, plain = make(20, 16, ALL[2:4])
+    table = torch.full((1, 3), -1, dtype=torch.int32, device="cuda")
+    p.extend(table, i32([0]).cuda(), i32([32]).cuda())
+    want = [[-1] * 3]
+    plain.extend(want, [0], [32])
+    for lens in ([20, 20, 17], [32, 20, 16], [16, 31, 0]):
+        kids, theirs = p.fork(table, None, i32([0, 0, 0]).cuda()), plain.fork(want, None, [0, 0, 0])
+        rows = bits(caches)
+        p.extend(kids, i32(lens).cuda(), i32(more).cuda()), plain.extend(theirs, lens, more)
+        same(kids, p, theirs, plain)
+        same_rows(caches, moved(rows, plain.copied))
+        p.free(kids), plain.free(theirs)
+
+
 def test_too_few_pages_change_nothing():
     caches, p, plain = make(6, 16)
     table = i32([[0, -1, -1], [0, -1, -1], [-9, -1, -1]]).cuda()

@@ -132,7 +132,7 @@ def test_plain_pages():
     kids = p.fork(table, [20], [0, 0, 0])
     assert p.refs[:2] == [4, 4]
     p.free(table)
-    p.extend(kids, [20] * 3, [1, 1, 0])  # the third holds page 1 as well and is not among those that get rows
+    p.extend(kids, [20] * 3, [1, 1, -1])  # the third holds page 1 as well and is left as it is
     assert kids == [[0, 2, -1], [0, 3, -1], [0, 1, -1]] and p.refs[:4] == [3, 1, 1, 1] and p.copied == [(1, 2), (1, 3)]
     p.extend(kids, [21, 21, 20], [1, 1, 12])
     assert kids == [[0, 2, -1], [0, 3, -1], [0, 1, -1]]
