@@ -56,7 +56,7 @@ class Rotary:
         self.device = self._turns.device
         at = self._turns.data_ptr()
         self._c = {t: C.pointer(fv_rotary(self.device.index, i, dim, part, LAYOUTS.index(layout), amplitude, at)) for i, t in enumerate((torch.bfloat16, torch.float16))}
-        self._i32, self._contiguous, self._index = torch.int32, torch.contiguous_format, self.device.index
+        self._i32, self._contiguous, self._empty_like, self._index = torch.int32, torch.contiguous_format, torch.empty_like, self.device.index
         self._grad, self._get_stream, self._rotate = torch.is_grad_enabled, torch._C._cuda_getCurrentRawStream, lib().fv_rotate_dev
         self._two = fv_rotary_rows * 2
 
@@ -71,7 +71,7 @@ class Rotary:
         r, h, d = x.stride()
         at = x.data_ptr()
         if out is None:
-            out = x.new_empty(shape)
+            out = self._empty_like(x, memory_format=self._contiguous)
             to, tr, th = out.data_ptr(), shape[1] * self.dim, self.dim
         else:
             tr, th, td = out.stride() if out.dim() == 3 else (0, 0, 0)

@@ -217,6 +217,48 @@ def test_scales_at_both_ends(new):
         check(c, p, q, table, lens, cu, None)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_few_rows_and_groups_that_are_no_numbers(dtype):
+    """Keys shared out to many CTAs: a key's reaches every query that sees it, whichever CTA has it, a value's its group only."""
+    heads, group, dim, page, lens, news = 2, 4, 128, 32, [3000, 2200], [6, 5]
+    c, p = pair(190, heads, dim, page, dtype)
+    table, cu = batch(2, 94, 190, 2), i32([0, 6, 11])
+    for name, b, pos, h, g in (("v", 0, 2996, 0, 2), ("v", 0, 17, 1, 1), ("k", 1, 2197, 0, 0), ("v", 1, 1500, 1, 3)):
+        at = int(table[b, pos // page])
+        getattr(c, name + "_scale")[at, h, pos % page, g] = 255
+        getattr(p, name)[at, h, pos % page, 32 * g : 32 * g + 32] = torch.nan
+    q = (queries(11, heads, group, dim, torch.float32, 3) * 0.1).to(dtype)  # weights of all rows
+    got = check(c, p, q, table, lens, cu, None)[0]
+    assert got[:2, :group, 64:96].isfinite().all() and got[3:6, :group, 64:96].isnan().all() and got[:6, group:, 32:64].isnan().all()
+    assert got[6:8, :group].isfinite().all() and got[8:, :group].isnan().all()
+
+
+def test_few_rows_captured_and_on_two_streams():
+    """Each call has its parts' place to itself."""
+    heads, group, dim, page = 2, 4, 128, 64
+    c, _ = pair(200, heads, dim, page, BF)
+    table, cu = batch(2, 90, 200, 2).cuda(), i32([0, 6, 12]).cuda()
+    q = [queries(12, heads, group, dim, BF, i).cuda() for i in range(2)]
+    lens, outs = i32([5000, 3000]).cuda(), [torch.zeros_like(x) for x in q]
+    for x, out in zip(q, outs):
+        c.attend(x, table, lens, cu=cu, out=out)
+    graphs = [torch.cuda.CUDAGraph() for _ in q]
+    for g, x, out in zip(graphs, q, outs):
+        with torch.cuda.graph(g):
+            c.attend(x, table, lens, cu=cu, out=out)
+    streams = [torch.cuda.Stream() for _ in q]
+    for n in (4000, 5700, 300):
+        lens.copy_(i32([n, n - 200]))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                for _ in range(3):
+                    g.replay()
+        torch.cuda.synchronize()
+        for x, out in zip(q, outs):
+            assert torch.equal(out, c.attend(x, table, lens, cu=cu))
+
+
 def test_attention_is_that_of_the_rows_read_back():
     """4-bit rows are exact in 16 bits: a 16-bit cache of what vectors gives has the same values, and the results are as near as two ways
     of rounding weights, 2^-9 and 2^-11 of each, and the result are."""
