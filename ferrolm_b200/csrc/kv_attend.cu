@@ -18,7 +18,7 @@
 // 32 blocks take 10.2 us in a graph, most of it dependent loads: the list, the table, the rows, and the shares that are joined.
 //
 // In 4 bits a row is half as long and its codes are taken apart by masks: 64 rows of 64 heads over 40 blocks (181 MB) take 57 us, 3.2 TB/s,
-// 0.49 of the copy rate; 12 whole sequences of heads of 96 in fp16 (210 MB) 77 us.  Copying alone would take 36 and 40: some 390 instructions for
+// 0.49 of the copy rate; 12 whole sequences of heads of 96 in fp16 (210 MB) 76 us.  Copying alone would take 36 and 40: some 390 instructions for
 // 16 rows and a head bound it (three fifths of the issue slots; 160 of them on the ALU, at half the others' rate: 80 take the codes apart).
 //
 // In 8 bits the codes are exact in fp16; a key's scale multiplies its score, a value's its weight, relative to the largest
@@ -62,6 +62,8 @@ bool kv_prompt_fits(const fv_kv_batch* b, size_t group, bool lists, size_t k);
 // CTAs saturate the bytes too: there only what leaves a third of the SMs without one, half of them where rows are 64 long, and a second
 // wave full to at most 0.6 in dim 128, where an SM holds two CTAs (of three or four the others cover for those that are gone).
 // Over 24 shapes and 4000 such points these lines are 0.5% from the better side on average, within 5% for 96% of them, 21% at worst.
+// 4 bits go by the lines of 8, with four CTAs to an SM: over 12 shapes and 700 points, 16 to 1024 tasks of 32 to 768 pieces, 0.5 to 1.4% from the
+// better side on average, 22% at worst (dim 128, us by tasks / in parts: 64 tasks of 128 pieces 29/20, of 768 129/41; 512 of 128 53/51).
 enum { KV_PARTS_TASKS = 1024, KV_PARTS_WARPS = 160 * 16, KV_SMS = 148 };
 constexpr int kv_ctas_an_sm(int kind, int dim) { return kind == FV_KV_INT4X32 ? 4 : dim == 64 ? 4 : dim == 96 && kind == FV_KV_SAME ? 3 : 2; }
 static bool in_parts(int kind, int dim, int group, bool alike, size_t tasks, size_t pieces) {
@@ -324,7 +326,12 @@ struct Share {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         shared_words<NG>(k[i], keys + (16 * h + 8 * i) * L::ROW);
-        L::halves_of(shared_bytes<NG>(key_scales + (16 * h + 8 * i) * NG), sc[i]);
+        if constexpr (NG == 3) {  // three bytes from an even or an odd address, by two halves
+          const uint32_t odd_row = L::token(g) & 1, from = key_scales + (16 * h + 8 * i) * NG - odd_row;
+          L::halves_of(__byte_perm(shared_bytes<2>(from), shared_bytes<2>(from + 2), odd_row ? 0x6541 : 0x6410), sc[i]);
+        } else {
+          L::halves_of(shared_bytes<NG>(key_scales + (16 * h + 8 * i) * NG), sc[i]);
+        }
       }
 #pragma unroll
       for (int y = 0; y < NG; ++y) {
@@ -351,7 +358,16 @@ struct Share {
 #pragma unroll
     for (int h = 0; h < P; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vs[h][i] = shared_bytes<NG>(value_scales + L::token(2 * t + (i & 1)) * NG + (16 * h + (i & 2) * 4) * NG);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (NG == 3) {  // those of two rows, six bytes, by three halves
+          if (i & 1) continue;
+          const uint32_t from = value_scales + 6 * t + (16 * h + 4 * i) * NG, last = shared_bytes<2>(from + 4);
+          const uint32_t four = __byte_perm(shared_bytes<2>(from), shared_bytes<2>(from + 2), 0x5410);
+          vs[h][i] = __byte_perm(four, last, t & 1 ? 0x6543 : 0x6210), vs[h][i + 1] = __byte_perm(four, last, t & 1 ? 0x6210 : 0x6543);
+        } else {
+          vs[h][i] = shared_bytes<NG>(value_scales + L::token(2 * t + (i & 1)) * NG + (16 * h + (i & 2) * 4) * NG);
+        }
+      }
     int least = visible[0];
     if constexpr (P > 1) least = min(least, visible[P - 1]);
     if (least < 16) {  // of rows that are not seen scores and scales are anything
