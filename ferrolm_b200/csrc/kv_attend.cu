@@ -1276,9 +1276,9 @@ int token_of(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAtte
 
 }  // namespace
 
-// Several rows of a sequence on average, and room for the union of their lists.
-static bool is_prompt(const fv_kv_batch* b, size_t group, bool lists, size_t k) {
-  return b->rows > 4 * b->nseq && kv_prompt_fits(b, group, lists, k);
+// Several rows of a sequence on average, room for the union of their lists, and a cache that has pages.
+static bool is_prompt(const fv_kv* kv, const fv_kv_batch* b, size_t group, bool lists, size_t k) {
+  return kv->pages && b->rows > 4 * b->nseq && kv_prompt_fits(b, group, lists, k);
 }
 
 int kv_token_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const KvAttend& a, void* work, size_t work_bytes) {
@@ -1289,7 +1289,7 @@ int kv_token_attend(const fv_kv* kv, cudaStream_t s, const fv_kv_batch* b, const
 
 extern "C" size_t fv_kv_attend_work(const fv_kv* kv, const fv_kv_batch* batch, size_t group) {
   if (!kv || !batch || group == 0 || group > 128) return 0;
-  if (fv::is_prompt(batch, group, false, 0)) return fv::kv_prompt_work(kv, batch, group);  // with lists too: a shorter union fits where the whole table does
+  if (fv::is_prompt(kv, batch, group, false, 0)) return fv::kv_prompt_work(kv, batch, group);  // with lists too: a shorter union fits where the whole table does
   if (batch->rows > fv::KV_PARTS_TASKS) return 0;
   const size_t cols = group <= 8 ? 8 : 16, tasks = batch->rows * kv->heads * ((group + cols - 1) / cols), pieces = batch->table_width * (kv->page_size / 16);
   const bool parts = fv::in_parts(kv->kind, int(kv->dim), int(group), false, tasks, pieces) || fv::in_parts(kv->kind, int(kv->dim), int(group), true, tasks, pieces);
@@ -1312,6 +1312,6 @@ extern "C" int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch
                        scale * 1.44269504088896341f, static_cast<const unsigned char*>(kv->k), static_cast<const unsigned char*>(kv->v),
                        kv->k_scale, kv->v_scale, static_cast<unsigned char*>(out), lse};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (kv->pages && fv::is_prompt(batch, group, blocks != nullptr, k)) return fv::kv_prompt_attend(kv, s, batch, a, work, work_bytes);
+  if (fv::is_prompt(kv, batch, group, blocks != nullptr, k)) return fv::kv_prompt_attend(kv, s, batch, a, work, work_bytes);
   return fv::kv_token_attend(kv, s, batch, a, work, work_bytes);
 }
