@@ -21,6 +21,25 @@ from ._lib import check, fv_pages, fv_table, lib
 from .kv import KvCache, _refuse
 
 
+def _shared(a: fv_table, b: fv_table) -> int:
+    """How many of a's entries are entries of b too.  Rows of a table do not overlap one another."""
+    size = lambda t: 4 * ((t.nseq - 1) * t.stride + t.width) if t.nseq and t.width else 0  # noqa: E731
+    begin_a, begin_b = a.table or 0, b.table or 0
+    if not size(a) or not size(b) or begin_a + size(a) <= begin_b or begin_b + size(b) <= begin_a:
+        return 0
+    if (begin_a, a.stride, a.width, a.nseq) == (begin_b, b.stride, b.width, b.nseq):
+        return a.nseq * a.width
+    found = 0
+    for i in range(a.nseq):
+        row = (begin_a - begin_b) // 4 + i * a.stride  # where row i of a begins in b
+        step = b.stride if b.nseq > 1 else max(b.stride, row + a.width + b.width, 1)
+        j = max((row - b.width) // step, 0)
+        while j < b.nseq and j * step < row + a.width:
+            found += max(min(row + a.width, j * step + b.width) - max(row, j * step), 0)
+            j += 1
+    return found
+
+
 class KvPages:
     """The pages of one cache or of several that share a table (a model's layers).
 
@@ -116,11 +135,22 @@ class KvPages:
         if status:
             check(status)
 
+    @staticmethod
+    def _once(tables):
+        """Those of the tables that are no part of another: an entry is renumbered once."""
+        inside = lambda a, b: _shared(a, b) == a.nseq * a.width  # noqa: E731
+        keep = [a for i, a in enumerate(tables) if not any(inside(a, b) and not (i < j and inside(b, a)) for j, b in enumerate(tables) if j != i)]
+        if any(_shared(a, b) for i, a in enumerate(keep) for b in keep[:i]):
+            _refuse("tables share some of their entries: give what holds both, or parts that share none")
+        return keep
+
     def compact(self, *tables):
         """Moves the n pages in use to 0 .. n - 1: those from n on go to the free ones below it, ascending to ascending, the others stay.
         The rows move in every cache, and the entries of `tables` become the pages' new numbers (-1 for a page that is free).  All
-        tables that hold pages are to be among them.  `used` becomes n."""
+        tables that hold pages are to be among them; one that is part of another counts once, and others share no entries.  `used` becomes n."""
         each = [self._table(t) for t in tables]
+        if len(each) > 1:
+            each = self._once(each)
         stream = self._get_stream(self._index)
         more = (self.pages + 3) // 4 * 4
         work = self._refs.new_empty((self._compact_work >> 2) + more)

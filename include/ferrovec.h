@@ -432,7 +432,8 @@ int fv_rotate_dev(const fv_rotary* r, void* stream, const fv_rotary_rows* x, siz
  * get none.  If there are fewer free pages than blocks to fill nothing is changed (entries that were none may have become -1), and *missing is how many
  * are lacking; otherwise it is 0.
  * compact: of the n pages in use those from n on move to the free ones below n, ascending to ascending; *used = n; map[p] is where
- * page p lies now (-1: free).  remap: entries of a table become map of what they were. */
+ * page p lies now (-1: free).  remap: entries of a table become map of what they were; an entry that lies in two tables is to be remapped
+ * once. */
 typedef struct fv_pages {
   int device;
   uint32_t page_size;

@@ -1,0 +1,55 @@
+"""KvPages where tables share memory with one another, and with more caches than one launch copies."""
+import pytest
+import torch
+
+from tests.test_gpu_kv_pages import ALL, bits, make, moved, same, same_rows
+from tests.test_gpu_kv_rows import i32
+
+pytestmark = pytest.mark.gpu
+
+
+def half_used(pages, page, layers, table):
+    """Every second of the pages that `table` names is in use, once for each of its rows that has it."""
+    caches, p, plain = make(pages, page, layers)
+    d = table.cuda()
+    for q in range(pages):
+        plain.refs[q] = int((table == q).sum()) if q % 2 else 0
+    p.refs.copy_(i32(plain.refs))
+    return caches, p, plain, d
+
+
+TABLE = torch.tensor([[9, 1, -1, 19], [7, 5, 13, 0], [15, 11, 3, 40], [17, 1, 4, -7]], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("which", ["twice", "a view first", "a view last", "columns", "rows between", "views that meet nowhere", "three times"])
+def test_an_entry_is_renumbered_once(which):
+    """A table given twice, or with views of itself, is as if it were given once."""
+    caches, p, plain, t = half_used(20, 16, ALL, TABLE)
+    want, rows = TABLE.tolist(), bits(caches)
+    p.compact(*{"twice": (t, t), "a view first": (t[1:3], t), "a view last": (t, t[:2]), "columns": (t, t[:, 1:3]), "rows between": (t[::2], t, t[1::2]),
+                "views that meet nowhere": (t[:, :1], t[:2, 1:], t[2:, 1:]), "three times": (t, t.view(4, 4), t)}[which])
+    plain.compact(want)
+    assert plain.copied
+    same(t, p, want, plain)
+    same_rows(caches, moved(rows, plain.copied))
+
+
+def test_pages_that_nobody_holds_are_none_in_the_end():
+    """An entry that names a free page becomes -1, also where another page moves to that place."""
+    _, p, _, t = half_used(6, 16, ALL[:1], i32([[1, 3, 5, 0, 2, 4]]))
+    p.compact(t, t)
+    assert t.tolist() == [[1, 0, 2, -1, -1, -1]]
+
+
+@pytest.mark.parametrize("views", [lambda t: (t[:3], t[2:]), lambda t: (t[:, :3], t[:, 2:]), lambda t: (t[:3, :3], t[1:, 1:]), lambda t: (t[::2], t[1:3])])
+def test_tables_that_share_some_entries_are_refused(views):
+    """Before anything moves."""
+    import ferrolm_b200 as fv
+
+    caches, p, plain, t = half_used(20, 16, ALL[:1], TABLE)
+    rows = bits(caches)
+    with pytest.raises(fv.FerrovecError, match="share"):
+        p.compact(*views(t))
+    same(t, p, TABLE.tolist(), plain)
+    same_rows(caches, rows)
+    assert int(p.used) == 0
