@@ -68,6 +68,7 @@ class KvPages:
         self._ref, self._index, self._get_stream = C.byref(self._c), self.device.index, torch._C._cuda_getCurrentRawStream
         self._handles = (C.c_void_p * len(self.caches))(*(C.addressof(c._c) for c in self.caches))
         self._lib = lib()
+        self._none = C.byref(fv_pages(self.device.index, self.page_size, 0, None))  # a call on no pages checks its table and does nothing
         self._compact_work, self._extend_work = self._lib.fv_pages_compact_work(self._ref), {}
 
     refs = property(lambda self: self._refs)
@@ -152,6 +153,10 @@ class KvPages:
         if len(each) > 1:
             each = self._once(each)
         stream = self._get_stream(self._index)
+        for t in each:  # before anything moves
+            status = self._lib.fv_pages_remap_dev(self._none, stream, None, t)
+            if status:
+                check(status)
         more = (self.pages + 3) // 4 * 4
         work = self._refs.new_empty((self._compact_work >> 2) + more)
         map_at = work.data_ptr() + self._compact_work

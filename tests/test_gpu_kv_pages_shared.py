@@ -53,3 +53,15 @@ def test_tables_that_share_some_entries_are_refused(views):
     same(t, p, TABLE.tolist(), plain)
     same_rows(caches, rows)
     assert int(p.used) == 0
+
+
+def test_a_table_that_cannot_be_renumbered_is_refused_before_anything_moves():
+    import ferrolm_b200 as fv
+
+    caches, p, plain, t = half_used(20, 16, ALL[:1], TABLE)
+    rows, wide = bits(caches), torch.full((1, (1 << 24) + 1), 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(fv.FerrovecError):
+        p.compact(t, wide)
+    same(t, p, TABLE.tolist(), plain)
+    same_rows(caches, rows)
+    assert int(p.used) == 0 and int(wide.min()) == 1
