@@ -497,6 +497,21 @@ int table_check(const fv_pages* p, const fv_table* t, const std::string& w) {
   if (!kv_aligned(t->table, 4)) return fail(FV_ERR_ARG, w + ": table does not begin on 4 bytes");
   return FV_OK;
 }
+// Whether an entry lies in both.  Rows of a table do not overlap one another.
+bool tables_meet(const fv_table* a, const fv_table* b) {
+  if (!a->nseq || !a->width || !b->nseq || !b->width) return false;
+  using wide = __int128;  // strides of tables that cannot be are not looked at closer
+  const wide step_a = a->nseq > 1 ? a->stride : 0, step_b = b->nseq > 1 ? b->stride : 0, width_a = a->width, width_b = b->width;
+  const wide begin = (wide(reinterpret_cast<uintptr_t>(a->table)) - wide(reinterpret_cast<uintptr_t>(b->table))) / 4;  // of a, in b
+  if (begin >= (b->nseq - 1) * step_b + width_b || begin + (a->nseq - 1) * step_a + width_a <= 0) return false;
+  for (size_t i = 0; i < a->nseq; ++i) {
+    const wide row = begin + i * step_a;
+    wide j = step_b && row > width_b ? (row - width_b) / step_b : 0;
+    for (; j < wide(b->nseq) && j * step_b < row + width_a; ++j)
+      if (row < j * step_b + width_b) return true;
+  }
+  return false;
+}
 int caches_check(const fv_pages* p, const fv_kv* const* caches, size_t n, const char* who) {
   const std::string w(who);
   if (n && !caches) return fail(FV_ERR_ARG, w + ": NULL caches");
@@ -540,7 +555,7 @@ extern "C" int fv_pages_fork_dev(const fv_pages* p, void* stream, const fv_table
   FV_TRY(fv::table_check(p, out, w));
   if (out->nseq == 0 || out->width == 0) return FV_OK;
   if (!parents || !fv::kv_aligned(parents, 4) || !fv::kv_aligned(lens, 4)) return fv::fail(FV_ERR_ARG, std::string(w) + ": parents is not there, or it or lens does not begin on 4 bytes");
-  if (from->table == out->table) return fv::fail(FV_ERR_ARG, std::string(w) + ": out is the table");
+  if (from->table == out->table || fv::tables_meet(from, out)) return fv::fail(FV_ERR_ARG, std::string(w) + ": out shares entries with the table");
   fv::DeviceGuard g(p->device);
   if (!g.ok) return fv::fail(FV_ERR_CUDA, "cudaSetDevice failed (there is no CPU path)");
   fv::pages_fork_kernel<<<fv::table_grid(out), 256, 0, static_cast<cudaStream_t>(stream)>>>(fv::pages_of(p), fv::table_of(from), lens, parents, fv::table_of(out));

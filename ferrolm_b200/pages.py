@@ -90,7 +90,7 @@ class KvPages:
     def fork(self, table, lens, parents, out=None):
         """A table whose row i is row `parents[i]` of `table`, up to the block of that row's last row (`lens`: those of `table`; None:
         the whole row), -1 behind it and everywhere where `parents[i]` is no row.  Pages are shared, not copied: every one counts
-        once more.  `out`: the table to write to, not `table` itself; what it held is not given back."""
+        once more.  `out`: the table to write to, which shares no entries with `table`; what it held is not given back."""
         t = self._table(table)
         at = None if lens is None else self._numbers(lens, t.nseq, "lens")
         if parents.dim() != 1:

@@ -423,7 +423,7 @@ int fv_rotate_dev(const fv_rotary* r, void* stream, const fv_rotary_rows* x, siz
  * a model), all of `pages` pages of `page_size` rows.  A table entry outside 0 .. pages-1 is none.
  *
  * fork: row i of `out` becomes row parents[i] of the table, up to the block of its lens' last row (NULL: all of it), and every page in it counts
- * one more; -1 behind them, and everywhere where parents[i] is no row.  out is not the table.
+ * one more; -1 behind them, and everywhere where parents[i] is no row.  out shares no entries with the table.
  * free: entries from the first block behind lens (NULL: all) on become -1, and their pages count one less (never below 0).
  * extend: room for more[b] rows behind lens[b]: of the blocks lens[b] / page_size up to the last that they come to, one without a page gets
  * a free one, and one whose page others hold as well gets a free one with a copy of its rows (a begun block also where more[b] is 0; where it

@@ -65,3 +65,20 @@ def test_a_table_that_cannot_be_renumbered_is_refused_before_anything_moves():
     same(t, p, TABLE.tolist(), plain)
     same_rows(caches, rows)
     assert int(p.used) == 0 and int(wide.min()) == 1
+
+
+def test_forks_into_the_table_itself_are_refused():
+    """Threads would read what others write.  Other parts of the same tensor are fine."""
+    import ferrolm_b200 as fv
+
+    _, p, plain, t = half_used(20, 16, ALL[:1], TABLE.repeat(2, 1))
+    n, parents = i32([64] * 4).cuda(), i32([3, 0, 1]).cuda()
+    for out in (t[1:4], t[:3], t[3:6], t[2:5, 1:]):
+        with pytest.raises(fv.FerrovecError, match="shares"):
+            p.fork(t[:4], n, parents, out=out)
+    assert torch.equal(t.cpu(), TABLE.repeat(2, 1)) and p.refs.tolist() == plain.refs
+    p.fork(t[:4], n, parents, out=t[4:7])
+    assert t[4:7].tolist() == plain.fork(TABLE.tolist(), [64] * 4, [3, 0, 1]) and torch.equal(t[:4].cpu(), TABLE)
+    assert p.refs.tolist() == plain.refs
+    p.fork(t[:3, :2], n[:3], parents[1:], out=t[:2, 2:])
+    assert t[:2, 2:].tolist() == plain.fork([r[:2] for r in TABLE.tolist()], [64] * 4, [0, 1])

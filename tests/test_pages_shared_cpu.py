@@ -1,9 +1,12 @@
 """Which entries two tables share, from their addresses alone, against sets."""
+import ctypes as C
 import random
 
 import pytest
+import torch
 
-from tests.test_kv_cpu import fv  # noqa: F401
+from tests.test_kv_cpu import ARG, AT, CUDA, fv  # noqa: F401
+from tests.test_rotary_pages_cpu import pages
 
 
 def entries(t):
@@ -42,3 +45,26 @@ def test_tables_that_are_part_of_others_count_once(fv):  # noqa: F811
         with pytest.raises(fv.FerrovecError, match="share"):
             once(tables)
     assert once([across, t, fv_table(4096, 8, 8, 8)])[0].nseq == 8
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses would be followed")
+@pytest.mark.parametrize("seed", range(3))
+def test_forks_into_the_table_itself(fv, seed):  # noqa: F811
+    """Refused where an entry lies in both; parts of one tensor that share none are not."""
+    from ferrolm_b200._lib import fv_table
+
+    L, r, met = fv.kv.lib(), random.Random(seed), 0
+    for _ in range(2000):
+        a, b = (fv_table(AT + 4 * r.randint(0, 60), (s := r.randint(1, 12)), r.randint(1, s), r.randint(1, 6)) for _ in range(2))
+        if r.random() < 0.5:
+            b.stride, b.width = a.stride, min(b.width, a.stride)
+        if r.random() < 0.2:
+            a.nseq, a.stride = 1, r.choice([0, 1, 3, 1 << 40])
+        both = bool(entries(a) & entries(b))
+        for x, y in ((a, b), (b, a)):
+            status = L.fv_pages_fork_dev(C.byref(pages()), None, C.byref(x), AT, AT, C.byref(y))
+            assert status == (ARG if both or a.table == b.table else CUDA), [(t.table, t.stride, t.width, t.nseq) for t in (a, b)]
+        met += both
+    assert met > 300
+    far = fv_table(AT + 8, 1 << 40, 2, 1 << 20)  # of no memory that there is
+    assert L.fv_pages_fork_dev(C.byref(pages()), None, C.byref(far), AT, AT, C.byref(fv_table(AT, 2, 2, 3))) == ARG
