@@ -82,3 +82,27 @@ def test_forks_into_the_table_itself_are_refused():
     assert p.refs.tolist() == plain.refs
     p.fork(t[:3, :2], n[:3], parents[1:], out=t[:2, 2:])
     assert t[:2, 2:].tolist() == plain.fork([r[:2] for r in TABLE.tolist()], [64] * 4, [0, 1])
+
+
+@pytest.mark.parametrize("layers", [8, 9, 16, 33])
+def test_many_caches(layers):
+    """More caches than one launch copies: every one has what the first has, and counts move once."""
+    caches, p, plain = make(60, 16, tuple(ALL[i % len(ALL)] for i in range(layers)), layers)
+    table, want = torch.full((4, 6), -1, dtype=torch.int32, device="cuda"), [[-1] * 6 for _ in range(4)]
+    lens, zero = [40, 17, 90, 3], [0] * 4
+    p.extend(table, i32(zero).cuda(), i32(lens).cuda()), plain.extend(want, zero, lens)
+    for step in range(3):
+        parents = [[0, 0, 1, 2], [3, 3, 3, 0], [2, 1, 1, 3]][step]
+        kids, theirs = p.fork(table, i32(lens).cuda(), i32(parents).cuda()), plain.fork(want, lens, parents)
+        lens, rows = [lens[b] for b in parents], bits(caches)
+        p.extend(kids, i32(lens).cuda(), i32([1, 20, 0, 5]).cuda()), plain.extend(theirs, lens, [1, 20, 0, 5])
+        assert plain.copied and int(p.missing) == plain.missing == 0
+        same(kids, p, theirs, plain)
+        same_rows(caches, moved(rows, plain.copied))
+        p.free(table), plain.free(want)
+        rows = bits(caches)
+        p.compact(kids), plain.compact(theirs)
+        same(kids, p, theirs, plain)
+        same_rows(caches, moved(rows, plain.copied))
+        table, want, lens = kids, theirs, [a + b for a, b in zip(lens, [1, 20, 0, 5])]
+        lens = [min(n, 96) for n in lens]
