@@ -76,7 +76,8 @@ class Rotary:
         else:
             tr, th, td = out.stride() if out.dim() == 3 else (0, 0, 0)
             to = out.data_ptr()
-            apart = (tr >= self.dim or shape[0] < 2) and (th >= self.dim or shape[1] < 2)
+            rows_span, head_span = (shape[0] - 1) * tr + self.dim, (shape[1] - 1) * th + self.dim  # of a head's rows, of a row's heads
+            apart = (tr >= head_span or shape[0] < 2) and (th >= self.dim or shape[1] < 2) or (th >= rows_span or shape[1] < 2) and (tr >= self.dim or shape[0] < 2)
             if out.shape != shape or out.dtype is not dtype or out.device != self.device or td != 1 or (tr | th) & 7 or to & 15 or not apart:
                 _refuse(f"what is written to is {dtype} of {tuple(shape)} on {self.device}, its rows on 16 bytes and apart from one another")
         if d != 1 or (r | h) & 7 or at & 15:
@@ -92,7 +93,7 @@ class Rotary:
         sequence brings one row.  Or row i stands at `positions[i]`.  Rows of no sequence and positions below 0 are skipped: what the
         result holds there is what was there before.  `back` turns the other way: what undoes a turn (times amplitude ** 2), and what a
         gradient of the result becomes one of the rows by.  `out`: the tensors to write to, a pair with `k`; each may be the rows
-        themselves, and otherwise does not overlap them.  Sums are of 32 bits, and results are rounded once."""
+        themselves, and otherwise overlaps neither those nor the other.  Sums are of 32 bits, and results are rounded once."""
         rows, dtype = q.shape[0] if q.dim() else 0, q.dtype
         c = self._c.get(dtype)
         if c is None:
@@ -121,6 +122,8 @@ class Rotary:
             status = self._rotate(c, self._get_stream(self._index), C.byref(x), 1, rows, lens_at, cu_at, n, pos_at, back)
         else:
             k, out_k, y = self._rows(k, to_k, dtype, rows, "k")
+            if out is not None and x.out == y.out and rows:
+                _refuse("the results of q and k are written to places that are apart from one another")
             status = self._rotate(c, self._get_stream(self._index), self._two(x, y), 2, rows, lens_at, cu_at, n, pos_at, back)
         if status:
             check(status)

@@ -397,7 +397,8 @@ size_t fv_kv_attend_work(const fv_kv* kv, const fv_kv_batch* batch, size_t group
  *
  * Row i of a call has the position that fv_kv_batch gives it (lens, cu), or positions[i].  Rows of no sequence and positions below 0
  * are skipped: nothing is read or written there.  One call turns up to four tensors of the same rows ([rows][heads][dim], strides in
- * elements, multiples of 8).  `out` may be `in` with the same strides; otherwise they do not overlap. */
+ * elements, multiples of 8).  `out` may be `in` with the same strides; otherwise they do not overlap.  Rows
+ * and heads of all the `out` lie apart from one another. */
 enum { FV_ROTARY_HALF = 0, FV_ROTARY_PAIRS = 1 }; /* layout */
 typedef struct fv_rotary {
   int device;
