@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotate_kernel(Rotary a, KvBatc
         } else {
           lo = r;
         }
-        pos = m.len(lo) - max(m.cu_at(lo + 1), r + 1) + r;
+        if (r >= m.cu_at(lo)) pos = m.len(lo) - max(m.cu_at(lo + 1), r + 1) + r;  // in front of the first there may be rows of no sequence
       }
     }
     s_pos[threadIdx.x] = pos;
