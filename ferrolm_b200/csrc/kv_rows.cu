@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(256) kv_vectors_kernel(KvPool pool, KvBatch m,
       } else {
         lo = r;
       }
-      const int pos = m.len(lo) - max(m.cu_at(lo + 1), r + 1) + r;
+      const int pos = r >= m.cu_at(lo) ? m.len(lo) - max(m.cu_at(lo + 1), r + 1) + r : -1;  // in front of the first there may be rows of no sequence
       if (pos >= 0) {
         const int page = m.page(lo, pos >> pool.page_shift);
         if (page >= 0) at = ((long long)(page) * pool.heads << pool.page_shift) + (pos & ((1 << pool.page_shift) - 1));

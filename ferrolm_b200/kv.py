@@ -7,8 +7,8 @@ all of them, is attention.
 
 A call is about a batch: `table[b, i]` is the page of block i of sequence b, `lens[b]` the sequence's rows, those of the call
 among them, and the call is about its last ones.  Row i of the n that sequence b brings stands at position
-`lens[b] - n + i` and is row `cu[b] + i` of the call's tensors; without `cu` every sequence brings one row.  Rows from
-`cu[-1]` on belong to no sequence (a padded batch): they are not read, and what a result holds there is what was there
+`lens[b] - n + i` and is row `cu[b] + i` of the call's tensors; without `cu` every sequence brings one row.  Rows before
+`cu[0]` and from `cu[-1]` on belong to no sequence (a padded batch): they are not read, and what a result holds there is what was there
 before.  Positions below 0 or in a block that the table has no column for, and blocks whose table entry is not a page of the
 cache (-1, say), are skipped: nothing is written or read there and nothing attends to them.
 

@@ -316,7 +316,7 @@ int fv_merge_topk_static_dev(int device, void* stream, const fv_neighbor* d_part
  *
  * A batch: sequence b has its pages in table[b][0..table_width) and lens[b] rows, those of this call among them.  The call
  * is about its last n_b rows: row i of them stands at position lens[b] - n_b + i, and they are rows cu[b] .. cu[b+1] of the
- * call's tensors (cu: nseq + 1 ascending numbers from 0; NULL: one row each, rows = nseq).  Rows from cu[nseq] on are not
+ * call's tensors (cu: nseq + 1 ascending numbers; NULL: one row each, rows = nseq).  Rows before cu[0] and from cu[nseq] on are not
  * touched.  A length below 0 counts as 0; table_width * page_size is less than 2^31.  Positions below 0 or in a block from table_width on, and blocks whose table entry is not a page of the cache
  * (-1, say), are skipped: nothing is read or written there, and nothing attends to them.  A page that add writes to is one
  * block of one sequence of the call. */
