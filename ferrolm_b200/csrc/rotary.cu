@@ -3,7 +3,8 @@
 //   y_i = a (x_i cos t - x_j sin t),  y_j = a (x_j cos t + x_i sin t),  t = position * w_i;  components behind the turned part as they are
 //
 // The angle is kept as a part of a whole turn, a fraction of 2^64: position * (w / 2 pi) modulo 1 is the low half of a product of
-// whole numbers, exact however far the position is, and its upper 32 bits give the sine and cosine to 2^-23.  A row's sines and
+// whole numbers, which adds nothing to w's own rounding, however far the position is.  Its upper 32 bits, rounded to 24, are off by less than
+// pi 2^-25 + pi 2^-31, and the sine and cosine of that by 2^-24: 2^-22.6 in all.  A row's sines and
 // cosines are worked out once and shared by its heads, so the bytes bound it: every row is read once and written once.
 #include <climits>
 

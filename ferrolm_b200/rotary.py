@@ -3,11 +3,48 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from decimal import Context, Decimal, localcontext
 
 from ._lib import check, fv_rotary, fv_rotary_rows, lib
 from .kv import _refuse
 
 LAYOUTS = ("half", "pairs")
+
+
+def _two_pi(digits: int) -> Decimal:
+    """By Machin's formula, 4 (4 arctan(1/5) - arctan(1/239)) = pi."""
+    with localcontext(Context(prec=digits + 10)):
+
+        def arctan(inverse):
+            power, total, k = Decimal(1) / inverse, Decimal(0), 1
+            while power.adjusted() > -(digits + 8):
+                total += power / k if k % 4 == 1 else -power / k
+                power, k = power / (inverse * inverse), k + 2
+            return total
+
+        return 8 * (4 * arctan(5) - arctan(239))
+
+
+def _frequencies(base, part, factor, original, fast, slow) -> list[Decimal]:
+    """w, to 55 digits and more."""
+    with localcontext(Context(prec=60)):
+        base, factor, fast, slow = (Decimal(float(x)) for x in (base, factor, fast, slow))
+        step, w = (base.ln() * -2 / part).exp(), [Decimal(1)]
+        while len(w) < part // 2:
+            w.append(w[-1] * step)
+        if original is None:
+            return [x / factor for x in w]
+        known = Decimal(float(original)) / _two_pi(60)
+        kept = [min(max((known * x - slow) / (fast - slow), Decimal(0)), Decimal(1)) for x in w]
+        return [x * (k + (1 - k) / factor) for x, k in zip(w, kept)]
+
+
+def _turns(w: list[Decimal]) -> list[int]:
+    """What pairs turn by at each position, in units of 2^-64 of a whole turn, to the nearest: a position of 31 bits is off by 2^-34 of a turn."""
+    digits = 60 + max(max(x.adjusted() for x in w), 0)  # those in front of the point too
+    with localcontext(Context(prec=digits)):
+        two_pi = _two_pi(digits)
+        return [int((x / two_pi % 1 * 2**64).to_integral_value()) % 2**64 for x in w]
 
 
 class Rotary:
@@ -36,23 +73,19 @@ class Rotary:
             w = [float(x) for x in frequencies]
             if len(w) != part // 2 or not all(map(math.isfinite, w)):
                 _refuse(f"frequencies are {part // 2} finite numbers")
+            w = [Decimal(x) for x in w]
         else:
-            w = [base ** (-2 * i / part) for i in range(part // 2)]
-            if original is None:
-                w = [x / factor for x in w]
-            else:
-                kept = [min(max((original * x / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0) for x in w]
-                w = [x * (k + (1 - k) / factor) for x, k in zip(w, kept)]
-                amplitude = 0.1 * math.log(factor) + 1.0 if amplitude is None and factor > 1 else amplitude
+            w = _frequencies(base, part, factor, original, fast, slow)
+            if original is not None and amplitude is None and factor > 1:
+                amplitude = 0.1 * math.log(factor) + 1.0
         amplitude = 1.0 if amplitude is None else float(amplitude)
         if not math.isfinite(amplitude):
             _refuse(f"amplitude is finite: got {amplitude}")
         device = torch.device("cuda" if device is None else device)
         if device.type != "cuda":
             _refuse("there is no CPU path")
-        self.dim, self.part, self.layout, self.amplitude, self.frequencies = dim, part, layout, amplitude, tuple(w)
-        turns = [round(math.fmod(x / (2 * math.pi), 1.0) * 2.0**64) % 2**64 for x in w]  # of whole turns, in units of 2^-64
-        self._turns = torch.tensor([x - 2**64 if x >= 2**63 else x for x in turns], dtype=torch.int64, device=device)
+        self.dim, self.part, self.layout, self.amplitude, self.frequencies = dim, part, layout, amplitude, tuple(map(float, w))
+        self._turns = torch.tensor([x - 2**64 if x >= 2**63 else x for x in _turns(w)], dtype=torch.int64, device=device)
         self.device = self._turns.device
         at = self._turns.data_ptr()
         self._c = {t: C.pointer(fv_rotary(self.device.index, i, dim, part, LAYOUTS.index(layout), amplitude, at)) for i, t in enumerate((torch.bfloat16, torch.float16))}

@@ -1,4 +1,7 @@
 """Rotary.rotate and KvCache.vectors: rows in front of the first sequence, results whose rows meet, far positions, tangents."""
+import math
+from decimal import Decimal, localcontext
+
 import pytest
 import torch
 
@@ -92,3 +95,64 @@ def test_calls_with_rows_in_front_of_the_first_sequence(kind, front, news):
         assert torch.equal(x[front : front + n].isnan(), y[:n].isnan())
         # a row's work may be cut in other places: weights and results are rounded to bf16, two ways
         assert x.dtype == torch.int32 and torch.equal(x[front:], y) or (x[front : front + n].float() - y[:n].float()).abs().max() <= 6 * 2.0**-8 * float(rows.float().abs().max())
+
+
+def pi_digits(n):
+    """Machin's formula, to n digits."""
+    with localcontext() as c:
+        c.prec = n + 10
+
+        def arctan_of_inverse(x):
+            term, total, k = Decimal(1) / x, Decimal(0), 0
+            while abs(term) > Decimal(10) ** -(n + 8):
+                total += term / (2 * k + 1) * (-1) ** k
+                term, k = term / (x * x), k + 1
+            return total
+
+        return 4 * (4 * arctan_of_inverse(5) - arctan_of_inverse(239))
+
+
+@pytest.mark.parametrize("how", [dict(), dict(base=500000.0), dict(factor=7.0), dict(factor=8.0, original=4096), dict(frequencies=[0.1 + 1.7 * i for i in range(64)])])
+def test_far_positions(how):
+    """As near as near ones.  An angle is off by half a unit of 2^-64 of a turn for each position, 2^-34 of a turn at most, by 2^-32 of half a
+    turn and its rounding to 24 bits, pi 2^-25 + pi 2^-31 in all, and sine and cosine by 2^-24: what a component of size 1 becomes is
+    off by less than 2^-22, with the product and the sum that are rounded to 32 bits."""
+    import ferrolm_b200 as fv
+
+    r = fv.Rotary(128, **how)
+    pos = [2**31 - 1, 2**31 - 1000, 2**30 + 12345, 2**27 + 1, 2**20, 70000, 3, 0]
+    with localcontext() as c:
+        c.prec = 60
+        two_pi, w = 2 * pi_digits(60), []
+        for i in range(64):
+            x = Decimal(how["frequencies"][i]) if "frequencies" in how else (Decimal(how.get("base", 10000.0)).ln() * (-2 * i) / 128).exp()
+            if "original" in how:
+                keep = min(max((how["original"] * x / two_pi - 1) / 31, Decimal(0)), Decimal(1))
+                x = x * (keep + (1 - keep) / Decimal(how["factor"]))
+            else:
+                x = x / Decimal(how.get("factor", 1.0))
+            w.append(x)
+        turn = [[float(p * x / two_pi % 1) for x in w] for p in pos]
+    angle = 2 * math.pi * torch.tensor(turn, dtype=torch.float64)
+    # a component that is turned to nearly nothing keeps the bits that its rounding would take from a larger one
+    x = torch.stack((angle.cos(), -angle.sin()), 1).to(FP)
+    near = (x[:, 1].double() * angle.cos() + x[:, 0].double() * angle.sin()) * r.amplitude
+    y = r.rotate(x.flatten(1).view(len(pos), 1, 128).cuda(), positions=i32(pos).cuda()).cpu().double()[:, 0, 64:]
+    assert near.abs().max() < 2.0**-10
+    assert ((y - near).abs() <= near.abs() * 2.0**-11 + 2.0**-25 + r.amplitude * 2.0**-22).all(), float((y - near).abs().max() * 2**22)
+
+
+def test_turns_are_exact():
+    """What a pair turns by at each position, to the nearest 2^-64 of a turn, from more than 64 bits."""
+    import ferrolm_b200 as fv
+
+    with localcontext() as c:
+        c.prec = 60
+        two_pi = 2 * pi_digits(60)
+        for base, factor, part in ((10000.0, 1.0, 128), (500000.0, 1.0, 80), (10000.0, 3.0, 16), (1.5, 0.3, 64), (1e-3, 1.0, 32)):
+            r = fv.Rotary(128, part=part, base=base, factor=factor)
+            for i, held in enumerate(r._turns.tolist()):
+                w = (Decimal(base).ln() * (-2 * i) / part).exp() / Decimal(factor)
+                off = abs((w / two_pi % 1) * 2**64 - held % 2**64)
+                assert min(off, 2**64 - off) <= Decimal("0.5001"), (base, i)
+                assert abs(Decimal(r.frequencies[i]) - w) <= w * Decimal(2) ** -53
