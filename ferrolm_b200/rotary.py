@@ -76,6 +76,8 @@ class Rotary:
             w = [Decimal(x) for x in w]
         else:
             w = _frequencies(base, part, factor, original, fast, slow)
+            if not all(math.isfinite(float(x)) for x in w):
+                _refuse(f"base {base} and factor {factor} make frequencies beyond what floats hold")
             if original is not None and amplitude is None and factor > 1:
                 amplitude = 0.1 * math.log(factor) + 1.0
         amplitude = 1.0 if amplitude is None else float(amplitude)
