@@ -13,7 +13,7 @@ before.  Positions below 0 or in a block that the table has no column for, and b
 cache (-1, say), are skipped: nothing is written or read there and nothing attends to them.
 
 The calls run on the current torch stream of the cache's device and do not wait for it; they can be captured into a CUDA
-graph.  Tensors are used on that stream only.  They know no gradients.  A length below 0 counts as 0.
+graph.  Tensors are used on that stream only.  They know no gradients, in neither mode.  A length below 0 counts as 0.
 """
 from __future__ import annotations
 
@@ -87,7 +87,7 @@ class KvCache:
 
         L = lib()
         self._ref, self._i32, self._f32, self._index = C.byref(self._c), torch.int32, torch.float32, self.device.index
-        self._grad = torch.is_grad_enabled
+        self._grad, self._dual = torch.is_grad_enabled, torch.autograd.forward_ad
         self._empty_like, self._contiguous = torch.empty_like, torch.contiguous_format
         self._get_stream, self._work_sizes = torch._C._cuda_getCurrentRawStream, {}
         self._add, self._vectors, self._search, self._attend = L.fv_kv_add_dev, L.fv_kv_vectors_dev, L.fv_kv_search_dev, L.fv_kv_attend_dev
@@ -124,6 +124,8 @@ class KvCache:
             _refuse(f"{what} is {self.dtype} on {self.device}: got {x.dtype} on {x.device}")
         if x.requires_grad and self._grad():
             _refuse(f"{what} wants a gradient, and the cache gives none: call it under torch.no_grad() or with a detached tensor")
+        if self._dual._current_level >= 0 and self._dual.unpack_dual(x).tangent is not None:
+            _refuse(f"{what} has a tangent, and the cache gives none: call it with the primal of unpack_dual")
         r, h, d = x.stride()
         at = x.data_ptr()
         if d != 1 or (r | h) & 7 or at & 15:

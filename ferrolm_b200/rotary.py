@@ -92,6 +92,7 @@ class Rotary:
         at = self._turns.data_ptr()
         self._c = {t: C.pointer(fv_rotary(self.device.index, i, dim, part, LAYOUTS.index(layout), amplitude, at)) for i, t in enumerate((torch.bfloat16, torch.float16))}
         self._i32, self._contiguous, self._empty_like, self._index = torch.int32, torch.contiguous_format, torch.empty_like, self.device.index
+        self._dual = torch.autograd.forward_ad
         self._grad, self._get_stream, self._rotate = torch.is_grad_enabled, torch._C._cuda_getCurrentRawStream, lib().fv_rotate_dev
         self._two = fv_rotary_rows * 2
 
@@ -103,6 +104,8 @@ class Rotary:
             _refuse(f"{what} is {dtype} on {self.device}: got {x.dtype} on {x.device}")
         if x.requires_grad and self._grad():
             _refuse(f"{what} wants a gradient, and none is recorded: call it under torch.no_grad() or with a detached tensor, and turn gradients with back=True")
+        if self._dual._current_level >= 0 and self._dual.unpack_dual(x).tangent is not None:
+            _refuse(f"{what} has a tangent, and none is worked out: the turn is linear, so turn the tangent by itself")
         r, h, d = x.stride()
         at = x.data_ptr()
         if out is None:

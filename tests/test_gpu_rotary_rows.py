@@ -4,6 +4,7 @@ from decimal import Decimal, localcontext
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from tests.test_gpu_kv_rows import batch, i32
 from tests.test_gpu_rotary import check, turned
@@ -156,3 +157,21 @@ def test_turns_are_exact():
                 off = abs((w / two_pi % 1) * 2**64 - held % 2**64)
                 assert min(off, 2**64 - off) <= Decimal("0.5001"), (base, i)
                 assert abs(Decimal(r.frequencies[i]) - w) <= w * Decimal(2) ** -53
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives are not recorded either."""
+    import ferrolm_b200 as fv
+
+    r, pos = fv.Rotary(64), i32([1, 2, 3]).cuda()
+    c = fv.KvCache(10, 2, 64, page_size=16)
+    x, table, lens = torch.randn((3, 2, 64)).to(BF).cuda(), torch.arange(6, dtype=torch.int32).view(3, 2).cuda(), i32([1, 2, 3]).cuda()
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: r.rotate(dual, positions=pos), lambda: r.rotate(x, dual, positions=pos), lambda: c.add(dual, x, table, lens), lambda: c.add(x, dual, table, lens),
+                     lambda: c.attend(dual, table, lens), lambda: c.search_blocks(dual, table, lens, 3)):
+            with pytest.raises(fv.FerrovecError, match="tangent"):
+                call()
+        plain = r.rotate(x, positions=pos)  # other rows are as ever
+        assert torch.equal(r.rotate(fwad.unpack_dual(dual).primal, positions=pos), plain)
+    assert torch.equal(r.rotate(x, positions=pos), plain)
