@@ -25,26 +25,30 @@ def _two_pi(digits: int) -> Decimal:
         return 8 * (4 * arctan(5) - arctan(239))
 
 
+DIGITS = 60
+TWO_PI = _two_pi(DIGITS)
+
+
 def _frequencies(base, part, factor, original, fast, slow) -> list[Decimal]:
     """w, to 55 digits and more."""
-    with localcontext(Context(prec=60)):
+    with localcontext(Context(prec=DIGITS)):
         base, factor, fast, slow = (Decimal(float(x)) for x in (base, factor, fast, slow))
         step, w = (base.ln() * -2 / part).exp(), [Decimal(1)]
         while len(w) < part // 2:
             w.append(w[-1] * step)
         if original is None:
             return [x / factor for x in w]
-        known = Decimal(float(original)) / _two_pi(60)
+        known = Decimal(float(original)) / TWO_PI
         kept = [min(max((known * x - slow) / (fast - slow), Decimal(0)), Decimal(1)) for x in w]
         return [x * (k + (1 - k) / factor) for x, k in zip(w, kept)]
 
 
 def _turns(w: list[Decimal]) -> list[int]:
     """What pairs turn by at each position, in units of 2^-64 of a whole turn, to the nearest: a position of 31 bits is off by 2^-34 of a turn."""
-    digits = 60 + max(max(x.adjusted() for x in w), 0)  # those in front of the point too
-    with localcontext(Context(prec=digits)):
-        two_pi = _two_pi(digits)
-        return [int((x / two_pi % 1 * 2**64).to_integral_value()) % 2**64 for x in w]
+    front = max(max(x.adjusted() for x in w), 0)  # digits in front of the point
+    with localcontext(Context(prec=DIGITS + front)):
+        unit = 2**64 / (_two_pi(DIGITS + front) if front else TWO_PI)
+        return [int((x * unit).to_integral_value()) % 2**64 for x in w]
 
 
 class Rotary:
