@@ -215,7 +215,6 @@ struct Stage<FV_KV_INT4X32, D> {
 };
 
 constexpr float KV_LAG = 6.f;  // 4 bits: log2 of what a maximum may lag behind by
-enum { KV_LEAST_UNIT = -15 };  // 2^15 is fp16's largest power of two
 
 // A warp's share of a row's attention: NT tiles of 8 queries.  A lane's queries are 8 x + 2 t and the next one.
 template <class T, int KIND, int D, int NT>
@@ -228,9 +227,7 @@ struct Share {
   float by[NT][2];  // scale of a lane's queries
   float o[D / 16][NT][4], m[NT][2], l[NT][2];
   uint32_t by_1024, by_64;  // 4 bits: what codes are added to
-  // 8 bits: values stand for multiples of 2^(unit - 126).  4 bits, results in bf16: the scales seen are below 2^(unit + 2); from 2 on a weight of 1 is
-  // 2^(ONE - unit), below that the scales are taken 2^-unit times, so that their products stay among fp16's normal numbers
-  int unit;
+  int unit;  // 8 bits: values stand for multiples of 2^(unit - 126)
   float far[NT][2];  // 4 bits: a maximum is replaced by one above this
 
   __device__ __forceinline__ void begin(const KvAttend& a, int row, int head, int first, int g, int t) {
@@ -294,7 +291,7 @@ struct Share {
       for (int x = 0; x < NT; ++x)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[u][x][i] = 0.f;
-    unit = FOUR && std::is_same<T, __nv_bfloat16>::value ? KV_LEAST_UNIT : 0;
+    unit = 0;
     if constexpr (FOUR) by_1024 = Four::magic(0x64006400u), by_64 = Four::magic(0x54005400u);
   }
 
@@ -305,17 +302,16 @@ struct Share {
       for (int h = 0; h < L::PIECES; ++h) take_four<1>(stage, h, g, t);
   }
 
-  // 4 bits: codes are exact in fp16.  A key's scales multiply the sums over their groups.  A value's multiply the weights, in fp16, which rounds
-  // them once more; for that not to cost small values their bits, scales are relative to the largest seen.  Results in
-  // fp16 would show that (0.00036 of them against 64 bits, where one rounding leaves 0.00028 and their own 0.00021): there scales
-  // multiply the codes, exactly, at 4 % of the time.  A maximum that grows by less than 2^KV_LAG is left as it was: with few pieces to a
-  // warp, most of them have a new one (a fifth of the instructions were for that).
+  // 4 bits: codes are exact in fp16.  A key's scales multiply the sums over their groups.  A value's multiply the codes, in fp16, which is exact:
+  // weights are rounded once, and values of any size keep their bits.  (On the weights, which are rounded twice then, they take 56.5 us for the
+  // 64 requests' 57.2, and small values lose most of their bits; relative to the largest scale seen they keep them, and take 56.9.)
+  // A maximum that grows by less than 2^KV_LAG is left as it was: with few pieces to a warp, most of them have a new one (a fifth of the
+  // instructions were for that).
   // (Codes below fp16's normal numbers, masked out of their words and not subtracted from, would be less work; the tensor cores
   // keep ten bits less of a sum of such products.)
   template <int P>
   __device__ __forceinline__ void take_four(uint32_t stage, int first, int g, int t) {
     constexpr int NG = D / 32;
-    constexpr bool ONCE = std::is_same<T, __half>::value;
     int visible[P], any = 0;
 #pragma unroll
     for (int h = 0; h < P; ++h) visible[h] = int(shared_bytes<4>(stage + L::SEEN + 4 * (first + h))), any = max(any, visible[h]);
@@ -383,15 +379,11 @@ struct Share {
           for (int x = 0; x < NT; ++x) s[h][x][i] = L::token(g) + (i & 2) * 4 < visible[h] ? s[h][x][i] : -INFINITY;
         }
     }
-    bool moved = false, odd = false;
-    {  // a scale that `unit` does not cover, or is no number: every lane looks at four of them, those of rows that are not seen too
-      constexpr int WORDS = 4 * NG * P;
-      const int lane = 4 * g + t;
-      const uint32_t w = shared_bytes<4>(value_scales + 4 * (WORDS == 24 ? (lane < 24 ? lane : lane - 24) : WORDS == 12 ? lane % 12 : lane & (WORDS - 1)));
-      const uint32_t from = ONCE ? 248u : uint32_t(8 * (unit + 17));  // the smallest byte that is not covered, from 16 to 248
-      const uint32_t up = (w & 0x7F7F7F7Fu) + 0x01010101u * (128u - (from & 127u)), both = from < 128u ? ~0u : 0u;  // byte by byte: lower seven bits not below those of `from`
-      moved = (((w & up) | ((w | up) & both)) & 0x80808080u) != 0u;
-    }
+    uint32_t high = 0u;
+#pragma unroll
+    for (int h = 0; h < P; ++h) high |= (vs[h][0] | vs[h][1]) | (vs[h][2] | vs[h][3]);
+    // Bytes from 248 on are no numbers.  Their bits together may reach that too where scales lie on both sides of 2: then it is looked at closer.
+    bool moved = (high & ((high & 0x7F7F7F7Fu) + 0x08080808u) & 0x80808080u) != 0u, odd = false;
     float to[NT][2];
 #pragma unroll
     for (int x = 0; x < NT; ++x)
@@ -403,19 +395,11 @@ struct Share {
         moved = moved || to[x][i] > far[x][i];
       }
     if (__any_sync(FV_FULL, moved)) {  // seldom, after the first pieces
-      uint32_t most = 0;  // of the scales that are numbers
 #pragma unroll
       for (int h = 0; h < P; ++h)
 #pragma unroll
-        for (int i = 0; i < 4 * NG; ++i) {
-          const uint32_t byte = vs[h][i / NG] >> (8 * (i % NG)) & 255u;
-          if (byte < 248u) most = max(most, byte);
-          odd = odd || byte >= 248u;
-        }
+        for (int i = 0; i < 4 * NG; ++i) odd = odd || (vs[h][i / NG] >> (8 * (i % NG)) & 255u) >= 248u;
       odd = __any_sync(FV_FULL, odd);
-      const int up = ONCE ? 0 : max(unit, int(__reduce_max_sync(FV_FULL, most) >> 3) - 16);  // below 2^(e - 14) = 2^(2 + unit)
-      const float less = __uint_as_float(uint32_t(127 + max(unit, 0) - max(up, 0)) << 23), less_o = __uint_as_float(uint32_t(127 + unit - up) << 23);  // of sums of weights, and of results
-      unit = up;
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -427,16 +411,15 @@ struct Share {
           y = y > far[x][i] ? y : m[x][i];
           const float down = y > m[x][i] ? exp2_of(m[x][i] - y) : 1.f;
           m[x][i] = y, far[x][i] = y == -INFINITY ? y : y + KV_LAG;
-          l[x][i] *= down * less;
+          l[x][i] *= down;
 #pragma unroll
-          for (int u = 0; u < D / 16; ++u) o[u][x][i] *= down * less_o, o[u][x][i + 2] *= down * less_o;
+          for (int u = 0; u < D / 16; ++u) o[u][x][i] *= down, o[u][x][i + 2] *= down;
         }
     }
     uint32_t b[P][NT][2];
-    const float one = ONE - float(max(unit, 0));
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
-      const float off[2] = {one - (m[x][0] == -INFINITY ? 0.f : m[x][0]), one - (m[x][1] == -INFINITY ? 0.f : m[x][1])};
+      const float off[2] = {ONE - (m[x][0] == -INFINITY ? 0.f : m[x][0]), ONE - (m[x][1] == -INFINITY ? 0.f : m[x][1])};
 #pragma unroll
       for (int h = 0; h < P; ++h) {
         float p[4];
@@ -460,7 +443,7 @@ struct Share {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const uint32_t w = shared_bytes<NG>(value_scales + L::token(g) * NG + (16 * h + 8 * r) * NG);
-              const bool weight = exp2_of(__fmaf_rn(s[h][x][2 * r + i], by[x][i], one - (m[x][i] == -INFINITY ? 0.f : m[x][i]))) != 0.f;
+              const bool weight = exp2_of(__fmaf_rn(s[h][x][2 * r + i], by[x][i], ONE - (m[x][i] == -INFINITY ? 0.f : m[x][i]))) != 0.f;
 #pragma unroll
               for (int y = 0; y < NG; ++y) bad |= L::token(g) + 8 * r < visible[h] && weight && (w >> (8 * y) & 255u) >= 248u ? 1u << y : 0u;
             }
@@ -497,44 +480,22 @@ struct Share {
           sc[z][y] = two[0];
           if (y + 1 < NG) sc[z][y + 1] = two[1];
         }
-      if constexpr (!ONCE) {  // exact: below 4, and not smaller than they were
-        const __half2 times = __half2half2(__ushort_as_half(uint16_t((15 - min(unit, 0)) << 10)));
-#pragma unroll
-        for (int z = 0; z < 2; ++z)
-#pragma unroll
-          for (int y = 0; y < NG; ++y) {
-            const __half2 c = __hmul2(*reinterpret_cast<const __half2*>(&sc[z][y]), times);
-            sc[z][y] = *reinterpret_cast<const uint32_t*>(&c);
-          }
-      }
 #pragma unroll
       for (int y = 0; y < NG; ++y) {
-        uint32_t a[2][4], w[NT][2];  // [rows 2 t, or 2 t + 8, and the next one][component]
+        uint32_t a[2][4];  // [rows 2 t, or 2 t + 8, and the next one][component]
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           Four::halves(__byte_perm(v[2 * z][y / 2], v[2 * z + 1][y / 2], y & 1 ? 0x7632 : 0x5410), a[z], by_1024, by_64);
-          const uint32_t f = sc[z][y];
-          if constexpr (ONCE) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __half2 c = __hmul2(*reinterpret_cast<const __half2*>(&a[z][e]), *reinterpret_cast<const __half2*>(&f));
-              a[z][e] = *reinterpret_cast<const uint32_t*>(&c);
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < NT; ++x) {
-            if constexpr (ONCE) {
-              w[x][z] = b[h][x][z];
-              continue;
-            }
-            const __half2 c = __hmul2(*reinterpret_cast<const __half2*>(&b[h][x][z]), *reinterpret_cast<const __half2*>(&f));
-            w[x][z] = *reinterpret_cast<const uint32_t*>(&c);
+          for (int e = 0; e < 4; ++e) {
+            const __half2 c = __hmul2(*reinterpret_cast<const __half2*>(&a[z][e]), *reinterpret_cast<const __half2*>(&sc[z][y]));
+            a[z][e] = *reinterpret_cast<const uint32_t*>(&c);
           }
         }
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
-          for (int z = 0; z < 2; ++z) mma_16<M>(o[2 * y + z][x], a[0][2 * z], a[0][2 * z + 1], a[1][2 * z], a[1][2 * z + 1], w[x][0], w[x][1]);
+          for (int z = 0; z < 2; ++z) mma_16<M>(o[2 * y + z][x], a[0][2 * z], a[0][2 * z + 1], a[1][2 * z], a[1][2 * z + 1], b[h][x][0], b[h][x][1]);
       }
     }
   }
@@ -691,11 +652,9 @@ struct Share {
   static constexpr int FLOATS = 8 * NT * (D + 2);
   __device__ __forceinline__ void store(float* to, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    const float f = SCALED ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : FOUR ? __uint_as_float(uint32_t(127 + unit) << 23) : 1.f;
-    [[maybe_unused]] const float f_l = FOUR ? __uint_as_float(uint32_t(127 + max(unit, 0)) << 23) : 1.f;
+    const float f = SCALED ? __uint_as_float(uint32_t(min(unit + 1, 254)) << 23) : 1.f;
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
-      if constexpr (FOUR) l[x][0] *= f_l, l[x][1] *= f_l;
 #pragma unroll
       for (int u = 0; u < D / 16; ++u)
         reinterpret_cast<float4*>(to)[(u * NT + x) * 32 + lane] = make_float4(o[u][x][0] * f, o[u][x][1] * f, o[u][x][2] * f, o[u][x][3] * f);

@@ -377,10 +377,8 @@ int fv_kv_search_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, co
  * attend to gets zeros and -inf.  Scores, maxima and sums are 32-bit floats; weights are rounded to 16 bits before they meet the
  * values.  Over 8 bits a weight is rounded together with its value's scale, relative to the largest scale among the rows that the
  * query sees, which costs a result up to 2^-38 of that scale times the largest code for each row, and bf16 queries become fp16, which
- * costs a component up to 2^-38 of the query's largest.  Over 4 bits queries become fp16 too, and a weight is off by up to 2^-32 of the largest
- * (times half the largest scale, if that is more than 1) besides its rounding; for single rows with results in bf16 it is rounded once more, as
- * the product with its value's scale, which besides is off by up to 2^-33 of the largest weight times the largest scale (or times 2^-14, if
- * that is more).  The largest scale is that of the values of the key head that the row sees.  The waits inside the kernels are bounded (about 2 s); results of one that ran out are NaN. */
+ * costs a component up to 2^-38 of the query's largest.  Over 4 bits queries become fp16 too, values are exact, and a weight
+ * is off by up to 2^-32 of the largest besides its one rounding to fp16.  The waits inside the kernels are bounded (about 2 s); results of one that ran out are NaN. */
 int fv_kv_attend_dev(const fv_kv* kv, void* stream, const fv_kv_batch* batch, const void* q, size_t q_row, size_t q_head,
                      size_t group, const int32_t* blocks, size_t k, float scale, void* out, float* lse, void* work, size_t work_bytes);
 /* Bytes of device memory that fv_kv_attend_dev wants as `work` (on 16 bytes, the caller's, used until the call's kernels are
