@@ -18,8 +18,9 @@
 // 32 blocks take 10.2 us in a graph, most of it dependent loads: the list, the table, the rows, and the shares that are joined.
 //
 // In 4 bits a row is half as long and its codes are taken apart by masks: 64 rows of 64 heads over 40 blocks (181 MB) take 57 us, 3.2 TB/s,
-// 0.49 of the copy rate; 12 whole sequences of heads of 96 in fp16 (210 MB) 76 us.  Copying alone would take 36 and 40: some 390 instructions for
-// 16 rows and a head bound it (three fifths of the issue slots; 160 of them on the ALU, at half the others' rate: 80 take the codes apart).
+// 0.48 of the copy rate; 12 whole sequences of heads of 96 in fp16 (210 MB) 76 us.  Copying alone would take 36 and 40: some 415 instructions for
+// 16 rows and a head (63 % of the issue slots; 163 of them on the ALU, at half the others' rate: 80 take the codes apart), and, with 12.8 warps
+// to an SM, the time that a warp waits for its own last step.
 //
 // In 8 bits the codes are exact in fp16; a key's scale multiplies its score, a value's its weight, relative to the largest
 // power of two of a scale that the row has seen.  Weights are rounded to 16 bits for the second product: fp16 with 2^14 for 1, so that

@@ -29,7 +29,7 @@
 // The tile's scales come relative to the same for all that the CTA's queries see, which mostly is the query's own power too; a warp
 // with a query for which it is not takes the scales as they are (as fast as one power for all: int8, dense 388 us, e4m3, lists 1160).
 // In 4 bits code times scale goes into shared memory as fp16, exactly, and the rest is as over 16 bits, but that 2^7 stands for a weight of 1 and
-// a maximum may lag behind by 2^8, for O to be scaled as seldom as in bf16 (2.8k rows over up to 6000, 195 GFLOP: 374 us, 428 with 2^14
+// a maximum may lag behind by 2^8, for O to be scaled as seldom as in bf16 (2.5k rows over up to 6000, 195 GFLOP: 373 us, 428 with 2^14
 // and a factor of 2; 396 for bf16 with whole sequences of 6000, 451 in 4 bits).  Taking the codes apart is 1400 of a tile's 3600 instructions.
 #include <climits>
 

@@ -33,9 +33,9 @@ struct Rotary {
 };
 
 // A CTA has ROWS rows.  Thread t takes piece t % units of a head: eight pairs of the two halves, or four neighbouring pairs (PAIRS), or
-// eight components that stay; it has the pieces of AHEAD heads on their way.  14k rows of 40 heads of 128 in halves: 54.0 us, 5.3 TB/s; half of a
+// eight components that stay; it has the pieces of AHEAD heads on their way.  13.6k rows of 40 heads of 128 in halves: 54.0 us, 5.3 TB/s; half of a
 // head in neighbours, 48.2 us, 5.9 TB/s, 0.91 of the copy rate (with four on their way, for which fewer CTAs have room, 57.2 and 50.9; with
-// eight rows to a CTA 59.9 and 49.9).  24 rows: 3.2 us, dependent loads (lengths, turns, rows).
+// eight rows to a CTA 59.9 and 49.9).  24 rows: 2.8 us, dependent loads (lengths, turns, rows).
 template <class T, bool PAIRS, int ROWS>
 __global__ void __launch_bounds__(ROTARY_THREADS) rotate_kernel(Rotary a, KvBatch m) {
   constexpr int AHEAD = 2;

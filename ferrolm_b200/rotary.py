@@ -57,9 +57,10 @@ class Rotary:
     `layout`: "half" pairs component i with i + part / 2, "pairs" 2 i with 2 i + 1.  dim and part (dim unless given) are multiples of 16.
     w[i] = base ** (-2 i / part).  For contexts that are `factor` times as long as those that a model was trained on: without
     `original` all w are divided by it; with `original`, the positions that the model was trained on, pairs that turn less than `slow`
-    times in these are divided, those that turn more than `fast` times are not, those between are in part, and what is turned is
-    multiplied by `amplitude`, 0.1 ln(factor) + 1 unless given (1 without `original`).  `frequencies` (part / 2 numbers) are
-    taken in place of all of that.  `dtype`: torch.bfloat16 or torch.float16, that of the rows.
+    times in these are divided, those that turn more than `fast` times are not, those between are in part (the share that is kept grows
+    linearly with the number of turns; where a checkpoint has it grow with the pair's index, give its `frequencies`), and what is turned is
+    multiplied by `amplitude`, 0.1 ln(factor) + 1 unless given (1 without `original`, and for factors up to 1).  `frequencies` (part / 2
+    numbers) are taken in place of all of that.  `dtype`: torch.bfloat16 or torch.float16, that of the rows.
     """
 
     def __init__(self, dim: int, part: int | None = None, layout: str = "half", base: float = 10000.0, factor: float = 1.0, original: int | None = None,

@@ -390,7 +390,7 @@ size_t fv_kv_attend_work(const fv_kv* kv, const fv_kv_batch* batch, size_t group
  * cache and attended to.  Of `dim` components the first `part` are turned in pairs, component i with i + part/2 (half) or 2 i with 2 i + 1
  * (pairs): y_i = amplitude (x_i cos t - x_j sin t), y_j = amplitude (x_j cos t + x_i sin t), t = 2 pi * position * turns[i] / 2^64.
  * `turns` (device memory, part/2 numbers) is what a pair turns by at each position, as a fraction of 2^64 of a whole turn, so that far
- * positions are as exact as near ones.  dim and part are multiples of 16, dim at most 1024.  `back`: the transposed turn (sin t -> -sin t),
+ * positions are as exact as near ones; sine and cosine are within 2^-22.  dim and part are multiples of 16, dim at most 1024.  `back`: the transposed turn (sin t -> -sin t),
  * which gradients take and which, but for the amplitude's square, undoes the other.
  *
  * Row i of a call has the position that fv_kv_batch gives it (lens, cu), or positions[i].  Rows of no sequence and positions below 0
