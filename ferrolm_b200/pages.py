@@ -29,9 +29,13 @@ def _shared(a: fv_table, b: fv_table) -> int:
         return 0
     if (begin_a, a.stride, a.width, a.nseq) == (begin_b, b.stride, b.width, b.nseq):
         return a.nseq * a.width
-    found = 0
+    begin, found = (begin_a - begin_b) // 4, 0  # of a, in b
+    if a.stride == b.stride and a.nseq > 1 and b.nseq > 1:  # row i of a begins in row i + k of b, and may end in the next one
+        k, at = divmod(begin, b.stride)
+        rows = lambda k: max(min(a.nseq, b.nseq - k) - max(-k, 0), 0)  # noqa: E731
+        return rows(k) * max(min(a.width, b.width - at), 0) + rows(k + 1) * max(min(at + a.width - b.stride, b.width), 0)
     for i in range(a.nseq):
-        row = (begin_a - begin_b) // 4 + i * a.stride  # where row i of a begins in b
+        row = begin + i * a.stride
         step = b.stride if b.nseq > 1 else max(b.stride, row + a.width + b.width, 1)
         j = max((row - b.width) // step, 0)
         while j < b.nseq and j * step < row + a.width:
